@@ -267,7 +267,7 @@ def _prepare_cached(case, g, dev):
           "q_lens": torch.tensor(valid, dtype=torch.int32).to(dev),
           "groups": torch.tensor(groups, dtype=torch.int32).to(dev) if shared else None,
           "prefix_lens": torch.full((len(groups) - 1,), shared * page, dtype=torch.int32).to(dev) if shared else None,
-          "host": (lens, valid), "max_len": max(lens)}
+          "host": (lens, valid)}
     if own:
         from tensorpack_amd.cache import PagedCache
         st["cache"] = PagedCache.from_buffers(pool, st["table"], st["lens"], st["refs"])
@@ -463,7 +463,7 @@ def _plain_verify(st):
     score = torch.where(rest > 0, rest * st["noise"], -1.0)
     best = score.amax(1, keepdim=True)
     first = torch.where(score == best, torch.arange(w.shape[1], device=x.device), w.shape[1]).amin(1)
-    first = torch.where(best[:, 0] > 0, first, -1)
+    first = torch.where(best[:, 0] >= 0, first, -1)
     tokens = torch.full((n, K + 1), -1, dtype=st["drafts"].dtype, device=x.device)
     tokens[:, :K] = torch.where(j < count[:, None], st["drafts"], -1)
     tokens[rows, count] = first.to(tokens.dtype)
@@ -479,7 +479,7 @@ def _own_prompt(st):
 def _own_cached(st):
     from tensorpack_amd.attention import cached_attention
     return cached_attention(st["q"], st["cache"], 0, st["seqs"], q_lens=st["q_lens"], groups=st["groups"],
-                            prefix_lens=st["prefix_lens"], max_len=st["max_len"])
+                            prefix_lens=st["prefix_lens"])
 
 
 def _own_pages(st):
