@@ -1,4 +1,4 @@
-"""ctypes mirror of include/mtc_hip.h (struct layout, constants, prototypes)."""
+"""ctypes mirror of include/mtc_hip.h and include/mtc_serve.h (struct layout, constants, prototypes)."""
 
 import ctypes
 
@@ -7,6 +7,7 @@ ABI_VERSION = 11
 MTC_OK = 0
 MTC_DTYPE_F32 = 0
 MTC_DTYPE_BF16 = 1
+MTC_DTYPE_F16 = 2                        # serving operators
 MTC_FLAG_FP32_SCALES = 0x1
 MTC_FLAG_MX_LAYOUT = 0x2                 # payload in the matrix-core decode layout (packer.LAYOUT_MX)
 MTC_FLAG_COLS_GATHERED = 0x4             # tile stream with columns in the original order (8-word cells)
@@ -22,6 +23,19 @@ EXPORTED = ("mtc_abi_version", "mtc_last_error", "mtc_check_desc", "mtc_dequant"
             "mtc_gemv_f32_batch", "mtc_gemv_noalloc_scratch_bytes", "mtc_gemv_f32_noalloc", "mtc_gemm_batch_plan",
             "mtc_gemm_bf16_batch", "mtc_gemm_f32_workspace_bytes", "mtc_gemm_f32", "mtc_tile_plan",
             "mtc_set_prefill_decode_once")
+
+SERVE_EXPORTED = ("mtc_prompt_attention", "mtc_check_cache_desc", "mtc_cache_scratch_ints", "mtc_cache_extend",
+                  "mtc_cache_fork", "mtc_cache_truncate", "mtc_cache_compact", "mtc_cache_copy_pages", "mtc_cache_append",
+                  "mtc_cached_attention_workspace_bytes", "mtc_cached_attention", "mtc_verify_workspace_bytes",
+                  "mtc_verify_drafts")
+
+ATTN_MAX_DIM = 128                       # MTC_ATTN_MAX_DIM
+CACHED_MAX_TOKENS = 16                   # MTC_CACHED_MAX_TOKENS
+CACHED_MAX_SEQS = 8192                   # MTC_CACHED_MAX_SEQS
+CACHE_MAX_SLOTS = 65536                  # MTC_CACHE_MAX_SLOTS
+CACHE_STATUS = {1: "sequence number out of range or twice in a list", 2: "not enough free pages",
+                4: "a sequence's table row is full", 8: "negative count, or a length above the present one",
+                16: "fork into a sequence that holds tokens or is a source"}
 
 
 class MtcStreamDesc(ctypes.Structure):
@@ -95,6 +109,50 @@ class MtcGemmBatchItem(ctypes.Structure):
     ]
 
 
+class MtcHeads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class MtcPromptArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("n_seqs", ctypes.c_int32), ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("dim", ctypes.c_int32), ("q_rows", ctypes.c_int32), ("k_rows", ctypes.c_int32),
+        ("causal", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("q", MtcHeads), ("k", MtcHeads), ("v", MtcHeads), ("o", MtcHeads),
+        ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p),
+    ]
+
+
+class MtcCacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("n_pages", ctypes.c_int32), ("n_layers", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("dim", ctypes.c_int32), ("page_size", ctypes.c_int32), ("max_seqs", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("pool", ctypes.c_void_p), ("table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("refs", ctypes.c_void_p),
+        ("state", ctypes.c_void_p), ("scratch", ctypes.c_void_p),
+    ]
+
+
+class MtcCachedArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_uint32), ("layer", ctypes.c_int32), ("n_seqs", ctypes.c_int32), ("tokens", ctypes.c_int32),
+        ("heads", ctypes.c_int32), ("n_groups", ctypes.c_int32), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("q", MtcHeads), ("o", MtcHeads),
+        ("seqs", ctypes.c_void_p), ("q_lens", ctypes.c_void_p), ("groups", ctypes.c_void_p), ("prefix_lens", ctypes.c_void_p),
+    ]
+
+
+class MtcVerifyArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("index_bytes", ctypes.c_int32), ("n_seqs", ctypes.c_int32),
+        ("n_drafted", ctypes.c_int32), ("vocab", ctypes.c_int32),
+        ("p", ctypes.c_void_p), ("p_stride", ctypes.c_int64 * 2), ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64 * 2),
+        ("u", ctypes.c_void_p), ("u_stride", ctypes.c_int64), ("noise", ctypes.c_void_p), ("noise_stride", ctypes.c_int64),
+        ("drafts", ctypes.c_void_p), ("drafts_stride", ctypes.c_int64), ("n_drafts", ctypes.c_void_p),
+        ("tokens", ctypes.c_void_p), ("accepted", ctypes.c_void_p),
+    ]
+
+
 MAX_GROUP = 4                        # MTC_MAX_GROUP: matrices per mtc_gemv_f32_group launch
 
 
@@ -152,6 +210,28 @@ def declare(lib: ctypes.CDLL) -> None:
     lib.mtc_gemm_bf16_group.restype = i32
     lib.mtc_gemm_bf16_group.argtypes = [ctypes.POINTER(TileDescP), i32, vp, i32, i64, ctypes.POINTER(vp), i32,
                                         ctypes.POINTER(i64), i32, vp, sz, vp]
+    declare_serve(lib)
+
+
+def declare_serve(lib: ctypes.CDLL) -> None:
+    vp, i32, sz, P = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.POINTER
+    cache = P(MtcCacheDesc)
+    for name, res, args in (
+            ("mtc_prompt_attention", i32, [P(MtcPromptArgs), vp]),
+            ("mtc_check_cache_desc", i32, [cache]),
+            ("mtc_cache_scratch_ints", sz, [i32, i32]),
+            ("mtc_cache_extend", i32, [cache, vp, vp, i32, vp]),
+            ("mtc_cache_fork", i32, [cache, vp, vp, i32, vp]),
+            ("mtc_cache_truncate", i32, [cache, vp, vp, i32, vp]),
+            ("mtc_cache_compact", i32, [cache, vp]),
+            ("mtc_cache_copy_pages", i32, [cache, vp, i32, vp, vp, i32, vp]),
+            ("mtc_cache_append", i32, [cache, i32, P(MtcHeads), P(MtcHeads), i32, i32, vp, vp, i32, vp]),
+            ("mtc_cached_attention_workspace_bytes", sz, [cache, P(MtcCachedArgs)]),
+            ("mtc_cached_attention", i32, [cache, P(MtcCachedArgs), vp, sz, vp]),
+            ("mtc_verify_workspace_bytes", sz, [P(MtcVerifyArgs)]),
+            ("mtc_verify_drafts", i32, [P(MtcVerifyArgs), vp, sz, vp])):
+        getattr(lib, name).restype = res
+        getattr(lib, name).argtypes = args
 
 
 class MtcError(RuntimeError):

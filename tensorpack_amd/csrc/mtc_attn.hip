@@ -1,0 +1,914 @@
+// gfx950 attention kernels and their C-ABI (include/mtc_serve.h).
+//
+//   k_prompt  : whole prompts, packed sequences, causal or not
+//   k_cached  : the newest tokens of each sequence over a paged cache; work split evenly over the blocks
+//   k_join    : joins k_cached's partial results per row
+//
+// Both multiply keys by queries with the keys as rows: S^T = K Q^T puts one query into each lane's
+// column, so a softmax row lives in one lane (plus its partners in the other lane groups), and the
+// same registers, rounded to 16 bits, are the right operand of O^T = V^T P^T without a shuffle: the
+// matrix instruction's reduction index may be numbered freely as long as both operands agree, and
+// V^T is read from LDS in that numbering by the transposing read.
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "mtc_attn.h"
+#include "mtc_host.h"
+#include "mtc_serve.h"
+
+#define MTC_API extern "C" __attribute__((visibility("default")))
+
+using mtc::host::check_launch;
+using mtc::host::fail;
+using mtc::host::ok;
+using namespace mtc::attn;
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// whole prompts
+// ---------------------------------------------------------------------------
+constexpr int kPromptWaves = 4;                   // 32 query rows each
+constexpr int kPromptRows = 32 * kPromptWaves;
+constexpr int kPromptKeys = 64;                   // keys per step
+
+struct PromptTile {
+  int tile;          // query tile of its sequence, -1: none
+  int q0, n, k0, m;  // the sequence's rows of q and k
+};
+
+__device__ __forceinline__ void prompt_range(const int32_t* cu, int b, int rows, int& at, int& n) {
+  at = min(max(cu[b], 0), rows);
+  n = min(max(cu[b + 1], at), rows) - at;
+}
+
+// The rank-th query tile of the call, the tiles with the largest place in their sequence first (with a
+// causal mask these see most keys; started last they would run alone at the end). Every lane gets it.
+__device__ PromptTile prompt_tile(const mtc_prompt_args& a, int rank) {
+  const int lane = threadIdx.x & 63;
+  auto tiles = [&](int b) {
+    int at, n;
+    prompt_range(a.cu_q, b, a.q_rows, at, n);
+    return (n + kPromptRows - 1) / kPromptRows;
+  };
+  const int t0 = lane < a.n_seqs ? tiles(lane) : 0;
+  auto count = [&](int level) {                     // tiles at `level` or above
+    int s = max(0, t0 - level);
+    for (int b = lane + 64; b < a.n_seqs; b += 64) s += max(0, tiles(b) - level);
+    return wave_sum(s);
+  };
+  PromptTile r;
+  r.tile = -1;
+  r.q0 = r.n = r.k0 = r.m = 0;
+  int seq = 0;
+  if (a.n_seqs == 1) {
+    const int t = __builtin_amdgcn_readfirstlane(t0);
+    if (rank >= t) return r;
+    r.tile = t - 1 - rank;
+  } else {
+    if (rank >= count(0)) return r;
+    int lo = 0, hi = (a.q_rows + kPromptRows - 1) / kPromptRows;     // count(lo) > rank >= count(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (count(mid) > rank) lo = mid; else hi = mid;
+    }
+    int left = rank - count(hi);                    // the left-th sequence with more than lo tiles
+    for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
+      const bool has = b0 + lane < a.n_seqs && (b0 ? tiles(b0 + lane) : t0) > lo;
+      const uint64_t mask = __ballot(has);
+      const int c = __popcll(mask);
+      if (left < c) {
+        const uint64_t hit = __ballot(has && __popcll(mask & ((1ull << lane) - 1)) == left);
+        seq = b0 + __ffsll((unsigned long long)hit) - 1;
+        break;
+      }
+      left -= c;
+    }
+    r.tile = lo;
+  }
+  prompt_range(a.cu_q, seq, a.q_rows, r.q0, r.n);
+  prompt_range(a.cu_k, seq, a.k_rows, r.k0, r.m);
+  r.tile = __builtin_amdgcn_readfirstlane(r.tile);
+  r.q0 = __builtin_amdgcn_readfirstlane(r.q0);
+  r.n = __builtin_amdgcn_readfirstlane(r.n);
+  r.k0 = __builtin_amdgcn_readfirstlane(r.k0);
+  r.m = __builtin_amdgcn_readfirstlane(r.m);
+  return r;
+}
+
+template <bool BF, int DP>
+__global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_prompt_args a) {
+  using E = Elem<BF>;
+  constexpr int kRow = DP * 2;                             // bytes of an LDS row
+  constexpr int kTile = kPromptKeys * kRow;
+  constexpr int kCopies = kTile / 1024 / kPromptWaves;     // 1 KiB copies per wave and tile
+  constexpr int kCopyRows = 1024 / kRow;
+  constexpr int kSteps = DP / 16;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kTile];   // K, V; two buffers each
+
+  const int H = a.heads, KV = a.kv_heads, D = a.dim;
+  // heads of one K/V head apart by KV places: blocks that share keys share an XCD (and its L2) when the
+  // count of K/V heads is a multiple or a divisor of 8
+  const int j = blockIdx.x % H;
+  const int kvh = j % KV, head = kvh * (H / KV) + j / KV;
+  const PromptTile pt = prompt_tile(a, blockIdx.x / H);
+  if (pt.tile < 0) return;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int half = lane >> 5, col = lane & 31;
+  const int row = pt.tile * kPromptRows + wave * 32 + col;         // this lane's query
+  const int shift = pt.m - pt.n + 1;
+  auto sees = [&](int r) { return a.causal ? min(max(r + shift, 0), pt.m) : pt.m; };
+  const int seen = row < pt.n ? sees(row) : 0;
+  const int last_row = min(pt.tile * kPromptRows + kPromptRows, pt.n) - 1;
+  const int wave_last = min(pt.tile * kPromptRows + wave * 32 + 31, pt.n - 1);
+  const int wave_first = pt.tile * kPromptRows + wave * 32;
+  const int wave_keys = wave_first < pt.n ? sees(wave_last) : 0;   // keys that any row of the wave sees
+  const int all_keys = wave_first + 31 < pt.n ? sees(wave_first) : 0;   // keys that all its rows see
+  const int steps = (sees(last_row) + kPromptKeys - 1) / kPromptKeys;
+
+  const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.data) + (int64_t)(pt.q0 + row) * a.q.row_stride +
+                       (int64_t)head * a.q.head_stride;
+  u32x4 qf[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int d = 16 * s + 8 * half;
+    qf[s] = row < pt.n && d < D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
+  }
+
+  const uint32_t k_bytes = (uint32_t)(a.k.row_stride * 2), v_bytes = (uint32_t)(a.v.row_stride * 2);
+  const uint64_t k_base = (uint64_t)(uintptr_t)a.k.data + 2 * ((int64_t)pt.k0 * a.k.row_stride + (int64_t)kvh * a.k.head_stride);
+  const uint64_t v_base = (uint64_t)(uintptr_t)a.v.data + 2 * ((int64_t)pt.k0 * a.v.row_stride + (int64_t)kvh * a.v.head_stride);
+  uint32_t k_off[kCopies], v_off[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const uint32_t r = (wave * kCopies + i) * kCopyRows + lane / (kRow / 16), place = lane % (kRow / 16);
+    const uint32_t kc = place ^ k_key<DP>(r), vc = place ^ v_key<DP>(r);
+    k_off[i] = (int)kc * 8 < D ? r * k_bytes + kc * 16 : kOutOfRange;
+    v_off[i] = (int)vc * 8 < D ? r * v_bytes + vc * 16 : kOutOfRange;
+  }
+  const uint32_t lds0 = lds_addr(lds);
+  auto copy_tile = [&](int t) {
+    const uint32_t rows = (uint32_t)min(kPromptKeys, pt.m - t * kPromptKeys);
+    const u32x4 kr = buffer_rsrc(k_base + (uint64_t)t * kPromptKeys * k_bytes, (rows - 1) * k_bytes + D * 2);
+    const u32x4 vr = buffer_rsrc(v_base + (uint64_t)t * kPromptKeys * v_bytes, (rows - 1) * v_bytes + D * 2);
+    const uint32_t dst = lds0 + (t & 1) * 2 * kTile + wave * kCopies * 1024;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) copy16(kr, k_off[i], __builtin_amdgcn_readfirstlane(dst + i * 1024));
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) copy16(vr, v_off[i], __builtin_amdgcn_readfirstlane(dst + kTile + i * 1024));
+  };
+
+  const float c = a.scale * kLog2e;
+  f32x16 o[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
+  float top = -INFINITY, sum = 0.0f;               // running maximum (times c) and this lane's share of the sum
+
+  if (steps > 0) copy_tile(0);
+  for (int t = 0; t < steps; ++t) {
+    wait_copies<0>();
+    lds_barrier();                                 // tile t is there; nobody reads the other buffer any more
+    if (t + 1 < steps) copy_tile(t + 1);
+    if (t * kPromptKeys >= wave_keys) continue;
+    const char* kt = lds + (t & 1) * 2 * kTile;
+    const char* vt = kt + kTile;
+    f32x16 s[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) s[g] = E::mfma32(read_k<DP>(kt, g * 32 + col, 2 * st + half), qf[st], s[g]);
+    // element e of s[g]: key g*32 + 8*(e/4) + 4*half + e%4, query col
+    if ((t + 1) * kPromptKeys > all_keys) {
+      const int left = seen - t * kPromptKeys - 4 * half;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (g * 32 + 8 * (e >> 2) + (e & 3) >= left) s[g][e] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[g][e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32)) * c;
+    const float was = top;
+    top = fmaxf(top, mx);
+    const float base = top == -INFINITY ? 0.0f : top;
+    const float fade = exp2_fast(was - base);
+    sum *= fade;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) o[d] *= fade;
+    u32x4 p[4];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float x = exp2_fast(__builtin_fmaf(s[g][e], c, -base));
+        const float y = exp2_fast(__builtin_fmaf(s[g][e + 1], c, -base));
+        sum += x + y;
+        p[g * 2 + (e >> 3)][(e & 7) >> 1] = E::pack(x, y);     // weights of 16 bits: the matrix core's operand
+      }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+        const uint32_t cl = d * 32 + 16 * ((lane >> 4) & 1);
+        const u32x2 lo = read_v<DP>(vt, ks * 16 + 4 * half, cl, lane & 15);
+        const u32x2 hi = read_v<DP>(vt, ks * 16 + 8 + 4 * half, cl, lane & 15);
+        o[d] = E::mfma32(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[ks], o[d]);
+      }
+  }
+
+  sum += __shfl_xor(sum, 32);
+  const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+  uint16_t* op = reinterpret_cast<uint16_t*>(a.o.data) + (int64_t)(pt.q0 + row) * a.o.row_stride +
+                 (int64_t)head * a.o.head_stride;
+  bool fine = true;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const float x0 = o[d][e] * inv, x1 = o[d][e + 1] * inv, x2 = o[d][e + 2] * inv, x3 = o[d][e + 3] * inv;
+      fine = fine && finite(x0) && finite(x1) && finite(x2) && finite(x3);
+      const int at = d * 32 + 2 * e + 4 * half;
+      if (row < pt.n && at < D) *reinterpret_cast<u32x2*>(op + at) = u32x2{E::pack(x0, x1), E::pack(x2, x3)};
+    }
+  uint64_t again = __ballot(row < pt.n && !fine);
+  again = (again | (again >> 32)) & 0xFFFFFFFFull;
+  while (again) {
+    const int r = wave_first + __ffsll((unsigned long long)again) - 1;
+    again &= again - 1;
+    float o0, o1;
+    plain_row<BF>(reinterpret_cast<const uint16_t*>(a.q.data) + (int64_t)(pt.q0 + r) * a.q.row_stride + (int64_t)head * a.q.head_stride,
+                  D, sees(r), c,
+                  [&](int key, const uint16_t*& k, const uint16_t*& v) {
+                    k = reinterpret_cast<const uint16_t*>((uintptr_t)k_base) + (int64_t)key * a.k.row_stride;
+                    v = reinterpret_cast<const uint16_t*>((uintptr_t)v_base) + (int64_t)key * a.v.row_stride;
+                  },
+                  o0, o1);
+    uint16_t* out = reinterpret_cast<uint16_t*>(a.o.data) + (int64_t)(pt.q0 + r) * a.o.row_stride + (int64_t)head * a.o.head_stride;
+    wait_copies<0>();                              // this wave's store of the same row is complete
+    if (lane < D) out[lane] = E::round(o0);
+    if (lane + 64 < D) out[lane + 64] = E::round(o1);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the newest tokens over a paged cache
+// ---------------------------------------------------------------------------
+// Work. An item is one K/V head and one tile of query rows over the keys of one entry: of a sequence's
+// own part (rows: its tokens x the heads of the K/V head) or of a group's prefix (rows: those of all members).
+// Items are cut into units of 128 keys; the units of all items, in order, are dealt out to the blocks in
+// equal runs, so short and long sequences fill the chip alike and nothing on the host depends on lengths. A
+// run crosses items; each crossing gives one partial result (maximum, sum, weighted values). Its slot is block +
+// item: both only grow along the runs and every crossing raises one of them, so no two share a slot.
+constexpr int kCachedWaves = 4;
+constexpr int kCachedThreads = 64 * kCachedWaves;
+constexpr int kUnit = 128;                 // keys per unit: 32 per wave
+constexpr int kWaveKeys = 32;
+constexpr int kXcds = 8;
+
+struct CachedCall {
+  const uint16_t* pool;
+  int64_t page_elems;                      // elements of a page, all layers
+  int64_t k_off, v_off;                    // of the layer's K and V within a page
+  int32_t kv_heads, dim, page_log, n_pages, max_pages, max_seqs;
+  const int32_t *table, *lens;
+  mtc_heads q, o;
+  const int32_t *seqs, *q_lens, *groups, *prefix_lens;
+  int32_t n_seqs, tokens, heads, n_groups;
+  float c;
+};
+struct Pass {                              // the own parts, or the prefixes
+  float* part;                             // [slot][tile_rows][dim]
+  float* ml;                               // [slot][tile_rows][2]: maximum (times c), sum
+  int32_t tile_rows, blocks, slots;
+};
+
+struct Seq {
+  int row, len, q_len;                     // table row (0 if out of range: it then holds nothing), tokens, queries
+};
+__device__ __forceinline__ Seq cached_seq(const CachedCall& a, int b) {
+  Seq s;
+  s.row = a.seqs ? a.seqs[b] : b;
+  const bool good = (uint32_t)s.row < (uint32_t)a.max_seqs;
+  if (!good) s.row = 0;
+  s.len = good ? min(max(a.lens[s.row], 0), a.max_pages << a.page_log) : 0;
+  s.q_len = a.q_lens ? min(max(a.q_lens[b], 0), a.tokens) : a.tokens;
+  return s;
+}
+__device__ __forceinline__ int row_sees(const Seq& s, int t) {
+  return t < s.q_len ? max(s.len - s.q_len + t + 1, 0) : 0;
+}
+__device__ __forceinline__ int group_start(const CachedCall& a, int g) { return min(max(a.groups[g], 0), a.n_seqs); }
+__device__ __forceinline__ int prefix_tokens(const CachedCall& a, int g) {
+  return min(max(a.prefix_lens[g], 0) >> a.page_log, a.max_pages) << a.page_log;
+}
+// The group g with groups[g] <= b < groups[g + 1], -1: none.
+__device__ __forceinline__ int group_of(const CachedCall& a, int b) {
+  int lo = 0, hi = a.n_groups;
+  if (hi == 0 || group_start(a, 0) > b || group_start(a, hi) <= b) return -1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (group_start(a, mid) <= b) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+struct Entry {
+  int tiles, items, units;                 // row tiles, items (tiles of every K/V head), units of each item
+  int from, to;                            // keys
+  int rows;
+};
+template <bool PREFIX>
+__device__ __forceinline__ Entry cached_entry(const CachedCall& a, int tile_rows, int e) {
+  Entry r;
+  const int per = a.tokens * (a.heads / a.kv_heads);
+  r.from = 0;
+  if constexpr (PREFIX) {
+    r.rows = max(group_start(a, e + 1) - group_start(a, e), 0) * per;
+    r.to = r.rows ? min(prefix_tokens(a, e), cached_seq(a, group_start(a, e)).len) : 0;
+  } else {
+    r.rows = per;
+    const int g = group_of(a, e);
+    if (g >= 0) r.from = prefix_tokens(a, g);
+    r.to = cached_seq(a, e).len;
+  }
+  r.tiles = (r.rows + tile_rows - 1) / tile_rows;
+  r.items = a.kv_heads * r.tiles;
+  r.units = (max(r.to - r.from, 0) + kUnit - 1) / kUnit;
+  return r;
+}
+
+// Running sums over the entries: every thread of the block has the sums before its run of entries [e0, e1).
+struct Scan {
+  int e0, e1, items;
+  int64_t units, own, total;
+};
+template <bool PREFIX>
+__device__ Scan cached_scan(const CachedCall& a, int tile_rows) {
+  __shared__ int64_t wave_u[kCachedWaves];
+  __shared__ int wave_i[kCachedWaves];
+  const int n = PREFIX ? a.n_groups : a.n_seqs, per = (n + kCachedThreads - 1) / kCachedThreads;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Scan r;
+  r.e0 = min((int)threadIdx.x * per, n);
+  r.e1 = min(r.e0 + per, n);
+  int64_t u = 0;
+  int it = 0;
+  for (int e = r.e0; e < r.e1; ++e) {
+    const Entry x = cached_entry<PREFIX>(a, tile_rows, e);
+    u += (int64_t)x.items * x.units;
+    it += x.items;
+  }
+  r.own = u;
+  const int own_items = it;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t xu = __shfl_up(u, d);
+    const int xi = __shfl_up(it, d);
+    if (lane >= d) {
+      u += xu;
+      it += xi;
+    }
+  }
+  __syncthreads();
+  if (lane == 63) {
+    wave_u[wave] = u;
+    wave_i[wave] = it;
+  }
+  __syncthreads();
+  r.units = u - r.own;
+  r.items = it - own_items;
+  r.total = 0;
+#pragma unroll
+  for (int w = 0; w < kCachedWaves; ++w) {
+    if (w < wave) {
+      r.units += wave_u[w];
+      r.items += wave_i[w];
+    }
+    r.total += wave_u[w];
+  }
+  return r;
+}
+
+// One item's keys [from, to) (from a multiple of 16) into a partial result.
+template <bool BF, int DP, int MT, bool PREFIX>
+__device__ void cached_segment(const CachedCall& a, const Pass& ps, char* lds, int e, const Entry& x, int item, int from, int to,
+                               int slot) {
+  using E = Elem<BF>;
+  constexpr int kRow = DP * 2;
+  constexpr int kHalf = 16 * kRow;                       // 16 keys, always of one page
+  constexpr int kHalfCopies = kHalf / 1024, kCopyRows = 1024 / kRow;
+  constexpr int kTileCopies = 2 * kHalfCopies;
+  constexpr int kSteps = DP / 32;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = lane & 15, w = lane >> 4;
+  const int D = a.dim, G = a.heads / a.kv_heads, per = a.tokens * G;
+  const int kvh = item / x.tiles, row0 = (item % x.tiles) * 16 * MT;
+  const int rows = min(x.rows - row0, 16 * MT);
+  const int first = PREFIX ? group_start(a, e) : e;
+  const int trow = __builtin_amdgcn_readfirstlane(cached_seq(a, first).row);
+
+  // this lane's query rows: 16 rt + n
+  u32x4 qf[MT][kSteps];
+  int seen[MT], all = 0x7FFFFFFF;                        // keys that a row sees, that all rows see
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt) {
+    const int rr = row0 + rt * 16 + n;
+    const bool good = rr < x.rows;
+    const int b = good ? first + rr / per : first, t = rr % per / G, h = kvh * G + rr % G;
+    seen[rt] = good ? row_sees(cached_seq(a, b), t) : 0;
+    if (good) all = min(all, seen[rt]);
+    const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.data) + ((int64_t)b * a.tokens + (good ? t : 0)) * a.q.row_stride +
+                         (int64_t)h * a.q.head_stride;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int d = 32 * s + 8 * w;
+      qf[rt][s] = good && d < D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
+    }
+  }
+#pragma unroll
+  for (int d = 8; d; d >>= 1) all = min(all, __shfl_xor(all, d));
+  all = __builtin_amdgcn_readfirstlane(all);
+
+  uint32_t k_lane[kHalfCopies], v_lane[kHalfCopies];     // byte offsets within 16 rows
+#pragma unroll
+  for (int i = 0; i < kHalfCopies; ++i) {
+    const uint32_t r = i * kCopyRows + lane / (kRow / 16), place = lane % (kRow / 16);
+    const uint32_t kc = place ^ k_key<DP>(r), vc = place ^ v_key<DP>(r);
+    k_lane[i] = (int)kc * 8 < D ? r * D * 2 + kc * 16 : kOutOfRange;
+    v_lane[i] = (int)vc * 8 < D ? r * D * 2 + vc * 16 : kOutOfRange;
+  }
+  char* const kt = lds + wave * 4 * kHalf;
+  char* const vt = kt + 2 * kHalf;
+  const uint32_t k_lds = __builtin_amdgcn_readfirstlane(lds_addr(kt)), v_lds = k_lds + 2 * kHalf;
+  const int32_t* table = a.table + (int64_t)trow * a.max_pages;
+  const int64_t head_off = ((int64_t)kvh << a.page_log) * D;
+  int window = 0, ids = -1;                              // page ids of the 64 table entries from `window`, one per lane
+  auto load_window = [&](int pos) {
+    window = pos >> a.page_log;
+    ids = window + lane < a.max_pages ? table[window + lane] : -1;
+  };
+  auto copy_keys = [&](int pos, int64_t off, uint32_t dst, const uint32_t* lanes) {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int p = pos + 16 * hf;
+      const int id = __builtin_amdgcn_readlane(ids, min((p >> a.page_log) - window, 63));
+      const int rows_left = min(to - p, 16);
+      const bool good = rows_left > 0 && (uint32_t)id < (uint32_t)a.n_pages;
+      const int64_t at = (int64_t)(good ? id : 0) * a.page_elems + off + head_off + (int64_t)(p & ((1 << a.page_log) - 1)) * D;
+      const u32x4 r = buffer_rsrc((uint64_t)(uintptr_t)(a.pool + at), good ? (uint32_t)(rows_left * D * 2) : 0u);
+#pragma unroll
+      for (int i = 0; i < kHalfCopies; ++i)
+        copy16(r, lanes[i], __builtin_amdgcn_readfirstlane(dst + hf * kHalf + i * 1024));
+    }
+  };
+
+  f32x4 o[MT][DP / 16];
+  float top[MT], sum[MT];
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt) {
+    top[rt] = -INFINITY;
+    sum[rt] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) o[rt][d] = f32x4{};
+  }
+  int pos = from + kWaveKeys * wave;
+  if (pos < to) {
+    load_window(pos);
+    copy_keys(pos, a.k_off, k_lds, k_lane);
+    copy_keys(pos, a.v_off, v_lds, v_lane);
+  }
+  while (pos < to) {
+    const int next = pos + kUnit;
+    const bool more = next < to;
+    wait_copies<kTileCopies>();                          // K is there
+    f32x4 s[MT][2];
+#pragma unroll
+    for (int rt = 0; rt < MT; ++rt) s[rt][0] = s[rt][1] = f32x4{};
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const u32x4 kf = read_k<DP>(kt, g * 16 + n, 4 * st + w);
+#pragma unroll
+        for (int rt = 0; rt < MT; ++rt) s[rt][g] = E::mfma16(kf, qf[rt][st], s[rt][g]);
+      }
+    wait_lds();
+    if (more) {
+      if (((next + kWaveKeys - 1) >> a.page_log) - window > 63) load_window(next);
+      copy_keys(next, a.k_off, k_lds, k_lane);
+    }
+    // element i of s[rt][g]: key pos + 16 g + 4 w + i, query row 16 rt + n
+    u32x4 p[MT];
+#pragma unroll
+    for (int rt = 0; rt < MT; ++rt) {
+      const int end = min(seen[rt], to);
+      if (pos + kWaveKeys > min(all, to)) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (pos + 16 * g + 4 * w + i >= end) s[rt][g][i] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][g][i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.c;
+      const float was = top[rt];
+      top[rt] = fmaxf(was, mx);
+      const float base = top[rt] == -INFINITY ? 0.0f : top[rt];
+      const float fade = exp2_fast(was - base);
+      sum[rt] *= fade;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) o[rt][d] *= fade;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float y0 = exp2_fast(__builtin_fmaf(s[rt][g][i], a.c, -base));
+          const float y1 = exp2_fast(__builtin_fmaf(s[rt][g][i + 1], a.c, -base));
+          sum[rt] += y0 + y1;
+          p[rt][2 * g + (i >> 1)] = E::pack(y0, y1);     // weights of 16 bits: the matrix core's operand
+        }
+    }
+    if (more) wait_copies<kTileCopies>();                // V is there
+    else wait_copies<0>();
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      const u32x2 lo = read_v<DP>(vt, 4 * w, d * 16, n), hi = read_v<DP>(vt, 16 + 4 * w, d * 16, n);
+#pragma unroll
+      for (int rt = 0; rt < MT; ++rt) o[rt][d] = E::mfma16(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[rt], o[rt][d]);
+    }
+    wait_lds();
+    if (more) copy_keys(next, a.v_off, v_lds, v_lane);
+    pos = next;
+  }
+
+  // join the four waves: element i of o[rt][d] is dim 16 d + 4 w + i of row 16 rt + n
+  constexpr int kPad = DP + 4;
+  float* const buf = reinterpret_cast<float*>(lds);                 // [wave][16][kPad]
+  float* const ml = buf + kCachedWaves * 16 * kPad;                 // [wave][16 MT][2]
+  __syncthreads();                                                  // every wave is done with its tiles
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt) {
+    sum[rt] += __shfl_xor(sum[rt], 16);
+    sum[rt] += __shfl_xor(sum[rt], 32);
+    if (w == 0) {
+      ml[(wave * 16 * MT + rt * 16 + n) * 2] = top[rt];
+      ml[(wave * 16 * MT + rt * 16 + n) * 2 + 1] = sum[rt];
+    }
+  }
+  __syncthreads();
+  const bool store = slot < ps.slots;
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt) {
+    const int r = rt * 16 + n;
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kCachedWaves; ++v) m = fmaxf(m, ml[(v * 16 * MT + r) * 2]);
+    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int v = 0; v < kCachedWaves; ++v) l += ml[(v * 16 * MT + r) * 2 + 1] * exp2_fast(ml[(v * 16 * MT + r) * 2] - base);
+    const float f = exp2_fast(top[rt] - base);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+      *reinterpret_cast<f32x4*>(buf + (wave * 16 + n) * kPad + d * 16 + 4 * w) = o[rt][d] * f;
+    if (store && wave == 0 && w == 0 && r < rows) {
+      float* at = ps.ml + ((int64_t)slot * ps.tile_rows + r) * 2;
+      at[0] = m;
+      at[1] = l;
+    }
+    __syncthreads();
+    for (int i = tid; i < 16 * (DP / 4); i += kCachedThreads) {
+      const int rr = i / (DP / 4), d = i % (DP / 4) * 4;
+      f32x4 y = f32x4{};
+#pragma unroll
+      for (int v = 0; v < kCachedWaves; ++v) y += *reinterpret_cast<const f32x4*>(buf + (v * 16 + rr) * kPad + d);
+      if (store && rt * 16 + rr < rows && d < D)
+        *reinterpret_cast<f32x4*>(ps.part + ((int64_t)slot * ps.tile_rows + rt * 16 + rr) * D + d) = y;
+    }
+    __syncthreads();
+  }
+}
+
+template <bool BF, int DP, int MT, bool PREFIX>
+__global__ __launch_bounds__(kCachedThreads, MT == 4 ? 1 : 2) void k_cached(const CachedCall a, const Pass ps) {
+  constexpr int kStage = kCachedWaves * 2 * kWaveKeys * DP * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[kStage];
+  static_assert(kCachedWaves * (16 * (DP + 4) + 16 * MT * 2) * 4 <= kStage, "the join fits the tiles' space");
+  __shared__ int64_t found[3];
+  const Scan sc = cached_scan<PREFIX>(a, ps.tile_rows);
+  const int blocks = (int)min((int64_t)ps.blocks, sc.total);
+  // consecutive runs on one XCD: row tiles that read the same keys then share its L2
+  const int per_xcd = ps.blocks / kXcds;
+  const int me = (int)(blockIdx.x % kXcds) * per_xcd + blockIdx.x / kXcds;
+  if (me >= blocks) return;
+  int64_t u = me * sc.total / blocks;
+  const int64_t end = (me + 1) * sc.total / blocks;
+  if (u >= sc.units && u < sc.units + sc.own) {          // one thread: its run of entries holds u
+    int64_t before = sc.units;
+    int items = sc.items;
+    for (int e = sc.e0; e < sc.e1; ++e) {
+      const Entry x = cached_entry<PREFIX>(a, ps.tile_rows, e);
+      const int64_t own = (int64_t)x.items * x.units;
+      if (u < before + own) {
+        found[0] = e;
+        found[1] = u - before;
+        found[2] = items;
+        break;
+      }
+      before += own;
+      items += x.items;
+    }
+  }
+  __syncthreads();
+  int e = __builtin_amdgcn_readfirstlane((int)found[0]);
+  int items = __builtin_amdgcn_readfirstlane((int)found[2]);
+  Entry x = cached_entry<PREFIX>(a, ps.tile_rows, e);
+  const int64_t in = found[1];
+  int item = __builtin_amdgcn_readfirstlane((int)(in / x.units)), unit = __builtin_amdgcn_readfirstlane((int)(in % x.units));
+  int left = __builtin_amdgcn_readfirstlane((int)(end - u));
+  while (true) {
+    const int run = min(left, x.units - unit);
+    const int from = x.from + unit * kUnit, to = min(from + run * kUnit, x.to);
+    cached_segment<BF, DP, MT, PREFIX>(a, ps, lds, e, x, item, from, to, me + items + item);
+    left -= run;
+    if (left <= 0) break;
+    unit = 0;
+    if (++item == x.items) {
+      item = 0;
+      do {                                               // left > 0: a further entry has units
+        items += x.items;
+        x = cached_entry<PREFIX>(a, ps.tile_rows, ++e);
+      } while (x.items == 0 || x.units == 0);
+    }
+  }
+}
+
+// One wave per (sequence, token, head): the partial results of its row, from the prefix and the own part.
+template <bool BF>
+__global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, const Pass own, const Pass pre) {
+  __shared__ int64_t at_u[2];
+  __shared__ int at_i[2];
+  const int b = blockIdx.x, lane = threadIdx.x & 63;
+  const int G = a.heads / a.kv_heads, D = a.dim;
+  const int g = group_of(a, b);
+  const Scan sc = cached_scan<false>(a, own.tile_rows);
+  Scan sp;
+  sp.total = 0;
+  if (g >= 0) sp = cached_scan<true>(a, pre.tile_rows);
+  if (b >= sc.e0 && b < sc.e1) {
+    int64_t u = sc.units;
+    int it = sc.items;
+    for (int e = sc.e0; e < b; ++e) {
+      const Entry x = cached_entry<false>(a, own.tile_rows, e);
+      u += (int64_t)x.items * x.units;
+      it += x.items;
+    }
+    at_u[0] = u;
+    at_i[0] = it;
+  }
+  if (g >= 0 && g >= sp.e0 && g < sp.e1) {
+    int64_t u = sp.units;
+    int it = sp.items;
+    for (int e = sp.e0; e < g; ++e) {
+      const Entry x = cached_entry<true>(a, pre.tile_rows, e);
+      u += (int64_t)x.items * x.units;
+      it += x.items;
+    }
+    at_u[1] = u;
+    at_i[1] = it;
+  }
+  __syncthreads();
+  const int row = blockIdx.y * kCachedWaves + (threadIdx.x >> 6);   // t * heads + h
+  if (row >= a.tokens * a.heads) return;
+  const int t = row / a.heads, h = row % a.heads, kvh = h / G;
+  const Seq s = cached_seq(a, b);
+  const int seen = row_sees(s, t);
+  float m = -INFINITY, l = 0.0f, y0 = 0.0f, y1 = 0.0f;
+  auto add = [&](const Pass& ps, const Entry& x, int rr, int64_t units, int items, int64_t total) {
+    if (x.units == 0) return;
+    const int64_t blocks = min((int64_t)ps.blocks, total);
+    const int item = kvh * x.tiles + rr / ps.tile_rows, r = rr % ps.tile_rows;
+    const int64_t u0 = units + (int64_t)item * x.units;
+    const int i0 = (int)(((u0 + 1) * blocks - 1) / total), i1 = (int)(((u0 + x.units) * blocks - 1) / total);
+    for (int i = i0; i <= i1; ++i) {
+      const int64_t slot = (int64_t)i + items + item;
+      if (slot >= ps.slots) return;
+      const float* p = ps.ml + (slot * ps.tile_rows + r) * 2;
+      const float pm = p[0], pl = p[1];
+      const float* po = ps.part + (slot * ps.tile_rows + r) * D;
+      const float z0 = lane < D ? po[lane] : 0.0f, z1 = lane + 64 < D ? po[lane + 64] : 0.0f;
+      const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.0f : top;
+      const float f = exp2_fast(m - base), pf = exp2_fast(pm - base);
+      l = l * f + pl * pf;
+      y0 = y0 * f + z0 * pf;
+      y1 = y1 * f + z1 * pf;
+      m = top;
+    }
+  };
+  if (g >= 0) {
+    const int rr = ((b - group_start(a, g)) * a.tokens + t) * G + h % G;
+    add(pre, cached_entry<true>(a, pre.tile_rows, g), rr, at_u[1], at_i[1], sp.total);
+  }
+  add(own, cached_entry<false>(a, own.tile_rows, b), t * G + h % G, at_u[0], at_i[0], sc.total);
+  const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+  y0 *= inv;
+  y1 *= inv;
+  if (__ballot(!finite(y0) || !finite(y1))) {
+    const int32_t* table = a.table + (int64_t)s.row * a.max_pages;
+    plain_row<BF>(reinterpret_cast<const uint16_t*>(a.q.data) + ((int64_t)b * a.tokens + t) * a.q.row_stride + (int64_t)h * a.q.head_stride,
+                  D, seen, a.c,
+                  [&](int key, const uint16_t*& k, const uint16_t*& v) {
+                    const int id = min(max(table[key >> a.page_log], 0), a.n_pages - 1);
+                    const uint16_t* p = a.pool + (int64_t)id * a.page_elems +
+                                        (((int64_t)kvh << a.page_log) + (key & ((1 << a.page_log) - 1))) * D;
+                    k = p + a.k_off;
+                    v = p + a.v_off;
+                  },
+                  y0, y1);
+  }
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.o.data) + ((int64_t)b * a.tokens + t) * a.o.row_stride + (int64_t)h * a.o.head_stride;
+  if (lane < D) out[lane] = Elem<BF>::round(y0);
+  if (lane + 64 < D) out[lane + 64] = Elem<BF>::round(y1);
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+int check_heads(const char* what, const mtc_heads& x, bool empty) {
+  if (!x.data && !empty) return fail(MTC_E_NULL, "%s is NULL", what);
+  if ((uintptr_t)x.data % 16) return fail(MTC_E_SHAPE, "%s must be 16-byte aligned", what);
+  if (x.row_stride < 0 || x.head_stride < 0 || x.row_stride % 8 || x.head_stride % 8)
+    return fail(MTC_E_SHAPE, "%s: strides %lld, %lld must be non-negative multiples of 8 elements", what,
+                (long long)x.row_stride, (long long)x.head_stride);
+  // offsets within a tile of 64 rows stay below 2^31 bytes
+  if (x.row_stride >= (1ll << 24)) return fail(MTC_E_SHAPE, "%s: row stride %lld is too large", what, (long long)x.row_stride);
+  return MTC_OK;
+}
+
+int check_attention(int dtype, int heads, int kv_heads, int dim, float scale) {
+  if (dtype != MTC_DTYPE_BF16 && dtype != MTC_DTYPE_F16) return fail(MTC_E_DTYPE, "attention takes bf16 or f16, got dtype %d", dtype);
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads)
+    return fail(MTC_E_SHAPE, "%d query heads over %d K/V heads", heads, kv_heads);
+  if (dim < 8 || dim > MTC_ATTN_MAX_DIM || dim % 8)
+    return fail(MTC_E_SHAPE, "head size %d: a multiple of 8 from 8 to %d", dim, MTC_ATTN_MAX_DIM);
+  if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(MTC_E_SHAPE, "scale must be positive and finite");
+  return MTC_OK;
+}
+
+template <bool BF>
+void launch_prompt(const mtc_prompt_args& a, unsigned grid, hipStream_t st) {
+  if (a.dim <= 64) k_prompt<BF, 64><<<grid, 64 * kPromptWaves, 0, st>>>(a);
+  else k_prompt<BF, 128><<<grid, 64 * kPromptWaves, 0, st>>>(a);
+}
+
+// Row tiles of a pass: 16, 32 or 64 rows per item, the least that hold the rows.
+int tile_rows_for(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+struct CachedPlan {
+  int own_rows, pre_rows;            // per item
+  int64_t own_slots, pre_slots;
+  size_t own_bytes, pre_bytes;       // part + ml of each pass
+  int blocks;
+};
+
+size_t round_up(size_t x, size_t to) { return (x + to - 1) / to * to; }
+
+int plan_cached(const mtc_cache_desc* c, const mtc_cached_args* a, CachedPlan* p) {
+  if (!a) return fail(MTC_E_NULL, "args is NULL");
+  if (int rc = mtc_check_cache_desc(c)) return rc;
+  if (a->abi_version != MTC_ABI_VERSION) return fail(MTC_E_VERSION, "args of ABI %u, library %d", a->abi_version, MTC_ABI_VERSION);
+  if (int rc = check_attention(c->dtype, a->heads, c->kv_heads, c->dim, a->scale)) return rc;
+  if (a->reserved != 0) return fail(MTC_E_SHAPE, "reserved must be 0");
+  if (a->layer < 0 || a->layer >= c->n_layers) return fail(MTC_E_SHAPE, "layer %d of %d", a->layer, c->n_layers);
+  if (a->n_seqs < 0 || a->n_seqs > MTC_CACHED_MAX_SEQS) return fail(MTC_E_SHAPE, "%d sequences, at most %d", a->n_seqs, MTC_CACHED_MAX_SEQS);
+  if (!a->seqs && a->n_seqs > c->max_seqs) return fail(MTC_E_SHAPE, "%d sequences, the cache holds %d", a->n_seqs, c->max_seqs);
+  if (a->tokens < 1 || a->tokens > MTC_CACHED_MAX_TOKENS)
+    return fail(MTC_E_SHAPE, "%d tokens per sequence: 1 to %d", a->tokens, MTC_CACHED_MAX_TOKENS);
+  if (a->n_groups < 0 || a->n_groups > a->n_seqs) return fail(MTC_E_SHAPE, "%d groups of %d sequences", a->n_groups, a->n_seqs);
+  const int64_t per = (int64_t)a->tokens * (a->heads / c->kv_heads);
+  if ((int64_t)a->tokens * a->heads > 0xFFFF || (int64_t)a->tokens * a->heads * a->n_seqs > 0x3FFFFFF)   // 2^32 threads a launch
+    return fail(MTC_E_SHAPE, "%d sequences of %d tokens of %d heads: too many query rows", a->n_seqs, a->tokens, a->heads);
+  p->blocks = 512;                   // two per CU
+  p->own_rows = tile_rows_for(per);
+  p->pre_rows = tile_rows_for(per * a->n_seqs);
+  p->own_slots = p->blocks + (int64_t)a->n_seqs * c->kv_heads * ((per + p->own_rows - 1) / p->own_rows);
+  p->pre_slots = a->n_groups ? p->blocks + (int64_t)c->kv_heads * ((per * a->n_seqs + p->pre_rows - 1) / p->pre_rows + a->n_groups) : 0;
+  p->own_bytes = round_up((size_t)p->own_slots * p->own_rows * (c->dim + 2) * 4, 256);
+  p->pre_bytes = round_up((size_t)p->pre_slots * p->pre_rows * (c->dim + 2) * 4, 256);
+  return MTC_OK;
+}
+
+template <bool BF, int DP, bool PREFIX>
+void launch_cached(const CachedCall& a, const Pass& ps, hipStream_t st) {
+  if (ps.tile_rows == 16) k_cached<BF, DP, 1, PREFIX><<<ps.blocks, kCachedThreads, 0, st>>>(a, ps);
+  else if (ps.tile_rows == 32) k_cached<BF, DP, 2, PREFIX><<<ps.blocks, kCachedThreads, 0, st>>>(a, ps);
+  else k_cached<BF, DP, 4, PREFIX><<<ps.blocks, kCachedThreads, 0, st>>>(a, ps);
+}
+
+template <bool BF>
+int run_cached(const CachedCall& a, const Pass& own, const Pass& pre, hipStream_t st) {
+  if (a.n_groups) {
+    if (a.dim <= 64) launch_cached<BF, 64, true>(a, pre, st);
+    else launch_cached<BF, 128, true>(a, pre, st);
+    if (int rc = check_launch("k_cached (prefixes)")) return rc;
+  }
+  if (a.dim <= 64) launch_cached<BF, 64, false>(a, own, st);
+  else launch_cached<BF, 128, false>(a, own, st);
+  if (int rc = check_launch("k_cached")) return rc;
+  const dim3 grid(a.n_seqs, (a.tokens * a.heads + kCachedWaves - 1) / kCachedWaves);
+  k_join<BF><<<grid, kCachedThreads, 0, st>>>(a, own, pre);
+  return check_launch("k_join");
+}
+
+}  // namespace
+
+MTC_API int mtc_prompt_attention(const mtc_prompt_args* a, void* hip_stream) {
+  if (!a) return fail(MTC_E_NULL, "args is NULL");
+  if (a->abi_version != MTC_ABI_VERSION) return fail(MTC_E_VERSION, "args of ABI %u, library %d", a->abi_version, MTC_ABI_VERSION);
+  if (int rc = check_attention(a->dtype, a->heads, a->kv_heads, a->dim, a->scale)) return rc;
+  if (a->n_seqs < 0 || a->q_rows < 0 || a->k_rows < 0) return fail(MTC_E_SHAPE, "negative sizes");
+  if (a->n_seqs == 0 || a->q_rows == 0) return ok();
+  if (!a->cu_q || !a->cu_k) return fail(MTC_E_NULL, "cu_q or cu_k is NULL");
+  if (int rc = check_heads("q", a->q, false)) return rc;
+  if (int rc = check_heads("k", a->k, a->k_rows == 0)) return rc;
+  if (int rc = check_heads("v", a->v, a->k_rows == 0)) return rc;
+  if (int rc = check_heads("o", a->o, false)) return rc;
+  // a tile's rows past the sequence's end must lie past its buffer's end: rows may not overlap
+  if ((a->k.row_stride < a->dim || a->v.row_stride < a->dim) && a->k_rows > 1)
+    return fail(MTC_E_SHAPE, "rows of k and v overlap: strides %lld, %lld", (long long)a->k.row_stride, (long long)a->v.row_stride);
+  const int64_t tiles = (int64_t)a->q_rows / kPromptRows + std::min(a->n_seqs, a->q_rows);    // at most
+  if (tiles * a->heads > 0xFFFFFF) return fail(MTC_E_SHAPE, "too many query tiles");     // 2^32 threads a launch
+  if (a->dtype == MTC_DTYPE_BF16) launch_prompt<true>(*a, (unsigned)(tiles * a->heads), (hipStream_t)hip_stream);
+  else launch_prompt<false>(*a, (unsigned)(tiles * a->heads), (hipStream_t)hip_stream);
+  return check_launch("k_prompt");
+}
+
+MTC_API size_t mtc_cached_attention_workspace_bytes(const mtc_cache_desc* c, const mtc_cached_args* a) {
+  CachedPlan p;
+  if (plan_cached(c, a, &p) != MTC_OK) return 0;
+  return p.own_bytes + p.pre_bytes;
+}
+
+MTC_API int mtc_cached_attention(const mtc_cache_desc* c, const mtc_cached_args* a, void* workspace, size_t workspace_bytes,
+                                 void* hip_stream) {
+  CachedPlan p;
+  if (int rc = plan_cached(c, a, &p)) return rc;
+  if (a->n_seqs == 0) return ok();
+  if (int rc = check_heads("q", a->q, false)) return rc;
+  if (int rc = check_heads("o", a->o, false)) return rc;
+  if (a->n_groups && (!a->groups || !a->prefix_lens)) return fail(MTC_E_NULL, "groups or prefix_lens is NULL");
+  if (!workspace || workspace_bytes < p.own_bytes + p.pre_bytes)
+    return fail(MTC_E_WORKSPACE, "workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : (size_t)0, p.own_bytes + p.pre_bytes);
+  if ((uintptr_t)workspace % 256) return fail(MTC_E_WORKSPACE, "workspace must be 256-byte aligned");
+  CachedCall k;
+  const int64_t head = (int64_t)c->page_size * c->dim;
+  k.pool = (const uint16_t*)c->pool;
+  k.page_elems = 2 * head * c->kv_heads * c->n_layers;
+  k.k_off = 2 * head * c->kv_heads * a->layer;
+  k.v_off = k.k_off + head * c->kv_heads;
+  k.kv_heads = c->kv_heads;
+  k.dim = c->dim;
+  k.page_log = __builtin_ctz((unsigned)c->page_size);
+  k.n_pages = c->n_pages;
+  k.max_pages = c->max_pages;
+  k.max_seqs = c->max_seqs;
+  k.table = c->table;
+  k.lens = c->lens;
+  k.q = a->q;
+  k.o = a->o;
+  k.seqs = a->seqs;
+  k.q_lens = a->q_lens;
+  k.groups = a->groups;
+  k.prefix_lens = a->prefix_lens;
+  k.n_seqs = a->n_seqs;
+  k.tokens = a->tokens;
+  k.heads = a->heads;
+  k.n_groups = a->n_groups;
+  k.c = a->scale * kLog2e;
+  auto pass = [&](char* at, int64_t slots, int rows) {
+    Pass x;
+    x.part = (float*)at;
+    x.ml = x.part + slots * rows * c->dim;
+    x.tile_rows = rows;
+    x.blocks = p.blocks;
+    x.slots = (int)slots;
+    return x;
+  };
+  const Pass own = pass((char*)workspace, p.own_slots, p.own_rows);
+  const Pass pre = pass((char*)workspace + p.own_bytes, p.pre_slots, p.pre_rows);
+  return c->dtype == MTC_DTYPE_BF16 ? run_cached<true>(k, own, pre, (hipStream_t)hip_stream)
+                                    : run_cached<false>(k, own, pre, (hipStream_t)hip_stream);
+}
