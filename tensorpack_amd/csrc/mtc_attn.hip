@@ -100,96 +100,42 @@ __device__ PromptTile prompt_tile(const mtc_prompt_args& a, int rank) {
   return r;
 }
 
+// 32 query rows of one wave (one per lane of either half) through tiles of 64 keys: S^T in two 32 x 32 blocks, O^T in
+// DP / 32. Element e of a block lies at row 8*(e/4) + 4*half + e%4 (key or dim), column `col` (query).
 template <bool BF, int DP>
-__global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_prompt_args a) {
+struct RowTile {
   using E = Elem<BF>;
-  constexpr int kRow = DP * 2;                             // bytes of an LDS row
-  constexpr int kTile = kPromptKeys * kRow;
-  constexpr int kCopies = kTile / 1024 / kPromptWaves;     // 1 KiB copies per wave and tile
-  constexpr int kCopyRows = 1024 / kRow;
-  constexpr int kSteps = DP / 16;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * kTile];   // K, V; two buffers each
-
-  const int H = a.heads, KV = a.kv_heads, D = a.dim;
-  // heads of one K/V head apart by KV places: blocks that share keys share an XCD (and its L2) when the
-  // count of K/V heads is a multiple or a divisor of 8
-  const int j = blockIdx.x % H;
-  const int kvh = j % KV, head = kvh * (H / KV) + j / KV;
-  const PromptTile pt = prompt_tile(a, blockIdx.x / H);
-  if (pt.tile < 0) return;
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int half = lane >> 5, col = lane & 31;
-  const int row = pt.tile * kPromptRows + wave * 32 + col;         // this lane's query
-  const int shift = pt.m - pt.n + 1;
-  auto sees = [&](int r) { return a.causal ? min(max(r + shift, 0), pt.m) : pt.m; };
-  const int seen = row < pt.n ? sees(row) : 0;
-  const int last_row = min(pt.tile * kPromptRows + kPromptRows, pt.n) - 1;
-  const int wave_last = min(pt.tile * kPromptRows + wave * 32 + 31, pt.n - 1);
-  const int wave_first = pt.tile * kPromptRows + wave * 32;
-  const int wave_keys = wave_first < pt.n ? sees(wave_last) : 0;   // keys that any row of the wave sees
-  const int all_keys = wave_first + 31 < pt.n ? sees(wave_first) : 0;   // keys that all its rows see
-  const int steps = (sees(last_row) + kPromptKeys - 1) / kPromptKeys;
-
-  const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.data) + (int64_t)(pt.q0 + row) * a.q.row_stride +
-                       (int64_t)head * a.q.head_stride;
+  static constexpr int kSteps = DP / 16;
   u32x4 qf[kSteps];
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int d = 16 * s + 8 * half;
-    qf[s] = row < pt.n && d < D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
-  }
-
-  const uint32_t k_bytes = (uint32_t)(a.k.row_stride * 2), v_bytes = (uint32_t)(a.v.row_stride * 2);
-  const uint64_t k_base = (uint64_t)(uintptr_t)a.k.data + 2 * ((int64_t)pt.k0 * a.k.row_stride + (int64_t)kvh * a.k.head_stride);
-  const uint64_t v_base = (uint64_t)(uintptr_t)a.v.data + 2 * ((int64_t)pt.k0 * a.v.row_stride + (int64_t)kvh * a.v.head_stride);
-  uint32_t k_off[kCopies], v_off[kCopies];
-#pragma unroll
-  for (int i = 0; i < kCopies; ++i) {
-    const uint32_t r = (wave * kCopies + i) * kCopyRows + lane / (kRow / 16), place = lane % (kRow / 16);
-    const uint32_t kc = place ^ k_key<DP>(r), vc = place ^ v_key<DP>(r);
-    k_off[i] = (int)kc * 8 < D ? r * k_bytes + kc * 16 : kOutOfRange;
-    v_off[i] = (int)vc * 8 < D ? r * v_bytes + vc * 16 : kOutOfRange;
-  }
-  const uint32_t lds0 = lds_addr(lds);
-  auto copy_tile = [&](int t) {
-    const uint32_t rows = (uint32_t)min(kPromptKeys, pt.m - t * kPromptKeys);
-    const u32x4 kr = buffer_rsrc(k_base + (uint64_t)t * kPromptKeys * k_bytes, (rows - 1) * k_bytes + D * 2);
-    const u32x4 vr = buffer_rsrc(v_base + (uint64_t)t * kPromptKeys * v_bytes, (rows - 1) * v_bytes + D * 2);
-    const uint32_t dst = lds0 + (t & 1) * 2 * kTile + wave * kCopies * 1024;
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) copy16(kr, k_off[i], __builtin_amdgcn_readfirstlane(dst + i * 1024));
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) copy16(vr, v_off[i], __builtin_amdgcn_readfirstlane(dst + kTile + i * 1024));
-  };
-
-  const float c = a.scale * kLog2e;
   f32x16 o[DP / 32];
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
-  float top = -INFINITY, sum = 0.0f;               // running maximum (times c) and this lane's share of the sum
+  float top, sum;                    // running maximum (times c), this lane's share of the sum
 
-  if (steps > 0) copy_tile(0);
-  for (int t = 0; t < steps; ++t) {
-    wait_copies<0>();
-    lds_barrier();                                 // tile t is there; nobody reads the other buffer any more
-    if (t + 1 < steps) copy_tile(t + 1);
-    if (t * kPromptKeys >= wave_keys) continue;
-    const char* kt = lds + (t & 1) * 2 * kTile;
-    const char* vt = kt + kTile;
+  __device__ __forceinline__ void start(const uint16_t* qp, bool good, int D, int half) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int d = 16 * s + 8 * half;
+      qf[s] = good && d < D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
+    top = -INFINITY;
+    sum = 0.0f;
+  }
+
+  // left: keys of the tile that this lane's row sees, used if `masked`
+  __device__ __forceinline__ void step(const char* kt, const char* vt, float c, bool masked, int left) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
     for (int st = 0; st < kSteps; ++st)
 #pragma unroll
       for (int g = 0; g < 2; ++g) s[g] = E::mfma32(read_k<DP>(kt, g * 32 + col, 2 * st + half), qf[st], s[g]);
-    // element e of s[g]: key g*32 + 8*(e/4) + 4*half + e%4, query col
-    if ((t + 1) * kPromptKeys > all_keys) {
-      const int left = seen - t * kPromptKeys - 4 * half;
+    if (masked) {
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (g * 32 + 8 * (e >> 2) + (e & 3) >= left) s[g][e] = -INFINITY;
+          if (g * 32 + 8 * (e >> 2) + (e & 3) >= left - 4 * half) s[g][e] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -224,8 +170,78 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
         o[d] = E::mfma32(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[ks], o[d]);
       }
   }
+};
 
-  sum += __shfl_xor(sum, 32);
+template <bool BF, int DP>
+__global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_prompt_args a) {
+  using E = Elem<BF>;
+  constexpr int kRow = DP * 2;                             // bytes of an LDS row
+  constexpr int kTile = kPromptKeys * kRow;
+  constexpr int kCopies = kTile / 1024 / kPromptWaves;     // 1 KiB copies per wave and tile
+  constexpr int kCopyRows = 1024 / kRow;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kTile];   // K, V; two buffers each
+
+  const int H = a.heads, KV = a.kv_heads, D = a.dim;
+  // heads of one K/V head apart by KV places: blocks that share keys share an XCD (and its L2) when the
+  // count of K/V heads is a multiple or a divisor of 8
+  const int j = blockIdx.x % H;
+  const int kvh = j % KV, head = kvh * (H / KV) + j / KV;
+  const PromptTile pt = prompt_tile(a, blockIdx.x / H);
+  if (pt.tile < 0) return;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int half = lane >> 5, col = lane & 31;
+  const int row = pt.tile * kPromptRows + wave * 32 + col;         // this lane's query
+  const int shift = pt.m - pt.n + 1;
+  auto sees = [&](int r) { return a.causal ? min(max(r + shift, 0), pt.m) : pt.m; };
+  const int seen = row < pt.n ? sees(row) : 0;
+  const int last_row = min(pt.tile * kPromptRows + kPromptRows, pt.n) - 1;
+  const int wave_last = min(pt.tile * kPromptRows + wave * 32 + 31, pt.n - 1);
+  const int wave_first = pt.tile * kPromptRows + wave * 32;
+  const int wave_keys = wave_first < pt.n ? sees(wave_last) : 0;   // keys that any row of the wave sees
+  const int all_keys = wave_first + 31 < pt.n ? sees(wave_first) : 0;   // keys that all its rows see
+  const int steps = (sees(last_row) + kPromptKeys - 1) / kPromptKeys;
+
+  const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.data) + (int64_t)(pt.q0 + row) * a.q.row_stride +
+                       (int64_t)head * a.q.head_stride;
+  RowTile<BF, DP> rt;
+  rt.start(qp, row < pt.n, D, half);
+
+  const uint32_t k_bytes = (uint32_t)(a.k.row_stride * 2), v_bytes = (uint32_t)(a.v.row_stride * 2);
+  const uint64_t k_base = (uint64_t)(uintptr_t)a.k.data + 2 * ((int64_t)pt.k0 * a.k.row_stride + (int64_t)kvh * a.k.head_stride);
+  const uint64_t v_base = (uint64_t)(uintptr_t)a.v.data + 2 * ((int64_t)pt.k0 * a.v.row_stride + (int64_t)kvh * a.v.head_stride);
+  uint32_t k_off[kCopies], v_off[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const uint32_t r = (wave * kCopies + i) * kCopyRows + lane / (kRow / 16), place = lane % (kRow / 16);
+    const uint32_t kc = place ^ k_key<DP>(r), vc = place ^ v_key<DP>(r);
+    k_off[i] = (int)kc * 8 < D ? r * k_bytes + kc * 16 : kOutOfRange;
+    v_off[i] = (int)vc * 8 < D ? r * v_bytes + vc * 16 : kOutOfRange;
+  }
+  const uint32_t lds0 = lds_addr(lds);
+  auto copy_tile = [&](int t) {
+    const uint32_t rows = (uint32_t)min(kPromptKeys, pt.m - t * kPromptKeys);
+    const u32x4 kr = buffer_rsrc(k_base + (uint64_t)t * kPromptKeys * k_bytes, (rows - 1) * k_bytes + D * 2);
+    const u32x4 vr = buffer_rsrc(v_base + (uint64_t)t * kPromptKeys * v_bytes, (rows - 1) * v_bytes + D * 2);
+    const uint32_t dst = lds0 + (t & 1) * 2 * kTile + wave * kCopies * 1024;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) copy16(kr, k_off[i], __builtin_amdgcn_readfirstlane(dst + i * 1024));
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) copy16(vr, v_off[i], __builtin_amdgcn_readfirstlane(dst + kTile + i * 1024));
+  };
+
+  const float c = a.scale * kLog2e;
+  if (steps > 0) copy_tile(0);
+  for (int t = 0; t < steps; ++t) {
+    wait_copies<0>();
+    lds_barrier();                                 // tile t is there; nobody reads the other buffer any more
+    if (t + 1 < steps) copy_tile(t + 1);
+    if (t * kPromptKeys >= wave_keys) continue;
+    const char* kt = lds + (t & 1) * 2 * kTile;
+    rt.step(kt, kt + kTile, c, (t + 1) * kPromptKeys > all_keys, seen - t * kPromptKeys);
+  }
+
+  const float sum = rt.sum + __shfl_xor(rt.sum, 32);
   const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
   uint16_t* op = reinterpret_cast<uint16_t*>(a.o.data) + (int64_t)(pt.q0 + row) * a.o.row_stride +
                  (int64_t)head * a.o.head_stride;
@@ -234,7 +250,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
-      const float x0 = o[d][e] * inv, x1 = o[d][e + 1] * inv, x2 = o[d][e + 2] * inv, x3 = o[d][e + 3] * inv;
+      const float x0 = rt.o[d][e] * inv, x1 = rt.o[d][e + 1] * inv, x2 = rt.o[d][e + 2] * inv, x3 = rt.o[d][e + 3] * inv;
       fine = fine && finite(x0) && finite(x1) && finite(x2) && finite(x3);
       const int at = d * 32 + 2 * e + 4 * half;
       if (row < pt.n && at < D) *reinterpret_cast<u32x2*>(op + at) = u32x2{E::pack(x0, x1), E::pack(x2, x3)};
@@ -264,16 +280,33 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
 // ---------------------------------------------------------------------------
 // Work. An item is one K/V head and one tile of query rows over the keys of one entry: of a sequence's
 // own part (rows: its tokens x the heads of the K/V head) or of a group's prefix (rows: those of all members).
-// Items are cut into units of 128 keys; the units of all items, in order, are dealt out to the blocks in
+// Items are cut into units of keys; the units of all items, in order, are dealt out to the blocks in
 // equal runs, so short and long sequences fill the chip alike and nothing on the host depends on lengths. A
 // run crosses items; each crossing gives one partial result (maximum, sum, weighted values). Its slot is block +
 // item: both only grow along the runs and every crossing raises one of them, so no two share a slot.
+//
+// Two ways through an item's keys:
+//   split keys   16 or 32 rows; each wave takes 32 keys of its own, the four waves are joined at the end. For few rows
+//                the keys' bytes are all that counts, and every wave keeps its own loads in flight.
+//   split rows   up to 128 rows, 32 per wave, as in k_prompt: the waves share each tile of 64 keys in LDS
 constexpr int kCachedWaves = 4;
 constexpr int kCachedThreads = 64 * kCachedWaves;
-constexpr int kUnit = 128;                 // keys per unit: 32 per wave
-constexpr int kWaveKeys = 32;
+constexpr int kCachedBlocks = 512;         // two per CU
 constexpr int kXcds = 8;
+constexpr int kWaveKeys = 32;              // split keys: per wave and step
+constexpr int kManyRows = 128;             // split rows: rows of a tile
+enum { kNone = 0, kOneTile = 1, kTwoTiles = 2, kRows = 3 };      // 16 rows, 32 rows, split rows
+__host__ __device__ constexpr int mode_rows(int mode) { return mode == kRows ? kManyRows : 16 * mode; }
+__host__ __device__ constexpr int mode_unit(int mode) { return mode == kRows ? kPromptKeys : kCachedWaves * kWaveKeys; }
 
+struct Pass {                              // the own parts, or the prefixes
+  float* part;                             // [slot][stride][dim]
+  float* ml;                               // [slot][stride][2]: maximum (times c), sum
+  int32_t stride, slots;
+};
+struct JoinEntry {                         // what k_join needs of a sequence, or of a group
+  int32_t units_before, items_before, units, tiles, group, first;
+};
 struct CachedCall {
   const uint16_t* pool;
   int64_t page_elems;                      // elements of a page, all layers
@@ -284,11 +317,8 @@ struct CachedCall {
   const int32_t *seqs, *q_lens, *groups, *prefix_lens;
   int32_t n_seqs, tokens, heads, n_groups;
   float c;
-};
-struct Pass {                              // the own parts, or the prefixes
-  float* part;                             // [slot][tile_rows][dim]
-  float* ml;                               // [slot][tile_rows][2]: maximum (times c), sum
-  int32_t tile_rows, blocks, slots;
+  Pass own, pre;
+  int32_t* join;                           // own units, own blocks, prefix units, prefix blocks; then the entries
 };
 
 struct Seq {
@@ -297,124 +327,164 @@ struct Seq {
 __device__ __forceinline__ Seq cached_seq(const CachedCall& a, int b) {
   Seq s;
   s.row = a.seqs ? a.seqs[b] : b;
+  s.q_len = a.q_lens ? min(max(a.q_lens[b], 0), a.tokens) : a.tokens;
   const bool good = (uint32_t)s.row < (uint32_t)a.max_seqs;
   if (!good) s.row = 0;
   s.len = good ? min(max(a.lens[s.row], 0), a.max_pages << a.page_log) : 0;
-  s.q_len = a.q_lens ? min(max(a.q_lens[b], 0), a.tokens) : a.tokens;
   return s;
 }
-__device__ __forceinline__ int row_sees(const Seq& s, int t) {
-  return t < s.q_len ? max(s.len - s.q_len + t + 1, 0) : 0;
-}
+__device__ __forceinline__ int row_sees(int len, int q_len, int t) { return t < q_len ? max(len - q_len + t + 1, 0) : 0; }
 __device__ __forceinline__ int group_start(const CachedCall& a, int g) { return min(max(a.groups[g], 0), a.n_seqs); }
 __device__ __forceinline__ int prefix_tokens(const CachedCall& a, int g) {
   return min(max(a.prefix_lens[g], 0) >> a.page_log, a.max_pages) << a.page_log;
 }
-// The group g with groups[g] <= b < groups[g + 1], -1: none.
-__device__ __forceinline__ int group_of(const CachedCall& a, int b) {
-  int lo = 0, hi = a.n_groups;
-  if (hi == 0 || group_start(a, 0) > b || group_start(a, hi) <= b) return -1;
+// The group g with start(g) <= b < start(g + 1), -1: none.
+template <class Start>
+__device__ __forceinline__ int group_of(int n_groups, int b, Start start) {
+  int lo = 0, hi = n_groups;
+  if (hi == 0 || start(0) > b || start(hi) <= b) return -1;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (group_start(a, mid) <= b) lo = mid; else hi = mid;
+    if (start(mid) <= b) lo = mid; else hi = mid;
   }
   return lo;
 }
 
 struct Entry {
-  int tiles, items, units;                 // row tiles, items (tiles of every K/V head), units of each item
+  int rows, tiles, items, units;           // query rows, row tiles, items (tiles of every K/V head), units of each
   int from, to;                            // keys
-  int rows;
+  int first, group;                        // batch entry that the keys belong to; own part: its group
+  Seq seq;                                 // of `first`
 };
-template <bool PREFIX>
-__device__ __forceinline__ Entry cached_entry(const CachedCall& a, int tile_rows, int e) {
+template <bool PREFIX, int MODE, class Start>
+__device__ __forceinline__ Entry cached_entry(const CachedCall& a, int e, Start start) {
   Entry r;
   const int per = a.tokens * (a.heads / a.kv_heads);
   r.from = 0;
   if constexpr (PREFIX) {
-    r.rows = max(group_start(a, e + 1) - group_start(a, e), 0) * per;
-    r.to = r.rows ? min(prefix_tokens(a, e), cached_seq(a, group_start(a, e)).len) : 0;
+    r.first = start(e);
+    r.rows = max(start(e + 1) - r.first, 0) * per;
+    r.group = e;
+    r.seq = cached_seq(a, min(r.first, a.n_seqs - 1));
+    r.to = r.rows ? min(prefix_tokens(a, e), r.seq.len) : 0;
   } else {
+    r.first = e;
     r.rows = per;
-    const int g = group_of(a, e);
-    if (g >= 0) r.from = prefix_tokens(a, g);
-    r.to = cached_seq(a, e).len;
+    r.seq = cached_seq(a, e);
+    r.group = group_of(a.n_groups, e, start);
+    if (r.group >= 0) r.from = prefix_tokens(a, r.group);
+    r.to = r.seq.len;
   }
-  r.tiles = (r.rows + tile_rows - 1) / tile_rows;
+  r.tiles = (r.rows + mode_rows(MODE) - 1) / mode_rows(MODE);
   r.items = a.kv_heads * r.tiles;
-  r.units = (max(r.to - r.from, 0) + kUnit - 1) / kUnit;
+  r.units = (max(r.to - r.from, 0) + mode_unit(MODE) - 1) / mode_unit(MODE);
   return r;
+}
+
+// Inclusive sum over the wave's lanes (row shifts, then the rows' totals).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);      // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);     // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);     // row_bcast:31 into rows 2 and 3
+  return x;
 }
 
 // Running sums over the entries: every thread of the block has the sums before its run of entries [e0, e1).
 struct Scan {
-  int e0, e1, items;
-  int64_t units, own, total;
+  int e0, e1, units, own, items, total;
 };
-template <bool PREFIX>
-__device__ Scan cached_scan(const CachedCall& a, int tile_rows) {
-  __shared__ int64_t wave_u[kCachedWaves];
-  __shared__ int wave_i[kCachedWaves];
+template <bool PREFIX, int MODE, class Start>
+__device__ Scan cached_scan(const CachedCall& a, int (&shared)[2][kCachedWaves], Start start) {
   const int n = PREFIX ? a.n_groups : a.n_seqs, per = (n + kCachedThreads - 1) / kCachedThreads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Scan r;
   r.e0 = min((int)threadIdx.x * per, n);
   r.e1 = min(r.e0 + per, n);
-  int64_t u = 0;
-  int it = 0;
+  int u = 0, it = 0;
   for (int e = r.e0; e < r.e1; ++e) {
-    const Entry x = cached_entry<PREFIX>(a, tile_rows, e);
-    u += (int64_t)x.items * x.units;
+    const Entry x = cached_entry<PREFIX, MODE>(a, e, start);
+    u += x.items * x.units;
     it += x.items;
   }
-  r.own = u;
-  const int own_items = it;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t xu = __shfl_up(u, d);
-    const int xi = __shfl_up(it, d);
-    if (lane >= d) {
-      u += xu;
-      it += xi;
-    }
-  }
-  __syncthreads();
+  const int su = wave_scan(u), si = wave_scan(it);
   if (lane == 63) {
-    wave_u[wave] = u;
-    wave_i[wave] = it;
+    shared[0][wave] = su;
+    shared[1][wave] = si;
   }
   __syncthreads();
-  r.units = u - r.own;
-  r.items = it - own_items;
+  r.own = u;
+  r.units = su - u;
+  r.items = si - it;
   r.total = 0;
 #pragma unroll
   for (int w = 0; w < kCachedWaves; ++w) {
     if (w < wave) {
-      r.units += wave_u[w];
-      r.items += wave_i[w];
+      r.units += shared[0][w];
+      r.items += shared[1][w];
     }
-    r.total += wave_u[w];
+    r.total += shared[0][w];
   }
   return r;
 }
 
-// One item's keys [from, to) (from a multiple of 16) into a partial result.
+// Page ids of 64 consecutive table entries, one per lane.
+struct PageWindow {
+  const int32_t* row;
+  int at, ids, max_pages;
+  __device__ __forceinline__ void load(int page) {
+    at = page;
+    const int i = page + (threadIdx.x & 63);
+    ids = i < max_pages ? row[i] : -1;
+  }
+  __device__ __forceinline__ int operator()(int page) const { return __builtin_amdgcn_readlane(ids, min(page - at, 63)); }
+};
+
+// Buffer over up to 16 rows (of one page) of K or V from token p on, cut at token `to`; no rows if the page id is bad.
+__device__ __forceinline__ u32x4 page_rows(const CachedCall& a, int id, int64_t off, int p, int to) {
+  const int rows = min(to - p, 16);
+  const bool good = rows > 0 && (uint32_t)id < (uint32_t)a.n_pages;
+  const int64_t at = (int64_t)(good ? id : 0) * a.page_elems + off + (int64_t)(p & ((1 << a.page_log) - 1)) * a.dim;
+  return buffer_rsrc((uint64_t)(uintptr_t)(a.pool + at), good ? (uint32_t)(rows * a.dim * 2) : 0u);
+}
+
+// Query row rr of an item: its place in q, and the keys it sees.
+template <bool PREFIX>
+__device__ __forceinline__ const uint16_t* cached_query(const CachedCall& a, const Entry& x, int kvh, int rr, int& seen) {
+  const int G = a.heads / a.kv_heads, per = a.tokens * G;
+  const bool good = rr < x.rows;
+  const int b = PREFIX && good ? x.first + rr / per : min(x.first, a.n_seqs - 1), t = good ? rr % per / G : 0, h = kvh * G + rr % G;
+  if constexpr (PREFIX) {
+    const Seq s = cached_seq(a, b);
+    seen = good ? row_sees(s.len, s.q_len, t) : 0;
+  } else {
+    seen = good ? row_sees(x.seq.len, x.seq.q_len, t) : 0;
+  }
+  return reinterpret_cast<const uint16_t*>(a.q.data) + ((int64_t)b * a.tokens + t) * a.q.row_stride + (int64_t)h * a.q.head_stride;
+}
+
+// One item's keys [from, to) (from a multiple of 16) into a partial result, the keys split over the waves.
 template <bool BF, int DP, int MT, bool PREFIX>
-__device__ void cached_segment(const CachedCall& a, const Pass& ps, char* lds, int e, const Entry& x, int item, int from, int to,
-                               int slot) {
+__device__ void split_keys(const CachedCall& a, char* lds, const Entry& x, int item, int from, int to, int slot) {
   using E = Elem<BF>;
   constexpr int kRow = DP * 2;
   constexpr int kHalf = 16 * kRow;                       // 16 keys, always of one page
   constexpr int kHalfCopies = kHalf / 1024, kCopyRows = 1024 / kRow;
   constexpr int kTileCopies = 2 * kHalfCopies;
   constexpr int kSteps = DP / 32;
+  constexpr int kUnit = kCachedWaves * kWaveKeys;
+  const Pass& ps = PREFIX ? a.pre : a.own;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = lane & 15, w = lane >> 4;
-  const int D = a.dim, G = a.heads / a.kv_heads, per = a.tokens * G;
+  const int D = a.dim;
   const int kvh = item / x.tiles, row0 = (item % x.tiles) * 16 * MT;
   const int rows = min(x.rows - row0, 16 * MT);
-  const int first = PREFIX ? group_start(a, e) : e;
-  const int trow = __builtin_amdgcn_readfirstlane(cached_seq(a, first).row);
+
+  PageWindow pages{a.table + (int64_t)x.seq.row * a.max_pages, 0, -1, a.max_pages};
+  int pos = from + kWaveKeys * wave;
+  if (pos < to) pages.load(pos >> a.page_log);
 
   // this lane's query rows: 16 rt + n
   u32x4 qf[MT][kSteps];
@@ -422,16 +492,12 @@ __device__ void cached_segment(const CachedCall& a, const Pass& ps, char* lds, i
 #pragma unroll
   for (int rt = 0; rt < MT; ++rt) {
     const int rr = row0 + rt * 16 + n;
-    const bool good = rr < x.rows;
-    const int b = good ? first + rr / per : first, t = rr % per / G, h = kvh * G + rr % G;
-    seen[rt] = good ? row_sees(cached_seq(a, b), t) : 0;
-    if (good) all = min(all, seen[rt]);
-    const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.data) + ((int64_t)b * a.tokens + (good ? t : 0)) * a.q.row_stride +
-                         (int64_t)h * a.q.head_stride;
+    const uint16_t* qp = cached_query<PREFIX>(a, x, kvh, rr, seen[rt]);
+    if (rr < x.rows) all = min(all, seen[rt]);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int d = 32 * s + 8 * w;
-      qf[rt][s] = good && d < D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
+      qf[rt][s] = rr < x.rows && d < D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
     }
   }
 #pragma unroll
@@ -449,22 +515,12 @@ __device__ void cached_segment(const CachedCall& a, const Pass& ps, char* lds, i
   char* const kt = lds + wave * 4 * kHalf;
   char* const vt = kt + 2 * kHalf;
   const uint32_t k_lds = __builtin_amdgcn_readfirstlane(lds_addr(kt)), v_lds = k_lds + 2 * kHalf;
-  const int32_t* table = a.table + (int64_t)trow * a.max_pages;
   const int64_t head_off = ((int64_t)kvh << a.page_log) * D;
-  int window = 0, ids = -1;                              // page ids of the 64 table entries from `window`, one per lane
-  auto load_window = [&](int pos) {
-    window = pos >> a.page_log;
-    ids = window + lane < a.max_pages ? table[window + lane] : -1;
-  };
-  auto copy_keys = [&](int pos, int64_t off, uint32_t dst, const uint32_t* lanes) {
+  auto copy_keys = [&](int at, int64_t off, uint32_t dst, const uint32_t* lanes) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const int p = pos + 16 * hf;
-      const int id = __builtin_amdgcn_readlane(ids, min((p >> a.page_log) - window, 63));
-      const int rows_left = min(to - p, 16);
-      const bool good = rows_left > 0 && (uint32_t)id < (uint32_t)a.n_pages;
-      const int64_t at = (int64_t)(good ? id : 0) * a.page_elems + off + head_off + (int64_t)(p & ((1 << a.page_log) - 1)) * D;
-      const u32x4 r = buffer_rsrc((uint64_t)(uintptr_t)(a.pool + at), good ? (uint32_t)(rows_left * D * 2) : 0u);
+      const int p = at + 16 * hf;
+      const u32x4 r = page_rows(a, pages(p >> a.page_log), off + head_off, p, to);
 #pragma unroll
       for (int i = 0; i < kHalfCopies; ++i)
         copy16(r, lanes[i], __builtin_amdgcn_readfirstlane(dst + hf * kHalf + i * 1024));
@@ -480,9 +536,7 @@ __device__ void cached_segment(const CachedCall& a, const Pass& ps, char* lds, i
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) o[rt][d] = f32x4{};
   }
-  int pos = from + kWaveKeys * wave;
   if (pos < to) {
-    load_window(pos);
     copy_keys(pos, a.k_off, k_lds, k_lane);
     copy_keys(pos, a.v_off, v_lds, v_lane);
   }
@@ -503,7 +557,7 @@ __device__ void cached_segment(const CachedCall& a, const Pass& ps, char* lds, i
       }
     wait_lds();
     if (more) {
-      if (((next + kWaveKeys - 1) >> a.page_log) - window > 63) load_window(next);
+      if (((next + kWaveKeys - 1) >> a.page_log) - pages.at > 63) pages.load(next >> a.page_log);
       copy_keys(next, a.k_off, k_lds, k_lane);
     }
     // element i of s[rt][g]: key pos + 16 g + 4 w + i, query row 16 rt + n
@@ -559,18 +613,20 @@ __device__ void cached_segment(const CachedCall& a, const Pass& ps, char* lds, i
   constexpr int kPad = DP + 4;
   float* const buf = reinterpret_cast<float*>(lds);                 // [wave][16][kPad]
   float* const ml = buf + kCachedWaves * 16 * kPad;                 // [wave][16 MT][2]
-  __syncthreads();                                                  // every wave is done with its tiles
 #pragma unroll
   for (int rt = 0; rt < MT; ++rt) {
     sum[rt] += __shfl_xor(sum[rt], 16);
     sum[rt] += __shfl_xor(sum[rt], 32);
+  }
+  __syncthreads();                                                  // every wave is done with its tiles
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt)
     if (w == 0) {
       ml[(wave * 16 * MT + rt * 16 + n) * 2] = top[rt];
       ml[(wave * 16 * MT + rt * 16 + n) * 2 + 1] = sum[rt];
     }
-  }
   __syncthreads();
-  const bool store = slot < ps.slots;
+  const bool store = slot >= 0 && slot < ps.slots;
 #pragma unroll
   for (int rt = 0; rt < MT; ++rt) {
     const int r = rt * 16 + n;
@@ -585,7 +641,7 @@ __device__ void cached_segment(const CachedCall& a, const Pass& ps, char* lds, i
     for (int d = 0; d < DP / 16; ++d)
       *reinterpret_cast<f32x4*>(buf + (wave * 16 + n) * kPad + d * 16 + 4 * w) = o[rt][d] * f;
     if (store && wave == 0 && w == 0 && r < rows) {
-      float* at = ps.ml + ((int64_t)slot * ps.tile_rows + r) * 2;
+      float* at = ps.ml + ((int64_t)slot * ps.stride + r) * 2;
       at[0] = m;
       at[1] = l;
     }
@@ -596,53 +652,124 @@ __device__ void cached_segment(const CachedCall& a, const Pass& ps, char* lds, i
 #pragma unroll
       for (int v = 0; v < kCachedWaves; ++v) y += *reinterpret_cast<const f32x4*>(buf + (v * 16 + rr) * kPad + d);
       if (store && rt * 16 + rr < rows && d < D)
-        *reinterpret_cast<f32x4*>(ps.part + ((int64_t)slot * ps.tile_rows + rt * 16 + rr) * D + d) = y;
+        *reinterpret_cast<f32x4*>(ps.part + ((int64_t)slot * ps.stride + rt * 16 + rr) * D + d) = y;
     }
     __syncthreads();
   }
 }
 
-template <bool BF, int DP, int MT, bool PREFIX>
-__global__ __launch_bounds__(kCachedThreads, MT == 4 ? 1 : 2) void k_cached(const CachedCall a, const Pass ps) {
-  constexpr int kStage = kCachedWaves * 2 * kWaveKeys * DP * 2;
-  __shared__ __attribute__((aligned(1024))) char lds[kStage];
-  static_assert(kCachedWaves * (16 * (DP + 4) + 16 * MT * 2) * 4 <= kStage, "the join fits the tiles' space");
-  __shared__ int64_t found[3];
-  const Scan sc = cached_scan<PREFIX>(a, ps.tile_rows);
-  const int blocks = (int)min((int64_t)ps.blocks, sc.total);
-  // consecutive runs on one XCD: row tiles that read the same keys then share its L2
-  const int per_xcd = ps.blocks / kXcds;
-  const int me = (int)(blockIdx.x % kXcds) * per_xcd + blockIdx.x / kXcds;
+// The same with the rows split over the waves, 32 each, and tiles of 64 keys shared by the block.
+template <bool BF, int DP, bool PREFIX>
+__device__ void split_rows(const CachedCall& a, char* lds, const Entry& x, int item, int from, int to, int slot) {
+  constexpr int kRow = DP * 2;
+  constexpr int kTile = kPromptKeys * kRow;
+  constexpr int kCopies = 16 * kRow / 1024, kCopyRows = 1024 / kRow;      // a wave copies 16 of the 64 keys
+  const Pass& ps = PREFIX ? a.pre : a.own;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int half = lane >> 5, col = lane & 31;
+  const int D = a.dim;
+  const int kvh = item / x.tiles, row0 = (item % x.tiles) * kManyRows + wave * 32;
+  const bool busy = row0 < x.rows;                       // the wave has rows
+
+  PageWindow pages{a.table + (int64_t)x.seq.row * a.max_pages, 0, -1, a.max_pages};
+  pages.load(from >> a.page_log);
+  RowTile<BF, DP> rt;
+  int seen;
+  const uint16_t* qp = cached_query<PREFIX>(a, x, kvh, row0 + col, seen);
+  rt.start(qp, row0 + col < x.rows, D, half);
+  seen = min(seen, to);
+  int all = row0 + col < x.rows ? seen : 0x7FFFFFFF;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) all = min(all, __shfl_xor(all, d));
+  all = __builtin_amdgcn_readfirstlane(all);
+
+  uint32_t k_lane[kCopies], v_lane[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const uint32_t r = i * kCopyRows + lane / (kRow / 16), place = lane % (kRow / 16);
+    const uint32_t kc = place ^ k_key<DP>(r), vc = place ^ v_key<DP>(r);      // 16 rows on, the keys are the same
+    k_lane[i] = (int)kc * 8 < D ? r * D * 2 + kc * 16 : kOutOfRange;
+    v_lane[i] = (int)vc * 8 < D ? r * D * 2 + vc * 16 : kOutOfRange;
+  }
+  const int64_t head_off = ((int64_t)kvh << a.page_log) * D;
+  const uint32_t lds0 = lds_addr(lds) + wave * 16 * kRow;
+  auto copy_tile = [&](int t) {
+    const int p = from + t * kPromptKeys + wave * 16;
+    if ((p >> a.page_log) - pages.at > 63) pages.load((from + t * kPromptKeys) >> a.page_log);
+    const int id = pages(p >> a.page_log);
+    const u32x4 kr = page_rows(a, id, a.k_off + head_off, p, to), vr = page_rows(a, id, a.v_off + head_off, p, to);
+    const uint32_t dst = lds0 + (t & 1) * 2 * kTile;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) copy16(kr, k_lane[i], __builtin_amdgcn_readfirstlane(dst + i * 1024));
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) copy16(vr, v_lane[i], __builtin_amdgcn_readfirstlane(dst + kTile + i * 1024));
+  };
+  const int steps = (to - from + kPromptKeys - 1) / kPromptKeys;
+  copy_tile(0);
+  for (int t = 0; t < steps; ++t) {
+    wait_copies<0>();
+    lds_barrier();
+    if (t + 1 < steps) copy_tile(t + 1);
+    const char* kt = lds + (t & 1) * 2 * kTile;
+    const int at = from + t * kPromptKeys;
+    if (busy) rt.step(kt, kt + kTile, a.c, at + kPromptKeys > all, seen - at);
+  }
+  lds_barrier();                                         // the next item may fill the tiles
+  const int r = wave * 32 + col;
+  rt.sum += __shfl_xor(rt.sum, 32);
+  if (slot >= 0 && slot < ps.slots && row0 + col < x.rows) {
+    float* po = ps.part + ((int64_t)slot * ps.stride + r) * D;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int dim = d * 32 + 2 * e + 4 * half;
+        if (dim < D) *reinterpret_cast<f32x4*>(po + dim) = f32x4{rt.o[d][e], rt.o[d][e + 1], rt.o[d][e + 2], rt.o[d][e + 3]};
+      }
+    if (half == 0) {
+      float* pm = ps.ml + ((int64_t)slot * ps.stride + r) * 2;
+      pm[0] = rt.top;
+      pm[1] = rt.sum;
+    }
+  }
+}
+
+// The run of units of block `me` of `blocks`.
+template <bool BF, int DP, int MODE, bool PREFIX>
+__device__ void cached_run(const CachedCall& a, char* lds, const Scan& sc, int me, int blocks) {
+  __shared__ int found[4];
+  auto start = [&](int g) { return group_start(a, g); };
   if (me >= blocks) return;
-  int64_t u = me * sc.total / blocks;
-  const int64_t end = (me + 1) * sc.total / blocks;
+  const int n = PREFIX ? a.n_groups : a.n_seqs;
+  const int u = (int)((int64_t)me * sc.total / blocks), end = (int)((int64_t)(me + 1) * sc.total / blocks);
+  if (threadIdx.x < 3) found[threadIdx.x] = 0;
+  __syncthreads();
   if (u >= sc.units && u < sc.units + sc.own) {          // one thread: its run of entries holds u
-    int64_t before = sc.units;
-    int items = sc.items;
+    int before = sc.units, items = sc.items;
     for (int e = sc.e0; e < sc.e1; ++e) {
-      const Entry x = cached_entry<PREFIX>(a, ps.tile_rows, e);
-      const int64_t own = (int64_t)x.items * x.units;
-      if (u < before + own) {
+      const Entry x = cached_entry<PREFIX, MODE>(a, e, start);
+      if (u < before + x.items * x.units) {
         found[0] = e;
         found[1] = u - before;
         found[2] = items;
         break;
       }
-      before += own;
+      before += x.items * x.units;
       items += x.items;
     }
   }
   __syncthreads();
-  int e = __builtin_amdgcn_readfirstlane((int)found[0]);
-  int items = __builtin_amdgcn_readfirstlane((int)found[2]);
-  Entry x = cached_entry<PREFIX>(a, ps.tile_rows, e);
-  const int64_t in = found[1];
-  int item = __builtin_amdgcn_readfirstlane((int)(in / x.units)), unit = __builtin_amdgcn_readfirstlane((int)(in % x.units));
-  int left = __builtin_amdgcn_readfirstlane((int)(end - u));
+  // (groups that are not in order can overflow the sums: what follows stays within the entries all the same)
+  int e = min(max(__builtin_amdgcn_readfirstlane(found[0]), 0), n - 1), items = __builtin_amdgcn_readfirstlane(found[2]);
+  const int in = max(__builtin_amdgcn_readfirstlane(found[1]), 0);
+  Entry x = cached_entry<PREFIX, MODE>(a, e, start);
+  if (x.units == 0 || x.items == 0) return;
+  int item = min(in / x.units, x.items - 1), unit = in % x.units, left = end - u;
   while (true) {
     const int run = min(left, x.units - unit);
-    const int from = x.from + unit * kUnit, to = min(from + run * kUnit, x.to);
-    cached_segment<BF, DP, MT, PREFIX>(a, ps, lds, e, x, item, from, to, me + items + item);
+    const int from = x.from + unit * mode_unit(MODE), to = min(from + run * mode_unit(MODE), x.to);
+    if constexpr (MODE == kRows) split_rows<BF, DP, PREFIX>(a, lds, x, item, from, to, me + items + item);
+    else split_keys<BF, DP, MODE, PREFIX>(a, lds, x, item, from, to, me + items + item);
     left -= run;
     if (left <= 0) break;
     unit = 0;
@@ -650,86 +777,133 @@ __global__ __launch_bounds__(kCachedThreads, MT == 4 ? 1 : 2) void k_cached(cons
       item = 0;
       do {                                               // left > 0: a further entry has units
         items += x.items;
-        x = cached_entry<PREFIX>(a, ps.tile_rows, ++e);
+        if (++e >= n) return;
+        x = cached_entry<PREFIX, MODE>(a, e, start);
       } while (x.items == 0 || x.units == 0);
     }
   }
 }
 
+template <bool BF, int DP, int OWN, int PRE>
+__global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a) {
+  constexpr int kStage = kCachedWaves * 2 * kWaveKeys * DP * 2;     // = 2 buffers of K and V tiles of 64 keys for split rows, halved
+  constexpr int kBytes = OWN == kRows || PRE == kRows ? 4 * kPromptKeys * DP * 2 : kStage;
+  __shared__ __attribute__((aligned(1024))) char lds[kBytes];
+  __shared__ int shared[2][2][kCachedWaves];
+  static_assert(kCachedWaves * (16 * (DP + 4) + 32 * 2) * 4 <= kStage, "the join fits the tiles' space");
+  auto start = [&](int g) { return group_start(a, g); };
+  const Scan own = cached_scan<false, OWN>(a, shared[0], start);
+  Scan pre;
+  pre.total = 0;
+  if constexpr (PRE != kNone) pre = cached_scan<true, PRE>(a, shared[1], start);
+
+  // blocks for the prefixes: their share of the keys' cost
+  int n_pre = 0;
+  if constexpr (PRE != kNone) {
+    const float wp = (float)pre.total * mode_unit(PRE), wo = (float)own.total * mode_unit(OWN);
+    if (pre.total) n_pre = own.total ? min(max((int)(kCachedBlocks / kXcds * wp / (wp + wo) + 0.5f), 1), kCachedBlocks / kXcds - 1) * kXcds : kCachedBlocks;
+  }
+  const int pre_blocks = min(n_pre, pre.total), own_blocks = min(kCachedBlocks - n_pre, own.total);
+  if (blockIdx.x == 0) {                                 // for k_join
+    if (threadIdx.x == 0) {
+      a.join[0] = own.total;
+      a.join[1] = own_blocks;
+      a.join[2] = pre.total;
+      a.join[3] = pre_blocks;
+    }
+    JoinEntry* je = reinterpret_cast<JoinEntry*>(a.join + 4);
+    int u = own.units, it = own.items;
+    for (int e = own.e0; e < own.e1; ++e) {
+      const Entry x = cached_entry<false, OWN>(a, e, start);
+      je[e] = JoinEntry{u, it, x.units, x.tiles, x.group, x.first};
+      u += x.items * x.units;
+      it += x.items;
+    }
+    if constexpr (PRE != kNone) {
+      u = pre.units;
+      it = pre.items;
+      for (int e = pre.e0; e < pre.e1; ++e) {
+        const Entry x = cached_entry<true, PRE>(a, e, start);
+        je[a.n_seqs + e] = JoinEntry{u, it, x.units, x.tiles, e, x.first};
+        u += x.items * x.units;
+        it += x.items;
+      }
+    }
+  }
+  // consecutive runs on one XCD: row tiles that read the same keys then share its L2
+  const int xcd = blockIdx.x % kXcds, at = blockIdx.x / kXcds, pre_each = n_pre / kXcds;
+  if constexpr (PRE != kNone) {
+    if (at < pre_each) {
+      cached_run<BF, DP, PRE, true>(a, lds, pre, xcd * pre_each + at, pre_blocks);
+      return;
+    }
+  }
+  cached_run<BF, DP, OWN, false>(a, lds, own, xcd * (kCachedBlocks / kXcds - pre_each) + at - pre_each, own_blocks);
+}
+
 // One wave per (sequence, token, head): the partial results of its row, from the prefix and the own part.
 template <bool BF>
-__global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, const Pass own, const Pass pre) {
-  __shared__ int64_t at_u[2];
-  __shared__ int at_i[2];
+__global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, int own_rows, int pre_rows) {
   const int b = blockIdx.x, lane = threadIdx.x & 63;
   const int G = a.heads / a.kv_heads, D = a.dim;
-  const int g = group_of(a, b);
-  const Scan sc = cached_scan<false>(a, own.tile_rows);
-  Scan sp;
-  sp.total = 0;
-  if (g >= 0) sp = cached_scan<true>(a, pre.tile_rows);
-  if (b >= sc.e0 && b < sc.e1) {
-    int64_t u = sc.units;
-    int it = sc.items;
-    for (int e = sc.e0; e < b; ++e) {
-      const Entry x = cached_entry<false>(a, own.tile_rows, e);
-      u += (int64_t)x.items * x.units;
-      it += x.items;
-    }
-    at_u[0] = u;
-    at_i[0] = it;
-  }
-  if (g >= 0 && g >= sp.e0 && g < sp.e1) {
-    int64_t u = sp.units;
-    int it = sp.items;
-    for (int e = sp.e0; e < g; ++e) {
-      const Entry x = cached_entry<true>(a, pre.tile_rows, e);
-      u += (int64_t)x.items * x.units;
-      it += x.items;
-    }
-    at_u[1] = u;
-    at_i[1] = it;
-  }
-  __syncthreads();
   const int row = blockIdx.y * kCachedWaves + (threadIdx.x >> 6);   // t * heads + h
   if (row >= a.tokens * a.heads) return;
   const int t = row / a.heads, h = row % a.heads, kvh = h / G;
-  const Seq s = cached_seq(a, b);
-  const int seen = row_sees(s, t);
+  const JoinEntry* je = reinterpret_cast<const JoinEntry*>(a.join + 4);
+  const JoinEntry own = je[b];
   float m = -INFINITY, l = 0.0f, y0 = 0.0f, y1 = 0.0f;
-  auto add = [&](const Pass& ps, const Entry& x, int rr, int64_t units, int items, int64_t total) {
+  auto add = [&](const Pass& ps, const JoinEntry& x, int tile_rows, int rr, int total, int blocks) {
     if (x.units == 0) return;
-    const int64_t blocks = min((int64_t)ps.blocks, total);
-    const int item = kvh * x.tiles + rr / ps.tile_rows, r = rr % ps.tile_rows;
-    const int64_t u0 = units + (int64_t)item * x.units;
+    const int item = kvh * x.tiles + rr / tile_rows, r = rr % tile_rows;
+    const int64_t u0 = x.units_before + (int64_t)item * x.units;
     const int i0 = (int)(((u0 + 1) * blocks - 1) / total), i1 = (int)(((u0 + x.units) * blocks - 1) / total);
-    for (int i = i0; i <= i1; ++i) {
-      const int64_t slot = (int64_t)i + items + item;
-      if (slot >= ps.slots) return;
-      const float* p = ps.ml + (slot * ps.tile_rows + r) * 2;
-      const float pm = p[0], pl = p[1];
-      const float* po = ps.part + (slot * ps.tile_rows + r) * D;
-      const float z0 = lane < D ? po[lane] : 0.0f, z1 = lane + 64 < D ? po[lane + 64] : 0.0f;
-      const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.0f : top;
-      const float f = exp2_fast(m - base), pf = exp2_fast(pm - base);
-      l = l * f + pl * pf;
-      y0 = y0 * f + z0 * pf;
-      y1 = y1 * f + z1 * pf;
+    const int64_t s0 = (int64_t)i0 + x.items_before + item;
+    const int n = s0 < 0 ? 0 : (int)min((int64_t)(i1 - i0 + 1), ps.slots - s0);
+    const float* pm = ps.ml + (s0 * ps.stride + r) * 2;
+    const float* po = ps.part + (s0 * ps.stride + r) * D;
+    for (int c0 = 0; c0 < n; c0 += 64) {                 // one slot per lane: maximum, weights, sum
+      const bool in = c0 + lane < n;
+      const float sm = in ? pm[(int64_t)(c0 + lane) * ps.stride * 2] : -INFINITY;
+      const float sl = in ? pm[(int64_t)(c0 + lane) * ps.stride * 2 + 1] : 0.0f;
+      const float top = fmaxf(m, wave_max(sm)), base = top == -INFINITY ? 0.0f : top;
+      const float f = exp2_fast(m - base), w = exp2_fast(sm - base);
+      l = l * f + wave_sum(sl * w);
+      y0 *= f;
+      y1 *= f;
       m = top;
+      const int k = min(64, n - c0);
+      for (int i = 0; i < k; i += 4) {                   // four slots' loads at a time
+        float z0[4], z1[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float* p = po + (int64_t)(c0 + min(i + v, k - 1)) * ps.stride * D;
+          z0[v] = lane < D ? p[lane] : 0.0f;
+          z1[v] = lane + 64 < D ? p[lane + 64] : 0.0f;
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float wi = i + v < k ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), min(i + v, 63))) : 0.0f;
+          if (i + v < k) {
+            y0 = __builtin_fmaf(z0[v], wi, y0);
+            y1 = __builtin_fmaf(z1[v], wi, y1);
+          }
+        }
+      }
     }
   };
-  if (g >= 0) {
-    const int rr = ((b - group_start(a, g)) * a.tokens + t) * G + h % G;
-    add(pre, cached_entry<true>(a, pre.tile_rows, g), rr, at_u[1], at_i[1], sp.total);
+  if (own.group >= 0) {
+    const JoinEntry pre = je[a.n_seqs + own.group];
+    add(a.pre, pre, pre_rows, ((b - pre.first) * a.tokens + t) * G + h % G, a.join[2], a.join[3]);
   }
-  add(own, cached_entry<false>(a, own.tile_rows, b), t * G + h % G, at_u[0], at_i[0], sc.total);
+  add(a.own, own, own_rows, t * G + h % G, a.join[0], a.join[1]);
   const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
   y0 *= inv;
   y1 *= inv;
   if (__ballot(!finite(y0) || !finite(y1))) {
+    const Seq s = cached_seq(a, b);
     const int32_t* table = a.table + (int64_t)s.row * a.max_pages;
     plain_row<BF>(reinterpret_cast<const uint16_t*>(a.q.data) + ((int64_t)b * a.tokens + t) * a.q.row_stride + (int64_t)h * a.q.head_stride,
-                  D, seen, a.c,
+                  D, row_sees(s.len, s.q_len, t), a.c,
                   [&](int key, const uint16_t*& k, const uint16_t*& v) {
                     const int id = min(max(table[key >> a.page_log], 0), a.n_pages - 1);
                     const uint16_t* p = a.pool + (int64_t)id * a.page_elems +
@@ -774,14 +948,15 @@ void launch_prompt(const mtc_prompt_args& a, unsigned grid, hipStream_t st) {
   else k_prompt<BF, 128><<<grid, 64 * kPromptWaves, 0, st>>>(a);
 }
 
-// Row tiles of a pass: 16, 32 or 64 rows per item, the least that hold the rows.
-int tile_rows_for(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// How an item's rows are taken: the least of 16, 32 and 128 rows that holds them.
+int mode_for(int64_t rows) { return rows <= 16 ? kOneTile : rows <= 32 ? kTwoTiles : kRows; }
 
 struct CachedPlan {
-  int own_rows, pre_rows;            // per item
+  int own_mode, pre_mode;
+  int own_stride, pre_stride;        // rows of a slot
   int64_t own_slots, pre_slots;
-  size_t own_bytes, pre_bytes;       // part + ml of each pass
-  int blocks;
+  size_t own_bytes, pre_bytes, join_bytes;
+  size_t bytes() const { return own_bytes + pre_bytes + join_bytes; }
 };
 
 size_t round_up(size_t x, size_t to) { return (x + to - 1) / to * to; }
@@ -798,38 +973,49 @@ int plan_cached(const mtc_cache_desc* c, const mtc_cached_args* a, CachedPlan* p
   if (a->tokens < 1 || a->tokens > MTC_CACHED_MAX_TOKENS)
     return fail(MTC_E_SHAPE, "%d tokens per sequence: 1 to %d", a->tokens, MTC_CACHED_MAX_TOKENS);
   if (a->n_groups < 0 || a->n_groups > a->n_seqs) return fail(MTC_E_SHAPE, "%d groups of %d sequences", a->n_groups, a->n_seqs);
-  const int64_t per = (int64_t)a->tokens * (a->heads / c->kv_heads);
   if ((int64_t)a->tokens * a->heads > 0xFFFF || (int64_t)a->tokens * a->heads * a->n_seqs > 0x3FFFFFF)   // 2^32 threads a launch
     return fail(MTC_E_SHAPE, "%d sequences of %d tokens of %d heads: too many query rows", a->n_seqs, a->tokens, a->heads);
-  p->blocks = 512;                   // two per CU
-  p->own_rows = tile_rows_for(per);
-  p->pre_rows = tile_rows_for(per * a->n_seqs);
-  p->own_slots = p->blocks + (int64_t)a->n_seqs * c->kv_heads * ((per + p->own_rows - 1) / p->own_rows);
-  p->pre_slots = a->n_groups ? p->blocks + (int64_t)c->kv_heads * ((per * a->n_seqs + p->pre_rows - 1) / p->pre_rows + a->n_groups) : 0;
-  p->own_bytes = round_up((size_t)p->own_slots * p->own_rows * (c->dim + 2) * 4, 256);
-  p->pre_bytes = round_up((size_t)p->pre_slots * p->pre_rows * (c->dim + 2) * 4, 256);
+  const int64_t per = (int64_t)a->tokens * (a->heads / c->kv_heads), all = per * a->n_seqs;
+  p->own_mode = mode_for(per);
+  // groups are on the device: the rows of an average one decide
+  p->pre_mode = a->n_groups ? mode_for(std::max<int64_t>(all / a->n_groups, 17)) : kNone;
+  auto tiles = [](int64_t rows, int mode) { return (rows + mode_rows(mode) - 1) / mode_rows(mode); };
+  auto stride = [](int64_t rows, int mode) { return (int)std::min<int64_t>((rows + 15) / 16 * 16, mode_rows(mode)); };
+  p->own_stride = stride(per, p->own_mode);
+  p->own_slots = kCachedBlocks + (int64_t)a->n_seqs * c->kv_heads * tiles(per, p->own_mode);
+  p->pre_stride = p->pre_mode ? stride(all, p->pre_mode) : 0;
+  p->pre_slots = p->pre_mode ? kCachedBlocks + (int64_t)c->kv_heads * (tiles(all, p->pre_mode) + a->n_groups) : 0;
+  // the kernels count units in 32 bits
+  const int64_t units = (int64_t)c->max_pages * c->page_size / kPromptKeys + 1;
+  if (units * (p->own_slots + p->pre_slots) > 0x7FFFFFFF)
+    return fail(MTC_E_SHAPE, "%d sequences of up to %d pages of %d tokens, %d row tiles: too much for one call", a->n_seqs, c->max_pages,
+                c->page_size, (int)tiles(per, p->own_mode));
+  p->own_bytes = round_up((size_t)p->own_slots * p->own_stride * (c->dim + 2) * 4, 256);
+  p->pre_bytes = round_up((size_t)p->pre_slots * p->pre_stride * (c->dim + 2) * 4, 256);
+  p->join_bytes = round_up(16 + sizeof(JoinEntry) * ((size_t)a->n_seqs + a->n_groups), 256);
   return MTC_OK;
 }
 
-template <bool BF, int DP, bool PREFIX>
-void launch_cached(const CachedCall& a, const Pass& ps, hipStream_t st) {
-  if (ps.tile_rows == 16) k_cached<BF, DP, 1, PREFIX><<<ps.blocks, kCachedThreads, 0, st>>>(a, ps);
-  else if (ps.tile_rows == 32) k_cached<BF, DP, 2, PREFIX><<<ps.blocks, kCachedThreads, 0, st>>>(a, ps);
-  else k_cached<BF, DP, 4, PREFIX><<<ps.blocks, kCachedThreads, 0, st>>>(a, ps);
+template <bool BF, int DP, int OWN>
+void launch_cached(const CachedCall& a, int pre, hipStream_t st) {
+  if (pre == kNone) k_cached<BF, DP, OWN, kNone><<<kCachedBlocks, kCachedThreads, 0, st>>>(a);
+  else if (pre == kTwoTiles) k_cached<BF, DP, OWN, kTwoTiles><<<kCachedBlocks, kCachedThreads, 0, st>>>(a);
+  else k_cached<BF, DP, OWN, kRows><<<kCachedBlocks, kCachedThreads, 0, st>>>(a);
+}
+template <bool BF, int DP>
+void launch_cached(const CachedCall& a, int own, int pre, hipStream_t st) {
+  if (own == kOneTile) launch_cached<BF, DP, kOneTile>(a, pre, st);
+  else if (own == kTwoTiles) launch_cached<BF, DP, kTwoTiles>(a, pre, st);
+  else launch_cached<BF, DP, kRows>(a, pre, st);
 }
 
 template <bool BF>
-int run_cached(const CachedCall& a, const Pass& own, const Pass& pre, hipStream_t st) {
-  if (a.n_groups) {
-    if (a.dim <= 64) launch_cached<BF, 64, true>(a, pre, st);
-    else launch_cached<BF, 128, true>(a, pre, st);
-    if (int rc = check_launch("k_cached (prefixes)")) return rc;
-  }
-  if (a.dim <= 64) launch_cached<BF, 64, false>(a, own, st);
-  else launch_cached<BF, 128, false>(a, own, st);
+int run_cached(const CachedCall& a, const CachedPlan& p, hipStream_t st) {
+  if (a.dim <= 64) launch_cached<BF, 64>(a, p.own_mode, p.pre_mode, st);
+  else launch_cached<BF, 128>(a, p.own_mode, p.pre_mode, st);
   if (int rc = check_launch("k_cached")) return rc;
   const dim3 grid(a.n_seqs, (a.tokens * a.heads + kCachedWaves - 1) / kCachedWaves);
-  k_join<BF><<<grid, kCachedThreads, 0, st>>>(a, own, pre);
+  k_join<BF><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_rows(p.pre_mode));
   return check_launch("k_join");
 }
 
@@ -859,7 +1045,7 @@ MTC_API int mtc_prompt_attention(const mtc_prompt_args* a, void* hip_stream) {
 MTC_API size_t mtc_cached_attention_workspace_bytes(const mtc_cache_desc* c, const mtc_cached_args* a) {
   CachedPlan p;
   if (plan_cached(c, a, &p) != MTC_OK) return 0;
-  return p.own_bytes + p.pre_bytes;
+  return p.bytes();
 }
 
 MTC_API int mtc_cached_attention(const mtc_cache_desc* c, const mtc_cached_args* a, void* workspace, size_t workspace_bytes,
@@ -870,8 +1056,8 @@ MTC_API int mtc_cached_attention(const mtc_cache_desc* c, const mtc_cached_args*
   if (int rc = check_heads("q", a->q, false)) return rc;
   if (int rc = check_heads("o", a->o, false)) return rc;
   if (a->n_groups && (!a->groups || !a->prefix_lens)) return fail(MTC_E_NULL, "groups or prefix_lens is NULL");
-  if (!workspace || workspace_bytes < p.own_bytes + p.pre_bytes)
-    return fail(MTC_E_WORKSPACE, "workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : (size_t)0, p.own_bytes + p.pre_bytes);
+  if (!workspace || workspace_bytes < p.bytes())
+    return fail(MTC_E_WORKSPACE, "workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : (size_t)0, p.bytes());
   if ((uintptr_t)workspace % 256) return fail(MTC_E_WORKSPACE, "workspace must be 256-byte aligned");
   CachedCall k;
   const int64_t head = (int64_t)c->page_size * c->dim;
@@ -898,17 +1084,12 @@ MTC_API int mtc_cached_attention(const mtc_cache_desc* c, const mtc_cached_args*
   k.heads = a->heads;
   k.n_groups = a->n_groups;
   k.c = a->scale * kLog2e;
-  auto pass = [&](char* at, int64_t slots, int rows) {
-    Pass x;
-    x.part = (float*)at;
-    x.ml = x.part + slots * rows * c->dim;
-    x.tile_rows = rows;
-    x.blocks = p.blocks;
-    x.slots = (int)slots;
-    return x;
+  auto pass = [&](char* at, int64_t slots, int stride) {
+    float* part = (float*)at;
+    return Pass{part, part + slots * stride * c->dim, stride, (int32_t)slots};
   };
-  const Pass own = pass((char*)workspace, p.own_slots, p.own_rows);
-  const Pass pre = pass((char*)workspace + p.own_bytes, p.pre_slots, p.pre_rows);
-  return c->dtype == MTC_DTYPE_BF16 ? run_cached<true>(k, own, pre, (hipStream_t)hip_stream)
-                                    : run_cached<false>(k, own, pre, (hipStream_t)hip_stream);
+  k.own = pass((char*)workspace, p.own_slots, p.own_stride);
+  k.pre = pass((char*)workspace + p.own_bytes, p.pre_slots, p.pre_stride);
+  k.join = (int32_t*)((char*)workspace + p.own_bytes + p.pre_bytes);
+  return c->dtype == MTC_DTYPE_BF16 ? run_cached<true>(k, p, (hipStream_t)hip_stream) : run_cached<false>(k, p, (hipStream_t)hip_stream);
 }
