@@ -11,7 +11,7 @@ import math
 from typing import Optional
 
 from . import _abi, _native
-from .device import _need, current_stream_handle, prefill_workspace, require_gpu
+from .device import raw_stream, require_gpu, stream_workspace
 
 
 def _dtype_code(dtype):
@@ -25,11 +25,11 @@ def _dtype_code(dtype):
 
 def _kernel_heads(x):
     """x (rows, heads, dim) itself when the kernels can read it in place (unit stride along dim, the other strides
-    multiples of 8 elements and rows that do not overlap, a 16-byte aligned start), else a contiguous copy."""
+    multiples of 8 elements, rows that do not overlap, a 16-byte aligned start), else a contiguous copy."""
     r, h, u = x.stride()
-    # (a stride along a length of one is never used)
-    ok = (u == 1 and h % 8 == 0 and r % 8 == 0 and h >= 0 and x.shape[2] <= r < 1 << 24 and x.data_ptr() % 16 == 0)
-    return x if ok else x.contiguous()
+    if u == 1 and not (h | r) & 7 and x.shape[2] <= r < 1 << 24 and not x.data_ptr() & 15:
+        return x
+    return x.contiguous()
 
 
 def _heads(x) -> "_abi.MtcHeads":
@@ -37,17 +37,21 @@ def _heads(x) -> "_abi.MtcHeads":
 
 
 def _int32(name, x, n, device):
+    """Address of a list of n (None: any number of) int32 on the device."""
     import torch
-    _need(isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.dim() == 1 and x.is_contiguous()
-          and x.device == device, f"{name} must be a contiguous 1-D int32 tensor on {device}")
-    _need(n is None or x.shape[0] == n, f"{name} must hold {n} numbers, got {x.shape[0]}")
+    if not (isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.dim() == 1 and x.is_contiguous() and x.device == device):
+        raise ValueError(f"{name} must be a contiguous 1-D int32 tensor on {device}")
+    if n is not None and x.shape[0] != n:
+        raise ValueError(f"{name} must hold {n} numbers, got {x.shape[0]}")
     return x.data_ptr()
 
 
 def _scale(scale: Optional[float], dim: int) -> float:
-    s = dim ** -0.5 if scale is None else float(scale)
-    _need(math.isfinite(s) and s > 0, f"scale must be positive and finite, got {scale}")
-    return s
+    if scale is None:
+        return dim ** -0.5
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return float(scale)
 
 
 def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: Optional[float] = None, out=None):
@@ -63,35 +67,40 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: Op
     they held); default: a new contiguous tensor.
     """
     import torch
-    dev = require_gpu(q.device)
-    _need(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k and v must be (tokens, heads, dim)")
+    dev = q.device if q.is_cuda else require_gpu(q.device)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+        raise ValueError(f"q, k and v must be (tokens, heads, dim), k and v alike: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     dt = _dtype_code(q.dtype)
-    _need(k.dtype == q.dtype and v.dtype == q.dtype, f"q, k and v must share a dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
-    _need(k.device == dev and v.device == dev, f"q, k and v must be on {dev}")
+    if not (k.dtype == q.dtype == v.dtype and k.device == dev == v.device):
+        raise ValueError(f"q, k and v must share dtype and device, got {q.dtype}, {k.dtype}, {v.dtype} on {dev}, {k.device}, {v.device}")
     rows, heads, dim = q.shape
-    _need(k.shape == v.shape and k.shape[2] == dim, f"k {tuple(k.shape)} and v {tuple(v.shape)} must be (keys, kv_heads, {dim})")
-    kv_heads = k.shape[1]
-    _need(kv_heads > 0 and heads > 0 and heads % kv_heads == 0, f"{heads} query heads over {kv_heads} K/V heads")
-    _need(8 <= dim <= _abi.ATTN_MAX_DIM and dim % 8 == 0, f"dim must be a multiple of 8 from 8 to {_abi.ATTN_MAX_DIM}, got {dim}")
+    keys, kv_heads, k_dim = k.shape
+    if k_dim != dim or kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads of {dim} over {kv_heads} K/V heads of {k_dim}")
+    if dim < 8 or dim > _abi.ATTN_MAX_DIM or dim % 8:
+        raise ValueError(f"dim must be a multiple of 8 from 8 to {_abi.ATTN_MAX_DIM}, got {dim}")
     scale = _scale(scale, dim)
-    n = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
-    _need(n >= 0, "cu_q must hold sequences + 1 offsets")
     cq = _int32("cu_q", cu_q, None, dev)
-    if cu_k is None:
-        _need(k.shape[0] == rows, f"without cu_k, k and v hold one row per query: {k.shape[0]} != {rows}")
+    n = cu_q.shape[0] - 1
+    if n < 0:
+        raise ValueError("cu_q must hold sequences + 1 offsets")
+    if cu_k is not None:
+        ck = _int32("cu_k", cu_k, n + 1, dev)
+    elif keys == rows:
         ck = cq
     else:
-        ck = _int32("cu_k", cu_k, n + 1, dev)
+        raise ValueError(f"without cu_k, k and v hold one row per query: {keys} != {rows}")
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=dev)
-    else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev and _kernel_heads(out) is out,
-              f"out must be {tuple(q.shape)} {q.dtype} on {dev} with 16-byte aligned rows")
-    q, k, v = _kernel_heads(q), _kernel_heads(k), _kernel_heads(v)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif not (out.shape == q.shape and out.dtype == q.dtype and out.device == dev and _kernel_heads(out) is out):
+        raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {dev} with 16-byte aligned rows")
     lib = _native.hip_lib()
-    args = _abi.MtcPromptArgs(_abi.ABI_VERSION, dt, n, heads, kv_heads, dim, rows, k.shape[0], int(causal), scale,
+    q, k, v = _kernel_heads(q), _kernel_heads(k), _kernel_heads(v)
+    args = _abi.MtcPromptArgs(_abi.ABI_VERSION, dt, n, heads, kv_heads, dim, rows, keys, causal, scale,
                               _heads(q), _heads(k), _heads(v), _heads(out), cq, ck)
-    _abi.check(lib, "mtc_prompt_attention", lib.mtc_prompt_attention(ctypes.byref(args), current_stream_handle(dev)))
+    rc = lib.mtc_prompt_attention(ctypes.byref(args), raw_stream(dev.index))
+    if rc:
+        _abi.check(lib, "mtc_prompt_attention", rc)
     return out
 
 
@@ -110,41 +119,49 @@ def cached_attention(q, cache, layer: int, seqs, *, q_lens=None, groups=None, pr
     """
     import torch
     dev = cache.device
-    _need(q.dim() == 4 and q.device == dev, f"q must be (sequences, tokens, heads, dim) on {dev}")
-    _need(q.dtype == cache.dtype, f"q must be {cache.dtype}, as the cache, got {q.dtype}")
+    if q.dim() != 4 or q.device != dev or q.dtype != cache.dtype:
+        raise ValueError(f"q must be (sequences, tokens, heads, dim) {cache.dtype} on {dev}, got {tuple(q.shape)} {q.dtype} on {q.device}")
     n, tokens, heads, dim = q.shape
-    _need(dim == cache.head_dim, f"head size {dim}, the cache holds {cache.head_dim}")
-    _need(heads > 0 and heads % cache.n_kv_heads == 0, f"{heads} query heads over {cache.n_kv_heads} K/V heads")
-    _need(1 <= tokens <= _abi.CACHED_MAX_TOKENS, f"1 to {_abi.CACHED_MAX_TOKENS} tokens per sequence, got {tokens}")
-    _need(n <= _abi.CACHED_MAX_SEQS, f"at most {_abi.CACHED_MAX_SEQS} sequences, got {n}")
-    _need(0 <= layer < cache.n_layers, f"layer {layer} of {cache.n_layers}")
-    _need((groups is None) == (prefix_lens is None), "groups and prefix_lens come together")
+    if dim != cache.head_dim or heads < 1 or heads % cache.n_kv_heads:
+        raise ValueError(f"{heads} query heads of {dim} over a cache of {cache.n_kv_heads} heads of {cache.head_dim}")
+    if not 1 <= tokens <= _abi.CACHED_MAX_TOKENS:
+        raise ValueError(f"1 to {_abi.CACHED_MAX_TOKENS} tokens per sequence, got {tokens}")
+    if n > _abi.CACHED_MAX_SEQS:
+        raise ValueError(f"at most {_abi.CACHED_MAX_SEQS} sequences, got {n}")
+    if not 0 <= layer < cache.n_layers:
+        raise ValueError(f"layer {layer} of {cache.n_layers}")
     scale = _scale(scale, dim)
     sp = _int32("seqs", seqs, n, dev)
     qp = None if q_lens is None else _int32("q_lens", q_lens, n, dev)
     gp = pp = None
     n_groups = 0
+    if (groups is None) != (prefix_lens is None):
+        raise ValueError("groups and prefix_lens come together")
     if groups is not None:
         n_groups = prefix_lens.shape[0]
         pp, gp = _int32("prefix_lens", prefix_lens, None, dev), _int32("groups", groups, n_groups + 1, dev)
-        _need(n_groups <= n, f"{n_groups} groups of {n} sequences")
+        if n_groups > n:
+            raise ValueError(f"{n_groups} groups of {n} sequences")
     if out is None:
-        out = torch.empty((n, tokens, heads, dim), dtype=q.dtype, device=dev)
-    else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.is_contiguous()
-              and out.data_ptr() % 16 == 0, f"out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {dev}")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif not (out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.is_contiguous() and out.data_ptr() % 16 == 0):
+        raise ValueError(f"out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {dev}")
     if n == 0:
         return out
+    # rows b * tokens + t
     if tokens > 1 and q.stride(0) != tokens * q.stride(1):
         q = q.contiguous()
-    # rows b * tokens + t
-    qr = _kernel_heads(q.squeeze(1) if tokens == 1 else q.flatten(0, 1))
+    row, head, unit = q.stride(0) if tokens == 1 else q.stride(1), q.stride(2), q.stride(3)
+    if unit != 1 or (row | head) & 7 or not dim <= row < 1 << 24 or q.data_ptr() & 15:
+        q = q.contiguous()
+        row, head = heads * dim, dim
     lib = cache.lib
-    args = _abi.MtcCachedArgs(_abi.ABI_VERSION, layer, n, tokens, heads, n_groups, scale, 0, _heads(qr),
+    args = _abi.MtcCachedArgs(_abi.ABI_VERSION, layer, n, tokens, heads, n_groups, scale, 0, _abi.MtcHeads(q.data_ptr(), row, head),
                               _abi.MtcHeads(out.data_ptr(), heads * dim, dim), sp, qp, gp, pp)
-    ref = ctypes.byref(args)
-    need = int(lib.mtc_cached_attention_workspace_bytes(cache.desc_ref, ref))
-    ws = prefill_workspace(dev, need) if need else None
-    _abi.check(lib, "mtc_cached_attention",
-               lib.mtc_cached_attention(cache.desc_ref, ref, ws.data_ptr() if need else None, need, current_stream_handle(dev)))
+    ref, stream = ctypes.byref(args), raw_stream(dev.index)
+    need = lib.mtc_cached_attention_workspace_bytes(cache.desc_ref, ref)
+    ws = stream_workspace(dev.index, stream, need).data_ptr() if need else None
+    rc = lib.mtc_cached_attention(cache.desc_ref, ref, ws, need, stream)
+    if rc:
+        _abi.check(lib, "mtc_cached_attention", rc)
     return out

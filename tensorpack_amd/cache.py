@@ -15,7 +15,7 @@ from typing import Optional
 
 from . import _abi, _native
 from .attention import _dtype_code, _int32
-from .device import _need, current_stream_handle, require_gpu
+from .device import _need, raw_stream, require_gpu
 
 STATE_WORDS = 4
 
@@ -87,35 +87,39 @@ class PagedCache:
 
     # ---- bookkeeping ----------------------------------------------------------------
     def _call(self, name, *args):
-        _abi.check(self.lib, name, getattr(self.lib, name)(self.desc_ref, *args, current_stream_handle(self.device)))
+        rc = getattr(self.lib, name)(self.desc_ref, *args, raw_stream(self.device.index))
+        if rc:
+            _abi.check(self.lib, name, rc)
 
     def _list(self, name, x, n=None):
-        p = _int32(name, x, n, self.device)
-        _need(x.shape[0] <= _abi.CACHED_MAX_SEQS, f"{name}: at most {_abi.CACHED_MAX_SEQS} sequences a call")
-        return p
+        if x.shape[0] > _abi.CACHED_MAX_SEQS:
+            raise ValueError(f"{name}: at most {_abi.CACHED_MAX_SEQS} sequences a call")
+        return _int32(name, x, n, self.device)
 
     def extend(self, seqs, counts) -> None:
         """Room for counts[i] more tokens of seqs[i]: lens grow, new pages are taken, a shared page that is
         partly filled is copied first. Write the tokens' K and V with `append`, layer by layer."""
         p = self._list("seqs", seqs)
-        _need(seqs.shape[0] <= self.max_seqs, f"{seqs.shape[0]} sequences, the cache holds {self.max_seqs}")
+        if seqs.shape[0] > self.max_seqs:
+            raise ValueError(f"{seqs.shape[0]} sequences, the cache holds {self.max_seqs}")
         self._call("mtc_cache_extend", p, self._list("counts", counts, seqs.shape[0]), seqs.shape[0])
 
     def append(self, layer: int, k, v, seqs, cu) -> None:
         """Writes K and V (rows, n_kv_heads, head_dim; the cache's dtype, or fp32 to be rounded) of the newest tokens:
         rows cu[i]:cu[i+1] are the last tokens of seqs[i]. cu: (sequences + 1) int32 offsets from 0."""
         import torch
-        _need(0 <= layer < self.n_layers, f"layer {layer} of {self.n_layers}")
-        shape = (k.shape[0], self.n_kv_heads, self.head_dim)
-        _need(tuple(k.shape) == shape and tuple(v.shape) == shape, f"k and v must be (rows, {shape[1]}, {shape[2]})")
-        _need(k.dtype == v.dtype and k.dtype in (self.dtype, torch.float32) and k.device == self.device and v.device == self.device,
-              f"k and v must be {self.dtype} or float32 on {self.device}")
+        if not 0 <= layer < self.n_layers:
+            raise ValueError(f"layer {layer} of {self.n_layers}")
+        if k.dim() != 3 or k.shape != v.shape or k.shape[1] != self.n_kv_heads or k.shape[2] != self.head_dim:
+            raise ValueError(f"k and v must be (rows, {self.n_kv_heads}, {self.head_dim}), got {tuple(k.shape)}, {tuple(v.shape)}")
+        if not (k.dtype == v.dtype and k.dtype in (self.dtype, torch.float32) and k.device == self.device == v.device):
+            raise ValueError(f"k and v must be {self.dtype} or float32 on {self.device}")
         p = self._list("seqs", seqs)
         c = _int32("cu", cu, seqs.shape[0] + 1, self.device)
-        per = 16 // k.element_size()
-        ok = lambda x: x.stride(2) == 1 and x.stride(0) % per == 0 and x.stride(1) % per == 0 and x.data_ptr() % 16 == 0
-        k, v = (x if ok(x) else x.contiguous() for x in (k, v))
-        hk, hv = (_abi.MtcHeads(x.data_ptr(), x.stride(0), x.stride(1)) for x in (k, v))
+        mask = 16 // k.element_size() - 1                        # rows of 16-byte pieces are read in place
+        hk, hv = (_abi.MtcHeads(x.data_ptr(), x.stride(0), x.stride(1)) for x in
+                  (x if x.stride(2) == 1 and not (x.stride(0) | x.stride(1)) & mask and not x.data_ptr() & 15 else x.contiguous()
+                   for x in (k, v)))
         code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self.desc.dtype
         self._call("mtc_cache_append", layer, ctypes.byref(hk), ctypes.byref(hv), code, k.shape[0], p, c, seqs.shape[0])
 

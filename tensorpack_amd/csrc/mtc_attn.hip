@@ -350,29 +350,58 @@ __device__ __forceinline__ int group_of(int n_groups, int b, Start start) {
   return lo;
 }
 
+// What the lists say of the sequences and groups: read once into LDS where they fit (two rounds of loads for
+// the whole call instead of a chain of them per lookup), else looked up in memory each time.
+constexpr int kBook = 512;
+struct Book {
+  int2* seq;                               // row | q_len << 16, len
+  int* group;                              // starts
+  int* prefix;                             // tokens
+  bool kept;
+  __device__ __forceinline__ Seq get(const CachedCall& a, int b) const {
+    if (!kept) return cached_seq(a, b);
+    const int2 x = seq[b];
+    return Seq{x.x & 0xFFFF, x.y, x.x >> 16};
+  }
+  __device__ __forceinline__ int start(const CachedCall& a, int g) const { return kept ? group[g] : group_start(a, g); }
+  __device__ __forceinline__ int tokens(const CachedCall& a, int g) const { return kept ? prefix[g] : prefix_tokens(a, g); }
+};
+__device__ void fill_book(const CachedCall& a, const Book& k) {
+  if (!k.kept) return;
+  for (int i = threadIdx.x; i < a.n_seqs; i += kCachedThreads) {
+    const Seq s = cached_seq(a, i);
+    k.seq[i] = make_int2(s.row | s.q_len << 16, s.len);
+  }
+  for (int i = threadIdx.x; i <= a.n_groups && a.n_groups; i += kCachedThreads) {
+    k.group[i] = group_start(a, i);
+    if (i < a.n_groups) k.prefix[i] = prefix_tokens(a, i);
+  }
+  __syncthreads();
+}
+
 struct Entry {
   int rows, tiles, items, units;           // query rows, row tiles, items (tiles of every K/V head), units of each
   int from, to;                            // keys
   int first, group;                        // batch entry that the keys belong to; own part: its group
   Seq seq;                                 // of `first`
 };
-template <bool PREFIX, int MODE, class Start>
-__device__ __forceinline__ Entry cached_entry(const CachedCall& a, int e, Start start) {
+template <bool PREFIX, int MODE>
+__device__ __forceinline__ Entry cached_entry(const CachedCall& a, const Book& book, int e) {
   Entry r;
   const int per = a.tokens * (a.heads / a.kv_heads);
   r.from = 0;
   if constexpr (PREFIX) {
-    r.first = start(e);
-    r.rows = max(start(e + 1) - r.first, 0) * per;
+    r.first = book.start(a, e);
+    r.rows = max(book.start(a, e + 1) - r.first, 0) * per;
     r.group = e;
-    r.seq = cached_seq(a, min(r.first, a.n_seqs - 1));
-    r.to = r.rows ? min(prefix_tokens(a, e), r.seq.len) : 0;
+    r.seq = book.get(a, min(r.first, a.n_seqs - 1));
+    r.to = r.rows ? min(book.tokens(a, e), r.seq.len) : 0;
   } else {
     r.first = e;
     r.rows = per;
-    r.seq = cached_seq(a, e);
-    r.group = group_of(a.n_groups, e, start);
-    if (r.group >= 0) r.from = prefix_tokens(a, r.group);
+    r.seq = book.get(a, e);
+    r.group = group_of(a.n_groups, e, [&](int g) { return book.start(a, g); });
+    if (r.group >= 0) r.from = book.tokens(a, r.group);
     r.to = r.seq.len;
   }
   r.tiles = (r.rows + mode_rows(MODE) - 1) / mode_rows(MODE);
@@ -396,8 +425,8 @@ __device__ __forceinline__ int wave_scan(int x) {
 struct Scan {
   int e0, e1, units, own, items, total;
 };
-template <bool PREFIX, int MODE, class Start>
-__device__ Scan cached_scan(const CachedCall& a, int (&shared)[2][kCachedWaves], Start start) {
+template <bool PREFIX, int MODE>
+__device__ Scan cached_scan(const CachedCall& a, const Book& book, int (&shared)[2][kCachedWaves]) {
   const int n = PREFIX ? a.n_groups : a.n_seqs, per = (n + kCachedThreads - 1) / kCachedThreads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Scan r;
@@ -405,7 +434,7 @@ __device__ Scan cached_scan(const CachedCall& a, int (&shared)[2][kCachedWaves],
   r.e1 = min(r.e0 + per, n);
   int u = 0, it = 0;
   for (int e = r.e0; e < r.e1; ++e) {
-    const Entry x = cached_entry<PREFIX, MODE>(a, e, start);
+    const Entry x = cached_entry<PREFIX, MODE>(a, book, e);
     u += x.items * x.units;
     it += x.items;
   }
@@ -452,12 +481,12 @@ __device__ __forceinline__ u32x4 page_rows(const CachedCall& a, int id, int64_t 
 
 // Query row rr of an item: its place in q, and the keys it sees.
 template <bool PREFIX>
-__device__ __forceinline__ const uint16_t* cached_query(const CachedCall& a, const Entry& x, int kvh, int rr, int& seen) {
+__device__ __forceinline__ const uint16_t* cached_query(const CachedCall& a, const Book& book, const Entry& x, int kvh, int rr, int& seen) {
   const int G = a.heads / a.kv_heads, per = a.tokens * G;
   const bool good = rr < x.rows;
   const int b = PREFIX && good ? x.first + rr / per : min(x.first, a.n_seqs - 1), t = good ? rr % per / G : 0, h = kvh * G + rr % G;
   if constexpr (PREFIX) {
-    const Seq s = cached_seq(a, b);
+    const Seq s = book.get(a, b);
     seen = good ? row_sees(s.len, s.q_len, t) : 0;
   } else {
     seen = good ? row_sees(x.seq.len, x.seq.q_len, t) : 0;
@@ -467,7 +496,7 @@ __device__ __forceinline__ const uint16_t* cached_query(const CachedCall& a, con
 
 // One item's keys [from, to) (from a multiple of 16) into a partial result, the keys split over the waves.
 template <bool BF, int DP, int MT, bool PREFIX>
-__device__ void split_keys(const CachedCall& a, char* lds, const Entry& x, int item, int from, int to, int slot) {
+__device__ void split_keys(const CachedCall& a, const Book& book, char* lds, const Entry& x, int item, int from, int to, int slot) {
   using E = Elem<BF>;
   constexpr int kRow = DP * 2;
   constexpr int kHalf = 16 * kRow;                       // 16 keys, always of one page
@@ -492,7 +521,7 @@ __device__ void split_keys(const CachedCall& a, char* lds, const Entry& x, int i
 #pragma unroll
   for (int rt = 0; rt < MT; ++rt) {
     const int rr = row0 + rt * 16 + n;
-    const uint16_t* qp = cached_query<PREFIX>(a, x, kvh, rr, seen[rt]);
+    const uint16_t* qp = cached_query<PREFIX>(a, book, x, kvh, rr, seen[rt]);
     if (rr < x.rows) all = min(all, seen[rt]);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -660,7 +689,7 @@ __device__ void split_keys(const CachedCall& a, char* lds, const Entry& x, int i
 
 // The same with the rows split over the waves, 32 each, and tiles of 64 keys shared by the block.
 template <bool BF, int DP, bool PREFIX>
-__device__ void split_rows(const CachedCall& a, char* lds, const Entry& x, int item, int from, int to, int slot) {
+__device__ void split_rows(const CachedCall& a, const Book& book, char* lds, const Entry& x, int item, int from, int to, int slot) {
   constexpr int kRow = DP * 2;
   constexpr int kTile = kPromptKeys * kRow;
   constexpr int kCopies = 16 * kRow / 1024, kCopyRows = 1024 / kRow;      // a wave copies 16 of the 64 keys
@@ -675,7 +704,7 @@ __device__ void split_rows(const CachedCall& a, char* lds, const Entry& x, int i
   pages.load(from >> a.page_log);
   RowTile<BF, DP> rt;
   int seen;
-  const uint16_t* qp = cached_query<PREFIX>(a, x, kvh, row0 + col, seen);
+  const uint16_t* qp = cached_query<PREFIX>(a, book, x, kvh, row0 + col, seen);
   rt.start(qp, row0 + col < x.rows, D, half);
   seen = min(seen, to);
   int all = row0 + col < x.rows ? seen : 0x7FFFFFFF;
@@ -736,9 +765,8 @@ __device__ void split_rows(const CachedCall& a, char* lds, const Entry& x, int i
 
 // The run of units of block `me` of `blocks`.
 template <bool BF, int DP, int MODE, bool PREFIX>
-__device__ void cached_run(const CachedCall& a, char* lds, const Scan& sc, int me, int blocks) {
+__device__ void cached_run(const CachedCall& a, const Book& book, char* lds, const Scan& sc, int me, int blocks) {
   __shared__ int found[4];
-  auto start = [&](int g) { return group_start(a, g); };
   if (me >= blocks) return;
   const int n = PREFIX ? a.n_groups : a.n_seqs;
   const int u = (int)((int64_t)me * sc.total / blocks), end = (int)((int64_t)(me + 1) * sc.total / blocks);
@@ -747,7 +775,7 @@ __device__ void cached_run(const CachedCall& a, char* lds, const Scan& sc, int m
   if (u >= sc.units && u < sc.units + sc.own) {          // one thread: its run of entries holds u
     int before = sc.units, items = sc.items;
     for (int e = sc.e0; e < sc.e1; ++e) {
-      const Entry x = cached_entry<PREFIX, MODE>(a, e, start);
+      const Entry x = cached_entry<PREFIX, MODE>(a, book, e);
       if (u < before + x.items * x.units) {
         found[0] = e;
         found[1] = u - before;
@@ -762,14 +790,14 @@ __device__ void cached_run(const CachedCall& a, char* lds, const Scan& sc, int m
   // (groups that are not in order can overflow the sums: what follows stays within the entries all the same)
   int e = min(max(__builtin_amdgcn_readfirstlane(found[0]), 0), n - 1), items = __builtin_amdgcn_readfirstlane(found[2]);
   const int in = max(__builtin_amdgcn_readfirstlane(found[1]), 0);
-  Entry x = cached_entry<PREFIX, MODE>(a, e, start);
+  Entry x = cached_entry<PREFIX, MODE>(a, book, e);
   if (x.units == 0 || x.items == 0) return;
   int item = min(in / x.units, x.items - 1), unit = in % x.units, left = end - u;
   while (true) {
     const int run = min(left, x.units - unit);
     const int from = x.from + unit * mode_unit(MODE), to = min(from + run * mode_unit(MODE), x.to);
-    if constexpr (MODE == kRows) split_rows<BF, DP, PREFIX>(a, lds, x, item, from, to, me + items + item);
-    else split_keys<BF, DP, MODE, PREFIX>(a, lds, x, item, from, to, me + items + item);
+    if constexpr (MODE == kRows) split_rows<BF, DP, PREFIX>(a, book, lds, x, item, from, to, me + items + item);
+    else split_keys<BF, DP, MODE, PREFIX>(a, book, lds, x, item, from, to, me + items + item);
     left -= run;
     if (left <= 0) break;
     unit = 0;
@@ -778,7 +806,7 @@ __device__ void cached_run(const CachedCall& a, char* lds, const Scan& sc, int m
       do {                                               // left > 0: a further entry has units
         items += x.items;
         if (++e >= n) return;
-        x = cached_entry<PREFIX, MODE>(a, e, start);
+        x = cached_entry<PREFIX, MODE>(a, book, e);
       } while (x.items == 0 || x.units == 0);
     }
   }
@@ -791,11 +819,14 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a
   __shared__ __attribute__((aligned(1024))) char lds[kBytes];
   __shared__ int shared[2][2][kCachedWaves];
   static_assert(kCachedWaves * (16 * (DP + 4) + 32 * 2) * 4 <= kStage, "the join fits the tiles' space");
-  auto start = [&](int g) { return group_start(a, g); };
-  const Scan own = cached_scan<false, OWN>(a, shared[0], start);
+  __shared__ int2 book_seq[kBook];
+  __shared__ int book_group[PRE == kNone ? 1 : kBook + 1], book_prefix[PRE == kNone ? 1 : kBook];
+  const Book book{book_seq, book_group, book_prefix, a.n_seqs <= kBook};
+  fill_book(a, book);
+  const Scan own = cached_scan<false, OWN>(a, book, shared[0]);
   Scan pre;
   pre.total = 0;
-  if constexpr (PRE != kNone) pre = cached_scan<true, PRE>(a, shared[1], start);
+  if constexpr (PRE != kNone) pre = cached_scan<true, PRE>(a, book, shared[1]);
 
   // blocks for the prefixes: their share of the keys' cost
   int n_pre = 0;
@@ -814,7 +845,7 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a
     JoinEntry* je = reinterpret_cast<JoinEntry*>(a.join + 4);
     int u = own.units, it = own.items;
     for (int e = own.e0; e < own.e1; ++e) {
-      const Entry x = cached_entry<false, OWN>(a, e, start);
+      const Entry x = cached_entry<false, OWN>(a, book, e);
       je[e] = JoinEntry{u, it, x.units, x.tiles, x.group, x.first};
       u += x.items * x.units;
       it += x.items;
@@ -823,7 +854,7 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a
       u = pre.units;
       it = pre.items;
       for (int e = pre.e0; e < pre.e1; ++e) {
-        const Entry x = cached_entry<true, PRE>(a, e, start);
+        const Entry x = cached_entry<true, PRE>(a, book, e);
         je[a.n_seqs + e] = JoinEntry{u, it, x.units, x.tiles, e, x.first};
         u += x.items * x.units;
         it += x.items;
@@ -834,11 +865,11 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a
   const int xcd = blockIdx.x % kXcds, at = blockIdx.x / kXcds, pre_each = n_pre / kXcds;
   if constexpr (PRE != kNone) {
     if (at < pre_each) {
-      cached_run<BF, DP, PRE, true>(a, lds, pre, xcd * pre_each + at, pre_blocks);
+      cached_run<BF, DP, PRE, true>(a, book, lds, pre, xcd * pre_each + at, pre_blocks);
       return;
     }
   }
-  cached_run<BF, DP, OWN, false>(a, lds, own, xcd * (kCachedBlocks / kXcds - pre_each) + at - pre_each, own_blocks);
+  cached_run<BF, DP, OWN, false>(a, book, lds, own, xcd * (kCachedBlocks / kXcds - pre_each) + at - pre_each, own_blocks);
 }
 
 // One wave per (sequence, token, head): the partial results of its row, from the prefix and the own part.
@@ -872,16 +903,16 @@ __global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, int
       y1 *= f;
       m = top;
       const int k = min(64, n - c0);
-      for (int i = 0; i < k; i += 4) {                   // four slots' loads at a time
-        float z0[4], z1[4];
+      for (int i = 0; i < k; i += 8) {                   // eight slots' loads at a time
+        float z0[8], z1[8];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
+        for (int v = 0; v < 8; ++v) {
           const float* p = po + (int64_t)(c0 + min(i + v, k - 1)) * ps.stride * D;
           z0[v] = lane < D ? p[lane] : 0.0f;
           z1[v] = lane + 64 < D ? p[lane + 64] : 0.0f;
         }
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
+        for (int v = 0; v < 8; ++v) {
           const float wi = i + v < k ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), min(i + v, 63))) : 0.0f;
           if (i + v < k) {
             y0 = __builtin_fmaf(z0[v], wi, y0);
