@@ -132,6 +132,26 @@ __device__ __forceinline__ float wave_max(float x) {
   return x;
 }
 
+// Maximum and sum over lanes l and l ^ 32: swapping the halves of two copies gives (low, low) and (high, high).
+// (The results go through scalars: a bit cast of a vector's element takes the vector's first.)
+__device__ __forceinline__ void both_halves(float x, float& low, float& high) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t a = r[0], b = r[1];
+  low = __builtin_bit_cast(float, a);
+  high = __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float half_max(float x) {
+  float low, high;
+  both_halves(x, low, high);
+  return fmaxf(low, high);
+}
+__device__ __forceinline__ float half_sum(float x) {
+  float low, high;
+  both_halves(x, low, high);
+  return low + high;
+}
+
 // One row by a plain loop over its `seen` keys (one wave; lane l ends with o for dims l and l + 64). The tile
 // kernels multiply keys that a row does not see by weights of 0, which is not 0 where V holds an infinity
 // or a NaN: rows that come out not finite are computed again here, where unseen keys are never read.

@@ -20,6 +20,12 @@
 #include "mtc_host.h"
 #include "mtc_serve.h"
 
+#ifndef MTC_MIN_ROWS
+#define MTC_MIN_ROWS 8
+#define MTC_MIN_KEYS 1
+#define MTC_COST_ROWS 1.0f
+#define MTC_COST_KEYS 6.0f
+#endif
 #define MTC_API extern "C" __attribute__((visibility("default")))
 
 using mtc::host::check_launch;
@@ -92,11 +98,6 @@ __device__ PromptTile prompt_tile(const mtc_prompt_args& a, int rank) {
   }
   prompt_range(a.cu_q, seq, a.q_rows, r.q0, r.n);
   prompt_range(a.cu_k, seq, a.k_rows, r.k0, r.m);
-  r.tile = __builtin_amdgcn_readfirstlane(r.tile);
-  r.q0 = __builtin_amdgcn_readfirstlane(r.q0);
-  r.n = __builtin_amdgcn_readfirstlane(r.n);
-  r.k0 = __builtin_amdgcn_readfirstlane(r.k0);
-  r.m = __builtin_amdgcn_readfirstlane(r.m);
   return r;
 }
 
@@ -108,7 +109,8 @@ struct RowTile {
   static constexpr int kSteps = DP / 16;
   u32x4 qf[kSteps];
   f32x16 o[DP / 32];
-  float top, sum;                    // running maximum (times c), this lane's share of the sum
+  static constexpr float kLag = 8.0f;
+  float top, sum;                    // running maximum (times c; up to kLag behind), this lane's share of the sum
 
   __device__ __forceinline__ void start(const uint16_t* qp, bool good, int D, int half) {
 #pragma unroll
@@ -122,34 +124,40 @@ struct RowTile {
     sum = 0.0f;
   }
 
-  // left: keys of the tile that this lane's row sees, used if `masked`
-  __device__ __forceinline__ void step(const char* kt, const char* vt, float c, bool masked, int left) {
+  // left (MASKED): keys of the tile that this lane's row sees
+  template <bool MASKED>
+  __device__ __forceinline__ void step(const char* kt, const char* vt, float c, int left) {
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
     for (int st = 0; st < kSteps; ++st)
 #pragma unroll
       for (int g = 0; g < 2; ++g) s[g] = E::mfma32(read_k<DP>(kt, g * 32 + col, 2 * st + half), qf[st], s[g]);
-    if (masked) {
+    if constexpr (MASKED) {
+      left -= 4 * half;
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (g * 32 + 8 * (e >> 2) + (e & 3) >= left - 4 * half) s[g][e] = -INFINITY;
+          if (g * 32 + 8 * (e >> 2) + (e & 3) >= left) s[g][e] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[g][e]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32)) * c;
-    const float was = top;
-    top = fmaxf(top, mx);
-    const float base = top == -INFINITY ? 0.0f : top;
-    const float fade = exp2_fast(was - base);
-    sum *= fade;
+    mx = half_max(mx) * c;
+    // The maximum may lag: weights up to 2^kLag keep their relative precision in 16 bits, and the common factor
+    // drops out of the quotient. After the first tiles it seldom moves, which saves the pass over o.
+    if (__ballot(mx > top + kLag)) {
+      const float was = top;
+      top = fmaxf(top, mx);
+      const float fade = top == -INFINITY ? 1.0f : exp2_fast(was - top);
+      sum *= fade;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) o[d] *= fade;
+      for (int d = 0; d < DP / 32; ++d) o[d] *= fade;
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
     u32x4 p[4];
 #pragma unroll
     for (int g = 0; g < 2; ++g)
@@ -186,10 +194,15 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
   // count of K/V heads is a multiple or a divisor of 8
   const int j = blockIdx.x % H;
   const int kvh = j % KV, head = kvh * (H / KV) + j / KV;
-  const PromptTile pt = prompt_tile(a, blockIdx.x / H);
+  PromptTile pt = prompt_tile(a, blockIdx.x / H);
+  pt.tile = __builtin_amdgcn_readfirstlane(pt.tile);      // the same in every lane: scalars from here on
+  pt.q0 = __builtin_amdgcn_readfirstlane(pt.q0);
+  pt.n = __builtin_amdgcn_readfirstlane(pt.n);
+  pt.k0 = __builtin_amdgcn_readfirstlane(pt.k0);
+  pt.m = __builtin_amdgcn_readfirstlane(pt.m);
   if (pt.tile < 0) return;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, col = lane & 31;
   const int row = pt.tile * kPromptRows + wave * 32 + col;         // this lane's query
   const int shift = pt.m - pt.n + 1;
@@ -232,16 +245,24 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
 
   const float c = a.scale * kLog2e;
   if (steps > 0) copy_tile(0);
-  for (int t = 0; t < steps; ++t) {
+  int t = 0;
+  auto next = [&]() {                              // tile t is there; nobody reads the other buffer any more
     wait_copies<0>();
-    lds_barrier();                                 // tile t is there; nobody reads the other buffer any more
+    lds_barrier();
     if (t + 1 < steps) copy_tile(t + 1);
-    if (t * kPromptKeys >= wave_keys) continue;
-    const char* kt = lds + (t & 1) * 2 * kTile;
-    rt.step(kt, kt + kTile, c, (t + 1) * kPromptKeys > all_keys, seen - t * kPromptKeys);
+    return lds + (t & 1) * 2 * kTile;
+  };
+  for (; (t + 1) * kPromptKeys <= all_keys; ++t) {           // every row sees every key
+    const char* kt = next();
+    rt.template step<false>(kt, kt + kTile, c, 0);
   }
+  for (; t * kPromptKeys < wave_keys; ++t) {
+    const char* kt = next();
+    rt.template step<true>(kt, kt + kTile, c, seen - t * kPromptKeys);
+  }
+  for (; t < steps; ++t) next();                   // keys for the other waves
 
-  const float sum = rt.sum + __shfl_xor(rt.sum, 32);
+  const float sum = half_sum(rt.sum);
   const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
   uint16_t* op = reinterpret_cast<uint16_t*>(a.o.data) + (int64_t)(pt.q0 + row) * a.o.row_stride +
                  (int64_t)head * a.o.head_stride;
@@ -304,8 +325,21 @@ struct Pass {                              // the own parts, or the prefixes
   float* ml;                               // [slot][stride][2]: maximum (times c), sum
   int32_t stride, slots;
 };
-struct JoinEntry {                         // what k_join needs of a sequence, or of a group
-  int32_t units_before, items_before, units, tiles, group, first;
+// Units dealt out to blocks: the first `rest` of them get each + 1, the others each.
+struct Deal {
+  int32_t each, rest;
+  __device__ __forceinline__ int start(int block) const { return block * each + min(block, rest); }
+  __device__ __forceinline__ int block_of(int unit) const {        // only where units were dealt: each + 1 > 0
+    const int big = rest * (each + 1);
+    return unit < big ? unit / (each + 1) : rest + (unit - big) / max(each, 1);
+  }
+};
+struct JoinPart {                          // what k_join needs of an entry
+  int32_t units_before, items_before, units, tiles;
+};
+struct JoinEntry {                         // of a sequence: its own part, its group's prefix (units 0: none)
+  JoinPart own, pre;
+  int32_t first, reserved;                 // first sequence of the group
 };
 struct CachedCall {
   const uint16_t* pool;
@@ -318,7 +352,7 @@ struct CachedCall {
   int32_t n_seqs, tokens, heads, n_groups;
   float c;
   Pass own, pre;
-  int32_t* join;                           // own units, own blocks, prefix units, prefix blocks; then the entries
+  int32_t* join;                           // Deal of the own parts, of the prefixes; then the entries
 };
 
 struct Seq {
@@ -505,7 +539,7 @@ __device__ void split_keys(const CachedCall& a, const Book& book, char* lds, con
   constexpr int kSteps = DP / 32;
   constexpr int kUnit = kCachedWaves * kWaveKeys;
   const Pass& ps = PREFIX ? a.pre : a.own;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, w = lane >> 4;
   const int D = a.dim;
   const int kvh = item / x.tiles, row0 = (item % x.tiles) * 16 * MT;
@@ -694,7 +728,7 @@ __device__ void split_rows(const CachedCall& a, const Book& book, char* lds, con
   constexpr int kTile = kPromptKeys * kRow;
   constexpr int kCopies = 16 * kRow / 1024, kCopyRows = 1024 / kRow;      // a wave copies 16 of the 64 keys
   const Pass& ps = PREFIX ? a.pre : a.own;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, col = lane & 31;
   const int D = a.dim;
   const int kvh = item / x.tiles, row0 = (item % x.tiles) * kManyRows + wave * 32;
@@ -735,17 +769,27 @@ __device__ void split_rows(const CachedCall& a, const Book& book, char* lds, con
   };
   const int steps = (to - from + kPromptKeys - 1) / kPromptKeys;
   copy_tile(0);
-  for (int t = 0; t < steps; ++t) {
+  int t = 0;
+  auto next = [&]() {
     wait_copies<0>();
     lds_barrier();
     if (t + 1 < steps) copy_tile(t + 1);
-    const char* kt = lds + (t & 1) * 2 * kTile;
-    const int at = from + t * kPromptKeys;
-    if (busy) rt.step(kt, kt + kTile, a.c, at + kPromptKeys > all, seen - at);
+    return lds + (t & 1) * 2 * kTile;
+  };
+  if (busy) {
+    for (; from + (t + 1) * kPromptKeys <= all; ++t) {
+      const char* kt = next();
+      rt.template step<false>(kt, kt + kTile, a.c, 0);
+    }
+    for (; t < steps; ++t) {
+      const char* kt = next();
+      rt.template step<true>(kt, kt + kTile, a.c, seen - from - t * kPromptKeys);
+    }
   }
+  for (; t < steps; ++t) next();
   lds_barrier();                                         // the next item may fill the tiles
   const int r = wave * 32 + col;
-  rt.sum += __shfl_xor(rt.sum, 32);
+  rt.sum = half_sum(rt.sum);
   if (slot >= 0 && slot < ps.slots && row0 + col < x.rows) {
     float* po = ps.part + ((int64_t)slot * ps.stride + r) * D;
 #pragma unroll
@@ -765,11 +809,11 @@ __device__ void split_rows(const CachedCall& a, const Book& book, char* lds, con
 
 // The run of units of block `me` of `blocks`.
 template <bool BF, int DP, int MODE, bool PREFIX>
-__device__ void cached_run(const CachedCall& a, const Book& book, char* lds, const Scan& sc, int me, int blocks) {
+__device__ void cached_run(const CachedCall& a, const Book& book, char* lds, const Scan& sc, const Deal& deal, int me, int blocks) {
   __shared__ int found[4];
   if (me >= blocks) return;
   const int n = PREFIX ? a.n_groups : a.n_seqs;
-  const int u = (int)((int64_t)me * sc.total / blocks), end = (int)((int64_t)(me + 1) * sc.total / blocks);
+  const int u = deal.start(me);
   if (threadIdx.x < 3) found[threadIdx.x] = 0;
   __syncthreads();
   if (u >= sc.units && u < sc.units + sc.own) {          // one thread: its run of entries holds u
@@ -792,7 +836,7 @@ __device__ void cached_run(const CachedCall& a, const Book& book, char* lds, con
   const int in = max(__builtin_amdgcn_readfirstlane(found[1]), 0);
   Entry x = cached_entry<PREFIX, MODE>(a, book, e);
   if (x.units == 0 || x.items == 0) return;
-  int item = min(in / x.units, x.items - 1), unit = in % x.units, left = end - u;
+  int item = min(in / x.units, x.items - 1), unit = in % x.units, left = deal.each + (me < deal.rest);
   while (true) {
     const int run = min(left, x.units - unit);
     const int from = x.from + unit * mode_unit(MODE), to = min(from + run * mode_unit(MODE), x.to);
@@ -812,6 +856,18 @@ __device__ void cached_run(const CachedCall& a, const Book& book, char* lds, con
   }
 }
 
+// Cost of a unit, for dealing blocks to the prefixes and the own parts; least units per block.
+__host__ __device__ constexpr float mode_cost(int mode) { return mode == kRows ? MTC_COST_ROWS : MTC_COST_KEYS; }
+__device__ __forceinline__ int deal_blocks(int blocks, int units, int mode) {
+  const int least = mode == kRows ? MTC_MIN_ROWS : MTC_MIN_KEYS;
+  return min(blocks, (units + least - 1) / least);
+}
+// Run of the at-th of `each` blocks of an XCD: XCD after XCD in consecutive runs, as many on each.
+__device__ __forceinline__ int spread(int xcd, int at, int each, int runs) {
+  const int per = (runs + kXcds - 1) / kXcds;
+  return at < per ? xcd * per + at : runs;
+}
+
 template <bool BF, int DP, int OWN, int PRE>
 __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a) {
   constexpr int kStage = kCachedWaves * 2 * kWaveKeys * DP * 2;     // = 2 buffers of K and V tiles of 64 keys for split rows, halved
@@ -828,111 +884,114 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a
   pre.total = 0;
   if constexpr (PRE != kNone) pre = cached_scan<true, PRE>(a, book, shared[1]);
 
-  // blocks for the prefixes: their share of the keys' cost
+  // blocks for the prefixes: their share of the cost
   int n_pre = 0;
   if constexpr (PRE != kNone) {
-    const float wp = (float)pre.total * mode_unit(PRE), wo = (float)own.total * mode_unit(OWN);
+    const float wp = (float)pre.total * mode_cost(PRE), wo = (float)own.total * mode_cost(OWN);
     if (pre.total) n_pre = own.total ? min(max((int)(kCachedBlocks / kXcds * wp / (wp + wo) + 0.5f), 1), kCachedBlocks / kXcds - 1) * kXcds : kCachedBlocks;
   }
-  const int pre_blocks = min(n_pre, pre.total), own_blocks = min(kCachedBlocks - n_pre, own.total);
-  if (blockIdx.x == 0) {                                 // for k_join
+  const int pre_blocks = deal_blocks(n_pre, pre.total, PRE), own_blocks = deal_blocks(kCachedBlocks - n_pre, own.total, OWN);
+  auto deal = [](int units, int blocks) { return Deal{units / max(blocks, 1), units % max(blocks, 1)}; };
+  const Deal own_deal = deal(own.total, own_blocks), pre_deal = deal(pre.total, pre_blocks);
+  if (blockIdx.x == kCachedBlocks - 1) {                 // for k_join
     if (threadIdx.x == 0) {
-      a.join[0] = own.total;
-      a.join[1] = own_blocks;
-      a.join[2] = pre.total;
-      a.join[3] = pre_blocks;
+      reinterpret_cast<Deal*>(a.join)[0] = own_deal;
+      reinterpret_cast<Deal*>(a.join)[1] = pre_deal;
     }
     JoinEntry* je = reinterpret_cast<JoinEntry*>(a.join + 4);
-    int u = own.units, it = own.items;
-    for (int e = own.e0; e < own.e1; ++e) {
-      const Entry x = cached_entry<false, OWN>(a, book, e);
-      je[e] = JoinEntry{u, it, x.units, x.tiles, x.group, x.first};
-      u += x.items * x.units;
-      it += x.items;
-    }
+    JoinPart* jg = reinterpret_cast<JoinPart*>(je + a.n_seqs);      // the groups' parts, until the sequences have them
+    int u, it;
     if constexpr (PRE != kNone) {
       u = pre.units;
       it = pre.items;
       for (int e = pre.e0; e < pre.e1; ++e) {
         const Entry x = cached_entry<true, PRE>(a, book, e);
-        je[a.n_seqs + e] = JoinEntry{u, it, x.units, x.tiles, e, x.first};
+        jg[e] = JoinPart{u, it, x.units, x.tiles};
         u += x.items * x.units;
         it += x.items;
       }
+      __syncthreads();
+    }
+    u = own.units;
+    it = own.items;
+    for (int e = own.e0; e < own.e1; ++e) {
+      const Entry x = cached_entry<false, OWN>(a, book, e);
+      je[e].own = JoinPart{u, it, x.units, x.tiles};
+      je[e].pre = PRE != kNone && x.group >= 0 ? jg[x.group] : JoinPart{0, 0, 0, 0};
+      je[e].first = PRE != kNone && x.group >= 0 ? book.start(a, x.group) : 0;
+      u += x.items * x.units;
+      it += x.items;
     }
   }
   // consecutive runs on one XCD: row tiles that read the same keys then share its L2
   const int xcd = blockIdx.x % kXcds, at = blockIdx.x / kXcds, pre_each = n_pre / kXcds;
   if constexpr (PRE != kNone) {
     if (at < pre_each) {
-      cached_run<BF, DP, PRE, true>(a, book, lds, pre, xcd * pre_each + at, pre_blocks);
+      cached_run<BF, DP, PRE, true>(a, book, lds, pre, pre_deal, spread(xcd, at, pre_each, pre_blocks), pre_blocks);
       return;
     }
   }
-  cached_run<BF, DP, OWN, false>(a, book, lds, own, xcd * (kCachedBlocks / kXcds - pre_each) + at - pre_each, own_blocks);
+  cached_run<BF, DP, OWN, false>(a, book, lds, own, own_deal, spread(xcd, at - pre_each, kCachedBlocks / kXcds - pre_each, own_blocks), own_blocks);
 }
 
-// One wave per (sequence, token, head): the partial results of its row, from the prefix and the own part.
-template <bool BF>
+// One wave per (sequence, token, head): the partial results of its row, the prefix's and the own part's. A lane holds
+// four dims: a quarter (DP 64) or half of the wave reads one slot's row, so one load covers several slots.
+template <bool BF, int DP>
 __global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, int own_rows, int pre_rows) {
+  constexpr int kLanes = DP / 4, kPer = 64 / kLanes, kBatch = 8;      // lanes and slots per load, loads in flight
   const int b = blockIdx.x, lane = threadIdx.x & 63;
   const int G = a.heads / a.kv_heads, D = a.dim;
-  const int row = blockIdx.y * kCachedWaves + (threadIdx.x >> 6);   // t * heads + h
+  const int row = blockIdx.y * kCachedWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // t * heads + h
   if (row >= a.tokens * a.heads) return;
   const int t = row / a.heads, h = row % a.heads, kvh = h / G;
-  const JoinEntry* je = reinterpret_cast<const JoinEntry*>(a.join + 4);
-  const JoinEntry own = je[b];
-  float m = -INFINITY, l = 0.0f, y0 = 0.0f, y1 = 0.0f;
-  auto add = [&](const Pass& ps, const JoinEntry& x, int tile_rows, int rr, int total, int blocks) {
-    if (x.units == 0) return;
+  const Deal* deals = reinterpret_cast<const Deal*>(a.join);
+  const JoinEntry je = reinterpret_cast<const JoinEntry*>(a.join + 4)[b];
+  const int sub = lane / kLanes, dim = lane % kLanes * 4;
+  float m = -INFINITY, l = 0.0f;
+  f32x4 y = f32x4{};
+  auto add = [&](const Pass& ps, const JoinPart& x, int tile_rows, int rr, const Deal& deal) {
+    if (x.units <= 0) return;
     const int item = kvh * x.tiles + rr / tile_rows, r = rr % tile_rows;
-    const int64_t u0 = x.units_before + (int64_t)item * x.units;
-    const int i0 = (int)(((u0 + 1) * blocks - 1) / total), i1 = (int)(((u0 + x.units) * blocks - 1) / total);
-    const int64_t s0 = (int64_t)i0 + x.items_before + item;
-    const int n = s0 < 0 ? 0 : (int)min((int64_t)(i1 - i0 + 1), ps.slots - s0);
-    const float* pm = ps.ml + (s0 * ps.stride + r) * 2;
-    const float* po = ps.part + (s0 * ps.stride + r) * D;
-    for (int c0 = 0; c0 < n; c0 += 64) {                 // one slot per lane: maximum, weights, sum
-      const bool in = c0 + lane < n;
-      const float sm = in ? pm[(int64_t)(c0 + lane) * ps.stride * 2] : -INFINITY;
-      const float sl = in ? pm[(int64_t)(c0 + lane) * ps.stride * 2 + 1] : 0.0f;
-      const float top = fmaxf(m, wave_max(sm)), base = top == -INFINITY ? 0.0f : top;
-      const float f = exp2_fast(m - base), w = exp2_fast(sm - base);
-      l = l * f + wave_sum(sl * w);
-      y0 *= f;
-      y1 *= f;
+    const int u0 = x.units_before + item * x.units;
+    const int i0 = deal.block_of(u0), i1 = deal.block_of(u0 + x.units - 1), s0 = i0 + x.items_before + item;
+    const int n = s0 < 0 ? 0 : min(i1 - i0 + 1, ps.slots - s0);
+    const float* pm = ps.ml + ((int64_t)s0 * ps.stride + r) * 2;
+    const float* po = ps.part + ((int64_t)s0 * ps.stride + r) * D + dim;
+    const int64_t step = (int64_t)ps.stride * D;
+    for (int c0 = 0; c0 < n; c0 += 64) {                 // one slot per lane: maximum, weight, sum
+      float2 ml = make_float2(-INFINITY, 0.0f);
+      if (c0 + lane < n) ml = *reinterpret_cast<const float2*>(pm + (int64_t)(c0 + lane) * ps.stride * 2);
+      const float top = fmaxf(m, wave_max(ml.x)), base = top == -INFINITY ? 0.0f : top;
+      const float f = exp2_fast(m - base), w = exp2_fast(ml.x - base);
+      l = l * f + wave_sum(ml.y * w);
+      y *= f;
       m = top;
       const int k = min(64, n - c0);
-      for (int i = 0; i < k; i += 8) {                   // eight slots' loads at a time
-        float z0[8], z1[8];
+      for (int i = 0; i < k; i += kPer * kBatch) {
+        f32x4 z[kBatch];
 #pragma unroll
-        for (int v = 0; v < 8; ++v) {
-          const float* p = po + (int64_t)(c0 + min(i + v, k - 1)) * ps.stride * D;
-          z0[v] = lane < D ? p[lane] : 0.0f;
-          z1[v] = lane + 64 < D ? p[lane + 64] : 0.0f;
+        for (int v = 0; v < kBatch; ++v) {
+          const int at = i + v * kPer + sub;
+          z[v] = at < k && dim < D ? *reinterpret_cast<const f32x4*>(po + (c0 + at) * step) : f32x4{};
         }
 #pragma unroll
-        for (int v = 0; v < 8; ++v) {
-          const float wi = i + v < k ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), min(i + v, 63))) : 0.0f;
-          if (i + v < k) {
-            y0 = __builtin_fmaf(z0[v], wi, y0);
-            y1 = __builtin_fmaf(z1[v], wi, y1);
-          }
-        }
+        for (int v = 0; v < kBatch; ++v) y += z[v] * __shfl(w, min(i + v * kPer + sub, 63));
       }
     }
   };
-  if (own.group >= 0) {
-    const JoinEntry pre = je[a.n_seqs + own.group];
-    add(a.pre, pre, pre_rows, ((b - pre.first) * a.tokens + t) * G + h % G, a.join[2], a.join[3]);
-  }
-  add(a.own, own, own_rows, t * G + h % G, a.join[0], a.join[1]);
+  add(a.pre, je.pre, max(pre_rows, 1), ((b - je.first) * a.tokens + t) * G + h % G, deals[1]);
+  add(a.own, je.own, own_rows, t * G + h % G, deals[0]);
+#pragma unroll
+  for (int d = kLanes; d < 64; d <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] += __shfl_xor(y[i], d);
   const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-  y0 *= inv;
-  y1 *= inv;
-  if (__ballot(!finite(y0) || !finite(y1))) {
+  y *= inv;
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.o.data) + ((int64_t)b * a.tokens + t) * a.o.row_stride + (int64_t)h * a.o.head_stride;
+  if (__ballot(!(finite(y[0]) && finite(y[1]) && finite(y[2]) && finite(y[3])))) {
     const Seq s = cached_seq(a, b);
     const int32_t* table = a.table + (int64_t)s.row * a.max_pages;
+    float y0, y1;
     plain_row<BF>(reinterpret_cast<const uint16_t*>(a.q.data) + ((int64_t)b * a.tokens + t) * a.q.row_stride + (int64_t)h * a.q.head_stride,
                   D, row_sees(s.len, s.q_len, t), a.c,
                   [&](int key, const uint16_t*& k, const uint16_t*& v) {
@@ -943,10 +1002,11 @@ __global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, int
                     v = p + a.v_off;
                   },
                   y0, y1);
+    if (lane < D) out[lane] = Elem<BF>::round(y0);
+    if (lane + 64 < D) out[lane + 64] = Elem<BF>::round(y1);
+    return;
   }
-  uint16_t* out = reinterpret_cast<uint16_t*>(a.o.data) + ((int64_t)b * a.tokens + t) * a.o.row_stride + (int64_t)h * a.o.head_stride;
-  if (lane < D) out[lane] = Elem<BF>::round(y0);
-  if (lane + 64 < D) out[lane + 64] = Elem<BF>::round(y1);
+  if (sub == 0 && dim < D) *reinterpret_cast<u32x2*>(out + dim) = u32x2{Elem<BF>::pack(y[0], y[1]), Elem<BF>::pack(y[2], y[3])};
 }
 
 // ---------------------------------------------------------------------------
@@ -1023,7 +1083,7 @@ int plan_cached(const mtc_cache_desc* c, const mtc_cached_args* a, CachedPlan* p
                 c->page_size, (int)tiles(per, p->own_mode));
   p->own_bytes = round_up((size_t)p->own_slots * p->own_stride * (c->dim + 2) * 4, 256);
   p->pre_bytes = round_up((size_t)p->pre_slots * p->pre_stride * (c->dim + 2) * 4, 256);
-  p->join_bytes = round_up(16 + sizeof(JoinEntry) * ((size_t)a->n_seqs + a->n_groups), 256);
+  p->join_bytes = round_up(16 + sizeof(JoinEntry) * (size_t)a->n_seqs + sizeof(JoinPart) * (size_t)a->n_groups, 256);
   return MTC_OK;
 }
 
@@ -1046,7 +1106,8 @@ int run_cached(const CachedCall& a, const CachedPlan& p, hipStream_t st) {
   else launch_cached<BF, 128>(a, p.own_mode, p.pre_mode, st);
   if (int rc = check_launch("k_cached")) return rc;
   const dim3 grid(a.n_seqs, (a.tokens * a.heads + kCachedWaves - 1) / kCachedWaves);
-  k_join<BF><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_rows(p.pre_mode));
+  if (a.dim <= 64) k_join<BF, 64><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_rows(p.pre_mode));
+  else k_join<BF, 128><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_rows(p.pre_mode));
   return check_launch("k_join");
 }
 
