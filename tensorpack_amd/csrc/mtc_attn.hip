@@ -20,12 +20,6 @@
 #include "mtc_host.h"
 #include "mtc_serve.h"
 
-#ifndef MTC_MIN_ROWS
-#define MTC_MIN_ROWS 8
-#define MTC_MIN_KEYS 1
-#define MTC_COST_ROWS 1.0f
-#define MTC_COST_KEYS 6.0f
-#endif
 #define MTC_API extern "C" __attribute__((visibility("default")))
 
 using mtc::host::check_launch;
@@ -303,22 +297,35 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
 // own part (rows: its tokens x the heads of the K/V head) or of a group's prefix (rows: those of all members).
 // Items are cut into units of keys; the units of all items, in order, are dealt out to the blocks in
 // equal runs, so short and long sequences fill the chip alike and nothing on the host depends on lengths. A
-// run crosses items; each crossing gives one partial result (maximum, sum, weighted values). Its slot is block +
+// run crosses items; each crossing gives one partial result (maximum, sum, weighted values). Its slot is run +
 // item: both only grow along the runs and every crossing raises one of them, so no two share a slot.
 //
-// Two ways through an item's keys:
-//   split keys   16 or 32 rows; each wave takes 32 keys of its own, the four waves are joined at the end. For few rows
-//                the keys' bytes are all that counts, and every wave keeps its own loads in flight.
-//   split rows   up to 128 rows, 32 per wave, as in k_prompt: the waves share each tile of 64 keys in LDS
+// Three ways through an item's keys:
+//   split keys   16 or 32 rows, units of 32 keys: for few rows the keys' bytes are all that counts, and every wave keeps
+//                loads of its own in flight. A run belongs to a block, whose waves take every fourth unit and are joined
+//                at the end, or, where items are short, to a single wave (64 sequences of 100 keys, 8 K/V heads: an item
+//                takes a block or a wave about 5 us of waiting whatever its length)
+//   split rows   up to 128 rows, units of 64 keys, a run per block: as in k_prompt, 32 rows per wave, and the waves share
+//                each tile of keys in LDS
 constexpr int kCachedWaves = 4;
 constexpr int kCachedThreads = 64 * kCachedWaves;
 constexpr int kCachedBlocks = 512;         // two per CU
 constexpr int kXcds = 8;
 constexpr int kWaveKeys = 32;              // split keys: per wave and step
 constexpr int kManyRows = 128;             // split rows: rows of a tile
+#ifndef K_SHORT
+#define K_SHORT 8
+#define K_LEAST 4
+#define K_COSTROWS 2.2f
+#define K_COSTKEYS 1.45f
+#define K_COSTITEM 1.0f
+#endif
+constexpr int kShortItem = K_SHORT;              // split keys: up to as many units per item on average, runs of single waves
+constexpr int kLeastRows = K_LEAST;              // split rows: units of a run at least
+constexpr float kCostRows = K_COSTROWS, kCostKeys = K_COSTKEYS, kCostItem = K_COSTITEM;   // of a unit, of an item; for dealing blocks to prefixes and own parts
 enum { kNone = 0, kOneTile = 1, kTwoTiles = 2, kRows = 3 };      // 16 rows, 32 rows, split rows
 __host__ __device__ constexpr int mode_rows(int mode) { return mode == kRows ? kManyRows : 16 * mode; }
-__host__ __device__ constexpr int mode_unit(int mode) { return mode == kRows ? kPromptKeys : kCachedWaves * kWaveKeys; }
+__host__ __device__ constexpr int mode_unit(int mode) { return mode == kRows ? kPromptKeys : kWaveKeys; }
 
 struct Pass {                              // the own parts, or the prefixes
   float* part;                             // [slot][stride][dim]
@@ -457,7 +464,8 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 // Running sums over the entries: every thread of the block has the sums before its run of entries [e0, e1).
 struct Scan {
-  int e0, e1, units, own, items, total;
+  int e0, e1, units, own, items;
+  int total, all_items;
 };
 template <bool PREFIX, int MODE>
 __device__ Scan cached_scan(const CachedCall& a, const Book& book, int (&shared)[2][kCachedWaves]) {
@@ -481,7 +489,7 @@ __device__ Scan cached_scan(const CachedCall& a, const Book& book, int (&shared)
   r.own = u;
   r.units = su - u;
   r.items = si - it;
-  r.total = 0;
+  r.total = r.all_items = 0;
 #pragma unroll
   for (int w = 0; w < kCachedWaves; ++w) {
     if (w < wave) {
@@ -489,6 +497,7 @@ __device__ Scan cached_scan(const CachedCall& a, const Book& book, int (&shared)
       r.items += shared[1][w];
     }
     r.total += shared[0][w];
+    r.all_items += shared[1][w];
   }
   return r;
 }
@@ -528,16 +537,17 @@ __device__ __forceinline__ const uint16_t* cached_query(const CachedCall& a, con
   return reinterpret_cast<const uint16_t*>(a.q.data) + ((int64_t)b * a.tokens + t) * a.q.row_stride + (int64_t)h * a.q.head_stride;
 }
 
-// One item's keys [from, to) (from a multiple of 16) into a partial result, the keys split over the waves.
+// One item's keys [from, to) (from a multiple of 16) into a partial result, by the block (the keys split over its waves)
+// or by this wave alone.
 template <bool BF, int DP, int MT, bool PREFIX>
-__device__ void split_keys(const CachedCall& a, const Book& book, char* lds, const Entry& x, int item, int from, int to, int slot) {
+__device__ void split_keys(const CachedCall& a, const Book& book, char* lds, const Entry& x, int item, int from, int to, int slot, bool alone) {
   using E = Elem<BF>;
   constexpr int kRow = DP * 2;
   constexpr int kHalf = 16 * kRow;                       // 16 keys, always of one page
   constexpr int kHalfCopies = kHalf / 1024, kCopyRows = 1024 / kRow;
   constexpr int kTileCopies = 2 * kHalfCopies;
   constexpr int kSteps = DP / 32;
-  constexpr int kUnit = kCachedWaves * kWaveKeys;
+  const int stride = alone ? kWaveKeys : kCachedWaves * kWaveKeys;
   const Pass& ps = PREFIX ? a.pre : a.own;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, w = lane >> 4;
@@ -546,7 +556,7 @@ __device__ void split_keys(const CachedCall& a, const Book& book, char* lds, con
   const int rows = min(x.rows - row0, 16 * MT);
 
   PageWindow pages{a.table + (int64_t)x.seq.row * a.max_pages, 0, -1, a.max_pages};
-  int pos = from + kWaveKeys * wave;
+  int pos = alone ? from : from + kWaveKeys * wave;
   if (pos < to) pages.load(pos >> a.page_log);
 
   // this lane's query rows: 16 rt + n
@@ -604,7 +614,7 @@ __device__ void split_keys(const CachedCall& a, const Book& book, char* lds, con
     copy_keys(pos, a.v_off, v_lds, v_lane);
   }
   while (pos < to) {
-    const int next = pos + kUnit;
+    const int next = pos + stride;
     const bool more = next < to;
     wait_copies<kTileCopies>();                          // K is there
     f32x4 s[MT][2];
@@ -640,8 +650,7 @@ __device__ void split_keys(const CachedCall& a, const Book& book, char* lds, con
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][g][i]);
-      mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.c;
+      mx = half_max(fmaxf(mx, __shfl_xor(mx, 16))) * a.c;
       const float was = top[rt];
       top[rt] = fmaxf(was, mx);
       const float base = top[rt] == -INFINITY ? 0.0f : top[rt];
@@ -672,15 +681,27 @@ __device__ void split_keys(const CachedCall& a, const Book& book, char* lds, con
     pos = next;
   }
 
-  // join the four waves: element i of o[rt][d] is dim 16 d + 4 w + i of row 16 rt + n
+  // element i of o[rt][d] is dim 16 d + 4 w + i of row 16 rt + n
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt) sum[rt] = half_sum(sum[rt] + __shfl_xor(sum[rt], 16));
+  const bool store = slot >= 0 && slot < ps.slots;
+  if (alone) {
+#pragma unroll
+    for (int rt = 0; rt < MT; ++rt) {
+      const int r = rt * 16 + n;
+      if (!store || r >= rows) continue;
+      const int64_t at = (int64_t)slot * ps.stride + r;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+        if (d * 16 + 4 * w < D) *reinterpret_cast<f32x4*>(ps.part + at * D + d * 16 + 4 * w) = o[rt][d];
+      if (w == 0) *reinterpret_cast<float2*>(ps.ml + at * 2) = make_float2(top[rt], sum[rt]);
+    }
+    return;
+  }
+  // join the four waves
   constexpr int kPad = DP + 4;
   float* const buf = reinterpret_cast<float*>(lds);                 // [wave][16][kPad]
   float* const ml = buf + kCachedWaves * 16 * kPad;                 // [wave][16 MT][2]
-#pragma unroll
-  for (int rt = 0; rt < MT; ++rt) {
-    sum[rt] += __shfl_xor(sum[rt], 16);
-    sum[rt] += __shfl_xor(sum[rt], 32);
-  }
   __syncthreads();                                                  // every wave is done with its tiles
 #pragma unroll
   for (int rt = 0; rt < MT; ++rt)
@@ -689,7 +710,6 @@ __device__ void split_keys(const CachedCall& a, const Book& book, char* lds, con
       ml[(wave * 16 * MT + rt * 16 + n) * 2 + 1] = sum[rt];
     }
   __syncthreads();
-  const bool store = slot >= 0 && slot < ps.slots;
 #pragma unroll
   for (int rt = 0; rt < MT; ++rt) {
     const int r = rt * 16 + n;
@@ -807,23 +827,41 @@ __device__ void split_rows(const CachedCall& a, const Book& book, char* lds, con
   }
 }
 
-// The run of units of block `me` of `blocks`.
+// How the units of a pass are dealt out.
+struct Plan {
+  Deal deal;
+  int runs;
+  bool alone;                              // runs of single waves, not of blocks
+};
+__device__ __forceinline__ Plan deal_out(int units, int items, int blocks, int mode) {
+  Plan p;
+  p.alone = mode != kRows && units <= kShortItem * items;
+  const int least = mode == kRows ? kLeastRows : 1;
+  p.runs = min(p.alone ? blocks * kCachedWaves : blocks, (units + least - 1) / least);
+  p.deal.each = units / max(p.runs, 1);
+  p.deal.rest = units % max(p.runs, 1);
+  return p;
+}
+
+// The runs of block `me` of `blocks`.
 template <bool BF, int DP, int MODE, bool PREFIX>
-__device__ void cached_run(const CachedCall& a, const Book& book, char* lds, const Scan& sc, const Deal& deal, int me, int blocks) {
-  __shared__ int found[4];
-  if (me >= blocks) return;
+__device__ void cached_run(const CachedCall& a, const Book& book, char* lds, const Scan& sc, const Plan& plan, int me, int blocks) {
+  __shared__ int found[kCachedWaves][3];
   const int n = PREFIX ? a.n_groups : a.n_seqs;
-  const int u = deal.start(me);
-  if (threadIdx.x < 3) found[threadIdx.x] = 0;
+  const int wave = plan.alone ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  if (me >= plan.runs) return;                                       // its other waves' runs come after
+  if (threadIdx.x < 3 * kCachedWaves) (&found[0][0])[threadIdx.x] = 0;
   __syncthreads();
-  if (u >= sc.units && u < sc.units + sc.own) {          // one thread: its run of entries holds u
+  for (int k = 0; k < (plan.alone ? kCachedWaves : 1); ++k) {
+    const int run = me + k * blocks, u = plan.deal.start(run);
+    if (run >= plan.runs || u < sc.units || u >= sc.units + sc.own) continue;   // one thread: its run of entries holds u
     int before = sc.units, items = sc.items;
     for (int e = sc.e0; e < sc.e1; ++e) {
       const Entry x = cached_entry<PREFIX, MODE>(a, book, e);
       if (u < before + x.items * x.units) {
-        found[0] = e;
-        found[1] = u - before;
-        found[2] = items;
+        found[k][0] = e;
+        found[k][1] = u - before;
+        found[k][2] = items;
         break;
       }
       before += x.items * x.units;
@@ -831,18 +869,21 @@ __device__ void cached_run(const CachedCall& a, const Book& book, char* lds, con
     }
   }
   __syncthreads();
+  const int run = me + wave * blocks;
+  if (run >= plan.runs) return;
   // (groups that are not in order can overflow the sums: what follows stays within the entries all the same)
-  int e = min(max(__builtin_amdgcn_readfirstlane(found[0]), 0), n - 1), items = __builtin_amdgcn_readfirstlane(found[2]);
-  const int in = max(__builtin_amdgcn_readfirstlane(found[1]), 0);
+  int e = min(max(__builtin_amdgcn_readfirstlane(found[wave][0]), 0), n - 1), items = __builtin_amdgcn_readfirstlane(found[wave][2]);
+  const int in = max(__builtin_amdgcn_readfirstlane(found[wave][1]), 0);
+  int left = plan.deal.each + (run < plan.deal.rest);
   Entry x = cached_entry<PREFIX, MODE>(a, book, e);
   if (x.units == 0 || x.items == 0) return;
-  int item = min(in / x.units, x.items - 1), unit = in % x.units, left = deal.each + (me < deal.rest);
+  int item = min(in / x.units, x.items - 1), unit = in % x.units;
   while (true) {
-    const int run = min(left, x.units - unit);
-    const int from = x.from + unit * mode_unit(MODE), to = min(from + run * mode_unit(MODE), x.to);
-    if constexpr (MODE == kRows) split_rows<BF, DP, PREFIX>(a, book, lds, x, item, from, to, me + items + item);
-    else split_keys<BF, DP, MODE, PREFIX>(a, book, lds, x, item, from, to, me + items + item);
-    left -= run;
+    const int units = min(left, x.units - unit);
+    const int from = x.from + unit * mode_unit(MODE), to = min(from + units * mode_unit(MODE), x.to);
+    if constexpr (MODE == kRows) split_rows<BF, DP, PREFIX>(a, book, lds, x, item, from, to, run + items + item);
+    else split_keys<BF, DP, MODE, PREFIX>(a, book, lds, x, item, from, to, run + items + item, plan.alone);
+    left -= units;
     if (left <= 0) break;
     unit = 0;
     if (++item == x.items) {
@@ -856,15 +897,9 @@ __device__ void cached_run(const CachedCall& a, const Book& book, char* lds, con
   }
 }
 
-// Cost of a unit, for dealing blocks to the prefixes and the own parts; least units per block.
-__host__ __device__ constexpr float mode_cost(int mode) { return mode == kRows ? MTC_COST_ROWS : MTC_COST_KEYS; }
-__device__ __forceinline__ int deal_blocks(int blocks, int units, int mode) {
-  const int least = mode == kRows ? MTC_MIN_ROWS : MTC_MIN_KEYS;
-  return min(blocks, (units + least - 1) / least);
-}
 // Run of the at-th of `each` blocks of an XCD: XCD after XCD in consecutive runs, as many on each.
 __device__ __forceinline__ int spread(int xcd, int at, int each, int runs) {
-  const int per = (runs + kXcds - 1) / kXcds;
+  const int per = (min(runs, each * kXcds) + kXcds - 1) / kXcds;
   return at < per ? xcd * per + at : runs;
 }
 
@@ -881,22 +916,25 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a
   fill_book(a, book);
   const Scan own = cached_scan<false, OWN>(a, book, shared[0]);
   Scan pre;
-  pre.total = 0;
+  pre.total = pre.all_items = 0;
   if constexpr (PRE != kNone) pre = cached_scan<true, PRE>(a, book, shared[1]);
 
   // blocks for the prefixes: their share of the cost
   int n_pre = 0;
   if constexpr (PRE != kNone) {
-    const float wp = (float)pre.total * mode_cost(PRE), wo = (float)own.total * mode_cost(OWN);
+    auto cost = [](const Scan& sc, int mode) {
+      return mode == kRows ? sc.total * kCostRows : sc.total * kCostKeys + min(sc.total, sc.all_items) * kCostItem;
+    };
+    const float wp = cost(pre, PRE), wo = cost(own, OWN);
     if (pre.total) n_pre = own.total ? min(max((int)(kCachedBlocks / kXcds * wp / (wp + wo) + 0.5f), 1), kCachedBlocks / kXcds - 1) * kXcds : kCachedBlocks;
   }
-  const int pre_blocks = deal_blocks(n_pre, pre.total, PRE), own_blocks = deal_blocks(kCachedBlocks - n_pre, own.total, OWN);
-  auto deal = [](int units, int blocks) { return Deal{units / max(blocks, 1), units % max(blocks, 1)}; };
-  const Deal own_deal = deal(own.total, own_blocks), pre_deal = deal(pre.total, pre_blocks);
+  const Plan own_plan = deal_out(own.total, own.all_items, kCachedBlocks - n_pre, OWN);
+  Plan pre_plan = own_plan;
+  if constexpr (PRE != kNone) pre_plan = deal_out(pre.total, pre.all_items, n_pre, PRE);
   if (blockIdx.x == kCachedBlocks - 1) {                 // for k_join
     if (threadIdx.x == 0) {
-      reinterpret_cast<Deal*>(a.join)[0] = own_deal;
-      reinterpret_cast<Deal*>(a.join)[1] = pre_deal;
+      reinterpret_cast<Deal*>(a.join)[0] = own_plan.deal;
+      reinterpret_cast<Deal*>(a.join)[1] = pre_plan.deal;
     }
     JoinEntry* je = reinterpret_cast<JoinEntry*>(a.join + 4);
     JoinPart* jg = reinterpret_cast<JoinPart*>(je + a.n_seqs);      // the groups' parts, until the sequences have them
@@ -924,14 +962,14 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a
     }
   }
   // consecutive runs on one XCD: row tiles that read the same keys then share its L2
-  const int xcd = blockIdx.x % kXcds, at = blockIdx.x / kXcds, pre_each = n_pre / kXcds;
+  const int xcd = blockIdx.x % kXcds, at = blockIdx.x / kXcds, pre_each = n_pre / kXcds, own_each = kCachedBlocks / kXcds - pre_each;
   if constexpr (PRE != kNone) {
     if (at < pre_each) {
-      cached_run<BF, DP, PRE, true>(a, book, lds, pre, pre_deal, spread(xcd, at, pre_each, pre_blocks), pre_blocks);
+      cached_run<BF, DP, PRE, true>(a, book, lds, pre, pre_plan, spread(xcd, at, pre_each, pre_plan.runs), n_pre);
       return;
     }
   }
-  cached_run<BF, DP, OWN, false>(a, book, lds, own, own_deal, spread(xcd, at - pre_each, kCachedBlocks / kXcds - pre_each, own_blocks), own_blocks);
+  cached_run<BF, DP, OWN, false>(a, book, lds, own, own_plan, spread(xcd, at - pre_each, own_each, own_plan.runs), kCachedBlocks - n_pre);
 }
 
 // One wave per (sequence, token, head): the partial results of its row, the prefix's and the own part's. A lane holds
@@ -1070,14 +1108,15 @@ int plan_cached(const mtc_cache_desc* c, const mtc_cached_args* a, CachedPlan* p
   p->own_mode = mode_for(per);
   // groups are on the device: the rows of an average one decide
   p->pre_mode = a->n_groups ? mode_for(std::max<int64_t>(all / a->n_groups, 17)) : kNone;
+  auto runs = [](int mode) { return kCachedBlocks * (mode == kRows ? 1 : kCachedWaves); };
   auto tiles = [](int64_t rows, int mode) { return (rows + mode_rows(mode) - 1) / mode_rows(mode); };
   auto stride = [](int64_t rows, int mode) { return (int)std::min<int64_t>((rows + 15) / 16 * 16, mode_rows(mode)); };
   p->own_stride = stride(per, p->own_mode);
-  p->own_slots = kCachedBlocks + (int64_t)a->n_seqs * c->kv_heads * tiles(per, p->own_mode);
+  p->own_slots = runs(p->own_mode) + (int64_t)a->n_seqs * c->kv_heads * tiles(per, p->own_mode);
   p->pre_stride = p->pre_mode ? stride(all, p->pre_mode) : 0;
-  p->pre_slots = p->pre_mode ? kCachedBlocks + (int64_t)c->kv_heads * (tiles(all, p->pre_mode) + a->n_groups) : 0;
+  p->pre_slots = p->pre_mode ? runs(p->pre_mode) + (int64_t)c->kv_heads * (tiles(all, p->pre_mode) + a->n_groups) : 0;
   // the kernels count units in 32 bits
-  const int64_t units = (int64_t)c->max_pages * c->page_size / kPromptKeys + 1;
+  const int64_t units = (int64_t)c->max_pages * c->page_size / kWaveKeys + 1;
   if (units * (p->own_slots + p->pre_slots) > 0x7FFFFFFF)
     return fail(MTC_E_SHAPE, "%d sequences of up to %d pages of %d tokens, %d row tiles: too much for one call", a->n_seqs, c->max_pages,
                 c->page_size, (int)tiles(per, p->own_mode));
