@@ -102,6 +102,9 @@ template <int DP>
 __device__ __forceinline__ uint32_t v_key(uint32_t row) {
   return DP == 128 ? (row & 7u) << 1 : ((row >> 1) & 3u) << 1;
 }
+__device__ __forceinline__ u32x4 lds_read16(uint32_t at) {
+  return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)at;
+}
 template <int DP>
 __device__ __forceinline__ u32x4 read_k(const char* tile, uint32_t row, uint32_t piece) {
   return *reinterpret_cast<const u32x4*>(tile + row * (DP * 2) + ((piece ^ k_key<DP>(row)) << 4));
@@ -110,11 +113,16 @@ __device__ __forceinline__ u32x4 read_k(const char* tile, uint32_t row, uint32_t
 // Transposed read: of the 16 lanes that share `row4` (a multiple of 4) and `col16` (a multiple of 16), lane i gets
 // elements (row4 .. row4+3, col16 + i). Lane i fetches 8 bytes: row row4 + i/4, columns col16 + 4 (i%4).
 template <int DP>
-__device__ __forceinline__ u32x2 read_v(const char* tile, uint32_t row4, uint32_t col16, uint32_t i) {
+__device__ __forceinline__ uint32_t v_place(uint32_t row4, uint32_t col16, uint32_t i) {
   const uint32_t row = row4 + (i >> 2), col = col16 + 4 * (i & 3);
-  const char* p = tile + row * (DP * 2) + (((col >> 3) ^ v_key<DP>(row)) << 4) + (col & 7) * 2;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       (__attribute__((address_space(3))) s16x4*)(uintptr_t)lds_addr(p)));
+  return row * (DP * 2) + (((col >> 3) ^ v_key<DP>(row)) << 4) + (col & 7) * 2;
+}
+__device__ __forceinline__ u32x2 lds_read_transposed(uint32_t at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
+}
+template <int DP>
+__device__ __forceinline__ u32x2 read_v(const char* tile, uint32_t row4, uint32_t col16, uint32_t i) {
+  return lds_read_transposed(lds_addr(tile) + v_place<DP>(row4, col16, i));
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }

@@ -97,52 +97,70 @@ __device__ PromptTile prompt_tile(const mtc_prompt_args& a, int rank) {
 
 // 32 query rows of one wave (one per lane of either half) through tiles of 64 keys: S^T in two 32 x 32 blocks, O^T in
 // DP / 32. Element e of a block lies at row 8*(e/4) + 4*half + e%4 (key or dim), column `col` (query).
+//
+// The scores of the next tile are computed beside the weights of this one: the matrix core multiplies while the vector
+// unit takes exponentials, within one wave. Tiles go in pairs, so that the places in LDS are constants and the scores'
+// registers change roles instead of being copied.
 template <bool BF, int DP>
 struct RowTile {
   using E = Elem<BF>;
-  static constexpr int kSteps = DP / 16;
+  static constexpr int kSteps = DP / 16, kRow = DP * 2, kTile = kPromptKeys * kRow;
+  // The maximum may lag: weights up to 2^kLag keep their relative precision in 16 bits, and the common factor drops out
+  // of the quotient. After the first tiles it seldom moves, which saves the pass over o.
+  static constexpr float kLag = 8.0f;
   u32x4 qf[kSteps];
   f32x16 o[DP / 32];
-  static constexpr float kLag = 8.0f;
   float top, sum;                    // running maximum (times c; up to kLag behind), this lane's share of the sum
+  float mx;                          // of the scores whose weights come next, times c
+  uint32_t k_at[kSteps], v_at[DP / 32];   // this lane's places in tiles of even turn: keys at lds, values two tiles on
 
-  __device__ __forceinline__ void start(const uint16_t* qp, bool good, int D, int half) {
+  __device__ __forceinline__ void start(const uint16_t* qp, bool good, int D, const char* lds) {
+    const uint32_t lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, i16 = lane & 15, base = lds_addr(lds);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int d = 16 * s + 8 * half;
-      qf[s] = good && d < D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
+    for (int i = 0; i < kSteps; ++i) {
+      const int d = 16 * i + 8 * half;
+      qf[i] = good && d < D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
+      k_at[i] = base + col * kRow + (((2 * i + half) ^ k_key<DP>(col)) << 4);          // 32 rows on, the key is the same
     }
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
+    for (int d = 0; d < DP / 32; ++d) {
+      o[d] = f32x16{};
+      v_at[d] = base + 2 * kTile + v_place<DP>(4 * half, d * 32 + 16 * ((lane >> 4) & 1), i16);   // 8 rows on, too
+    }
     top = -INFINITY;
     sum = 0.0f;
   }
 
+  // Scores of the keys in the place `at` bytes on
+  __device__ __forceinline__ void multiply(uint32_t at, f32x16 (&r)[2]) const {
+    r[0] = r[1] = f32x16{};
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) r[g] = E::mfma32(lds_read16(k_at[i] + (at + g * 32 * kRow)), qf[i], r[g]);
+  }
   // left (MASKED): keys of the tile that this lane's row sees
   template <bool MASKED>
-  __device__ __forceinline__ void step(const char* kt, const char* vt, float c, int left) {
-    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
-    f32x16 s[2] = {f32x16{}, f32x16{}};
-#pragma unroll
-    for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-      for (int g = 0; g < 2; ++g) s[g] = E::mfma32(read_k<DP>(kt, g * 32 + col, 2 * st + half), qf[st], s[g]);
+  __device__ __forceinline__ void maximum(f32x16 (&s)[2], float c, int left) {
     if constexpr (MASKED) {
-      left -= 4 * half;
+      left -= 4 * ((threadIdx.x >> 5) & 1);
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (g * 32 + 8 * (e >> 2) + (e & 3) >= left) s[g][e] = -INFINITY;
     }
-    float mx = -INFINITY;
+    mx = -INFINITY;
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[g][e]);
     mx = half_max(mx) * c;
-    // The maximum may lag: weights up to 2^kLag keep their relative precision in 16 bits, and the common factor
-    // drops out of the quotient. After the first tiles it seldom moves, which saves the pass over o.
+  }
+
+  // Weights of s times the values `v` bytes on; NEXT: n becomes the scores of the keys `k` bytes on (MASKED, left: as above)
+  template <bool NEXT, bool MASKED>
+  __device__ __forceinline__ void step(f32x16 (&s)[2], f32x16 (&n)[2], uint32_t v, uint32_t k, float c, int left) {
     if (__ballot(mx > top + kLag)) {
       const float was = top;
       top = fmaxf(top, mx);
@@ -152,6 +170,7 @@ struct RowTile {
       for (int d = 0; d < DP / 32; ++d) o[d] *= fade;
     }
     const float base = top == -INFINITY ? 0.0f : top;
+    if constexpr (NEXT) multiply(k, n);
     u32x4 p[4];
 #pragma unroll
     for (int g = 0; g < 2; ++g)
@@ -166,11 +185,42 @@ struct RowTile {
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d) {
-        const uint32_t cl = d * 32 + 16 * ((lane >> 4) & 1);
-        const u32x2 lo = read_v<DP>(vt, ks * 16 + 4 * half, cl, lane & 15);
-        const u32x2 hi = read_v<DP>(vt, ks * 16 + 8 + 4 * half, cl, lane & 15);
+        const u32x2 lo = lds_read_transposed(v_at[d] + (v + ks * 16 * kRow));
+        const u32x2 hi = lds_read_transposed(v_at[d] + (v + (ks * 16 + 8) * kRow));
         o[d] = E::mfma32(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[ks], o[d]);
       }
+    if constexpr (NEXT) maximum<MASKED>(n, c, left);
+  }
+
+  // All tiles: `mine` of them have keys for this wave, of which all rows see the first `full` whole. first_keys() makes tile
+  // 0's keys readable, turn(t) tile t's values and tile t + 1's keys, and starts the copies of what comes after; left(t):
+  // keys of tile t that this lane's row sees.
+  template <class First, class Turn, class Left>
+  __device__ __forceinline__ void run(int tiles, int mine, int full, float c, First first_keys, Turn turn, Left left) {
+    if (tiles <= 0) return;
+    f32x16 a[2], b[2];
+    int t = 0;
+    first_keys();
+    if (mine > 0) {
+      multiply(0, a);
+      maximum<true>(a, c, left(0));
+      for (; t + 2 < full; t += 2) {
+        turn(t);
+        step<true, false>(a, b, 0, kTile, c, 0);
+        turn(t + 1);
+        step<true, false>(b, a, kTile, 0, c, 0);
+      }
+      for (; t + 1 < mine; ++t) {
+        turn(t);
+        step<true, true>(a, b, (t & 1) * kTile, ((t + 1) & 1) * kTile, c, left(t + 1));
+        a[0] = b[0];
+        a[1] = b[1];
+      }
+      turn(t);
+      step<false, false>(a, b, (t & 1) * kTile, 0, c, 0);
+      ++t;
+    }
+    for (; t < tiles; ++t) turn(t);                  // copies for the other waves
   }
 };
 
@@ -212,7 +262,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
   const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.data) + (int64_t)(pt.q0 + row) * a.q.row_stride +
                        (int64_t)head * a.q.head_stride;
   RowTile<BF, DP> rt;
-  rt.start(qp, row < pt.n, D, half);
+  rt.start(qp, row < pt.n, D, lds);
 
   const uint32_t k_bytes = (uint32_t)(a.k.row_stride * 2), v_bytes = (uint32_t)(a.v.row_stride * 2);
   const uint64_t k_base = (uint64_t)(uintptr_t)a.k.data + 2 * ((int64_t)pt.k0 * a.k.row_stride + (int64_t)kvh * a.k.head_stride);
@@ -226,35 +276,34 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
     v_off[i] = (int)vc * 8 < D ? r * v_bytes + vc * 16 : kOutOfRange;
   }
   const uint32_t lds0 = lds_addr(lds);
-  auto copy_tile = [&](int t) {
+  auto copy = [&](uint64_t base, uint32_t bytes, const uint32_t* off, int t, uint32_t place) {
     const uint32_t rows = (uint32_t)min(kPromptKeys, pt.m - t * kPromptKeys);
-    const u32x4 kr = buffer_rsrc(k_base + (uint64_t)t * kPromptKeys * k_bytes, (rows - 1) * k_bytes + D * 2);
-    const u32x4 vr = buffer_rsrc(v_base + (uint64_t)t * kPromptKeys * v_bytes, (rows - 1) * v_bytes + D * 2);
-    const uint32_t dst = lds0 + (t & 1) * 2 * kTile + wave * kCopies * 1024;
+    const u32x4 r = buffer_rsrc(base + (uint64_t)t * kPromptKeys * bytes, (rows - 1) * bytes + D * 2);
+    const uint32_t dst = lds0 + place * kTile + wave * kCopies * 1024;
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) copy16(kr, k_off[i], __builtin_amdgcn_readfirstlane(dst + i * 1024));
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) copy16(vr, v_off[i], __builtin_amdgcn_readfirstlane(dst + kTile + i * 1024));
+    for (int i = 0; i < kCopies; ++i) copy16(r, off[i], __builtin_amdgcn_readfirstlane(dst + i * 1024));
   };
+  // places: keys of even and odd tiles, values of even and odd tiles
+  auto copy_keys = [&](int t) { copy(k_base, k_bytes, k_off, t, t & 1); };
+  auto copy_values = [&](int t) { copy(v_base, v_bytes, v_off, t, 2 + (t & 1)); };
 
   const float c = a.scale * kLog2e;
-  if (steps > 0) copy_tile(0);
-  int t = 0;
-  auto next = [&]() {                              // tile t is there; nobody reads the other buffer any more
-    wait_copies<0>();
-    lds_barrier();
-    if (t + 1 < steps) copy_tile(t + 1);
-    return lds + (t & 1) * 2 * kTile;
-  };
-  for (; (t + 1) * kPromptKeys <= all_keys; ++t) {           // every row sees every key
-    const char* kt = next();
-    rt.template step<false>(kt, kt + kTile, c, 0);
-  }
-  for (; t * kPromptKeys < wave_keys; ++t) {
-    const char* kt = next();
-    rt.template step<true>(kt, kt + kTile, c, seen - t * kPromptKeys);
-  }
-  for (; t < steps; ++t) next();                   // keys for the other waves
+  rt.run(
+      steps, (wave_keys + kPromptKeys - 1) / kPromptKeys, all_keys / kPromptKeys, c,
+      [&]() {
+        copy_keys(0);
+        copy_values(0);
+        if (steps > 1) copy_keys(1);
+        if (steps > 1) wait_copies<2 * kCopies>(); else wait_copies<kCopies>();
+        lds_barrier();
+      },
+      [&](int t) {
+        wait_copies<0>();
+        lds_barrier();                               // and nobody reads tile t's keys or tile t - 1's values any more
+        if (t + 1 < steps) copy_values(t + 1);
+        if (t + 2 < steps) copy_keys(t + 2);
+      },
+      [&](int t) { return seen - t * kPromptKeys; });
 
   const float sum = half_sum(rt.sum);
   const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
@@ -759,12 +808,13 @@ __device__ void split_rows(const CachedCall& a, const Book& book, char* lds, con
   RowTile<BF, DP> rt;
   int seen;
   const uint16_t* qp = cached_query<PREFIX>(a, book, x, kvh, row0 + col, seen);
-  rt.start(qp, row0 + col < x.rows, D, half);
+  rt.start(qp, row0 + col < x.rows, D, lds);
   seen = min(seen, to);
   int all = row0 + col < x.rows ? seen : 0x7FFFFFFF;
 #pragma unroll
   for (int d = 16; d; d >>= 1) all = min(all, __shfl_xor(all, d));
-  all = __builtin_amdgcn_readfirstlane(all);
+  all = min(__builtin_amdgcn_readfirstlane(all), to);
+  all = max(all, from);
 
   uint32_t k_lane[kCopies], v_lane[kCopies];
 #pragma unroll
@@ -776,37 +826,34 @@ __device__ void split_rows(const CachedCall& a, const Book& book, char* lds, con
   }
   const int64_t head_off = ((int64_t)kvh << a.page_log) * D;
   const uint32_t lds0 = lds_addr(lds) + wave * 16 * kRow;
-  auto copy_tile = [&](int t) {
+  auto copy = [&](int64_t off, const uint32_t* lanes, int t, uint32_t place) {
     const int p = from + t * kPromptKeys + wave * 16;
-    if ((p >> a.page_log) - pages.at > 63) pages.load((from + t * kPromptKeys) >> a.page_log);
-    const int id = pages(p >> a.page_log);
-    const u32x4 kr = page_rows(a, id, a.k_off + head_off, p, to), vr = page_rows(a, id, a.v_off + head_off, p, to);
-    const uint32_t dst = lds0 + (t & 1) * 2 * kTile;
+    const u32x4 r = page_rows(a, pages(p >> a.page_log), off + head_off, p, to);
+    const uint32_t dst = lds0 + place * kTile;
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) copy16(kr, k_lane[i], __builtin_amdgcn_readfirstlane(dst + i * 1024));
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) copy16(vr, v_lane[i], __builtin_amdgcn_readfirstlane(dst + kTile + i * 1024));
+    for (int i = 0; i < kCopies; ++i) copy16(r, lanes[i], __builtin_amdgcn_readfirstlane(dst + i * 1024));
   };
+  auto copy_keys = [&](int t) { copy(a.k_off, k_lane, t, t & 1); };
+  auto copy_values = [&](int t) { copy(a.v_off, v_lane, t, 2 + (t & 1)); };
   const int steps = (to - from + kPromptKeys - 1) / kPromptKeys;
-  copy_tile(0);
-  int t = 0;
-  auto next = [&]() {
-    wait_copies<0>();
-    lds_barrier();
-    if (t + 1 < steps) copy_tile(t + 1);
-    return lds + (t & 1) * 2 * kTile;
-  };
-  if (busy) {
-    for (; from + (t + 1) * kPromptKeys <= all; ++t) {
-      const char* kt = next();
-      rt.template step<false>(kt, kt + kTile, a.c, 0);
-    }
-    for (; t < steps; ++t) {
-      const char* kt = next();
-      rt.template step<true>(kt, kt + kTile, a.c, seen - from - t * kPromptKeys);
-    }
-  }
-  for (; t < steps; ++t) next();
+  rt.run(
+      steps, busy ? steps : 0, (all - from) / kPromptKeys, a.c,
+      [&]() {
+        copy_keys(0);
+        copy_values(0);
+        if (steps > 1) copy_keys(1);
+        if (steps > 1) wait_copies<2 * kCopies>(); else wait_copies<kCopies>();
+        lds_barrier();
+      },
+      [&](int t) {
+        wait_copies<0>();
+        lds_barrier();
+        const int next = from + (t + 1) * kPromptKeys;
+        if (((next + 2 * kPromptKeys - 1) >> a.page_log) - pages.at > 63) pages.load(next >> a.page_log);
+        if (t + 1 < steps) copy_values(t + 1);
+        if (t + 2 < steps) copy_keys(t + 2);
+      },
+      [&](int t) { return seen - from - t * kPromptKeys; });
   lds_barrier();                                         // the next item may fill the tiles
   const int r = wave * 32 + col;
   rt.sum = half_sum(rt.sum);
