@@ -92,15 +92,15 @@ __device__ __forceinline__ void lds_barrier() {
 // place c ^ key(r). The copies put it there by choosing each lane's source, so a row needs no padding.
 // Two readings, one key each:
 //   keys (K)    every lane one piece, the same c of consecutive rows: the rows must spread over the banks
-//   values (V)  the transposing read, 16 lanes taking 32 bytes of 4 consecutive rows: pairs of pieces stay
-//               together, rows spread in steps of 32 bytes
+//   values (V)  the transposing read: 32 lanes take 64 bytes of 4 consecutive rows (k_prompt) or 32 bytes of 8 (one wave's
+//               keys): pairs of pieces stay together, 4 rows spread in steps of 64 bytes, 8 rows in steps of 32
 template <int DP>
 __device__ __forceinline__ uint32_t k_key(uint32_t row) {
   return DP == 128 ? (row & 15u) : ((row >> 1) & 7u);
 }
 template <int DP>
 __device__ __forceinline__ uint32_t v_key(uint32_t row) {
-  return DP == 128 ? (row & 7u) << 1 : ((row >> 1) & 3u) << 1;
+  return DP == 128 ? (row & 3u) << 2 | (row & 4u) >> 1 : (row & 2u) << 1 | (row & 4u) >> 1;
 }
 __device__ __forceinline__ u32x4 lds_read16(uint32_t at) {
   return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)at;

@@ -344,10 +344,11 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
 // ---------------------------------------------------------------------------
 // Work. An item is one K/V head and one tile of query rows over the keys of one entry: of a sequence's
 // own part (rows: its tokens x the heads of the K/V head) or of a group's prefix (rows: those of all members).
-// Items are cut into units of keys; the units of all items, in order, are dealt out to the blocks in
-// equal runs, so short and long sequences fill the chip alike and nothing on the host depends on lengths. A
-// run crosses items; each crossing gives one partial result (maximum, sum, weighted values). Its slot is run +
-// item: both only grow along the runs and every crossing raises one of them, so no two share a slot.
+// Items are cut into units of keys, with a few more at their start that stand for the time an item takes whatever its
+// length; the units of all items, in order, are dealt out to the blocks in equal runs, so short and long sequences
+// fill the chip alike and nothing on the host depends on lengths. A run crosses items; each crossing gives one partial
+// result (maximum, sum, weighted values). Its slot is run + item: both only grow along the runs and every crossing
+// raises one of them, so no two share a slot.
 //
 // Three ways through an item's keys:
 //   split keys   16 or 32 rows, units of 32 keys: for few rows the keys' bytes are all that counts, and every wave keeps
@@ -362,18 +363,17 @@ constexpr int kCachedBlocks = 512;         // two per CU
 constexpr int kXcds = 8;
 constexpr int kWaveKeys = 32;              // split keys: per wave and step
 constexpr int kManyRows = 128;             // split rows: rows of a tile
-#ifndef K_SHORT
-#define K_SHORT 8
-#define K_LEAST 4
-#define K_COSTROWS 2.2f
-#define K_COSTKEYS 1.45f
-#define K_COSTITEM 1.0f
-#endif
-constexpr int kShortItem = K_SHORT;              // split keys: up to as many units per item on average, runs of single waves
-constexpr int kLeastRows = K_LEAST;              // split rows: units of a run at least
-constexpr float kCostRows = K_COSTROWS, kCostKeys = K_COSTKEYS, kCostItem = K_COSTITEM;   // of a unit, of an item; for dealing blocks to prefixes and own parts
+// Measured on the device with 64 sequences on one prefix of 8192, 16 x 6 drafts on prefixes of 1536, 32 sequences of 0 to
+// 16384 and 64 of 1 to 512 (14/2 heads of 64, 32/8 of 128): starts of 1/2, 2/3, 2/5 and 3/3 units are within 6 %
+// of each other but for 1/2 (32 ragged: 48 us against 43); a prefix's unit at 0.9, 1.5 and 2.8 times a unit of keys
+// gives the first case 47, 37 and 34 us, at 5 times 38.
+constexpr int kStartRows = 2, kStartKeys = 4;    // units that stand for an item's start
+constexpr int kShortItem = 8;                    // split keys: up to as many units per item on average, runs of single waves
+constexpr int kLeastRows = 2;                    // split rows: units of a run (drafts 14.9 us; 4: 17.4, 8: 21)
+constexpr float kCostRows = 2.2f, kCostKeys = 0.8f;      // of a unit, for dealing blocks to prefixes and own parts
 enum { kNone = 0, kOneTile = 1, kTwoTiles = 2, kRows = 3 };      // 16 rows, 32 rows, split rows
 __host__ __device__ constexpr int mode_rows(int mode) { return mode == kRows ? kManyRows : 16 * mode; }
+__host__ __device__ constexpr int mode_start(int mode) { return mode == kRows ? kStartRows : kStartKeys; }
 __host__ __device__ constexpr int mode_unit(int mode) { return mode == kRows ? kPromptKeys : kWaveKeys; }
 
 struct Pass {                              // the own parts, or the prefixes
@@ -381,11 +381,11 @@ struct Pass {                              // the own parts, or the prefixes
   float* ml;                               // [slot][stride][2]: maximum (times c), sum
   int32_t stride, slots;
 };
-// Units dealt out to blocks: the first `rest` of them get each + 1, the others each.
+// Units dealt out to runs: the first `rest` of them get each + 1, the others each.
 struct Deal {
   int32_t each, rest;
-  __device__ __forceinline__ int start(int block) const { return block * each + min(block, rest); }
-  __device__ __forceinline__ int block_of(int unit) const {        // only where units were dealt: each + 1 > 0
+  __device__ __forceinline__ int start(int run) const { return run * each + min(run, rest); }
+  __device__ __forceinline__ int run_of(int unit) const {        // only where units were dealt: each + 1 > 0
     const int big = rest * (each + 1);
     return unit < big ? unit / (each + 1) : rest + (unit - big) / max(each, 1);
   }
@@ -470,7 +470,8 @@ __device__ void fill_book(const CachedCall& a, const Book& k) {
 }
 
 struct Entry {
-  int rows, tiles, items, units;           // query rows, row tiles, items (tiles of every K/V head), units of each
+  int rows, tiles, items;                  // query rows, row tiles, items (tiles of every K/V head)
+  int units;                               // of each item, its start among them; 0: no keys
   int from, to;                            // keys
   int first, group;                        // batch entry that the keys belong to; own part: its group
   Seq seq;                                 // of `first`
@@ -496,7 +497,7 @@ __device__ __forceinline__ Entry cached_entry(const CachedCall& a, const Book& b
   }
   r.tiles = (r.rows + mode_rows(MODE) - 1) / mode_rows(MODE);
   r.items = a.kv_heads * r.tiles;
-  r.units = (max(r.to - r.from, 0) + mode_unit(MODE) - 1) / mode_unit(MODE);
+  r.units = r.to > r.from ? (r.to - r.from + mode_unit(MODE) - 1) / mode_unit(MODE) + mode_start(MODE) : 0;
   return r;
 }
 
@@ -882,7 +883,7 @@ struct Plan {
 };
 __device__ __forceinline__ Plan deal_out(int units, int items, int blocks, int mode) {
   Plan p;
-  p.alone = mode != kRows && units <= kShortItem * items;
+  p.alone = mode != kRows && units <= (kShortItem + mode_start(mode)) * items;
   const int least = mode == kRows ? kLeastRows : 1;
   p.runs = min(p.alone ? blocks * kCachedWaves : blocks, (units + least - 1) / least);
   p.deal.each = units / max(p.runs, 1);
@@ -927,9 +928,12 @@ __device__ void cached_run(const CachedCall& a, const Book& book, char* lds, con
   int item = min(in / x.units, x.items - 1), unit = in % x.units;
   while (true) {
     const int units = min(left, x.units - unit);
-    const int from = x.from + unit * mode_unit(MODE), to = min(from + units * mode_unit(MODE), x.to);
-    if constexpr (MODE == kRows) split_rows<BF, DP, PREFIX>(a, book, lds, x, item, from, to, run + items + item);
-    else split_keys<BF, DP, MODE, PREFIX>(a, book, lds, x, item, from, to, run + items + item, plan.alone);
+    const int from = x.from + max(unit - mode_start(MODE), 0) * mode_unit(MODE);
+    const int to = min(x.from + (unit + units - mode_start(MODE)) * mode_unit(MODE), x.to);
+    if (to > from) {
+      if constexpr (MODE == kRows) split_rows<BF, DP, PREFIX>(a, book, lds, x, item, from, to, run + items + item);
+      else split_keys<BF, DP, MODE, PREFIX>(a, book, lds, x, item, from, to, run + items + item, plan.alone);
+    }
     left -= units;
     if (left <= 0) break;
     unit = 0;
@@ -970,7 +974,7 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a
   int n_pre = 0;
   if constexpr (PRE != kNone) {
     auto cost = [](const Scan& sc, int mode) {
-      return mode == kRows ? sc.total * kCostRows : sc.total * kCostKeys + min(sc.total, sc.all_items) * kCostItem;
+      return sc.total * (mode == kRows ? kCostRows : kCostKeys);
     };
     const float wp = cost(pre, PRE), wo = cost(own, OWN);
     if (pre.total) n_pre = own.total ? min(max((int)(kCachedBlocks / kXcds * wp / (wp + wo) + 0.5f), 1), kCachedBlocks / kXcds - 1) * kXcds : kCachedBlocks;
@@ -1022,7 +1026,7 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a
 // One wave per (sequence, token, head): the partial results of its row, the prefix's and the own part's. A lane holds
 // four dims: a quarter (DP 64) or half of the wave reads one slot's row, so one load covers several slots.
 template <bool BF, int DP>
-__global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, int own_rows, int pre_rows) {
+__global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, int own_rows, int own_start, int pre_rows, int pre_start) {
   constexpr int kLanes = DP / 4, kPer = 64 / kLanes, kBatch = 8;      // lanes and slots per load, loads in flight
   const int b = blockIdx.x, lane = threadIdx.x & 63;
   const int G = a.heads / a.kv_heads, D = a.dim;
@@ -1034,11 +1038,11 @@ __global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, int
   const int sub = lane / kLanes, dim = lane % kLanes * 4;
   float m = -INFINITY, l = 0.0f;
   f32x4 y = f32x4{};
-  auto add = [&](const Pass& ps, const JoinPart& x, int tile_rows, int rr, const Deal& deal) {
-    if (x.units <= 0) return;
+  auto add = [&](const Pass& ps, const JoinPart& x, int tile_rows, int start, int rr, const Deal& deal) {
+    if (x.units <= start) return;
     const int item = kvh * x.tiles + rr / tile_rows, r = rr % tile_rows;
     const int u0 = x.units_before + item * x.units;
-    const int i0 = deal.block_of(u0), i1 = deal.block_of(u0 + x.units - 1), s0 = i0 + x.items_before + item;
+    const int i0 = deal.run_of(u0 + start), i1 = deal.run_of(u0 + x.units - 1), s0 = i0 + x.items_before + item;
     const int n = s0 < 0 ? 0 : min(i1 - i0 + 1, ps.slots - s0);
     const float* pm = ps.ml + ((int64_t)s0 * ps.stride + r) * 2;
     const float* po = ps.part + ((int64_t)s0 * ps.stride + r) * D + dim;
@@ -1064,8 +1068,8 @@ __global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, int
       }
     }
   };
-  add(a.pre, je.pre, max(pre_rows, 1), ((b - je.first) * a.tokens + t) * G + h % G, deals[1]);
-  add(a.own, je.own, own_rows, t * G + h % G, deals[0]);
+  add(a.pre, je.pre, max(pre_rows, 1), pre_start, ((b - je.first) * a.tokens + t) * G + h % G, deals[1]);
+  add(a.own, je.own, own_rows, own_start, t * G + h % G, deals[0]);
 #pragma unroll
   for (int d = kLanes; d < 64; d <<= 1)
 #pragma unroll
@@ -1163,7 +1167,7 @@ int plan_cached(const mtc_cache_desc* c, const mtc_cached_args* a, CachedPlan* p
   p->pre_stride = p->pre_mode ? stride(all, p->pre_mode) : 0;
   p->pre_slots = p->pre_mode ? runs(p->pre_mode) + (int64_t)c->kv_heads * (tiles(all, p->pre_mode) + a->n_groups) : 0;
   // the kernels count units in 32 bits
-  const int64_t units = (int64_t)c->max_pages * c->page_size / kWaveKeys + 1;
+  const int64_t units = (int64_t)c->max_pages * c->page_size / kWaveKeys + 1 + std::max(mode_start(kOneTile), mode_start(kRows));
   if (units * (p->own_slots + p->pre_slots) > 0x7FFFFFFF)
     return fail(MTC_E_SHAPE, "%d sequences of up to %d pages of %d tokens, %d row tiles: too much for one call", a->n_seqs, c->max_pages,
                 c->page_size, (int)tiles(per, p->own_mode));
@@ -1192,8 +1196,8 @@ int run_cached(const CachedCall& a, const CachedPlan& p, hipStream_t st) {
   else launch_cached<BF, 128>(a, p.own_mode, p.pre_mode, st);
   if (int rc = check_launch("k_cached")) return rc;
   const dim3 grid(a.n_seqs, (a.tokens * a.heads + kCachedWaves - 1) / kCachedWaves);
-  if (a.dim <= 64) k_join<BF, 64><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_rows(p.pre_mode));
-  else k_join<BF, 128><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_rows(p.pre_mode));
+  if (a.dim <= 64) k_join<BF, 64><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_start(p.own_mode), mode_rows(p.pre_mode), mode_start(p.pre_mode));
+  else k_join<BF, 128><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_start(p.own_mode), mode_rows(p.pre_mode), mode_start(p.pre_mode));
   return check_launch("k_join");
 }
 
