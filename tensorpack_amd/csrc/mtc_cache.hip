@@ -82,6 +82,11 @@ __device__ __forceinline__ bool mark(uint32_t* marks, int s) {         // true: 
   return (atomicOr(&marks[s >> 5], 1u << (s & 31)) >> (s & 31)) & 1;
 }
 
+// One block. A thread plans sequence i of each round of 1024; lists of up to 1024 (any but the largest batches) take
+// one round, whose plan stays in registers. Loads come in three dependent steps (list, lengths, last page and its count).
+struct Extend {
+  int s, len, count, old, need;            // need: new pages, the copy of a shared last page (old >= 0) first
+};
 __global__ __launch_bounds__(kThreads) void k_extend(const mtc_cache_desc c, const int32_t* seqs, const int32_t* counts, int n) {
   __shared__ uint32_t marks[kMarkWords];
   __shared__ int freed;
@@ -92,45 +97,42 @@ __global__ __launch_bounds__(kThreads) void k_extend(const mtc_cache_desc c, con
   if (tid == 0) freed = c.n_pages;
   __syncthreads();
 
-  // pages that sequence i needs; copy: its last page is partly filled and shared
-  auto wants = [&](int i, int& len, int& count, bool& copy) {
-    const int s = seqs[i];
-    len = c.lens[s];
-    count = counts[i];
-    copy = false;
-    if (len % c.page_size && count > 0) {
-      const int p = c.table[(int64_t)s * c.max_pages + len / c.page_size];
-      copy = (uint32_t)p < (uint32_t)c.n_pages && c.refs[p] > 1;
-    }
-    return pages_of(c, len + count) - pages_of(c, len) + copy;
-  };
-
   int bad = 0;
-  for (int i = tid; i < n; i += kThreads) {
-    const int s = seqs[i];
-    if ((uint32_t)s >= (uint32_t)c.max_seqs || mark(marks, s)) {
+  auto plan = [&](int i, bool check) {
+    Extend x{0, 0, 0, -1, 0};
+    if (i >= n) return x;
+    x.s = seqs[i];
+    x.count = counts[i];
+    if ((uint32_t)x.s >= (uint32_t)c.max_seqs || (check && mark(marks, x.s))) {
       bad |= MTC_CACHE_BAD_SEQ;
-      continue;
+      return x;
     }
-    if (counts[i] < 0) bad |= MTC_CACHE_BAD_LENGTH;
-    else if ((int64_t)c.lens[s] + counts[i] > (int64_t)c.max_pages * c.page_size) bad |= MTC_CACHE_TABLE_FULL;
+    x.len = c.lens[x.s];
+    if (x.count < 0) bad |= MTC_CACHE_BAD_LENGTH;
+    else if ((int64_t)x.len + x.count > (int64_t)c.max_pages * c.page_size) bad |= MTC_CACHE_TABLE_FULL;
+    if (bad) return x;
+    if (x.len % c.page_size && x.count > 0) {
+      const int p = c.table[(int64_t)x.s * c.max_pages + x.len / c.page_size];
+      if ((uint32_t)p < (uint32_t)c.n_pages && c.refs[p] > 1) x.old = p;
+    }
+    x.need = pages_of(c, x.len + x.count) - pages_of(c, x.len) + (x.old >= 0);
+    return x;
+  };
+  constexpr uint64_t kLow = (1ull << 44) - 1;              // 1024 x 2^26 pages stay below 2^44
+  int64_t need = 0, copies = 0;
+  Extend mine{};
+  int64_t my_copy = 0;
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    mine = plan(i0 + tid, true);
+    uint64_t total;
+    const uint64_t at = block_scan((uint64_t)(mine.old >= 0) << 44 | (uint64_t)mine.need, total);
+    if (i0 + tid < n) start[i0 + tid] = (int)min(need + (int64_t)(at & kLow), (int64_t)c.n_pages);
+    my_copy = copies + (int64_t)(at >> 44);
+    need += (int64_t)(total & kLow);
+    copies += (int64_t)(total >> 44);
   }
   bad = block_or(bad);
-  int64_t need = 0, copies = 0;
-  if (!bad) {
-    for (int i0 = 0; i0 < n; i0 += kThreads) {
-      int len, count, w = 0;
-      bool copy = false;
-      if (i0 + tid < n) w = wants(i0 + tid, len, count, copy);
-      uint64_t total;
-      const uint64_t at = block_scan((uint64_t)copy << 44 | (uint64_t)w, total);      // 1024 x 2^26 pages stay below 2^44
-      if (i0 + tid < n) start[i0 + tid] = (int)(need + (int64_t)(at & ((1ull << 44) - 1)));
-      need += (int64_t)(total & ((1ull << 44) - 1));
-      copies += (int64_t)(total >> 44);
-      if (need > c.n_pages) break;
-    }
-    if (need > c.n_pages) bad = MTC_CACHE_NO_PAGES;
-  }
+  if (!bad && need > c.n_pages) bad = MTC_CACHE_NO_PAGES;
   // the lowest free ids, in order
   int64_t found = 0;
   int next_free = c.state[kFirstFree];
@@ -146,7 +148,7 @@ __global__ __launch_bounds__(kThreads) void k_extend(const mtc_cache_desc c, con
     }
     if (found < need) bad = MTC_CACHE_NO_PAGES;
   }
-  __syncthreads();                                       // ids and start are written
+  __syncthreads();                                         // ids and start are written
   if (bad) {
     if (tid == 0) {
       c.state[kStatus] |= bad;
@@ -155,49 +157,52 @@ __global__ __launch_bounds__(kThreads) void k_extend(const mtc_cache_desc c, con
     return;
   }
   if (need) next_free = ids[need - 1] + 1;
-  // one wave per sequence; the copies' pairs are ranked in the list's order
+  // pairs of pages to copy, in the list's order
   int64_t before = 0;
   for (int i0 = 0; i0 < n; i0 += kThreads) {
-    int len, count;
-    bool copy = false;
-    if (i0 + tid < n) wants(i0 + tid, len, count, copy);
-    uint64_t total;
-    const int64_t at = before + (int64_t)block_scan(copy, total);
-    if (copy) {
-      const int64_t slot = (int64_t)seqs[i0 + tid] * c.max_pages + len / c.page_size;
-      scratch_src(c)[at] = c.table[slot];
-      scratch_dst(c)[at] = ids[start[i0 + tid]];
+    if (n > kThreads) {
+      mine = plan(i0 + tid, false);
+      uint64_t total;
+      my_copy = before + (int64_t)block_scan(mine.old >= 0, total);
+      before += (int64_t)total;
     }
-    before += (int64_t)total;
+    if (mine.old >= 0) {
+      scratch_src(c)[my_copy] = mine.old;
+      scratch_dst(c)[my_copy] = ids[start[i0 + tid]];
+    }
   }
-  __syncthreads();
-  for (int i = wave; i < n; i += kWaves) {
-    int len, count;
-    bool copy;
-    wants(i, len, count, copy);
-    const int s = seqs[i], first = start[i], have = pages_of(c, len), more = pages_of(c, len + count) - have;
-    int32_t* const row = c.table + (int64_t)s * c.max_pages;
-    for (int k = lane; k < more; k += 64) {
-      const int p = ids[first + copy + k];
-      row[have + k] = p;
+  // new pages: by the sequence's thread where there are a few, by a wave where there are many
+  auto take = [&](const Extend& x, int first, int k0, int step) {
+    const int have = pages_of(c, x.len), more = x.need - (x.old >= 0);
+    for (int k = k0; k < more; k += step) {
+      const int p = ids[first + (x.old >= 0) + k];
+      c.table[(int64_t)x.s * c.max_pages + have + k] = p;
       c.refs[p] = 1;
     }
-    // the table entry of a copied page is written after every wave has judged its own last page (below)
+  };
+  constexpr int kFew = 4;
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    if (n > kThreads) mine = plan(i0 + tid, false);
+    const int first = i0 + tid < n ? start[i0 + tid] : 0;
+    if (mine.need <= kFew) take(mine, first, 0, 1);
+    for (uint64_t many = __ballot(mine.need > kFew); many; many &= many - 1) {
+      const int l = __ffsll((unsigned long long)many) - 1;
+      const Extend x{__shfl(mine.s, l), __shfl(mine.len, l), 0, __shfl(mine.old, l), __shfl(mine.need, l)};
+      take(x, __shfl(first, l), lane, 64);
+    }
   }
-  __syncthreads();
+  __syncthreads();                                         // every last page has been judged by its count
   for (int i = tid; i < (int)copies; i += kThreads) {
     const int old = scratch_src(c)[i];
     if (atomicSub(&c.refs[old], 1) == 1) atomicMin(&freed, old);
     c.refs[scratch_dst(c)[i]] = 1;
   }
-  before = 0;
   for (int i = tid; i < n; i += kThreads) {
     const int s = seqs[i], len = c.lens[s], count = counts[i];
     if (len % c.page_size && count > 0) {
-      // copied: the first of the sequence's new ids is one of the copies' targets
-      const int have = pages_of(c, len), more = pages_of(c, len + count) - have;
-      const int end = i + 1 < n ? start[i + 1] : (int)need;
-      if (end - start[i] > more) c.table[(int64_t)s * c.max_pages + have - 1] = ids[start[i]];
+      // copied, if its new ids are one more than its new pages: the first of them takes the last page's place
+      const int have = pages_of(c, len), end = i + 1 < n ? start[i + 1] : (int)need;
+      if (end - start[i] > pages_of(c, len + count) - have) c.table[(int64_t)s * c.max_pages + have - 1] = ids[start[i]];
     }
     c.lens[s] = len + count;
   }
@@ -210,13 +215,11 @@ __global__ __launch_bounds__(kThreads) void k_extend(const mtc_cache_desc c, con
 
 // Whole pages: unit = 16 KiB of one page (or what is left of it). Pairs of ids out of range are left out.
 constexpr int kCopyThreads = 256;
-__global__ __launch_bounds__(kCopyThreads) void k_copy_pages(char* pool, const char* from, int64_t page_bytes, int n_pages,
-                                                             int from_pages, const int32_t* src, const int32_t* dst,
-                                                             const int32_t* count, int n) {
+__device__ void copy_pages(char* pool, const char* from, int64_t page_bytes, int n_pages, int from_pages, const int32_t* src,
+                           const int32_t* dst, int n, int block, int blocks) {
   constexpr int kUnitBytes = kCopyThreads * 16 * 4;
-  if (count) n = *count;
   const int64_t per = (page_bytes + kUnitBytes - 1) / kUnitBytes;
-  for (int64_t u = blockIdx.x; u < per * n; u += gridDim.x) {
+  for (int64_t u = block; u < per * n; u += blocks) {
     const int i = (int)(u / per);
     const int a = src[i], b = dst[i];
     if ((uint32_t)a >= (uint32_t)from_pages || (uint32_t)b >= (uint32_t)n_pages) continue;
@@ -232,16 +235,24 @@ __global__ __launch_bounds__(kCopyThreads) void k_copy_pages(char* pool, const c
       if (at + k * kCopyThreads * 16 < page_bytes) *reinterpret_cast<u32x4*>(d + at + k * kCopyThreads * 16) = x[k];
   }
 }
+__global__ __launch_bounds__(kCopyThreads) void k_copy_pages(char* pool, const char* from, int64_t page_bytes, int n_pages,
+                                                             int from_pages, const int32_t* src, const int32_t* dst,
+                                                             const int32_t* count, int n) {
+  copy_pages(pool, from, page_bytes, n_pages, from_pages, src, dst, count ? *count : n, blockIdx.x, gridDim.x);
+}
 
-// Every block checks the whole list (lens change only after the last block has done so), then does its share.
-// Returns true in the one block that finishes last.
+// Every block checks the whole list, then does its share; lens change only in the block that comes here last, when every
+// block has read them. (The count orders those reads before its writes; nothing written by one block is read by another,
+// so no fence, whose write-back of the caches costs more than the kernel.) One block alone needs no count.
 __device__ bool last_block(int32_t* done) {
   __shared__ int last;
-  __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+  if (gridDim.x == 1) return true;
+  if (threadIdx.x == 0) {
+    last = __hip_atomic_fetch_add(done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+    if (last) __hip_atomic_store(done, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
   __syncthreads();
-  if (last) __threadfence();
   return last;
 }
 
@@ -275,10 +286,7 @@ __global__ __launch_bounds__(kThreads) void k_truncate(const mtc_cache_desc c, c
   if (!last_block(&c.state[kDone])) return;
   if (!bad)
     for (int i = threadIdx.x; i < n; i += kThreads) c.lens[seqs[i]] = new_lens ? new_lens[i] : 0;
-  if (threadIdx.x == 0) {
-    c.state[kDone] = 0;
-    if (bad) c.state[kStatus] |= bad;
-  }
+  if (threadIdx.x == 0 && bad) c.state[kStatus] |= bad;
 }
 
 __global__ __launch_bounds__(kThreads) void k_fork(const mtc_cache_desc c, const int32_t* src, const int32_t* dst, int n) {
@@ -314,35 +322,47 @@ __global__ __launch_bounds__(kThreads) void k_fork(const mtc_cache_desc c, const
   if (!last_block(&c.state[kDone])) return;
   if (!bad)
     for (int i = threadIdx.x; i < n; i += kThreads) c.lens[dst[i]] = c.lens[src[i]];
-  if (threadIdx.x == 0) {
-    c.state[kDone] = 0;
-    if (bad) c.state[kStatus] |= bad;
-  }
+  if (threadIdx.x == 0 && bad) c.state[kStatus] |= bad;
 }
 
+// One block; a thread takes four consecutive pages of each round of 4096.
 __global__ __launch_bounds__(kThreads) void k_compact_plan(const mtc_cache_desc c) {
+  constexpr int kEach = 4;
   const int tid = threadIdx.x;
-  int used = 0;
-  for (int p = tid; p < c.n_pages; p += kThreads) used += c.refs[p] > 0;
+  auto counts = [&](int64_t p, int (&r)[kEach]) {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) r[k] = p + k < c.n_pages ? c.refs[p + k] : -1;
+  };
+  int used = 0, r[kEach];
+  for (int64_t p = (int64_t)tid * kEach; p < c.n_pages; p += kThreads * kEach) {
+    counts(p, r);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) used += r[k] > 0;
+  }
   uint64_t total;
   block_scan(used, total);
   const int64_t live = (int64_t)total;
   int64_t movers = 0, holes = 0;
-  for (int64_t p0 = 0; p0 < c.n_pages; p0 += kThreads) {
-    const int64_t p = p0 + tid;
-    const bool in = p < c.n_pages, is_used = in && c.refs[p] > 0;
-    const bool moves = is_used && p >= live, hole = in && !is_used && p < live;
-    const uint64_t at = block_scan((uint64_t)moves << 32 | (uint32_t)hole, total);
-    if (moves) scratch_src(c)[movers + (int64_t)(at >> 32)] = (int)p;
-    if (hole) scratch_dst(c)[holes + (int64_t)(at & 0xFFFFFFFFu)] = (int)p;
-    if (in) scratch_ids(c)[p] = (int)p;
+  for (int64_t p0 = 0; p0 < c.n_pages; p0 += kThreads * kEach) {
+    const int64_t p = p0 + (int64_t)tid * kEach;
+    if (p0 || c.n_pages > kThreads * kEach) counts(p, r);
+    uint64_t n = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) n += p + k >= live ? (uint64_t)(r[k] > 0) << 32 : (uint64_t)(r[k] == 0);
+    const uint64_t at = block_scan(n, total);
+    int64_t m = movers + (int64_t)(at >> 32), h = holes + (int64_t)(at & 0xFFFFFFFFu);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      if (p + k >= live && r[k] > 0) scratch_src(c)[m++] = (int)(p + k);
+      if (p + k < live && r[k] == 0) scratch_dst(c)[h++] = (int)(p + k);
+    }
     movers += (int64_t)(total >> 32);
     holes += (int64_t)(total & 0xFFFFFFFFu);
   }
   __syncthreads();
   for (int64_t i = tid; i < movers; i += kThreads) {
     const int a = scratch_src(c)[i], b = scratch_dst(c)[i];
-    scratch_ids(c)[a] = b;
+    scratch_ids(c)[a] = b;                                 // where page a went; read for ids from `live` on only
     c.refs[b] = c.refs[a];
     c.refs[a] = 0;
   }
@@ -352,14 +372,20 @@ __global__ __launch_bounds__(kThreads) void k_compact_plan(const mtc_cache_desc 
   }
 }
 
-__global__ __launch_bounds__(256) void k_compact_table(const mtc_cache_desc c) {
-  const int lane = threadIdx.x & 63;
-  for (int s = blockIdx.x * 4 + (threadIdx.x >> 6); s < c.max_seqs; s += gridDim.x * 4) {
+// The first blocks rename the moved pages in the table, the others copy them.
+__global__ __launch_bounds__(kCopyThreads) void k_compact(const mtc_cache_desc c, int64_t page_bytes, int table_blocks) {
+  if ((int)blockIdx.x >= table_blocks) {
+    copy_pages((char*)c.pool, (const char*)c.pool, page_bytes, c.n_pages, c.n_pages, scratch_src(c), scratch_dst(c), c.state[kPairs],
+               blockIdx.x - table_blocks, gridDim.x - table_blocks);
+    return;
+  }
+  const int live = c.state[kFirstFree], lane = threadIdx.x & 63;
+  for (int s = blockIdx.x * 4 + (threadIdx.x >> 6); s < c.max_seqs; s += table_blocks * 4) {
     const int have = min(pages_of(c, c.lens[s]), c.max_pages);
     int32_t* const row = c.table + (int64_t)s * c.max_pages;
     for (int k = lane; k < have; k += 64) {
       const int p = row[k];
-      if ((uint32_t)p < (uint32_t)c.n_pages) row[k] = scratch_ids(c)[p];
+      if (p >= live && p < c.n_pages) row[k] = scratch_ids(c)[p];
     }
   }
 }
@@ -410,6 +436,10 @@ constexpr int kMaxDrafted = 64;
 struct Best {
   float rest, all;                 // largest score over w = max(p - q, 0) (or p where nothing was rejected), and over p
   int32_t rest_i, all_i;           // its first index, -1: none
+};
+struct Found {                     // of one block
+  Best best;
+  int32_t accepted, reserved[3];
 };
 __device__ __forceinline__ void better(float& a, int32_t& ai, float b, int32_t bi) {
   if (bi >= 0 && (ai < 0 || b > a || (b == a && bi < ai))) {
@@ -467,64 +497,75 @@ __device__ int accepted(const mtc_verify_args& a, int b, int& k) {
   return wrong ? __ffsll((unsigned long long)wrong) - 1 : k;
 }
 
-template <int DT>
-__global__ __launch_bounds__(kVerifyThreads) void k_verify(const mtc_verify_args a, Best* best, int span) {
+// One block per sequence and span of the vocabulary. The noise does not depend on how many drafts were accepted, so its
+// loads are in flight while that chain of three dependent loads (count, drafts, their probabilities) is followed.
+template <int DT, int ROUNDS>
+__global__ __launch_bounds__(kVerifyThreads) void k_verify(const mtc_verify_args a, Found* found) {
   typedef typename Prob<DT>::type T;
   using P = Prob<DT>;
+  constexpr int kSpan = kVerifyThreads * 8;
   const int b = blockIdx.y, tid = threadIdx.x;
+  const float* e = a.noise + (int64_t)b * a.noise_stride;
+  const int from = blockIdx.x * (ROUNDS * kSpan) + tid * 8;
+  Eight<float> ev[ROUNDS];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
+    if (from + r * kSpan + 8 <= a.vocab) ev[r] = *reinterpret_cast<const Eight<float>*>(e + from + r * kSpan);
   int k;
   const int n = accepted<DT>(a, b, k);
   const bool minus = n < k;
   const T* p = reinterpret_cast<const T*>(a.p) + (int64_t)b * a.p_stride[0] + (int64_t)n * a.p_stride[1];
   const T* q = minus ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.q_stride[0] + (int64_t)n * a.q_stride[1] : p;
-  const float* e = a.noise + (int64_t)b * a.noise_stride;
-  Best r{0.0f, 0.0f, -1, -1};
+  Best best{0.0f, 0.0f, -1, -1};
   auto one = [&](int i, float w, float d, float z) {
-    if (w > 0.0f) better(r.all, r.all_i, w * z, i);
-    if (d > 0.0f) better(r.rest, r.rest_i, d * z, i);
+    if (w > 0.0f) better(best.all, best.all_i, w * z, i);
+    if (d > 0.0f) better(best.rest, best.rest_i, d * z, i);
   };
-  const int from = blockIdx.x * span, to = min(from + span, a.vocab);
-  for (int i = from + tid * 8; i < to; i += kVerifyThreads * 8) {
-    if (i + 8 <= to) {
-      const Eight<T> pv = *reinterpret_cast<const Eight<T>*>(p + i);
-      const Eight<float> ev = *reinterpret_cast<const Eight<float>*>(e + i);
-      if (minus) {
-        const Eight<T> qv = *reinterpret_cast<const Eight<T>*>(q + i);
+  Eight<T> pv[ROUNDS], qv[ROUNDS];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) one(i + j, P::get(pv.x[j]), P::get(pv.x[j]) - P::get(qv.x[j]), ev.x[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) one(i + j, P::get(pv.x[j]), 0.0f, ev.x[j]);
-      }
-    } else {
-      for (int j = i; j < to; ++j) one(j, P::get(p[j]), minus ? P::get(p[j]) - P::get(q[j]) : 0.0f, e[j]);
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int i = from + r * kSpan;
+    if (i + 8 <= a.vocab) {
+      pv[r] = *reinterpret_cast<const Eight<T>*>(p + i);
+      if (minus) qv[r] = *reinterpret_cast<const Eight<T>*>(q + i);
     }
   }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    better(r.rest, r.rest_i, __shfl_xor(r.rest, d), __shfl_xor(r.rest_i, d));
-    better(r.all, r.all_i, __shfl_xor(r.all, d), __shfl_xor(r.all_i, d));
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int i = from + r * kSpan;
+    if (i + 8 <= a.vocab) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) one(i + j, P::get(pv[r].x[j]), minus ? P::get(pv[r].x[j]) - P::get(qv[r].x[j]) : 0.0f, ev[r].x[j]);
+    } else {
+      for (int j = i; j < a.vocab; ++j) one(j, P::get(p[j]), minus ? P::get(p[j]) - P::get(q[j]) : 0.0f, e[j]);
+    }
   }
+  auto fold = [&]() {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+      better(best.rest, best.rest_i, __shfl_xor(best.rest, d), __shfl_xor(best.rest_i, d));
+      better(best.all, best.all_i, __shfl_xor(best.all, d), __shfl_xor(best.all_i, d));
+    }
+  };
+  fold();
   __shared__ Best waves[kVerifyThreads / 64];
-  if ((tid & 63) == 0) waves[tid >> 6] = r;
+  if ((tid & 63) == 0) waves[tid >> 6] = best;
   __syncthreads();
   if (tid == 0) {
     for (int w = 1; w < kVerifyThreads / 64; ++w) {
-      better(r.rest, r.rest_i, waves[w].rest, waves[w].rest_i);
-      better(r.all, r.all_i, waves[w].all, waves[w].all_i);
+      better(best.rest, best.rest_i, waves[w].rest, waves[w].rest_i);
+      better(best.all, best.all_i, waves[w].all, waves[w].all_i);
     }
-    best[(int64_t)b * gridDim.x + blockIdx.x] = r;
+    found[(int64_t)b * gridDim.x + blockIdx.x] = Found{best, n, {0, 0, 0}};
   }
 }
 
-template <int DT>
-__global__ __launch_bounds__(64) void k_verify_join(const mtc_verify_args a, const Best* best, int splits) {
+__global__ __launch_bounds__(64) void k_verify_join(const mtc_verify_args a, const Found* found, int splits) {
   const int b = blockIdx.x, lane = threadIdx.x;
-  int k;
-  const int n = accepted<DT>(a, b, k);
+  const int n = found[(int64_t)b * splits].accepted;
   Best r{0.0f, 0.0f, -1, -1};
   for (int i = lane; i < splits; i += 64) {
-    const Best x = best[(int64_t)b * splits + i];
+    const Best x = found[(int64_t)b * splits + i].best;
     better(r.rest, r.rest_i, x.rest, x.rest_i);
     better(r.all, r.all_i, x.all, x.all_i);
   }
@@ -563,13 +604,11 @@ int check_list(const mtc_cache_desc* c, const int32_t* a, const char* what, int 
 
 unsigned list_grid(int n) { return (unsigned)std::min((n + kWaves - 1) / kWaves, 256); }
 
-int verify_splits(const mtc_verify_args* a, int* span) {
-  // enough blocks to fill the chip, at least two rounds of a block's loads each
-  int64_t per = ((int64_t)a->n_seqs * a->vocab + 2047) / 2048;
-  per = std::max<int64_t>(per, 2 * kVerifyThreads * 8);
-  per = (per + kVerifyThreads * 8 - 1) / (kVerifyThreads * 8) * (kVerifyThreads * 8);
-  *span = (int)std::min<int64_t>(per, 0x40000000);
-  return (int)(((int64_t)a->vocab + *span - 1) / *span);
+// Two rounds of a block's loads per block once that still gives every CU several blocks, else one.
+int verify_rounds(const mtc_verify_args* a) { return (int64_t)a->n_seqs * a->vocab >= (4 << 20) ? 2 : 1; }
+int verify_splits(const mtc_verify_args* a) {
+  const int span = kVerifyThreads * 8 * verify_rounds(a);
+  return (a->vocab + span - 1) / span;
 }
 
 int check_verify(const mtc_verify_args* a) {
@@ -581,14 +620,19 @@ int check_verify(const mtc_verify_args* a) {
   if (a->n_seqs < 0 || a->n_seqs > 65535) return fail(MTC_E_SHAPE, "%d sequences: 0 to 65535", a->n_seqs);
   if (a->n_drafted < 0 || a->n_drafted > kMaxDrafted) return fail(MTC_E_SHAPE, "%d drafts: 0 to %d", a->n_drafted, kMaxDrafted);
   if (a->vocab < 1 || a->vocab > 0x3FFFFFFF) return fail(MTC_E_SHAPE, "vocabulary of %d", a->vocab);
+  if ((int64_t)verify_splits(a) * a->n_seqs > 0xFFFFFF)                                    // 2^32 threads a launch
+    return fail(MTC_E_SHAPE, "%d sequences of a vocabulary of %d: too many", a->n_seqs, a->vocab);
   return MTC_OK;
 }
 
 template <int DT>
-int run_verify(const mtc_verify_args& a, Best* best, int splits, int span, hipStream_t st) {
-  k_verify<DT><<<dim3(splits, a.n_seqs), kVerifyThreads, 0, st>>>(a, best, span);
+int run_verify(const mtc_verify_args& a, Found* found, hipStream_t st) {
+  const int splits = verify_splits(&a);
+  const dim3 grid(splits, a.n_seqs);
+  if (verify_rounds(&a) == 2) k_verify<DT, 2><<<grid, kVerifyThreads, 0, st>>>(a, found);
+  else k_verify<DT, 1><<<grid, kVerifyThreads, 0, st>>>(a, found);
   if (int rc = check_launch("k_verify")) return rc;
-  k_verify_join<DT><<<a.n_seqs, 64, 0, st>>>(a, best, splits);
+  k_verify_join<<<a.n_seqs, 64, 0, st>>>(a, found, splits);
   return check_launch("k_verify_join");
 }
 
@@ -652,11 +696,9 @@ MTC_API int mtc_cache_compact(const mtc_cache_desc* c, void* hip_stream) {
   hipStream_t st = (hipStream_t)hip_stream;
   k_compact_plan<<<1, kThreads, 0, st>>>(*c);
   if (int rc = check_launch("k_compact_plan")) return rc;
-  k_compact_table<<<std::min((c->max_seqs + 3) / 4, 1024), 256, 0, st>>>(*c);
-  if (int rc = check_launch("k_compact_table")) return rc;
-  k_copy_pages<<<copy_grid(c, c->n_pages / 2 + 1), kCopyThreads, 0, st>>>((char*)c->pool, (const char*)c->pool, page_bytes(c), c->n_pages,
-                                                                          c->n_pages, scratch_src(*c), scratch_dst(*c), c->state + kPairs, 0);
-  return check_launch("k_copy_pages");
+  const int table_blocks = std::min((c->max_seqs + 3) / 4, 256);
+  k_compact<<<table_blocks + copy_grid(c, c->n_pages / 2 + 1), kCopyThreads, 0, st>>>(*c, page_bytes(c), table_blocks);
+  return check_launch("k_compact");
 }
 
 MTC_API int mtc_cache_copy_pages(const mtc_cache_desc* c, const void* from_pool, int from_pages, const int32_t* src,
@@ -697,8 +739,7 @@ MTC_API int mtc_cache_append(const mtc_cache_desc* c, int layer, const mtc_heads
 
 MTC_API size_t mtc_verify_workspace_bytes(const mtc_verify_args* a) {
   if (check_verify(a) != MTC_OK) return 0;
-  int span;
-  return (size_t)a->n_seqs * verify_splits(a, &span) * sizeof(Best);
+  return (size_t)a->n_seqs * verify_splits(a) * sizeof(Found);
 }
 
 MTC_API int mtc_verify_drafts(const mtc_verify_args* a, void* workspace, size_t workspace_bytes, void* hip_stream) {
@@ -706,15 +747,13 @@ MTC_API int mtc_verify_drafts(const mtc_verify_args* a, void* workspace, size_t 
   if (a->n_seqs == 0) return ok();
   if (!a->p || !a->noise || !a->tokens || !a->accepted) return fail(MTC_E_NULL, "p, noise, tokens or accepted is NULL");
   if (a->n_drafted && (!a->q || !a->u || !a->drafts)) return fail(MTC_E_NULL, "q, u or drafts is NULL");
-  int span;
-  const int splits = verify_splits(a, &span);
-  const size_t need = (size_t)a->n_seqs * splits * sizeof(Best);
+  const size_t need = (size_t)a->n_seqs * verify_splits(a) * sizeof(Found);
   if (!workspace || workspace_bytes < need)
     return fail(MTC_E_WORKSPACE, "workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : (size_t)0, need);
   if ((uintptr_t)workspace % 256) return fail(MTC_E_WORKSPACE, "workspace must be 256-byte aligned");
-  Best* best = (Best*)workspace;
+  Found* found = (Found*)workspace;
   hipStream_t st = (hipStream_t)hip_stream;
-  if (a->dtype == MTC_DTYPE_F32) return run_verify<MTC_DTYPE_F32>(*a, best, splits, span, st);
-  if (a->dtype == MTC_DTYPE_BF16) return run_verify<MTC_DTYPE_BF16>(*a, best, splits, span, st);
-  return run_verify<MTC_DTYPE_F16>(*a, best, splits, span, st);
+  if (a->dtype == MTC_DTYPE_F32) return run_verify<MTC_DTYPE_F32>(*a, found, st);
+  if (a->dtype == MTC_DTYPE_BF16) return run_verify<MTC_DTYPE_BF16>(*a, found, st);
+  return run_verify<MTC_DTYPE_F16>(*a, found, st);
 }
