@@ -441,11 +441,12 @@ struct Found {                     // of one block
   Best best;
   int32_t accepted, reserved[3];
 };
+constexpr float kNoScore = -1.0f;  // below every score of a w > 0
+// Without branches: of 16 elements a thread, each would be taken by some lane.
 __device__ __forceinline__ void better(float& a, int32_t& ai, float b, int32_t bi) {
-  if (bi >= 0 && (ai < 0 || b > a || (b == a && bi < ai))) {
-    a = b;
-    ai = bi;
-  }
+  const bool take = b > a || (b == a && (uint32_t)bi < (uint32_t)ai);
+  a = take ? b : a;
+  ai = take ? bi : ai;
 }
 
 template <int DT>
@@ -482,23 +483,21 @@ template <int DT>
 __device__ int accepted(const mtc_verify_args& a, int b, int& k) {
   typedef typename Prob<DT>::type T;
   const int j = threadIdx.x & 63;
+  const int64_t x = j < a.n_drafted ? draft_at(a, b, j) : -1;
+  const float u = j < a.n_drafted ? a.u[(int64_t)b * a.u_stride + j] : 0.0f;
   k = a.n_drafts ? min(max(a.n_drafts[b], 0), a.n_drafted) : a.n_drafted;
-  bool good = true;                // past the last draft: stops the run below by k
-  if (j < k) {
-    const int64_t x = draft_at(a, b, j);
-    good = false;
-    if (x >= 0 && x < a.vocab) {
-      const float p = Prob<DT>::get(reinterpret_cast<const T*>(a.p)[(int64_t)b * a.p_stride[0] + (int64_t)j * a.p_stride[1] + x]);
-      const float q = Prob<DT>::get(reinterpret_cast<const T*>(a.q)[(int64_t)b * a.q_stride[0] + (int64_t)j * a.q_stride[1] + x]);
-      good = a.u[(int64_t)b * a.u_stride + j] * q < p;
-    }
+  float p = 0.0f, q = 0.0f;        // outside the vocabulary: never accepted
+  if (x >= 0 && x < a.vocab) {
+    p = Prob<DT>::get(reinterpret_cast<const T*>(a.p)[(int64_t)b * a.p_stride[0] + (int64_t)j * a.p_stride[1] + x]);
+    q = Prob<DT>::get(reinterpret_cast<const T*>(a.q)[(int64_t)b * a.q_stride[0] + (int64_t)j * a.q_stride[1] + x]);
   }
+  const bool good = j >= k || u * q < p;           // past the last draft: k ends the run below
   const uint64_t wrong = __ballot(!good);
   return wrong ? __ffsll((unsigned long long)wrong) - 1 : k;
 }
 
 // One block per sequence and span of the vocabulary. The noise does not depend on how many drafts were accepted, so its
-// loads are in flight while that chain of three dependent loads (count, drafts, their probabilities) is followed.
+// loads are in flight while that chain of dependent loads (drafts, their probabilities) is followed.
 template <int DT, int ROUNDS>
 __global__ __launch_bounds__(kVerifyThreads) void k_verify(const mtc_verify_args a, Found* found) {
   typedef typename Prob<DT>::type T;
@@ -516,10 +515,14 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify(const mtc_verify_args
   const bool minus = n < k;
   const T* p = reinterpret_cast<const T*>(a.p) + (int64_t)b * a.p_stride[0] + (int64_t)n * a.p_stride[1];
   const T* q = minus ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.q_stride[0] + (int64_t)n * a.q_stride[1] : p;
-  Best best{0.0f, 0.0f, -1, -1};
-  auto one = [&](int i, float w, float d, float z) {
-    if (w > 0.0f) better(best.all, best.all_i, w * z, i);
-    if (d > 0.0f) better(best.rest, best.rest_i, d * z, i);
+  Best best{kNoScore, kNoScore, -1, -1};
+  auto one = [&](int i, float w, float d, float z) {       // i ascends in a thread: the first of equals stays
+    const float all = w > 0.0f ? w * z : kNoScore, rest = d > 0.0f ? d * z : kNoScore;
+    const bool x = all > best.all, y = rest > best.rest;
+    best.all = x ? all : best.all;
+    best.all_i = x ? i : best.all_i;
+    best.rest = y ? rest : best.rest;
+    best.rest_i = y ? i : best.rest_i;
   };
   Eight<T> pv[ROUNDS], qv[ROUNDS];
 #pragma unroll
@@ -563,7 +566,7 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify(const mtc_verify_args
 __global__ __launch_bounds__(64) void k_verify_join(const mtc_verify_args a, const Found* found, int splits) {
   const int b = blockIdx.x, lane = threadIdx.x;
   const int n = found[(int64_t)b * splits].accepted;
-  Best r{0.0f, 0.0f, -1, -1};
+  Best r{kNoScore, kNoScore, -1, -1};
   for (int i = lane; i < splits; i += 64) {
     const Best x = found[(int64_t)b * splits + i].best;
     better(r.rest, r.rest_i, x.rest, x.rest_i);
