@@ -189,7 +189,40 @@ struct RowTile {
         const u32x2 hi = lds_read_transposed(v_at[d] + (v + (ks * 16 + 8) * kRow));
         o[d] = E::mfma32(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[ks], o[d]);
       }
-    if constexpr (NEXT) maximum<MASKED>(n, c, left);
+    if constexpr (NEXT) {
+      maximum<MASKED>(n, c, left);
+    }
+    if constexpr (NEXT && DP == 128) {
+      // Order: LDS reads four ahead of the multiplications that take them, the weights spread over the first half of those
+      // (1 x 16384, 32/8 x 128: 1981 -> 1937 us; with 64 dims it costs a wave per SIMD: 39 -> 45 us for 24 ragged 14/2)
+      constexpr int kQK = 2 * kSteps, kPV = 4 * (DP / 32), kValu = 6, kExp = (32 + kQK - 1) / kQK;
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < kQK - 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, kValu, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, kExp, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, kValu, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, kExp, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kPV - 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      }
+    }
   }
 
   // All tiles: `mine` of them have keys for this wave, of which all rows see the first `full` whole. first_keys() makes tile
