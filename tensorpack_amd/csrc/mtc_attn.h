@@ -160,10 +160,17 @@ __device__ __forceinline__ float half_sum(float x) {
   return low + high;
 }
 
+template <bool BF>
+__device__ __forceinline__ bool finite16(uint16_t x) {
+  constexpr uint32_t exponent = BF ? 0x7F80u : 0x7C00u;
+  return (x & exponent) != exponent;
+}
+
 // One row by a plain loop over its `seen` keys (one wave; lane l ends with o for dims l and l + 64). The tile
 // kernels multiply keys that a row does not see by weights of 0, which is not 0 where V holds an infinity
-// or a NaN: rows that come out not finite are computed again here, where unseen keys are never read.
-// kv(j) gives the addresses of key j's K and V.
+// or a NaN: rows that come out not finite beside such keys are computed again here, where unseen keys are never read.
+// From the last key back, so that a row that itself sees a NaN score (its result is NaN) mostly ends soon.
+// kv(j) gives the addresses of key j's K and V (16-byte aligned rows).
 template <bool BF, class KV>
 __device__ void plain_row(const uint16_t* q, int dim, int seen, float c, KV kv, float& o0, float& o1) {
   const int lane = threadIdx.x & 63;
@@ -171,11 +178,27 @@ __device__ void plain_row(const uint16_t* q, int dim, int seen, float c, KV kv, 
     const uint16_t *k, *v;
     kv(j, k, v);
     float s = 0.0f;
-    for (int d = 0; d < dim; ++d) s = __builtin_fmaf(Elem<BF>::widen(q[d]), Elem<BF>::widen(k[d]), s);
+    for (int d = 0; d < dim; d += 8) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(q + d), y = *reinterpret_cast<const u32x4*>(k + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = x[i], b = y[i];
+        s = __builtin_fmaf(Elem<BF>::widen((uint16_t)a), Elem<BF>::widen((uint16_t)b), s);
+        s = __builtin_fmaf(Elem<BF>::widen((uint16_t)(a >> 16)), Elem<BF>::widen((uint16_t)(b >> 16)), s);
+      }
+    }
     return s;
   };
   float top = -INFINITY;
-  for (int j = lane; j < seen; j += 64) top = fmaxf(top, score(j));
+  for (int j0 = seen; j0 > 0; j0 -= 64) {
+    const int j = j0 - 1 - lane;
+    const float s = j >= 0 ? score(j) : -INFINITY;
+    if (__ballot(s != s)) {
+      o0 = o1 = __builtin_nanf("");
+      return;
+    }
+    top = fmaxf(top, s);
+  }
   top = wave_max(top);
   float sum = 0.0f;
   o0 = o1 = 0.0f;
@@ -192,6 +215,7 @@ __device__ void plain_row(const uint16_t* q, int dim, int seen, float c, KV kv, 
     }
   }
   sum = wave_sum(sum);
+  if (sum == 0.0f) return;                         // no keys, or none with a weight: 0
   o0 /= sum;
   o1 /= sum;
 }

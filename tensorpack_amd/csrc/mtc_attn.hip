@@ -354,9 +354,16 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
     }
   uint64_t again = __ballot(row < pt.n && !fine);
   again = (again | (again >> 32)) & 0xFFFFFFFFull;
+  const int read = min((wave_keys + kPromptKeys - 1) / kPromptKeys * kPromptKeys, pt.m);    // keys that the wave multiplied
   while (again) {
     const int r = wave_first + __ffsll((unsigned long long)again) - 1;
     again &= again - 1;
+    bool clean = true;                             // nothing unseen can have got in: the row's own keys made it so
+    for (int key = sees(r); key < read; ++key) {
+      const uint16_t* v = reinterpret_cast<const uint16_t*>((uintptr_t)v_base) + (int64_t)key * a.v.row_stride;
+      clean = clean && !(lane < D && !finite16<BF>(v[lane])) && !(lane + 64 < D && !finite16<BF>(v[lane + 64]));
+    }
+    if (!__ballot(!clean)) continue;
     float o0, o1;
     plain_row<BF>(reinterpret_cast<const uint16_t*>(a.q.data) + (int64_t)(pt.q0 + r) * a.q.row_stride + (int64_t)head * a.q.head_stride,
                   D, sees(r), c,
@@ -1110,12 +1117,20 @@ __global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, int
   const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
   y *= inv;
   uint16_t* out = reinterpret_cast<uint16_t*>(a.o.data) + ((int64_t)b * a.tokens + t) * a.o.row_stride + (int64_t)h * a.o.head_stride;
-  if (__ballot(!(finite(y[0]) && finite(y[1]) && finite(y[2]) && finite(y[3])))) {
-    const Seq s = cached_seq(a, b);
+  bool again = __ballot(!(finite(y[0]) && finite(y[1]) && finite(y[2]) && finite(y[3])));
+  Seq s{0, 0, 0};
+  int seen = 0;
+  if (again) {                                           // only if keys were read that the row does not see
+    s = cached_seq(a, b);
+    seen = row_sees(s.len, s.q_len, t);
+    const int g = group_of(a.n_groups, b, [&](int i) { return group_start(a, i); });
+    again = seen < s.len || (g >= 0 && seen < prefix_tokens(a, g));
+  }
+  if (again) {
     const int32_t* table = a.table + (int64_t)s.row * a.max_pages;
     float y0, y1;
     plain_row<BF>(reinterpret_cast<const uint16_t*>(a.q.data) + ((int64_t)b * a.tokens + t) * a.q.row_stride + (int64_t)h * a.q.head_stride,
-                  D, row_sees(s.len, s.q_len, t), a.c,
+                  D, seen, a.c,
                   [&](int key, const uint16_t*& k, const uint16_t*& v) {
                     const int id = min(max(table[key >> a.page_log], 0), a.n_pages - 1);
                     const uint16_t* p = a.pool + (int64_t)id * a.page_elems +

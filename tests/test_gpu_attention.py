@@ -148,6 +148,33 @@ def test_prompt_ignores_what_it_does_not_see(gpu):
         a += n
 
 
+def test_rows_without_keys_beside_a_nan(gpu):
+    # rows that see nothing are 0 also where the tile's keys hold a NaN
+    import torch
+    from tensorpack_amd.attention import cached_attention, prompt_attention
+    q, k, v = (_normal(s, (n, 2, 64), _dtype("bf16"), gpu) for s, n in ((1, 100), (2, 40), (3, 40)))
+    v[0], k[39] = math.nan, math.nan
+    got = prompt_attention(q, k, v, _offsets([100], gpu), _offsets([40], gpu))    # the first 60 queries precede every key
+    assert not got[:60].any() and torch.isnan(got[60:]).all()
+    v[0] = 0
+    assert not torch.isnan(prompt_attention(q, k, v, _offsets([100], gpu), _offsets([40], gpu))[:99]).any()
+    cache = _cache(gpu, [70], 16, 1, 64, "bf16", layers=1)
+    cache.pool[int(cache.table[0, 0]), 0, 1, :, 3] = math.inf
+    q = _normal(9, (1, 8, 2, 64), _dtype("bf16"), gpu)
+    got = cached_attention(q, cache, 0, _ints([0], gpu), q_lens=_ints([5], gpu))
+    assert not got[0, 5:].any() and not torch.isfinite(got[0, :5]).any()
+
+
+def test_prompt_all_nan_ends(gpu):
+    # every key a NaN: the rows are NaN, without a plain loop over all of them
+    import torch
+    from tensorpack_amd.attention import prompt_attention
+    q, k, v = (_normal(s, (4096, 4, 64), _dtype("bf16"), gpu) for s in (1, 2, 3))
+    k[2048:], v[2048:] = math.nan, math.nan
+    got = prompt_attention(q, k, v, _offsets([4096], gpu))
+    assert torch.isnan(got[2048:]).all() and torch.isfinite(got[:2048]).all()
+
+
 def test_prompt_large_scores(gpu):
     # one key takes all the weight; scores of the type's range; a scale of its own
     from tensorpack_amd.attention import prompt_attention
