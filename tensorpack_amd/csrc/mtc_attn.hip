@@ -257,6 +257,15 @@ struct RowTile {
   }
 };
 
+// One block per tile of 128 queries and head: softmax in one pass over the keys (running maximum m and sum l; o and l are
+// scaled by 2^(m - m') when m moves to m'), 64 keys a step, K and V copied to LDS a step ahead of their use. 128 queries in
+// four waves let two blocks share a CU, whose barriers then do not stop each other: four waves of 32 queries read 16
+// KiB of each tile per 32 matrix instructions, which LDS supplies while they run.
+// Bound by the matrix and vector units: of a wave's 2950 cycles a step with 128 dims (two waves a SIMD), 975 are matrix
+// instructions, 860 vector issue, 680 waits for LDS and barriers. 1 x 16384, 32/8 heads of 128, causal: 1937 to 2080 us,
+// 1.06 to 1.14 PFLOP/s, the clock at 1.7 GHz under the load (an 8192^3 library product: 1.22 PFLOP/s). Calls of few blocks wait for
+// the longest (512 new queries on 4608 keys: 72 steps of 1.6 us, 119 us). Not kept: two waves per 32 queries with half the
+// keys each (129 us), two sets of four waves on alternate tiles (130 us).
 template <bool BF, int DP>
 __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_prompt_args a) {
   using E = Elem<BF>;
@@ -994,6 +1003,12 @@ __device__ __forceinline__ int spread(int xcd, int at, int each, int runs) {
   return at < per ? xcd * per + at : runs;
 }
 
+// 512 blocks whatever the call. Every block reads the lists and sums the units by itself (3.5 us until its first keys'
+// copies start, 4.5 with groups), which is less than a planning launch would take.
+// Bound by memory for few rows: 32 sequences of 8192, 32/8 heads of 128: 1.07 GB in 185 us, 5.8 TB/s (a 1 GiB copy: 5.2);
+// 32 ragged up to 16384: 252 MB in 41 us. 64 sequences on one prefix of 8192: 35 us, where the prefix's 2048 units of
+// 128 rows take 9.6 us of the whole chip and 26 MB of own keys 4.6; what is left is the start, the partial results (64 KB a
+// run) and blocks that share a CU. Smallest calls: 6 us.
 template <bool BF, int DP, int OWN, int PRE>
 __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a) {
   constexpr int kStage = kCachedWaves * 2 * kWaveKeys * DP * 2;     // = 2 buffers of K and V tiles of 64 keys for split rows, halved
@@ -1064,7 +1079,8 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const CachedCall a
 }
 
 // One wave per (sequence, token, head): the partial results of its row, the prefix's and the own part's. A lane holds
-// four dims: a quarter (DP 64) or half of the wave reads one slot's row, so one load covers several slots.
+// four dims: a quarter (DP 64) or half of the wave reads one slot's row, so one load covers several slots, and eight
+// loads are in flight (one dim a lane and four loads: 9 to 15 us for 32 ragged sequences, now 4.8).
 template <bool BF, int DP>
 __global__ __launch_bounds__(kCachedThreads) void k_join(const CachedCall a, int own_rows, int own_start, int pre_rows, int pre_start) {
   constexpr int kLanes = DP / 4, kPer = 64 / kLanes, kBatch = 8;      // lanes and slots per load, loads in flight
