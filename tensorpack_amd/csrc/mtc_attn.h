@@ -34,6 +34,9 @@ struct Elem<true> {
     x2 p = {(__bf16)a, (__bf16)b};
     return __builtin_bit_cast(uint32_t, p);
   }
+  static __device__ __forceinline__ float add2(uint32_t p, float s) {      // s + both elements of p, in fp32
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(x2, p), x2{(__bf16)1.0f, (__bf16)1.0f}, s, false);
+  }
   static __device__ __forceinline__ uint16_t round(float a) { return __builtin_bit_cast(uint16_t, (__bf16)a); }
   static __device__ __forceinline__ float widen(uint16_t a) { return __builtin_bit_cast(float, (uint32_t)a << 16); }
 };
@@ -50,6 +53,9 @@ struct Elem<false> {
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     x2 p = {(_Float16)a, (_Float16)b};
     return __builtin_bit_cast(uint32_t, p);
+  }
+  static __device__ __forceinline__ float add2(uint32_t p, float s) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(x2, p), x2{(_Float16)1.0f, (_Float16)1.0f}, s, false);
   }
   static __device__ __forceinline__ uint16_t round(float a) { return __builtin_bit_cast(uint16_t, (_Float16)a); }
   static __device__ __forceinline__ float widen(uint16_t a) { return (float)__builtin_bit_cast(_Float16, a); }

@@ -172,15 +172,18 @@ struct RowTile {
     const float base = top == -INFINITY ? 0.0f : top;
     if constexpr (NEXT) multiply(k, n);
     u32x4 p[4];
+    float add[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         const float x = exp2_fast(__builtin_fmaf(s[g][e], c, -base));
         const float y = exp2_fast(__builtin_fmaf(s[g][e + 1], c, -base));
-        sum += x + y;
-        p[g * 2 + (e >> 3)][(e & 7) >> 1] = E::pack(x, y);     // weights of 16 bits: the matrix core's operand
+        const uint32_t w = E::pack(x, y);          // weights of 16 bits: the matrix core's operand
+        add[(e >> 1) & 1] = E::add2(w, add[(e >> 1) & 1]);     // and what is summed, so that the quotient's parts agree
+        p[g * 2 + (e >> 3)][(e & 7) >> 1] = w;
       }
+    sum += add[0] + add[1];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
