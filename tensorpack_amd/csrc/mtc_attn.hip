@@ -29,6 +29,17 @@ using namespace mtc::attn;
 
 namespace {
 
+// Inclusive sum over the wave's lanes (row shifts, then the rows' totals).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);      // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);     // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);     // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
 // ---------------------------------------------------------------------------
 // whole prompts
 // ---------------------------------------------------------------------------
@@ -47,19 +58,26 @@ __device__ __forceinline__ void prompt_range(const int32_t* cu, int b, int rows,
 }
 
 // The rank-th query tile of the call, the tiles with the largest place in their sequence first (with a
-// causal mask these see most keys; started last they would run alone at the end). Every lane gets it.
+// causal mask these see most keys; started last they would run alone at the end). Every lane gets it. The ranges of the first
+// 64 sequences stay in the lanes, one each: one round of loads for calls of up to 64.
 __device__ PromptTile prompt_tile(const mtc_prompt_args& a, int rank) {
   const int lane = threadIdx.x & 63;
-  auto tiles = [&](int b) {
-    int at, n;
-    prompt_range(a.cu_q, b, a.q_rows, at, n);
-    return (n + kPromptRows - 1) / kPromptRows;
-  };
-  const int t0 = lane < a.n_seqs ? tiles(lane) : 0;
+  auto tiles = [](int n) { return (n + kPromptRows - 1) / kPromptRows; };
+  auto range = [&](int b, int& q0, int& n) { prompt_range(a.cu_q, b, a.q_rows, q0, n); };
+  int q0 = 0, n0 = 0, k0 = 0, m0 = 0;               // of sequence `lane`
+  if (lane < a.n_seqs) {
+    range(lane, q0, n0);
+    prompt_range(a.cu_k, lane, a.k_rows, k0, m0);
+  }
+  const int t0 = tiles(n0);
   auto count = [&](int level) {                     // tiles at `level` or above
     int s = max(0, t0 - level);
-    for (int b = lane + 64; b < a.n_seqs; b += 64) s += max(0, tiles(b) - level);
-    return wave_sum(s);
+    for (int b = lane + 64; b < a.n_seqs; b += 64) {
+      int at, n;
+      range(b, at, n);
+      s += max(0, tiles(n) - level);
+    }
+    return __builtin_amdgcn_readlane(wave_scan(s), 63);
   };
   PromptTile r;
   r.tile = -1;
@@ -78,11 +96,16 @@ __device__ PromptTile prompt_tile(const mtc_prompt_args& a, int rank) {
     }
     int left = rank - count(hi);                    // the left-th sequence with more than lo tiles
     for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
-      const bool has = b0 + lane < a.n_seqs && (b0 ? tiles(b0 + lane) : t0) > lo;
-      const uint64_t mask = __ballot(has);
+      int t = t0;
+      if (b0) {
+        int at, n = 0;
+        if (b0 + lane < a.n_seqs) range(b0 + lane, at, n);
+        t = tiles(n);
+      }
+      const uint64_t mask = __ballot(t > lo);
       const int c = __popcll(mask);
       if (left < c) {
-        const uint64_t hit = __ballot(has && __popcll(mask & ((1ull << lane) - 1)) == left);
+        const uint64_t hit = __ballot(t > lo && __popcll(mask & ((1ull << lane) - 1)) == left);
         seq = b0 + __ffsll((unsigned long long)hit) - 1;
         break;
       }
@@ -90,8 +113,16 @@ __device__ PromptTile prompt_tile(const mtc_prompt_args& a, int rank) {
     }
     r.tile = lo;
   }
-  prompt_range(a.cu_q, seq, a.q_rows, r.q0, r.n);
-  prompt_range(a.cu_k, seq, a.k_rows, r.k0, r.m);
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  if (seq < 64) {
+    r.q0 = __builtin_amdgcn_readlane(q0, seq);
+    r.n = __builtin_amdgcn_readlane(n0, seq);
+    r.k0 = __builtin_amdgcn_readlane(k0, seq);
+    r.m = __builtin_amdgcn_readlane(m0, seq);
+  } else {
+    range(seq, r.q0, r.n);
+    prompt_range(a.cu_k, seq, a.k_rows, r.k0, r.m);
+  }
   return r;
 }
 
@@ -358,11 +389,18 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const float x0 = rt.o[d][e] * inv, x1 = rt.o[d][e + 1] * inv, x2 = rt.o[d][e + 2] * inv, x3 = rt.o[d][e + 3] * inv;
-      fine = fine && finite(x0) && finite(x1) && finite(x2) && finite(x3);
-      const int at = d * 32 + 2 * e + 4 * half;
-      if (row < pt.n && at < D) *reinterpret_cast<u32x2*>(op + at) = u32x2{E::pack(x0, x1), E::pack(x2, x3)};
+    for (int e = 0; e < 16; e += 8) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = rt.o[d][e + 2 * i] * inv, y = rt.o[d][e + 2 * i + 1] * inv;
+        fine = fine && finite(x) && finite(y);
+        w[i] = E::pack(x, y);
+      }
+      // the halves hold dims 4 half + 0..3 of 8-dim groups e/4 and e/4 + 1: after the swap each has one group whole
+      const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+      const int at = d * 32 + 2 * e + 8 * half;
+      if (row < pt.n && at < D) *reinterpret_cast<u32x4*>(op + at) = u32x4{x[0], y[0], x[1], y[1]};
     }
   uint64_t again = __ballot(row < pt.n && !fine);
   again = (again | (again >> 32)) & 0xFFFFFFFFull;
@@ -551,17 +589,6 @@ __device__ __forceinline__ Entry cached_entry(const CachedCall& a, const Book& b
   r.items = a.kv_heads * r.tiles;
   r.units = r.to > r.from ? (r.to - r.from + mode_unit(MODE) - 1) / mode_unit(MODE) + mode_start(MODE) : 0;
   return r;
-}
-
-// Inclusive sum over the wave's lanes (row shifts, then the rows' totals).
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);      // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);     // row_bcast:15 into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);     // row_bcast:31 into rows 2 and 3
-  return x;
 }
 
 // Running sums over the entries: every thread of the block has the sums before its run of entries [e0, e1).
