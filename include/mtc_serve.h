@@ -42,6 +42,8 @@ typedef struct mtc_heads {
  * being the last tokens. A row that sees no key is 0. Keys that a row does not see have no part in it,
  * whatever they hold (infinities and NaN included). dtype: bf16 or f16 for q, k, v and o; products
  * on the matrix cores, sums and softmax in fp32. Rows of o outside every sequence are not written.
+ * Workspace: mtc_prompt_attention_workspace_bytes (0 but for calls of few rows on many keys, whose keys are split over
+ * blocks), 256-byte aligned, no initialisation.
  */
 typedef struct mtc_prompt_args {
   uint32_t abi_version;
@@ -62,7 +64,8 @@ typedef struct mtc_prompt_args {
   const int32_t* cu_k;
 } mtc_prompt_args;
 
-int mtc_prompt_attention(const mtc_prompt_args* a, void* hip_stream);
+size_t mtc_prompt_attention_workspace_bytes(const mtc_prompt_args* a);
+int mtc_prompt_attention(const mtc_prompt_args* a, void* workspace, size_t workspace_bytes, void* hip_stream);
 
 /*
  * The paged cache. The pool holds n_pages pages, each contiguous:

@@ -24,7 +24,7 @@ EXPORTED = ("mtc_abi_version", "mtc_last_error", "mtc_check_desc", "mtc_dequant"
             "mtc_gemm_bf16_batch", "mtc_gemm_f32_workspace_bytes", "mtc_gemm_f32", "mtc_tile_plan",
             "mtc_set_prefill_decode_once")
 
-SERVE_EXPORTED = ("mtc_prompt_attention", "mtc_check_cache_desc", "mtc_cache_scratch_ints", "mtc_cache_extend",
+SERVE_EXPORTED = ("mtc_prompt_attention_workspace_bytes", "mtc_prompt_attention", "mtc_check_cache_desc", "mtc_cache_scratch_ints", "mtc_cache_extend",
                   "mtc_cache_fork", "mtc_cache_truncate", "mtc_cache_compact", "mtc_cache_copy_pages", "mtc_cache_append",
                   "mtc_cached_attention_workspace_bytes", "mtc_cached_attention", "mtc_verify_workspace_bytes",
                   "mtc_verify_drafts")
@@ -217,7 +217,8 @@ def declare_serve(lib: ctypes.CDLL) -> None:
     vp, i32, sz, P = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.POINTER
     cache = P(MtcCacheDesc)
     for name, res, args in (
-            ("mtc_prompt_attention", i32, [P(MtcPromptArgs), vp]),
+            ("mtc_prompt_attention_workspace_bytes", sz, [P(MtcPromptArgs)]),
+            ("mtc_prompt_attention", i32, [P(MtcPromptArgs), vp, sz, vp]),
             ("mtc_check_cache_desc", i32, [cache]),
             ("mtc_cache_scratch_ints", sz, [i32, i32]),
             ("mtc_cache_extend", i32, [cache, vp, vp, i32, vp]),

@@ -98,7 +98,10 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: Op
     q, k, v = _kernel_heads(q), _kernel_heads(k), _kernel_heads(v)
     args = _abi.MtcPromptArgs(_abi.ABI_VERSION, dt, n, heads, kv_heads, dim, rows, keys, causal, scale,
                               _heads(q), _heads(k), _heads(v), _heads(out), cq, ck)
-    rc = lib.mtc_prompt_attention(ctypes.byref(args), raw_stream(dev.index))
+    ref, stream = ctypes.byref(args), raw_stream(dev.index)
+    need = lib.mtc_prompt_attention_workspace_bytes(ref)
+    ws = stream_workspace(dev.index, stream, need).data_ptr() if need else None
+    rc = lib.mtc_prompt_attention(ref, ws, need, stream)
     if rc:
         _abi.check(lib, "mtc_prompt_attention", rc)
     return out

@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "mtc_attn.h"
 #include "mtc_host.h"
@@ -300,8 +301,18 @@ struct RowTile {
 // 1.06 to 1.14 PFLOP/s, the clock at 1.7 GHz under the load (an 8192^3 library product: 1.22 PFLOP/s). Calls of few blocks wait for
 // the longest (512 new queries on 4608 keys: 72 steps of 1.6 us, 119 us). Not kept: two waves per 32 queries with half the
 // keys each (129 us), two sets of four waves on alternate tiles (130 us).
-template <bool BF, int DP>
-__global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_prompt_args a) {
+//
+// PARTS: for calls of few tiles (a short chunk of new tokens on many older ones), `parts.n` blocks share a tile, each with a run
+// of its steps, and k_prompt_join joins their partial results (4 to 5 us). A call, unsplit and split: 117 queries on 5175 keys,
+// 14/2 heads of 40: 83.6 -> 18.4 us; 100 on 2000, 32/8 of 128: 62.1 -> 25.2; 400 on 16000, 8/1 of 128: 454 -> 54.3; 1 on 600,
+// 32/8 of 128: 22.6 -> 12.1; 300 on 600, 14/2 of 64, the least gain: 14.1 -> 13.3.
+struct PromptParts {
+  float* o;                // [part][row of q][head][dim]
+  float* ml;               // [part][row of q][head][2]: maximum (times c), sum (0: no keys, o is not written)
+  int32_t n;
+};
+template <bool BF, int DP, bool PARTS>
+__global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_prompt_args a, const PromptParts parts) {
   using E = Elem<BF>;
   constexpr int kRow = DP * 2;                             // bytes of an LDS row
   constexpr int kTile = kPromptKeys * kRow;
@@ -314,7 +325,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
   // count of K/V heads is a multiple or a divisor of 8
   const int j = blockIdx.x % H;
   const int kvh = j % KV, head = kvh * (H / KV) + j / KV;
-  PromptTile pt = prompt_tile(a, blockIdx.x / H);
+  const int rank_part = blockIdx.x / H, part = PARTS ? rank_part % parts.n : 0;
+  PromptTile pt = prompt_tile(a, PARTS ? rank_part / parts.n : rank_part);
   pt.tile = __builtin_amdgcn_readfirstlane(pt.tile);      // the same in every lane: scalars from here on
   pt.q0 = __builtin_amdgcn_readfirstlane(pt.q0);
   pt.n = __builtin_amdgcn_readfirstlane(pt.n);
@@ -333,7 +345,9 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
   const int wave_first = pt.tile * kPromptRows + wave * 32;
   const int wave_keys = wave_first < pt.n ? sees(wave_last) : 0;   // keys that any row of the wave sees
   const int all_keys = wave_first + 31 < pt.n ? sees(wave_first) : 0;   // keys that all its rows see
-  const int steps = (sees(last_row) + kPromptKeys - 1) / kPromptKeys;
+  const int all_steps = (sees(last_row) + kPromptKeys - 1) / kPromptKeys;
+  const int step0 = PARTS ? all_steps * part / parts.n : 0;          // this block's tiles of keys: step0 ..
+  const int steps = (PARTS ? all_steps * (part + 1) / parts.n : all_steps) - step0;
 
   const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q.data) + (int64_t)(pt.q0 + row) * a.q.row_stride +
                        (int64_t)head * a.q.head_stride;
@@ -353,8 +367,9 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
   }
   const uint32_t lds0 = lds_addr(lds);
   auto copy = [&](uint64_t base, uint32_t bytes, const uint32_t* off, int t, uint32_t place) {
-    const uint32_t rows = (uint32_t)min(kPromptKeys, pt.m - t * kPromptKeys);
-    const u32x4 r = buffer_rsrc(base + (uint64_t)t * kPromptKeys * bytes, (rows - 1) * bytes + D * 2);
+    const int at = (step0 + t) * kPromptKeys;
+    const uint32_t rows = (uint32_t)min(kPromptKeys, pt.m - at);
+    const u32x4 r = buffer_rsrc(base + (uint64_t)at * bytes, (rows - 1) * bytes + D * 2);
     const uint32_t dst = lds0 + place * kTile + wave * kCopies * 1024;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) copy16(r, off[i], __builtin_amdgcn_readfirstlane(dst + i * 1024));
@@ -365,7 +380,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
 
   const float c = a.scale * kLog2e;
   rt.run(
-      steps, (wave_keys + kPromptKeys - 1) / kPromptKeys, all_keys / kPromptKeys, c,
+      steps, min(max((wave_keys + kPromptKeys - 1) / kPromptKeys - step0, 0), steps), min(max(all_keys / kPromptKeys - step0, 0), steps), c,
       [&]() {
         copy_keys(0);
         copy_values(0);
@@ -379,9 +394,23 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
         if (t + 1 < steps) copy_values(t + 1);
         if (t + 2 < steps) copy_keys(t + 2);
       },
-      [&](int t) { return seen - t * kPromptKeys; });
+      [&](int t) { return seen - (step0 + t) * kPromptKeys; });
 
   const float sum = half_sum(rt.sum);
+  if constexpr (PARTS) {
+    if (row >= pt.n) return;
+    const int64_t at = ((int64_t)part * a.q_rows + pt.q0 + row) * H + head;
+    if (half == 0) *reinterpret_cast<float2*>(parts.ml + at * 2) = make_float2(rt.top, sum);
+    if (sum == 0.0f) return;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int dim = d * 32 + 2 * e + 4 * half;
+        if (dim < D) *reinterpret_cast<f32x4*>(parts.o + at * D + dim) = f32x4{rt.o[d][e], rt.o[d][e + 1], rt.o[d][e + 2], rt.o[d][e + 3]};
+      }
+    return;
+  }
   const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
   uint16_t* op = reinterpret_cast<uint16_t*>(a.o.data) + (int64_t)(pt.q0 + row) * a.o.row_stride +
                  (int64_t)head * a.o.head_stride;
@@ -426,6 +455,97 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
     wait_copies<0>();                              // this wave's store of the same row is complete
     if (lane < D) out[lane] = E::round(o0);
     if (lane + 64 < D) out[lane + 64] = E::round(o1);
+  }
+}
+
+// Joins the parts of a call: a row is DP / 4 lanes, four dims each, so a wave joins two or four rows at once, with four parts'
+// loads under way. A lane also holds its part's maximum and sum (kMostParts <= DP / 4).
+constexpr int kMostParts = 16;
+template <int DP>
+constexpr int kJoinRows = kPromptWaves * 256 / DP;              // of a block
+template <bool BF, int DP>
+__global__ __launch_bounds__(64 * kPromptWaves) void k_prompt_join(const mtc_prompt_args a, const PromptParts parts) {
+  constexpr int kLanes = DP / 4, kChunks = kPromptRows / kJoinRows<DP>;
+  const int H = a.heads, D = a.dim, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.x % H, kvh = head / (H / a.kv_heads);
+  PromptTile pt = prompt_tile(a, blockIdx.x / H / kChunks);
+  pt.tile = __builtin_amdgcn_readfirstlane(pt.tile);
+  pt.q0 = __builtin_amdgcn_readfirstlane(pt.q0);
+  pt.n = __builtin_amdgcn_readfirstlane(pt.n);
+  pt.k0 = __builtin_amdgcn_readfirstlane(pt.k0);
+  pt.m = __builtin_amdgcn_readfirstlane(pt.m);
+  if (pt.tile < 0) return;
+  const int row0 = pt.tile * kPromptRows + blockIdx.x / H % kChunks * kJoinRows<DP> + wave * (64 / kLanes);
+  if (row0 >= pt.n) return;
+  const int in = lane % kLanes, row = row0 + lane / kLanes;
+  const int64_t at = (int64_t)(pt.q0 + min(row, pt.n - 1)) * H + head;
+  const int64_t step = (int64_t)a.q_rows * H;                  // from a part to the next
+  float2 ml = make_float2(-INFINITY, 0.0f);
+  if (in < parts.n) ml = *reinterpret_cast<const float2*>(parts.ml + (at + in * step) * 2);
+  const bool has = ml.y != 0.0f;                               // a NaN too
+  float top = has ? ml.x : -INFINITY;
+#pragma unroll
+  for (int x = 1; x < kMostParts; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+  top = __shfl(top, lane - in);
+  const float w = has ? exp2_fast(ml.x - (top == -INFINITY ? 0.0f : top)) : 0.0f;
+  float l = has ? ml.y * w : 0.0f;
+#pragma unroll
+  for (int x = 1; x < kMostParts; x *= 2) l += __shfl_xor(l, x);
+  l = __shfl(l, lane - in);
+  const uint64_t with = __ballot(has);
+  float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const bool mine = 4 * in < D;
+  for (int p = 0; p < parts.n; p += 4) {
+    f32x4 z[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {                              // a part without keys wrote nothing: not looked at
+      z[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (mine && (with >> (lane - in + p + j) & 1))
+        z[j] = *reinterpret_cast<const f32x4*>(parts.o + (at + (p + j) * step) * D + 4 * in);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float wp = __shfl(w, lane - in + p + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(z[j][e], wp, y[e]);
+    }
+  }
+  const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] *= inv;
+  uint16_t* op = reinterpret_cast<uint16_t*>(a.o.data) + (int64_t)pt.q0 * a.o.row_stride + (int64_t)head * a.o.head_stride;
+  if (mine && row < pt.n) {
+    u32x2 packed = {Elem<BF>::pack(y[0], y[1]), Elem<BF>::pack(y[2], y[3])};
+    *reinterpret_cast<u32x2*>(op + (int64_t)row * a.o.row_stride + 4 * in) = packed;
+  }
+  uint64_t bad = __ballot(row < pt.n && !(finite(y[0]) && finite(y[1]) && finite(y[2]) && finite(y[3])));
+  if (!bad) return;
+  // as in k_prompt: not of the row's own making if a key that it does not see, in the tiles taken for its wave, holds one
+  const float c = a.scale * kLog2e;
+  const int64_t hk = (int64_t)kvh * a.k.head_stride, hv = (int64_t)kvh * a.v.head_stride;
+  const uint16_t* kb = reinterpret_cast<const uint16_t*>(a.k.data) + (int64_t)pt.k0 * a.k.row_stride + hk;
+  const uint16_t* vb = reinterpret_cast<const uint16_t*>(a.v.data) + (int64_t)pt.k0 * a.v.row_stride + hv;
+  for (int i = 0; i < 64 / kLanes; ++i) {
+    if (!(bad >> (i * kLanes) & ((1ull << kLanes) - 1))) continue;
+    const int r = row0 + i, seen = a.causal ? min(max(r + pt.m - pt.n + 1, 0), pt.m) : pt.m;
+    bool clean = true;
+    for (int key = seen; key < min(seen + kPromptKeys + 32, pt.m); ++key) {      // the wave's last row saw up to 31 more
+      const uint16_t* v = vb + (int64_t)key * a.v.row_stride;
+      clean = clean && !(lane < D && !finite16<BF>(v[lane])) && !(lane + 64 < D && !finite16<BF>(v[lane + 64]));
+    }
+    if (!__ballot(!clean)) continue;
+    float o0, o1;
+    plain_row<BF>(reinterpret_cast<const uint16_t*>(a.q.data) + (int64_t)(pt.q0 + r) * a.q.row_stride + (int64_t)head * a.q.head_stride,
+                  D, seen, c,
+                  [&](int key, const uint16_t*& k, const uint16_t*& v) {
+                    k = kb + (int64_t)key * a.k.row_stride;
+                    v = vb + (int64_t)key * a.v.row_stride;
+                  },
+                  o0, o1);
+    uint16_t* out = op + (int64_t)r * a.o.row_stride;
+    wait_copies<0>();                              // this wave's store of the same row is complete
+    if (lane < D) out[lane] = Elem<BF>::round(o0);
+    if (lane + 64 < D) out[lane + 64] = Elem<BF>::round(o1);
   }
 }
 
@@ -1216,10 +1336,55 @@ int check_attention(int dtype, int heads, int kv_heads, int dim, float scale) {
   return MTC_OK;
 }
 
+// At most so many query tiles (the sequences' lengths are on the device): n rows are (n - 1) / kPromptRows + 1 tiles.
+int64_t prompt_tiles(const mtc_prompt_args& a) {
+  const int seqs = std::min(a.n_seqs, a.q_rows);
+  return (int64_t)(a.q_rows - seqs) / kPromptRows + seqs;
+}
+
+// Blocks that share a tile's keys, from the sizes that the host knows (as if one sequence had all the keys): as many as fill the
+// chip's 512 places, with two steps or more each, where the steps that a part saves (1.6 us each at 128 dims, 0.8 at 64) are
+// worth its partial results (0.7 us a MB, out and back): steps t / n + n MB 0.7 is least at n = sqrt(steps t / (0.7 MB)).
+// Below eight steps the join's launch costs more than it saves (1 query on 300 keys: 8.9 -> 9.6 us, 4 x 64: 5.4 -> 8.8).
+int prompt_parts(const mtc_prompt_args& a) {
+  const int64_t blocks = prompt_tiles(a) * a.heads, steps = a.k_rows / kPromptKeys;
+  if (steps < 8 || blocks > 256) return 1;
+  const double mb = 1e-6 * a.q_rows * a.heads * (a.dim + 2) * 4;
+  const int64_t worth = (int64_t)std::min(std::sqrt((double)steps * (a.dim <= 64 ? 0.8 : 1.6) / (0.7 * mb)), (double)kMostParts);
+  return (int)std::max<int64_t>(std::min(std::min(512 / blocks, steps / 2), worth), 1);
+}
+size_t prompt_workspace(const mtc_prompt_args& a) {
+  const int n = prompt_parts(a);
+  return n < 2 ? 0 : (size_t)n * a.q_rows * a.heads * (a.dim + 2) * 4 + 16;
+}
+
+template <bool BF, int DP>
+int launch_prompt(const mtc_prompt_args& a, void* workspace, hipStream_t st) {
+  const unsigned blocks = (unsigned)(prompt_tiles(a) * a.heads);
+  PromptParts parts{nullptr, nullptr, prompt_parts(a)};
+  if (parts.n < 2) {
+    k_prompt<BF, DP, false><<<blocks, 64 * kPromptWaves, 0, st>>>(a, parts);
+    return check_launch("k_prompt");
+  }
+  parts.ml = (float*)workspace;                    // an even count of floats: the rows of o stay 16-byte aligned below
+  parts.o = parts.ml + (((size_t)parts.n * a.q_rows * a.heads * 2 + 3) & ~(size_t)3);
+  k_prompt<BF, DP, true><<<blocks * parts.n, 64 * kPromptWaves, 0, st>>>(a, parts);
+  if (int rc = check_launch("k_prompt")) return rc;
+  k_prompt_join<BF, DP><<<blocks * (kPromptRows / kJoinRows<DP>), 64 * kPromptWaves, 0, st>>>(a, parts);
+  return check_launch("k_prompt_join");
+}
 template <bool BF>
-void launch_prompt(const mtc_prompt_args& a, unsigned grid, hipStream_t st) {
-  if (a.dim <= 64) k_prompt<BF, 64><<<grid, 64 * kPromptWaves, 0, st>>>(a);
-  else k_prompt<BF, 128><<<grid, 64 * kPromptWaves, 0, st>>>(a);
+int launch_prompt(const mtc_prompt_args& a, void* workspace, hipStream_t st) {
+  return a.dim <= 64 ? launch_prompt<BF, 64>(a, workspace, st) : launch_prompt<BF, 128>(a, workspace, st);
+}
+
+int check_prompt(const mtc_prompt_args* a) {
+  if (!a) return fail(MTC_E_NULL, "args is NULL");
+  if (a->abi_version != MTC_ABI_VERSION) return fail(MTC_E_VERSION, "args of ABI %u, library %d", a->abi_version, MTC_ABI_VERSION);
+  if (int rc = check_attention(a->dtype, a->heads, a->kv_heads, a->dim, a->scale)) return rc;
+  if (a->n_seqs < 0 || a->q_rows < 0 || a->k_rows < 0) return fail(MTC_E_SHAPE, "negative sizes");
+  if (prompt_tiles(*a) * a->heads > 0xFFFFFF) return fail(MTC_E_SHAPE, "too many query tiles");     // 2^32 threads a launch
+  return MTC_OK;
 }
 
 // How an item's rows are taken: the least of 16, 32 and 128 rows that holds them.
@@ -1297,11 +1462,13 @@ int run_cached(const CachedCall& a, const CachedPlan& p, hipStream_t st) {
 
 }  // namespace
 
-MTC_API int mtc_prompt_attention(const mtc_prompt_args* a, void* hip_stream) {
-  if (!a) return fail(MTC_E_NULL, "args is NULL");
-  if (a->abi_version != MTC_ABI_VERSION) return fail(MTC_E_VERSION, "args of ABI %u, library %d", a->abi_version, MTC_ABI_VERSION);
-  if (int rc = check_attention(a->dtype, a->heads, a->kv_heads, a->dim, a->scale)) return rc;
-  if (a->n_seqs < 0 || a->q_rows < 0 || a->k_rows < 0) return fail(MTC_E_SHAPE, "negative sizes");
+MTC_API size_t mtc_prompt_attention_workspace_bytes(const mtc_prompt_args* a) {
+  if (check_prompt(a) != MTC_OK || a->n_seqs == 0 || a->q_rows == 0) return 0;
+  return prompt_workspace(*a);
+}
+
+MTC_API int mtc_prompt_attention(const mtc_prompt_args* a, void* workspace, size_t workspace_bytes, void* hip_stream) {
+  if (int rc = check_prompt(a)) return rc;
   if (a->n_seqs == 0 || a->q_rows == 0) return ok();
   if (!a->cu_q || !a->cu_k) return fail(MTC_E_NULL, "cu_q or cu_k is NULL");
   if (int rc = check_heads("q", a->q, false)) return rc;
@@ -1311,11 +1478,13 @@ MTC_API int mtc_prompt_attention(const mtc_prompt_args* a, void* hip_stream) {
   // a tile's rows past the sequence's end must lie past its buffer's end: rows may not overlap
   if ((a->k.row_stride < a->dim || a->v.row_stride < a->dim) && a->k_rows > 1)
     return fail(MTC_E_SHAPE, "rows of k and v overlap: strides %lld, %lld", (long long)a->k.row_stride, (long long)a->v.row_stride);
-  const int64_t tiles = (int64_t)a->q_rows / kPromptRows + std::min(a->n_seqs, a->q_rows);    // at most
-  if (tiles * a->heads > 0xFFFFFF) return fail(MTC_E_SHAPE, "too many query tiles");     // 2^32 threads a launch
-  if (a->dtype == MTC_DTYPE_BF16) launch_prompt<true>(*a, (unsigned)(tiles * a->heads), (hipStream_t)hip_stream);
-  else launch_prompt<false>(*a, (unsigned)(tiles * a->heads), (hipStream_t)hip_stream);
-  return check_launch("k_prompt");
+  if (const size_t need = prompt_workspace(*a)) {
+    if (!workspace || workspace_bytes < need)
+      return fail(MTC_E_WORKSPACE, "workspace of %zu bytes, needs %zu", workspace ? workspace_bytes : (size_t)0, need);
+    if ((uintptr_t)workspace % 256) return fail(MTC_E_WORKSPACE, "workspace must be 256-byte aligned");
+  }
+  hipStream_t st = (hipStream_t)hip_stream;
+  return a->dtype == MTC_DTYPE_BF16 ? launch_prompt<true>(*a, workspace, st) : launch_prompt<false>(*a, workspace, st);
 }
 
 MTC_API size_t mtc_cached_attention_workspace_bytes(const mtc_cache_desc* c, const mtc_cached_args* a) {

@@ -95,6 +95,37 @@ def test_prompt(gpu, lengths, causal, heads, kv, dim, dtype):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("heads,kv,dim,dtype,causal", [(14, 2, 64, "bf16", True), (4, 4, 128, "fp16", True), (2, 1, 40, "bf16", False)])
+@pytest.mark.parametrize("new,keys", [([1], [3000]), ([130], [1500]), ([5, 0, 60, 3], [700, 100, 61, 2500])])
+def test_prompt_few_rows_on_many_keys(gpu, new, keys, heads, kv, dim, dtype, causal):
+    # keys split over blocks: parts with no keys for some rows, for some waves, for a whole sequence
+    import torch
+    from tensorpack_amd.attention import prompt_attention
+    print("parts", new, keys, heads, kv, dim, dtype, causal, flush=True)
+    q, k, v = (_normal(s, (sum(n), h, dim), _dtype(dtype), gpu, f) for s, n, h, f in
+               ((1, new, heads, 2.0), (2, keys, kv, 1.0), (3, keys, kv, 1.0)))
+    cq, ck = _offsets(new, gpu), _offsets(keys, gpu)
+    got = prompt_attention(q, k, v, cq, ck, causal=causal)
+    _check(got, *_prompt64(q, k, v, new, keys, causal, dim ** -0.5), dtype)
+    assert torch.equal(got, prompt_attention(q, k, v, cq, ck, causal=causal))
+
+
+def test_prompt_parts_ignore_what_they_do_not_see(gpu):
+    import torch
+    from tensorpack_amd.attention import prompt_attention
+    q, k, v = (_normal(s, (n, 2, 64), _dtype("bf16"), gpu) for s, n in ((1, 50), (2, 2000), (3, 2000)))
+    clean = prompt_attention(q, k, v, _offsets([50], gpu), _offsets([2000], gpu)).double().cpu().numpy()
+    o, A = _prompt64(q, k, v, [50], [2000], True, 0.125)
+    k[1980], v[1980] = math.nan, math.inf
+    got = prompt_attention(q, k, v, _offsets([50], gpu), _offsets([2000], gpu))
+    _check(got[:30], o[:30], A[:30], "bf16")
+    assert torch.isnan(got[30:]).all() and np.isfinite(clean).all()
+    v[5] = math.nan                                              # seen by all
+    assert torch.isnan(prompt_attention(q, k, v, _offsets([50], gpu), _offsets([2000], gpu))).all()
+    few = prompt_attention(q, k[:1030], v[:1030], _offsets([20, 30], gpu), _offsets([1030, 0], gpu))   # a sequence without keys
+    assert torch.isnan(few[:20]).all() and not few[20:].any()
+
+
 def test_prompt_many_sequences(gpu):
     # more sequences than a wave has lanes, tiles of several levels
     from tensorpack_amd.attention import prompt_attention

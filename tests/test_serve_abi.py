@@ -61,7 +61,7 @@ def _prompt(**kw):
 
 
 def test_prompt_checks(lib):
-    f = lib.mtc_prompt_attention
+    f = lambda a, stream: lib.mtc_prompt_attention(a, None, 0, stream)
     assert f(None, None) == -1
     for kw, code in (({"abi_version": 3}, -7), ({"dtype": 0}, -4), ({"dtype": 9}, -4), ({"heads": 7}, -3), ({"kv_heads": 0}, -3),
                      ({"dim": 60}, -3), ({"dim": 136}, -3), ({"dim": 0}, -3), ({"scale": 0.0}, -3), ({"scale": float("inf")}, -3),
@@ -71,6 +71,13 @@ def test_prompt_checks(lib):
         assert f(_prompt(**kw), None) == code, kw
         assert lib.mtc_last_error()
     assert f(_prompt(n_seqs=0), None) == 0 and f(_prompt(q_rows=0), None) == 0
+    ws, few = lib.mtc_prompt_attention_workspace_bytes, dict(q_rows=100, k_rows=5000)
+    assert ws(_prompt()) == 0 and ws(_prompt(q_rows=100000, k_rows=100000)) == 0 and ws(_prompt(heads=7)) == 0
+    need = ws(_prompt(**few))                                    # few rows on many keys: partial results
+    assert need >= 2 * 100 * 8 * 66 * 4
+    full = lib.mtc_prompt_attention
+    assert full(_prompt(**few), None, need, None) == -5 and full(_prompt(**few), 0x100, need - 1, None) == -5
+    assert full(_prompt(**few), 0x180, need, None) == -5
 
 
 def _cache(**kw):
