@@ -297,9 +297,9 @@ struct RowTile {
 // four waves let two blocks share a CU, whose barriers then do not stop each other: four waves of 32 queries read 16
 // KiB of each tile per 32 matrix instructions, which LDS supplies while they run.
 // Bound by the matrix and vector units: of a wave's 2950 cycles a step with 128 dims (two waves a SIMD), 975 are matrix
-// instructions, 860 vector issue, 680 waits for LDS and barriers. 1 x 16384, 32/8 heads of 128, causal: 1937 to 2080 us,
-// 1.06 to 1.14 PFLOP/s, the clock at 1.7 GHz under the load (an 8192^3 library product: 1.22 PFLOP/s). Calls of few blocks wait for
-// the longest (512 new queries on 4608 keys: 72 steps of 1.6 us, 119 us). Not kept: two waves per 32 queries with half the
+// instructions, 860 vector issue, 680 waits for LDS and barriers. 1 x 16384, 32/8 heads of 128, causal: 1912 to 2084 us,
+// 1.06 to 1.15 PFLOP/s, the clock at 1.7 GHz under the load (an 8192^3 library product: 1.22 PFLOP/s). Calls of few blocks wait for
+// the longest (512 new queries on 4608 keys: 72 steps of 1.6 us, 118 to 128 us). Not kept: two waves per 32 queries with half the
 // keys each (129 us), two sets of four waves on alternate tiles (130 us).
 //
 // PARTS: for calls of few tiles (a short chunk of new tokens on many older ones), `parts.n` blocks share a tile, each with a run
