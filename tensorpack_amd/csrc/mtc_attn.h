@@ -75,10 +75,12 @@ __device__ __forceinline__ u32x4 buffer_rsrc(uint64_t base, uint32_t bytes) {
 // Global -> LDS copy of 16 bytes per lane: lane l's bytes land at lds + 16 l (lds uniform); a lane whose
 // offset is past the buffer's end writes zeros, so the rows past a sequence's end hold zeros and
 // nothing beyond it is read. Assembly, so the compiler does not make every LDS read wait for it: the
-// kernels wait with counted s_waitcnt (the copies are their only vector memory loads in flight there).
+// kernels wait with counted s_waitcnt (the copies are their only vector memory loads in flight there). The wait states that
+// the instruction needs are its own too, since the compiler adds none inside assembly: 1 after m0 is written, 5 after a
+// vector instruction writes a scalar register that it reads (the resource by v_readfirstlane, or a spilled one by v_readlane).
 __device__ __forceinline__ void copy16(u32x4 rsrc, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "s"(lds)
-               : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "s"(lds)
+               : "memory", "m0");
 }
 
 template <int N>

@@ -125,10 +125,12 @@ __device__ __forceinline__ u32x4_t buffer_rsrc(const void* base, uint32_t bytes)
 // a lane whose offset is past the buffer's end writes zeros. Inline assembly, so the
 // compiler neither counts it among its own loads nor makes LDS reads wait for it: the
 // consumer waves, which issue no other vector memory loads in their loop, wait for
-// these copies with their own counted s_waitcnt.
+// these copies with their own counted s_waitcnt. The wait states that the instruction needs are its own too (the compiler
+// adds none inside assembly): 1 after m0 is written, 5 after a vector instruction writes a scalar register that it
+// reads (a resource or address by v_readfirstlane, or a spilled one by v_readlane).
 __device__ __forceinline__ void dma16(u32x4_t rsrc, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "s"(lds)
-               : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "s"(lds)
+               : "memory", "m0");
 }
 
 // Workgroup barrier that orders LDS only: waits for this wave's LDS accesses, not for its
