@@ -79,13 +79,14 @@ int mtc_prompt_attention(const mtc_prompt_args* a, void* workspace, size_t works
  * Bookkeeping calls take device lists of distinct sequence numbers. A call whose list names a sequence
  * out of range or twice, that runs out of pages or of table entries, or whose lengths do not fit, changes
  * nothing and sets its bit in state[0] (no host synchronisation; the caller reads it when it likes).
+ * A length outside 0 .. max_pages * page_size counts as the nearest of the two; extend refuses it.
  * Results do not depend on the order in which blocks run.
  */
 enum {
   MTC_CACHE_BAD_SEQ = 1,      /* sequence number out of range or twice in a list */
   MTC_CACHE_NO_PAGES = 2,     /* not enough free pages */
   MTC_CACHE_TABLE_FULL = 4,   /* a sequence would need more than max_pages entries */
-  MTC_CACHE_BAD_LENGTH = 8,   /* negative count, or a length above the present one */
+  MTC_CACHE_BAD_LENGTH = 8,   /* negative count or present length, or a length above the present one */
   MTC_CACHE_NOT_EMPTY = 16    /* fork into a sequence that holds tokens, or that is a source of the call */
 };
 

@@ -34,7 +34,7 @@ CACHED_MAX_TOKENS = 16                   # MTC_CACHED_MAX_TOKENS
 CACHED_MAX_SEQS = 8192                   # MTC_CACHED_MAX_SEQS
 CACHE_MAX_SLOTS = 65536                  # MTC_CACHE_MAX_SLOTS
 CACHE_STATUS = {1: "sequence number out of range or twice in a list", 2: "not enough free pages",
-                4: "a sequence's table row is full", 8: "negative count, or a length above the present one",
+                4: "a sequence's table row is full", 8: "negative count or present length, or a length above the present one",
                 16: "fork into a sequence that holds tokens or is a source"}
 
 

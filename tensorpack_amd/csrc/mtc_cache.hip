@@ -42,6 +42,10 @@ __host__ __device__ inline int32_t* scratch_start(const mtc_cache_desc& c) { ret
 __device__ __forceinline__ int pages_of(const mtc_cache_desc& c, int tokens) {
   return (tokens + c.page_size - 1) / c.page_size;
 }
+// Tokens of sequence s, as far as its table row can hold them: lens may hold anything.
+__device__ __forceinline__ int held(const mtc_cache_desc& c, int s) {
+  return min(max(c.lens[s], 0), c.max_pages * c.page_size);
+}
 
 // Exclusive sum over the block's threads (two counts at once where they are packed); the total in `total`.
 __device__ uint64_t block_scan(uint64_t x, uint64_t& total) {
@@ -112,7 +116,7 @@ __global__ __launch_bounds__(kThreads) void k_extend(const mtc_cache_desc c, con
       return x;
     }
     x.len = c.lens[x.s];
-    if (x.count < 0) bad |= MTC_CACHE_BAD_LENGTH;
+    if (x.count < 0 || x.len < 0) bad |= MTC_CACHE_BAD_LENGTH;
     else if ((int64_t)x.len + x.count > (int64_t)c.max_pages * c.page_size) bad |= MTC_CACHE_TABLE_FULL;
     if (bad) return x;
     if (x.len % c.page_size && x.count > 0) {
@@ -268,13 +272,13 @@ __global__ __launch_bounds__(kThreads) void k_truncate(const mtc_cache_desc c, c
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int s = seqs[i];
     if ((uint32_t)s >= (uint32_t)c.max_seqs || mark(marks, s)) bad |= MTC_CACHE_BAD_SEQ;
-    else if (new_lens && (new_lens[i] < 0 || new_lens[i] > c.lens[s])) bad |= MTC_CACHE_BAD_LENGTH;
+    else if (new_lens && (new_lens[i] < 0 || new_lens[i] > held(c, s))) bad |= MTC_CACHE_BAD_LENGTH;
   }
   bad = block_or(bad);
   if (!bad) {
     const int lane = threadIdx.x & 63;
     for (int i = blockIdx.x * kWaves + (threadIdx.x >> 6); i < n; i += gridDim.x * kWaves) {
-      const int s = seqs[i], keep = pages_of(c, new_lens ? new_lens[i] : 0), have = min(pages_of(c, c.lens[s]), c.max_pages);
+      const int s = seqs[i], keep = pages_of(c, new_lens ? new_lens[i] : 0), have = pages_of(c, held(c, s));
       int32_t* const row = c.table + (int64_t)s * c.max_pages;
       int lowest = c.n_pages;
       for (int k = keep + lane; k < have; k += 64) {
@@ -313,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void k_fork(const mtc_cache_desc c, const
   if (!bad) {
     const int lane = threadIdx.x & 63;
     for (int i = blockIdx.x * kWaves + (threadIdx.x >> 6); i < n; i += gridDim.x * kWaves) {
-      const int have = min(pages_of(c, c.lens[src[i]]), c.max_pages);
+      const int have = pages_of(c, held(c, src[i]));
       const int32_t* const from = c.table + (int64_t)src[i] * c.max_pages;
       int32_t* const to = c.table + (int64_t)dst[i] * c.max_pages;
       for (int k = lane; k < have; k += 64) {
@@ -325,7 +329,7 @@ __global__ __launch_bounds__(kThreads) void k_fork(const mtc_cache_desc c, const
   }
   if (!last_block(&c.state[kDone])) return;
   if (!bad)
-    for (int i = threadIdx.x; i < n; i += kThreads) c.lens[dst[i]] = c.lens[src[i]];
+    for (int i = threadIdx.x; i < n; i += kThreads) c.lens[dst[i]] = held(c, src[i]);
   if (threadIdx.x == 0 && bad) c.state[kStatus] |= bad;
 }
 
@@ -385,7 +389,7 @@ __global__ __launch_bounds__(kCopyThreads) void k_compact(const mtc_cache_desc c
   }
   const int live = c.state[kFirstFree], lane = threadIdx.x & 63;
   for (int s = blockIdx.x * 4 + (threadIdx.x >> 6); s < c.max_seqs; s += table_blocks * 4) {
-    const int have = min(pages_of(c, c.lens[s]), c.max_pages);
+    const int have = pages_of(c, held(c, s));
     int32_t* const row = c.table + (int64_t)s * c.max_pages;
     for (int k = lane; k < have; k += 64) {
       const int p = row[k];
@@ -412,7 +416,7 @@ __global__ __launch_bounds__(256) void k_append(const mtc_cache_desc c, int laye
   }
   const int s = seqs[lo];
   if ((uint32_t)s >= (uint32_t)c.max_seqs) return;
-  const int pos = c.lens[s] - (cu[lo + 1] - r);
+  const int pos = held(c, s) - (cu[lo + 1] - r);
   if (pos < 0 || pos >= c.max_pages * c.page_size) return;
   const int page = c.table[(int64_t)s * c.max_pages + pos / c.page_size];
   if ((uint32_t)page >= (uint32_t)c.n_pages) return;

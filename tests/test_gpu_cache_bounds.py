@@ -1,0 +1,71 @@
+"""Bookkeeping calls on a cache whose device arrays hold values that no call wrote. All arrays of the bookkeeping are
+compared for equality (they lie one after another in one tensor, so that an index outside one shows in its neighbour)."""
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+TOP = (1 << 31) - 1
+
+
+def _ints(x, dev):
+    import torch
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def _fresh(dev, n_pages=40, max_seqs=6, max_pages=5):
+    from tensorpack_amd.cache import PagedCache
+    return PagedCache(n_pages, 1, 1, 64, max_seqs=max_seqs, max_pages=max_pages, device=dev)
+
+
+def _refused(c, bits, call):
+    import torch
+    from tensorpack_amd.cache import CacheError
+    before = c.book.clone()
+    call()
+    with pytest.raises(CacheError) as e:
+        c.check()
+    assert e.value.bits == bits
+    assert torch.equal(c.book[4:], before[4:]) and c.state[1] == before[1]
+
+
+@pytest.mark.parametrize("seq", [0, 3])
+@pytest.mark.parametrize("length,count", [(-1, 1), (-40, 60), (-100, 200), (-TOP - 1, TOP)])
+def test_extend_refuses_a_negative_length(gpu, seq, length, count):
+    print("extend", seq, length, count, flush=True)
+    c = _fresh(gpu)
+    c.extend(_ints([1, 2], gpu), _ints([20, 3], gpu))
+    c.lens[seq] = length
+    _refused(c, 8, lambda: c.extend(_ints([seq], gpu), _ints([count], gpu)))
+    _refused(c, 8, lambda: c.extend(_ints([1, seq], gpu), _ints([20, count], gpu)))
+
+
+def test_lengths_above_the_table(gpu):
+    c = _fresh(gpu)
+    c.extend(_ints([0, 1], gpu), _ints([40, 70], gpu))
+    c.lens[1] = TOP                                              # counts as 80: the five pages of its row
+    _refused(c, 4, lambda: c.extend(_ints([1], gpu), _ints([1], gpu)))
+    _refused(c, 8, lambda: c.truncate(_ints([1], gpu), _ints([TOP], gpu)))
+    _refused(c, 8, lambda: c.truncate(_ints([1], gpu), _ints([81], gpu)))
+    c.fork(_ints([1], gpu), _ints([4], gpu))
+    assert c.table[4].tolist() == c.table[1].tolist() and c.lens[4] == 80
+    assert c.refs.tolist() == [1] * 3 + [2] * 5 + [0] * 32
+    c.free(_ints([1, 4], gpu))
+    assert c.lens.tolist() == [40, 0, 0, 0, 0, 0] and c.refs.tolist() == [1] * 3 + [0] * 37
+    assert c.table[1:].eq(-1).all()
+    c.check()
+
+
+def test_append_after_a_length_that_no_call_wrote(gpu):
+    import torch
+    c = _fresh(gpu)
+    c.pool.zero_()
+    c.extend(_ints([1], gpu), _ints([70], gpu))
+    k = torch.ones((3, 1, 64), dtype=c.dtype, device=gpu)
+    for length in (-TOP - 1, -5):
+        c.lens[1] = length
+        c.append(0, k, k, _ints([1], gpu), _ints([0, 3], gpu))
+    assert not c.pool.any()
+    c.lens[1] = TOP                                              # the last tokens of the row: 77, 78 and 79
+    c.append(0, k, k, _ints([1], gpu), _ints([0, 3], gpu))
+    page = int(c.table[1, 4])
+    assert c.pool[page, 0, :, 0, 13:].eq(1).all() and c.pool.count_nonzero() == 2 * 3 * 64
