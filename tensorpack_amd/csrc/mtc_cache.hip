@@ -341,7 +341,8 @@ __global__ __launch_bounds__(kThreads) void k_compact_plan(const mtc_cache_desc 
 #pragma unroll
     for (int k = 0; k < kEach; ++k) r[k] = p + k < c.n_pages ? c.refs[p + k] : -1;
   };
-  int used = 0, r[kEach];
+  int used = 0, r[kEach];                                // the counts of round 0 stay here where it is the only one
+  counts(c.n_pages, r);                                  // threads past the last page: no pages
   for (int64_t p = (int64_t)tid * kEach; p < c.n_pages; p += kThreads * kEach) {
     counts(p, r);
 #pragma unroll

@@ -69,3 +69,33 @@ def test_append_after_a_length_that_no_call_wrote(gpu):
     c.append(0, k, k, _ints([1], gpu), _ints([0, 3], gpu))
     page = int(c.table[1, 4])
     assert c.pool[page, 0, :, 0, 13:].eq(1).all() and c.pool.count_nonzero() == 2 * 3 * 64
+
+
+@pytest.mark.parametrize("n_pages", [1, 3, 5, 63, 1000, 4095, 4096, 4097, 9001])
+def test_compact_takes_the_pool_s_pages_only(gpu, n_pages):
+    """Pools that the planning block's threads do not divide, after another pool's counts were in the same registers."""
+    import torch
+    from tensorpack_amd.cache import PagedCache
+    print("compact", n_pages, flush=True)
+    make = lambda n: PagedCache(n, 1, 1, 8, max_seqs=2, max_pages=n, device=gpu)
+    full, c = make(8192), make(n_pages)
+    full.refs.fill_(7)
+    full.compact()
+    pages = torch.randperm(n_pages, generator=torch.Generator().manual_seed(n_pages))[:(n_pages + 1) // 2].int().to(gpu)
+    held = torch.arange(n_pages, device=gpu, dtype=c.dtype)[:, None, None, None, None, None].expand_as(c.pool)
+    c.pool.copy_(held)
+    c.table[1, :len(pages)], c.lens[1] = pages, 16 * len(pages)
+    c.refs[pages.long()] = 1
+    c.scratch.fill_(-5)
+    want = pages.tolist()
+    holes = [p for p in range(len(want)) if p not in set(want)]
+    moved = dict(zip(sorted(p for p in want if p >= len(want)), holes))
+    c.compact()
+    assert c.table[1, :len(want)].tolist() == [moved.get(p, p) for p in want]
+    assert c.refs.tolist() == [1] * len(want) + [0] * (n_pages - len(want))
+    assert torch.equal(c.pool[c.table[1, :len(want)].long()], held[pages.long()])
+    assert c.state.tolist() == [0, len(want), len(moved), 0]
+    assert c.scratch[:len(moved)].tolist() == sorted(moved) and c.scratch[len(moved):n_pages].eq(-5).all()
+    assert c.scratch[n_pages:n_pages + len(moved)].tolist() == holes and c.scratch[n_pages + len(moved):2 * n_pages].eq(-5).all()
+    assert c.scratch[3 * n_pages:].eq(-5).all()
+    c.check()
