@@ -333,13 +333,14 @@ __global__ __launch_bounds__(kThreads) void k_fork(const mtc_cache_desc c, const
   if (threadIdx.x == 0 && bad) c.state[kStatus] |= bad;
 }
 
-// One block; a thread takes four consecutive pages of each round of 4096.
+// One block; a thread takes four consecutive pages of each round of 4096. A page is held or free (a count below 0 is free),
+// so that there are as many free pages below `live` as held ones from there on.
 __global__ __launch_bounds__(kThreads) void k_compact_plan(const mtc_cache_desc c) {
   constexpr int kEach = 4;
   const int tid = threadIdx.x;
   auto counts = [&](int64_t p, int (&r)[kEach]) {
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) r[k] = p + k < c.n_pages ? c.refs[p + k] : -1;
+    for (int k = 0; k < kEach; ++k) r[k] = p + k < c.n_pages ? max(c.refs[p + k], 0) : -1;
   };
   int used = 0, r[kEach];                                // the counts of round 0 stay here where it is the only one
   counts(c.n_pages, r);                                  // threads past the last page: no pages

@@ -99,3 +99,18 @@ def test_compact_takes_the_pool_s_pages_only(gpu, n_pages):
     assert c.scratch[n_pages:n_pages + len(moved)].tolist() == holes and c.scratch[n_pages + len(moved):2 * n_pages].eq(-5).all()
     assert c.scratch[3 * n_pages:].eq(-5).all()
     c.check()
+
+
+def test_compact_takes_negative_counts_as_free(gpu):
+    import torch
+    c = _fresh(gpu, n_pages=20)
+    c.pool.copy_(torch.arange(20, device=gpu)[:, None, None, None, None, None].expand_as(c.pool))
+    c.table[2, :4], c.lens[2] = _ints([19, 1, 7, 3], gpu), 60
+    c.refs[c.table[2, :4].long()] = 1
+    c.refs[0], c.refs[2], c.refs[5] = -1, -TOP - 1, -7
+    c.scratch.fill_(TOP)
+    c.compact()
+    assert c.table[2].tolist() == [2, 1, 0, 3, -1] and c.refs[:4].tolist() == [1, 1, 1, 1]
+    assert c.refs[4:].tolist() == [0, -7] + [0] * 14
+    assert c.pool[:4, 0, 0, 0, 0, 0].tolist() == [7, 1, 19, 3]
+    c.check()
