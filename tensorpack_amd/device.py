@@ -6,6 +6,7 @@ no GPU or no built library these functions raise.
 """
 
 import ctypes
+import threading
 from typing import Dict, Optional, Tuple
 
 import numpy as np
@@ -316,7 +317,7 @@ class DeviceTiles:
 
     def workspace(self, M: int, x_dtype: int, need: int = None):
         """The prefill workspace of an M-row call (prefill_workspace: shared by every matrix's calls
-        on the current stream)."""
+        of this thread on the current stream)."""
         if need is None:
             need = int(self.lib.mtc_gemm_workspace_bytes(ctypes.byref(self.desc), int(M), int(x_dtype)))
         if need == 0:
@@ -449,30 +450,38 @@ class GemmBatch:
         return self.outs
 
 
-_PREFILL_WS: dict = {}
+_WORKSPACES = threading.local()
 
 
 def prefill_workspace(device, need: int):
     """A device buffer of at least `need` bytes for the prefill calls on the current HIP stream of
-    `device`, shared by every matrix and group: calls ordered on one stream never overlap, calls on
-    two streams may, so each stream has its own. The buffer only grows, to at least twice its last
-    size, and a buffer it outgrows is kept, never freed: a HIP graph captured earlier still
-    addresses it."""
+    `device` (stream_workspace)."""
     torch = _torch()
     index = torch.device(device).index
     return stream_workspace(torch.cuda.current_device() if index is None else index, current_stream_handle(device), need)
 
 
 def stream_workspace(index: int, stream: int, need: int):
-    """prefill_workspace for callers that have the device's index and the stream's handle already."""
+    """A device buffer of at least `need` bytes for one call on `stream`, the current stream of device `index`. Hold it until
+    the call has returned.
+
+    A call launches several kernels that hand partial results on in it, so a buffer belongs to a thread and stream: calls of one
+    thread on one stream never overlap, but another thread's launches can come between those of a call, on the same stream too.
+    It is shared by every matrix and operator and only grows, to at least twice its last size.
+    While the stream is captured the buffer comes from the graph's own memory: graphs captured on one stream can be replayed
+    at the same time on others."""
     torch = _torch()
-    held = _PREFILL_WS.get((index, stream))
-    if held is None:
-        held = _PREFILL_WS[index, stream] = []
-    if not held or held[-1].numel() < need:
-        size = max(int(need), 2 * held[-1].numel() if held else 0)
-        held.append(torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index)))
-    return held[-1]
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(int(need), dtype=torch.uint8, device=torch.device("cuda", index))
+    try:
+        held = _WORKSPACES.held
+    except AttributeError:
+        held = _WORKSPACES.held = {}
+    mine = held.get((index, stream))
+    if mine is None or mine.numel() < need:
+        size = max(int(need), 2 * mine.numel() if mine is not None else 0)
+        mine = held[index, stream] = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
+    return mine
 
 
 def raw_stream(index: int) -> int:
@@ -484,8 +493,8 @@ def raw_stream(index: int) -> int:
 def gemm_bf16_group(tiles, X, outs=None, out_dtype=None):
     """Y_i = X @ W_hat_i for 1..MAX_GROUP tile streams that share X (same K), one launch per
     kernel (mtc_gemm_bf16_group). Each Y_i is bit-identical to tiles[i].gemm_bf16(X). The
-    workspace is cached per device and HIP stream (calls on one stream are ordered; calls on
-    two streams may overlap, so they do not share one)."""
+    workspace is stream_workspace's (calls of one thread on one stream are ordered; others
+    may overlap, so they do not share one)."""
     torch = _torch()
     tiles = list(tiles)
     n = len(tiles)

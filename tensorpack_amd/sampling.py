@@ -57,7 +57,8 @@ def verify_drafts(drafts, p, q, u, noise, *, n_drafts=None):
                               drafts.stride(0), np_, tokens.data_ptr(), accepted.data_ptr())
     ref, stream = ctypes.byref(args), raw_stream(dev.index)
     need = lib.mtc_verify_workspace_bytes(ref)
-    rc = lib.mtc_verify_drafts(ref, stream_workspace(dev.index, stream, need).data_ptr(), need, stream)
+    ws = stream_workspace(dev.index, stream, need)
+    rc = lib.mtc_verify_drafts(ref, ws.data_ptr(), need, stream)
     if rc:
         _abi.check(lib, "mtc_verify_drafts", rc)
     return tokens, accepted
