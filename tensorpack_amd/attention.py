@@ -11,7 +11,7 @@ import math
 from typing import Optional
 
 from . import _abi, _native
-from .device import raw_stream, require_gpu, stream_workspace
+from .device import on_device, raw_stream, require_gpu, stream_workspace
 
 
 def _dtype_code(dtype):
@@ -100,10 +100,11 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: Op
                               _heads(q), _heads(k), _heads(v), _heads(out), cq, ck)
     ref, stream = ctypes.byref(args), raw_stream(dev.index)
     need = lib.mtc_prompt_attention_workspace_bytes(ref)
-    ws = stream_workspace(dev.index, stream, need) if need else None
-    rc = lib.mtc_prompt_attention(ref, ws.data_ptr() if need else None, need, stream)
-    if rc:
-        _abi.check(lib, "mtc_prompt_attention", rc)
+    with on_device(dev.index):
+        ws = stream_workspace(dev.index, stream, need) if need else None
+        rc = lib.mtc_prompt_attention(ref, ws.data_ptr() if need else None, need, stream)
+        if rc:
+            _abi.check(lib, "mtc_prompt_attention", rc)
     return out
 
 
@@ -163,8 +164,9 @@ def cached_attention(q, cache, layer: int, seqs, *, q_lens=None, groups=None, pr
                               _abi.MtcHeads(out.data_ptr(), heads * dim, dim), sp, qp, gp, pp)
     ref, stream = ctypes.byref(args), raw_stream(dev.index)
     need = lib.mtc_cached_attention_workspace_bytes(cache.desc_ref, ref)
-    ws = stream_workspace(dev.index, stream, need) if need else None
-    rc = lib.mtc_cached_attention(cache.desc_ref, ref, ws.data_ptr() if need else None, need, stream)
-    if rc:
-        _abi.check(lib, "mtc_cached_attention", rc)
+    with on_device(dev.index):
+        ws = stream_workspace(dev.index, stream, need) if need else None
+        rc = lib.mtc_cached_attention(cache.desc_ref, ref, ws.data_ptr() if need else None, need, stream)
+        if rc:
+            _abi.check(lib, "mtc_cached_attention", rc)
     return out

@@ -15,7 +15,7 @@ from typing import Optional
 
 from . import _abi, _native
 from .attention import _dtype_code, _int32
-from .device import _need, raw_stream, require_gpu
+from .device import _need, on_device, raw_stream, require_gpu
 
 STATE_WORDS = 4
 
@@ -87,9 +87,10 @@ class PagedCache:
 
     # ---- bookkeeping ----------------------------------------------------------------
     def _call(self, name, *args):
-        rc = getattr(self.lib, name)(self.desc_ref, *args, raw_stream(self.device.index))
-        if rc:
-            _abi.check(self.lib, name, rc)
+        with on_device(self.device.index):
+            rc = getattr(self.lib, name)(self.desc_ref, *args, raw_stream(self.device.index))
+            if rc:
+                _abi.check(self.lib, name, rc)
 
     def _list(self, name, x, n=None):
         if x.shape[0] > _abi.CACHED_MAX_SEQS:

@@ -5,6 +5,7 @@ every computation goes through libmtc_hip.so. There is no CPU fallback: with
 no GPU or no built library these functions raise.
 """
 
+import contextlib
 import ctypes
 import threading
 from typing import Dict, Optional, Tuple
@@ -482,6 +483,15 @@ def stream_workspace(index: int, stream: int, need: int):
         size = max(int(need), 2 * mine.numel() if mine is not None else 0)
         mine = held[index, stream] = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
     return mine
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(index: int):
+    """A context with device `index` current, where the library launches its kernels, whatever device the stream is of."""
+    torch = _torch()
+    return _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def raw_stream(index: int) -> int:

@@ -8,7 +8,7 @@ model's distribution.
 import ctypes
 
 from . import _abi, _native
-from .device import raw_stream, require_gpu, stream_workspace
+from .device import on_device, raw_stream, require_gpu, stream_workspace
 
 
 def verify_drafts(drafts, p, q, u, noise, *, n_drafts=None):
@@ -57,8 +57,9 @@ def verify_drafts(drafts, p, q, u, noise, *, n_drafts=None):
                               drafts.stride(0), np_, tokens.data_ptr(), accepted.data_ptr())
     ref, stream = ctypes.byref(args), raw_stream(dev.index)
     need = lib.mtc_verify_workspace_bytes(ref)
-    ws = stream_workspace(dev.index, stream, need)
-    rc = lib.mtc_verify_drafts(ref, ws.data_ptr(), need, stream)
-    if rc:
-        _abi.check(lib, "mtc_verify_drafts", rc)
+    with on_device(dev.index):
+        ws = stream_workspace(dev.index, stream, need)
+        rc = lib.mtc_verify_drafts(ref, ws.data_ptr(), need, stream)
+        if rc:
+            _abi.check(lib, "mtc_verify_drafts", rc)
     return tokens, accepted
