@@ -23,13 +23,22 @@ def _dtype_code(dtype):
     raise ValueError(f"attention takes bfloat16 or float16, got {dtype}")
 
 
-def _kernel_heads(x):
-    """x (rows, heads, dim) itself when the kernels can read it in place (unit stride along dim, the other strides
-    multiples of 8 elements, rows that do not overlap, a 16-byte aligned start), else a contiguous copy."""
+def _in_place(x) -> bool:
+    """The kernels can take x (rows, heads, dim) where it is: unit stride along dim, the other strides multiples of 8
+    elements, rows that do not overlap, a 16-byte aligned start."""
     r, h, u = x.stride()
-    if u == 1 and not (h | r) & 7 and x.shape[2] <= r < 1 << 24 and not x.data_ptr() & 15:
-        return x
-    return x.contiguous()
+    return u == 1 and not (h | r) & 7 and x.shape[2] <= r < 1 << 24 and not x.data_ptr() & 15
+
+
+def _copy(x):
+    """A contiguous copy in memory of its own. (contiguous() returns x itself where only its start or the stride of an
+    axis of size 1 is in the way.)"""
+    import torch
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _kernel_heads(x):
+    return x if _in_place(x) else _copy(x)
 
 
 def _heads(x) -> "_abi.MtcHeads":
@@ -58,7 +67,7 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: Op
     """Attention over whole prompts packed one after another (mtc_prompt_attention).
 
     q (rows, heads, dim), k and v (keys, kv_heads, dim): bf16 or f16; strided views are read in place when their
-    rows are 16-byte aligned. heads is a multiple of kv_heads, dim a multiple of 8 up to 128.
+    rows are 16-byte aligned, others are copied. heads is a multiple of kv_heads, dim a multiple of 8 up to 128.
     cu_q, cu_k (sequences + 1) int32 on the device: sequence b owns rows cu_q[b]:cu_q[b+1] of q and
     cu_k[b]:cu_k[b+1] of k and v, from 0 to the end (cu_k None: cu_q). A sequence may have more keys than queries
     (the queries are then its last tokens), fewer, or none of either.
@@ -92,7 +101,7 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: Op
         raise ValueError(f"without cu_k, k and v hold one row per query: {keys} != {rows}")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif not (out.shape == q.shape and out.dtype == q.dtype and out.device == dev and _kernel_heads(out) is out):
+    elif not (out.shape == q.shape and out.dtype == q.dtype and out.device == dev and _in_place(out)):
         raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {dev} with 16-byte aligned rows")
     lib = _native.hip_lib()
     q, k, v = _kernel_heads(q), _kernel_heads(k), _kernel_heads(v)
@@ -157,7 +166,7 @@ def cached_attention(q, cache, layer: int, seqs, *, q_lens=None, groups=None, pr
         q = q.contiguous()
     row, head, unit = q.stride(0) if tokens == 1 else q.stride(1), q.stride(2), q.stride(3)
     if unit != 1 or (row | head) & 7 or not dim <= row < 1 << 24 or q.data_ptr() & 15:
-        q = q.contiguous()
+        q = _copy(q)
         row, head = heads * dim, dim
     lib = cache.lib
     args = _abi.MtcCachedArgs(_abi.ABI_VERSION, layer, n, tokens, heads, n_groups, scale, 0, _abi.MtcHeads(q.data_ptr(), row, head),
