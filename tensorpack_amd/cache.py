@@ -118,9 +118,9 @@ class PagedCache:
         p = self._list("seqs", seqs)
         c = _int32("cu", cu, seqs.shape[0] + 1, self.device)
         mask = 16 // k.element_size() - 1                        # rows of 16-byte pieces are read in place, others copied
-        hk, hv = (_abi.MtcHeads(x.data_ptr(), x.stride(0), x.stride(1)) for x in
-                  (x if x.stride(2) == 1 and not (x.stride(0) | x.stride(1)) & mask and not x.data_ptr() & 15 else _copy(x)
-                   for x in (k, v)))
+        k, v = (x if x.stride(2) == 1 and not (x.stride(0) | x.stride(1)) & mask and not x.data_ptr() & 15 else _copy(x)
+                for x in (k, v))
+        hk, hv = (_abi.MtcHeads(x.data_ptr(), x.stride(0), x.stride(1)) for x in (k, v))
         code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self.desc.dtype
         self._call("mtc_cache_append", layer, ctypes.byref(hk), ctypes.byref(hv), code, k.shape[0], p, c, seqs.shape[0])
 

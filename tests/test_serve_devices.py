@@ -93,3 +93,23 @@ def test_launches_go_to_the_tensors_device(world):
                                         "mtc_cache_append", "mtc_cache_fork", "mtc_cache_truncate", "mtc_cache_truncate", "mtc_cache_compact"]
     assert all(x[1:] == (1, 1001) for x in world.calls), world.calls
     assert len(world.calls) == len(launches) + 3 and world.current == 0
+
+
+def test_append_holds_its_copies_until_the_launch(world, monkeypatch):
+    """K and V that have to be copied: both copies live when the library is called (another thread could get the
+    memory of a released one on the same stream)."""
+    import weakref
+    from tensorpack_amd import cache
+    copies, alive = [], []
+
+    def copy(x):
+        y = Tensor(*x.shape)
+        copies.append(weakref.ref(y))
+        return y
+    monkeypatch.setattr(cache, "_copy", copy)
+    world.cache.lib.__class__.mtc_cache_append = lambda self, *a: alive.extend(r() is not None for r in copies) or 0
+    k, v = Tensor(5, 2, 64), Tensor(5, 2, 64)
+    k.data_ptr = v.data_ptr = lambda: 0x100002
+    import torch
+    world.cache.append(0, k, v, Tensor(2, dtype=torch.int32), Tensor(3, dtype=torch.int32))
+    assert alive == [True, True]
