@@ -156,9 +156,10 @@ class PagedCache:
         return self.book.clone()
 
     def restore(self, snapshot) -> None:
-        """Puts the bookkeeping back. Pages written or moved since hold what was written."""
+        """Puts the bookkeeping back, but for the status: `check()` still raises, once, for a call since the last check.
+        Pages written or moved since hold what was written."""
         _need(snapshot.shape == self.book.shape and snapshot.dtype == self.book.dtype, "not a snapshot of this cache")
-        self.book.copy_(snapshot)
+        self.book[1:].copy_(snapshot[1:])
 
     def check(self) -> None:
         """Waits for the GPU; raises CacheError if a call since the last check could not be done."""

@@ -114,3 +114,21 @@ def test_compact_takes_negative_counts_as_free(gpu):
     assert c.refs[4:].tolist() == [0, -7] + [0] * 14
     assert c.pool[:4, 0, 0, 0, 0, 0].tolist() == [7, 1, 19, 3]
     c.check()
+
+
+def test_restore_leaves_the_status(gpu):
+    import torch
+    from tensorpack_amd.cache import CacheError
+    c = _fresh(gpu)
+    c.extend(_ints([0], gpu), _ints([20], gpu))
+    clean = c.snapshot()
+    c.extend(_ints([1, 1], gpu), _ints([1, 1], gpu))             # refused after the snapshot
+    c.extend(_ints([2], gpu), _ints([30], gpu))
+    c.restore(clean)
+    assert c.lens.tolist() == [20, 0, 0, 0, 0, 0] and torch.equal(c.book[1:], clean[1:])
+    pending = c.snapshot()                                       # with the refusal still to be reported
+    with pytest.raises(CacheError) as e:
+        c.check()
+    assert e.value.bits == 1
+    c.restore(pending)
+    c.check()                                                    # reported once
