@@ -41,7 +41,8 @@ typedef struct mtc_heads {
  * over all keys of its sequence, or with `causal` over keys j <= t + (keys - queries), the queries
  * being the last tokens. A row that sees no key is 0. Keys that a row does not see have no part in it,
  * whatever they hold (infinities and NaN included). dtype: bf16 or f16 for q, k, v and o; products
- * on the matrix cores, sums and softmax in fp32. Rows of o outside every sequence are not written.
+ * on the matrix cores, sums and softmax in fp32. Rows of o outside every sequence are not written. o may be q itself
+ * (the same address and strides); it shares no other memory with q, k or v.
  * Workspace: mtc_prompt_attention_workspace_bytes (0 but for calls of few rows on many keys, whose keys are split over
  * blocks), 256-byte aligned, no initialisation.
  */
@@ -144,6 +145,7 @@ int mtc_cache_append(const mtc_cache_desc* c, int layer, const mtc_heads* k, con
  * cache, their own K and V included (append first). q and o: rows b * tokens + t. q_lens[b]
  * (NULL: tokens) rows of sequence b count: row t < q_lens[b] sees the first
  * lens[s] - q_lens[b] + t + 1 tokens of s = seqs[b] (NULL: b); a row that sees none, or t >= q_lens[b], is 0.
+ * o may be q itself (the same address and strides); it shares no other memory with q or the cache.
  *
  * Shared prefixes: groups (n_groups + 1 offsets into the batch, from 0 to n_seqs, not falling) and
  * prefix_lens (n_groups): the sequences groups[g] .. groups[g+1] hold the same pages for their first

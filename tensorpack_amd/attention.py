@@ -73,7 +73,7 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: Op
     (the queries are then its last tokens), fewer, or none of either.
     causal: query t sees keys up to its own place; a query that sees none gives zeros.
     scale: of the scores; default dim ** -0.5. out: result tensor like q (rows outside every sequence keep what
-    they held); default: a new contiguous tensor.
+    they held); it may be q itself, but shares no other memory with q, k or v; default: a new contiguous tensor.
     """
     import torch
     dev = q.device if q.is_cuda else require_gpu(q.device)
@@ -103,6 +103,8 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: Op
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif not (out.shape == q.shape and out.dtype == q.dtype and out.device == dev and _in_place(out)):
         raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {dev} with 16-byte aligned rows")
+    elif rows and keys and out.data_ptr() in (k.data_ptr(), v.data_ptr()):
+        raise ValueError("out is k or v, which other rows still read")
     lib = _native.hip_lib()
     q, k, v = _kernel_heads(q), _kernel_heads(k), _kernel_heads(v)
     args = _abi.MtcPromptArgs(_abi.ABI_VERSION, dt, n, heads, kv_heads, dim, rows, keys, causal, scale,

@@ -412,37 +412,44 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
     return;
   }
   const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+  bool fine = true;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      rt.o[d][e] *= inv;
+      fine = fine && finite(rt.o[d][e]);
+    }
+  // rows to compute again: their q is still needed, and o may be q
+  uint64_t again = __ballot(row < pt.n && !fine);
+  again = (again | (again >> 32)) & 0xFFFFFFFFull;
+  const int read = min((wave_keys + kPromptKeys - 1) / kPromptKeys * kPromptKeys, pt.m);    // keys that the wave multiplied
+  for (uint64_t ask = again; ask; ask &= ask - 1) {
+    const int i = __ffsll((unsigned long long)ask) - 1;
+    bool clean = true;                             // nothing unseen can have got in: the row's own keys made it so
+    for (int key = sees(wave_first + i); key < read; ++key) {
+      const uint16_t* v = reinterpret_cast<const uint16_t*>((uintptr_t)v_base) + (int64_t)key * a.v.row_stride;
+      clean = clean && !(lane < D && !finite16<BF>(v[lane])) && !(lane + 64 < D && !finite16<BF>(v[lane + 64]));
+    }
+    if (!__ballot(!clean)) again &= ~(1ull << i);
+  }
   uint16_t* op = reinterpret_cast<uint16_t*>(a.o.data) + (int64_t)(pt.q0 + row) * a.o.row_stride +
                  (int64_t)head * a.o.head_stride;
-  bool fine = true;
+  const bool store = row < pt.n && !(again >> col & 1);
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
     for (int e = 0; e < 16; e += 8) {
       uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = rt.o[d][e + 2 * i] * inv, y = rt.o[d][e + 2 * i + 1] * inv;
-        fine = fine && finite(x) && finite(y);
-        w[i] = E::pack(x, y);
-      }
+      for (int i = 0; i < 4; ++i) w[i] = E::pack(rt.o[d][e + 2 * i], rt.o[d][e + 2 * i + 1]);
       // the halves hold dims 4 half + 0..3 of 8-dim groups e/4 and e/4 + 1: after the swap each has one group whole
       const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
       const int at = d * 32 + 2 * e + 8 * half;
-      if (row < pt.n && at < D) *reinterpret_cast<u32x4*>(op + at) = u32x4{x[0], y[0], x[1], y[1]};
+      if (store && at < D) *reinterpret_cast<u32x4*>(op + at) = u32x4{x[0], y[0], x[1], y[1]};
     }
-  uint64_t again = __ballot(row < pt.n && !fine);
-  again = (again | (again >> 32)) & 0xFFFFFFFFull;
-  const int read = min((wave_keys + kPromptKeys - 1) / kPromptKeys * kPromptKeys, pt.m);    // keys that the wave multiplied
-  while (again) {
+  for (; again; again &= again - 1) {
     const int r = wave_first + __ffsll((unsigned long long)again) - 1;
-    again &= again - 1;
-    bool clean = true;                             // nothing unseen can have got in: the row's own keys made it so
-    for (int key = sees(r); key < read; ++key) {
-      const uint16_t* v = reinterpret_cast<const uint16_t*>((uintptr_t)v_base) + (int64_t)key * a.v.row_stride;
-      clean = clean && !(lane < D && !finite16<BF>(v[lane])) && !(lane + 64 < D && !finite16<BF>(v[lane + 64]));
-    }
-    if (!__ballot(!clean)) continue;
     float o0, o1;
     plain_row<BF>(reinterpret_cast<const uint16_t*>(a.q.data) + (int64_t)(pt.q0 + r) * a.q.row_stride + (int64_t)head * a.q.head_stride,
                   D, sees(r), c,
@@ -452,7 +459,6 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void k_prompt(const mtc_promp
                   },
                   o0, o1);
     uint16_t* out = reinterpret_cast<uint16_t*>(a.o.data) + (int64_t)(pt.q0 + r) * a.o.row_stride + (int64_t)head * a.o.head_stride;
-    wait_copies<0>();                              // this wave's store of the same row is complete
     if (lane < D) out[lane] = E::round(o0);
     if (lane + 64 < D) out[lane + 64] = E::round(o1);
   }
@@ -514,18 +520,14 @@ __global__ __launch_bounds__(64 * kPromptWaves) void k_prompt_join(const mtc_pro
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] *= inv;
   uint16_t* op = reinterpret_cast<uint16_t*>(a.o.data) + (int64_t)pt.q0 * a.o.row_stride + (int64_t)head * a.o.head_stride;
-  if (mine && row < pt.n) {
-    u32x2 packed = {Elem<BF>::pack(y[0], y[1]), Elem<BF>::pack(y[2], y[3])};
-    *reinterpret_cast<u32x2*>(op + (int64_t)row * a.o.row_stride + 4 * in) = packed;
-  }
-  uint64_t bad = __ballot(row < pt.n && !(finite(y[0]) && finite(y[1]) && finite(y[2]) && finite(y[3])));
-  if (!bad) return;
   // as in k_prompt: not of the row's own making if a key that it does not see, in the tiles taken for its wave, holds one
+  const uint64_t bad = __ballot(row < pt.n && !(finite(y[0]) && finite(y[1]) && finite(y[2]) && finite(y[3])));
+  uint32_t again = 0;                              // bit i: row row0 + i is computed again (before it is stored: o may be q)
   const float c = a.scale * kLog2e;
   const int64_t hk = (int64_t)kvh * a.k.head_stride, hv = (int64_t)kvh * a.v.head_stride;
   const uint16_t* kb = reinterpret_cast<const uint16_t*>(a.k.data) + (int64_t)pt.k0 * a.k.row_stride + hk;
   const uint16_t* vb = reinterpret_cast<const uint16_t*>(a.v.data) + (int64_t)pt.k0 * a.v.row_stride + hv;
-  for (int i = 0; i < 64 / kLanes; ++i) {
+  for (int i = 0; bad && i < 64 / kLanes; ++i) {
     if (!(bad >> (i * kLanes) & ((1ull << kLanes) - 1))) continue;
     const int r = row0 + i, seen = a.causal ? min(max(r + pt.m - pt.n + 1, 0), pt.m) : pt.m;
     bool clean = true;
@@ -534,6 +536,7 @@ __global__ __launch_bounds__(64 * kPromptWaves) void k_prompt_join(const mtc_pro
       clean = clean && !(lane < D && !finite16<BF>(v[lane])) && !(lane + 64 < D && !finite16<BF>(v[lane + 64]));
     }
     if (!__ballot(!clean)) continue;
+    again |= 1u << i;
     float o0, o1;
     plain_row<BF>(reinterpret_cast<const uint16_t*>(a.q.data) + (int64_t)(pt.q0 + r) * a.q.row_stride + (int64_t)head * a.q.head_stride,
                   D, seen, c,
@@ -543,9 +546,12 @@ __global__ __launch_bounds__(64 * kPromptWaves) void k_prompt_join(const mtc_pro
                   },
                   o0, o1);
     uint16_t* out = op + (int64_t)r * a.o.row_stride;
-    wait_copies<0>();                              // this wave's store of the same row is complete
     if (lane < D) out[lane] = Elem<BF>::round(o0);
     if (lane + 64 < D) out[lane + 64] = Elem<BF>::round(o1);
+  }
+  if (mine && row < pt.n && !(again >> (lane / kLanes) & 1)) {
+    u32x2 packed = {Elem<BF>::pack(y[0], y[1]), Elem<BF>::pack(y[2], y[3])};
+    *reinterpret_cast<u32x2*>(op + (int64_t)row * a.o.row_stride + 4 * in) = packed;
   }
 }
 
