@@ -1,6 +1,7 @@
 """Serving calls on tensors of a device that is not the current one, on the CPU: a library in the native one's place notes
 which device is current when it is called, and stand-ins take the tensors' places."""
 
+import itertools
 import types
 
 import pytest
@@ -9,10 +10,12 @@ import pytest
 class Tensor:
     """Shape, type and place of a tensor on cuda:1."""
     is_cuda = True
+    made = itertools.count(1)
 
     def __init__(self, *shape, dtype=None):
         import torch
         self.shape, self.dtype, self.device = torch.Size(shape), dtype or torch.bfloat16, torch.device("cuda", 1)
+        self.at = next(self.made) << 20
 
     def dim(self):
         return len(self.shape)
@@ -27,7 +30,7 @@ class Tensor:
         return True
 
     def data_ptr(self):
-        return 0x100000
+        return self.at
 
     def element_size(self):
         return self.dtype.itemsize
