@@ -7,6 +7,7 @@ no GPU or no built library these functions raise.
 
 import contextlib
 import ctypes
+import functools
 import threading
 from typing import Dict, Optional, Tuple
 
@@ -17,6 +18,7 @@ from .packer import LAYOUT_MX, PanelStream
 from .tilestream import TileStream
 
 
+@functools.lru_cache(maxsize=None)                 # asked for several times a call
 def _torch():
     import torch
     return torch
