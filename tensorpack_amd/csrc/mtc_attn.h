@@ -18,6 +18,10 @@ constexpr uint32_t kOutOfRange = 0xFFFFFF00u;   // byte offset past any buffer's
 constexpr float kLog2e = 1.4426950408889634f;
 
 // The two 16-bit types: BF true for bf16, false for f16.
+//
+// raise(lag): softmax weights that grow up to 2^lag over the running maximum are kept 2^raise larger than that, which drops out of
+// the quotient. f16 has 5 exponent bits: a weight below 2^-14 loses bits and one below 2^-25 is zero. Raised to the top of the
+// range (2^15), a row's weights lose less than 2^(lag - 40) of its largest one, each.
 template <bool BF>
 struct Elem;
 template <>
@@ -38,6 +42,7 @@ struct Elem<true> {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(x2, p), x2{(__bf16)1.0f, (__bf16)1.0f}, s, false);
   }
   static __device__ __forceinline__ uint16_t round(float a) { return __builtin_bit_cast(uint16_t, (__bf16)a); }
+  static constexpr float raise(float) { return 0.0f; }
   static __device__ __forceinline__ float widen(uint16_t a) { return __builtin_bit_cast(float, (uint32_t)a << 16); }
 };
 template <>
@@ -58,6 +63,7 @@ struct Elem<false> {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(x2, p), x2{(_Float16)1.0f, (_Float16)1.0f}, s, false);
   }
   static __device__ __forceinline__ uint16_t round(float a) { return __builtin_bit_cast(uint16_t, (_Float16)a); }
+  static constexpr float raise(float lag) { return 15.0f - lag; }
   static __device__ __forceinline__ float widen(uint16_t a) { return (float)__builtin_bit_cast(_Float16, a); }
 };
 

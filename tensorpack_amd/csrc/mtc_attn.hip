@@ -139,7 +139,8 @@ struct RowTile {
   static constexpr int kSteps = DP / 16, kRow = DP * 2, kTile = kPromptKeys * kRow;
   // The maximum may lag: weights up to 2^kLag keep their relative precision in 16 bits, and the common factor drops out
   // of the quotient. After the first tiles it seldom moves, which saves the pass over o.
-  static constexpr float kLag = 8.0f;
+  // (f16, which raises its weights by 15 - lag: 512 on 4608 117 us with lags of 0, 2 and 4 at 126, 122 and 120.)
+  static constexpr float kLag = 8.0f, kRaise = E::raise(kLag);
   u32x4 qf[kSteps];
   f32x16 o[DP / 32];
   float top, sum;                    // running maximum (times c; up to kLag behind), this lane's share of the sum
@@ -187,7 +188,7 @@ struct RowTile {
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[g][e]);
-    mx = half_max(mx) * c;
+    mx = half_max(mx) * c - kRaise;
   }
 
   // Weights of s times the values `v` bytes on; NEXT: n becomes the scores of the keys `k` bytes on (MASKED, left: as above)
@@ -905,7 +906,7 @@ __device__ void split_keys(const CachedCall& a, const Book& book, char* lds, con
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][g][i]);
-      mx = half_max(fmaxf(mx, __shfl_xor(mx, 16))) * a.c;
+      mx = half_max(fmaxf(mx, __shfl_xor(mx, 16))) * a.c - E::raise(0.0f);
       const float was = top[rt];
       top[rt] = fmaxf(was, mx);
       const float base = top[rt] == -INFINITY ? 0.0f : top[rt];
