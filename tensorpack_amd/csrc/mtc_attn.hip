@@ -920,8 +920,9 @@ __device__ void split_keys(const CachedCall& a, const Book& book, char* lds, con
         for (int i = 0; i < 4; i += 2) {
           const float y0 = exp2_fast(__builtin_fmaf(s[rt][g][i], a.c, -base));
           const float y1 = exp2_fast(__builtin_fmaf(s[rt][g][i + 1], a.c, -base));
-          sum[rt] += y0 + y1;
-          p[rt][2 * g + (i >> 1)] = E::pack(y0, y1);     // weights of 16 bits: the matrix core's operand
+          const uint32_t y = E::pack(y0, y1);            // weights of 16 bits: the matrix core's operand
+          sum[rt] = E::add2(y, sum[rt]);                 // and what is summed, so that the quotient's parts agree
+          p[rt][2 * g + (i >> 1)] = y;
         }
     }
     if (more) wait_copies<kTileCopies>();                // V is there

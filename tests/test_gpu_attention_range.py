@@ -77,3 +77,29 @@ def test_cached(gpu, case, dtype, heads, prefix, at_end):
     kw = {"groups": _ints([0, 2], gpu), "prefix_lens": _ints([prefix], gpu)} if prefix else {}
     _check(cached_attention(q, cache, 0, _ints([0, 1], gpu), **kw), k, v, dtype)
     cache.check()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("heads", [1, 20, 40])                   # 16, 32 and more rows: each has a way of its own
+@pytest.mark.parametrize("keys", [2, 40, 200])
+def test_cached_weights_add_up(gpu, dtype, heads, keys):
+    """A constant V comes out as it is: the weights that are summed are those that V is multiplied with, so their rounding drops
+    out. All weights but one lie just below the middle of two values of the type (all round down, by nearly u of each), and
+    V has the largest mantissa, whose half unit is u / 2 of it. With agreeing sums each weight times v and each sum is an fp32
+    rounding (2^-24 for each of 200 keys: under 2^-16 of the result), far below that half unit."""
+    import torch
+    from tensorpack_amd.attention import cached_attention
+    from tensorpack_amd.cache import PagedCache
+    print(dtype, heads, keys, flush=True)
+    dt, u = (torch.float16, 2.0 ** -11) if dtype == "fp16" else (torch.bfloat16, 2.0 ** -8)
+    cache = PagedCache(30, 1, 1, DIM, max_seqs=1, max_pages=20, dtype=dt, device=gpu)
+    cache.extend(_ints([0], gpu), _ints([keys], gpu))
+    k = torch.zeros((keys, 1, DIM), dtype=dt, device=gpu)
+    k[1:, 0, 0] = -1.0
+    v = torch.full((keys, 1, DIM), 2.0 - 2.0 * u, dtype=dt, device=gpu)
+    cache.append(0, k, v, _ints([0], gpu), _ints([0, keys], gpu))
+    q = torch.zeros((1, 1, heads, DIM), dtype=dt, device=gpu)
+    q[..., 0] = 1.0
+    scale = float(np.log(2.0) - np.log1p(0.9 * u))               # weights 1 and 1/2 + 0.45 u
+    got = cached_attention(q, cache, 0, _ints([0], gpu), scale=scale)
+    assert torch.equal(got, v[:1].expand(1, 1, heads, DIM))
