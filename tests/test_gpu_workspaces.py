@@ -127,3 +127,35 @@ def test_a_captured_prefill_keeps_out_of_eager_calls(gpu):
             assert torch.equal(t.gemm_bf16(big), large)
         torch.cuda.synchronize()
         assert torch.equal(Y, want)
+
+
+def test_a_captured_decode_keeps_its_workspace(gpu):
+    """A split-K decode of 2 rows captured, then calls of other row counts on the same stream, whose workspaces have other sizes:
+    the graph's stays where it was."""
+    import torch
+    from tensorpack_amd.core.quadtree import QuadtreeRD
+    from tensorpack_amd.kernels.gemm import MTCMatrix
+    rng = np.random.RandomState(1)
+    m = MTCMatrix.from_quadtree(QuadtreeRD((rng.randn(512, 256) * 0.05).astype(np.float32), None, (32, 16, 8, 4)).select(4.0))
+    ds, s = m.device_stream(64, gpu, 2), torch.cuda.Stream()
+    X = {n: torch.from_numpy(rng.randn(n, 512).astype(np.float32)).to(gpu) for n in (1, 2, 16)}
+    want = {n: ds.gemv_f32(x) for n, x in X.items()}
+    Y, g = torch.empty_like(want[2]), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        ds.gemv_f32(X[2], out=Y)
+        held = ds.workspace(2)[0]
+    sizes = {int(ds.lib.mtc_gemv_workspace_bytes(ds.desc, n)) for n in X}
+    assert len(sizes) > 1 and held is not None
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        ds.gemv_f32(X[2], out=Y)
+    for n in (16, 1, 16):
+        with torch.cuda.stream(s):
+            assert torch.equal(ds.gemv_f32(X[n]), want[n])
+            assert ds.workspace(2)[0] is held
+        torch.cuda.synchronize()
+        Y.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(Y, want[2])
