@@ -297,15 +297,15 @@ struct RowTile {
 // scaled by 2^(m - m') when m moves to m'), 64 keys a step, K and V copied to LDS a step ahead of their use. 128 queries in
 // four waves let two blocks share a CU, whose barriers then do not stop each other: four waves of 32 queries read 16
 // KiB of each tile per 32 matrix instructions, which LDS supplies while they run.
-// Bound by the matrix and vector units: of a wave's 2950 cycles a step with 128 dims (two waves a SIMD), 975 are matrix
-// instructions, 860 vector issue, 680 waits for LDS and barriers. 1 x 16384, 32/8 heads of 128, causal: 1912 to 2084 us,
-// 1.06 to 1.15 PFLOP/s, the clock at 1.7 GHz under the load (an 8192^3 library product: 1.22 PFLOP/s). Calls of few blocks wait for
-// the longest (512 new queries on 4608 keys: 72 steps of 1.6 us, 118 to 128 us). Not kept: two waves per 32 queries with half the
+// Bound by the matrix and vector units: of a wave's 3100 cycles a step with 128 dims (two waves a SIMD), 975 are matrix
+// instructions, 815 vector issue, 760 waits for LDS and barriers. 1 x 16384, 32/8 heads of 128, causal: 1951 to 2012 us,
+// 1.09 to 1.13 PFLOP/s, the clock at 1.75 GHz under the load (an 8192^3 library product: 1.22 PFLOP/s). Calls of few blocks wait for
+// the longest (512 new queries on 4608 keys: 72 steps of 1.6 us, 117 to 124 us). Not kept: two waves per 32 queries with half the
 // keys each (129 us), two sets of four waves on alternate tiles (130 us).
 //
 // PARTS: for calls of few tiles (a short chunk of new tokens on many older ones), `parts.n` blocks share a tile, each with a run
-// of its steps, and k_prompt_join joins their partial results (4 to 5 us). A call, unsplit and split: 117 queries on 5175 keys,
-// 14/2 heads of 40: 83.6 -> 18.4 us; 100 on 2000, 32/8 of 128: 62.1 -> 25.2; 400 on 16000, 8/1 of 128: 454 -> 54.3; 1 on 600,
+// of its steps, and k_prompt_join joins their partial results (5 to 7 us). A call, unsplit and split: 117 queries on 5175 keys,
+// 14/2 heads of 40: 83.6 -> 18.6 us; 100 on 2000, 32/8 of 128: 62.1 -> 25.2; 400 on 16000, 8/1 of 128: 454 -> 51.0; 1 on 600,
 // 32/8 of 128: 22.6 -> 12.1; 300 on 600, 14/2 of 64, the least gain: 14.1 -> 13.3.
 struct PromptParts {
   float* o;                // [part][row of q][head][dim]
@@ -1163,7 +1163,7 @@ __device__ __forceinline__ int spread(int xcd, int at, int each, int runs) {
 
 // 512 blocks whatever the call. Every block reads the lists and sums the units by itself (3.5 us until its first keys'
 // copies start, 4.5 with groups), which is less than a planning launch would take.
-// Bound by memory for few rows: 32 sequences of 8192, 32/8 heads of 128: 1.07 GB in 185 us, 5.8 TB/s (a 1 GiB copy: 5.2);
+// Bound by memory for few rows: 32 sequences of 8192, 32/8 heads of 128: 1.07 GB in 190 to 194 us, 5.6 TB/s (a 1 GiB copy: 5.2);
 // 32 ragged up to 16384: 252 MB in 41 us. 64 sequences on one prefix of 8192: 35 us, where the prefix's 2048 units of
 // 128 rows take 9.6 us of the whole chip and 26 MB of own keys 4.6; what is left is the start, the partial results (64 KB a
 // run) and blocks that share a CU. Smallest calls: 6 us.
