@@ -91,7 +91,7 @@ class DeviceStream:
         d.n_steps = 0 if ps.steps is None else int(ps.steps.shape[0])
         self.desc = d
         _abi.check(self.lib, "mtc_check_desc", self.lib.mtc_check_desc(ctypes.byref(d)))
-        self._ws: Dict[tuple, object] = {}             # (HIP stream handle, bytes) -> tensor
+        self._ws: Dict[tuple, object] = {}             # (thread, HIP stream handle, bytes) -> tensor
 
     def clone(self) -> "DeviceStream":
         """A second device copy of the same stream (distinct buffers, same contents)."""
@@ -130,14 +130,15 @@ class DeviceStream:
         return self.host.nbytes()
 
     def workspace(self, M: int):
-        """Zero-initialised GEMV workspace for M rows, one per HIP stream and size (its counters reset
-        themselves at the end of each call, so calls ordered on one stream can share it;
-        calls on different streams could overlap, so each stream gets its own). Kept while the
+        """Zero-initialised GEMV workspace for M rows, one per thread, HIP stream and size (its counters reset
+        themselves at the end of each call, so a thread's calls on one stream can share it; calls on
+        different streams could overlap, and another thread's call could come between the two launches
+        of one of 5 rows or more). Kept while the
         matrix lives: a graph captured earlier still addresses it after calls of another M."""
         need = int(self.lib.mtc_gemv_workspace_bytes(ctypes.byref(self.desc), int(M)))
         if need == 0:
             return None, 0
-        key = current_stream_handle(self.device), need
+        key = threading.get_ident(), current_stream_handle(self.device), need
         have = self._ws.get(key)
         if have is None:
             torch = _torch()

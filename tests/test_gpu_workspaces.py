@@ -159,3 +159,38 @@ def test_a_captured_decode_keeps_its_workspace(gpu):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(Y, want[2])
+
+
+@pytest.mark.parametrize("rows", [3, 16])
+def test_decodes_of_two_threads_on_one_stream(gpu, rows):
+    """Split-K decode (counters) and, from 5 rows, X laid out by a launch of its own: the threads' workspaces are apart."""
+    import torch
+    from tensorpack_amd.core.quadtree import QuadtreeRD
+    from tensorpack_amd.kernels.gemm import MTCMatrix
+    rng = np.random.RandomState(2)
+    m = MTCMatrix.from_quadtree(QuadtreeRD((rng.randn(512, 256) * 0.05).astype(np.float32), None, (32, 16, 8, 4)).select(4.0))
+    ds = m.device_stream(64, gpu, rows)
+    X = [torch.from_numpy(rng.randn(rows, 512).astype(np.float32)).to(gpu) for _ in range(2)]
+    want = [ds.gemv_f32(x) for x in X]
+    torch.cuda.synchronize()
+    got, spans, errs, ready = [None, None], [None, None], [], threading.Barrier(2)
+
+    def run(i):
+        try:
+            ready.wait()
+            got[i] = [ds.gemv_f32(X[i]) for _ in range(50)]
+            ws, n = ds.workspace(rows)
+            spans[i] = [(0, ws.data_ptr(), ws.data_ptr() + n)]
+            ready.wait()
+        except Exception as e:                                   # reported below
+            errs.append(e)
+            ready.abort()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errs, errs
+    assert _apart(*spans)
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
