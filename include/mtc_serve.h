@@ -21,6 +21,7 @@ extern "C" {
 enum { MTC_DTYPE_F16 = 2 };            /* beside MTC_DTYPE_F32 and MTC_DTYPE_BF16 */
 
 #define MTC_ATTN_MAX_DIM 128           /* head size: a multiple of 8 up to this */
+#define MTC_ROTARY_MAX_DIM 1024        /* head size of mtc_rotary */
 #define MTC_CACHED_MAX_TOKENS 16       /* queries per sequence of mtc_cached_attention */
 #define MTC_CACHED_MAX_SEQS 8192       /* sequences of one cached or bookkeeping call */
 #define MTC_CACHE_MAX_SLOTS 65536      /* sequences that one cache can hold (max_seqs) */
@@ -82,14 +83,23 @@ int mtc_prompt_attention(const mtc_prompt_args* a, void* workspace, size_t works
  * nothing and sets its bit in state[0] (no host synchronisation; the caller reads it when it likes).
  * A length outside 0 .. max_pages * page_size counts as the nearest of the two; extend refuses it.
  * Results do not depend on the order in which blocks run.
+ *
+ * 8-bit caches: dtype MTC_DTYPE_BF16 or MTC_DTYPE_F16 with MTC_CACHE_CODES8. A page is
+ *   [n_layers][2 (K, V)][kv_heads][page_size][dim rounded up to a multiple of 16] int8 codes, then
+ *   [n_layers][2][kv_heads][page_size / MTC_CODES8_BLOCK] bf16 scales, rounded up to a multiple of 16 bytes;
+ * a value is code * scale, of a scale for each MTC_CODES8_BLOCK tokens of one head, a power of two from 2^-100 to 2^100 (bf16)
+ * or 2^-24 to 2^9 (f16): every value is a number of the dtype. Bookkeeping calls and mtc_cached_attention take both kinds.
  */
 enum {
   MTC_CACHE_BAD_SEQ = 1,      /* sequence number out of range or twice in a list */
   MTC_CACHE_NO_PAGES = 2,     /* not enough free pages */
   MTC_CACHE_TABLE_FULL = 4,   /* a sequence would need more than max_pages entries */
   MTC_CACHE_BAD_LENGTH = 8,   /* negative count or present length, or a length above the present one */
-  MTC_CACHE_NOT_EMPTY = 16    /* fork into a sequence that holds tokens, or that is a source of the call */
+  MTC_CACHE_NOT_EMPTY = 16,   /* fork into a sequence that holds tokens, or that is a source of the call */
+  MTC_CACHE_SHARED_PAGE = 32  /* append to an 8-bit cache into a page that several sequences hold */
 };
+enum { MTC_CACHE_CODES8 = 16 };        /* flag of mtc_cache_desc.dtype */
+#define MTC_CODES8_BLOCK 16            /* tokens of a scale */
 
 typedef struct mtc_cache_desc {
   uint32_t abi_version;
@@ -139,6 +149,20 @@ int mtc_cache_copy_pages(const mtc_cache_desc* c, const void* from_pool, int fro
  * pool's). Rows that would fall before token 0 or on no page are not written. */
 int mtc_cache_append(const mtc_cache_desc* c, int layer, const mtc_heads* k, const mtc_heads* v, int src_dtype,
                      int rows, const int32_t* seqs, const int32_t* cu, int n, void* hip_stream);
+/* Into an 8-bit cache: a block's exponent e is the least with max |x| <= 127 2^e over its new tokens (finite ones), not less than
+ * that of the older tokens it holds; new codes are x 2^-e, rounded to nearest even and cut to -127 .. 127 (NaN: 0), codes of the older
+ * tokens code 2^(old e - e), rounded. A block's tokens come from one sequence of a call: nothing is written into a page that several
+ * sequences hold (MTC_CACHE_SHARED_PAGE), nor for a sequence that the list names twice (MTC_CACHE_BAD_SEQ). */
+
+/* Reads an 8-bit cache back: rows cu[i] .. cu[i+1] of k and v (offsets from 0, cut at `rows`; as many heads and dims as the cache)
+ * become the last cu[i+1] - cu[i] tokens of sequence seqs[i] in `layer`. dst_dtype: the cache's (exact) or fp32. Rows before
+ * token 0 or on no page become 0, those of no sequence stay as they are. Strides are multiples of 16 bytes. */
+int mtc_cache_read(const mtc_cache_desc* c, int layer, const mtc_heads* k, const mtc_heads* v, int dst_dtype, int rows,
+                   const int32_t* seqs, const int32_t* cu, int n, void* hip_stream);
+
+/* Sequence seqs[i] becomes a holder of what seqs[parents[i]] held before the call, i < n, all at once: pages that nobody
+ * holds any more become free. parents may repeat; one out of 0 .. n-1 is MTC_CACHE_BAD_SEQ. No data moves. */
+int mtc_cache_reorder(const mtc_cache_desc* c, const int32_t* seqs, const int32_t* parents, int n, void* hip_stream);
 
 /*
  * Attention of the newest `tokens` tokens (1 .. MTC_CACHED_MAX_TOKENS) of n_seqs sequences over the
@@ -213,6 +237,36 @@ typedef struct mtc_verify_args {
 
 size_t mtc_verify_workspace_bytes(const mtc_verify_args* a);
 int mtc_verify_drafts(const mtc_verify_args* a, void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/*
+ * Rotary positions. Pair i < rotated / 2 of row r turns by t = positions[r] f_i radians:
+ *   (x, y) -> amplitude (x cos t - y sin t, x sin t + y cos t)
+ * of dims (i, i + rotated / 2), or (2 i, 2 i + 1) if interleaved; dims from `rotated` on are copied. turns[i] =
+ * round(2^64 f_i / 2 pi) modulo 2^64: the product with a position, modulo 2^64, is the exact fraction of a turn.
+ *   q (rows, heads, dim) -> oq, k (rows, kv_heads, dim) -> ok: dtype fp32, bf16 or f16; heads or kv_heads may be 0. dim: a multiple of 8 up to
+ *   MTC_ROTARY_MAX_DIM. Strides are multiples of 16 bytes. oq may be q itself (the same address and strides), ok k; they
+ *   share no other memory with q or k.
+ */
+typedef struct mtc_rotary_args {
+  uint32_t abi_version;
+  int32_t dtype;
+  int32_t rows;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t dim;
+  int32_t rotated;
+  int32_t interleaved;
+  float amplitude;
+  int32_t reserved;           /* 0 */
+  mtc_heads q;
+  mtc_heads k;
+  mtc_heads oq;
+  mtc_heads ok;
+  const int32_t* positions;
+  const uint64_t* turns;
+} mtc_rotary_args;
+
+int mtc_rotary(const mtc_rotary_args* a, void* hip_stream);
 
 #ifdef __cplusplus
 }

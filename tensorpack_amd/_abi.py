@@ -27,15 +27,19 @@ EXPORTED = ("mtc_abi_version", "mtc_last_error", "mtc_check_desc", "mtc_dequant"
 SERVE_EXPORTED = ("mtc_prompt_attention_workspace_bytes", "mtc_prompt_attention", "mtc_check_cache_desc", "mtc_cache_scratch_ints", "mtc_cache_extend",
                   "mtc_cache_fork", "mtc_cache_truncate", "mtc_cache_compact", "mtc_cache_copy_pages", "mtc_cache_append",
                   "mtc_cached_attention_workspace_bytes", "mtc_cached_attention", "mtc_verify_workspace_bytes",
-                  "mtc_verify_drafts")
+                  "mtc_verify_drafts", "mtc_rotary", "mtc_cache_read", "mtc_cache_reorder")
 
 ATTN_MAX_DIM = 128                       # MTC_ATTN_MAX_DIM
+ROTARY_MAX_DIM = 1024                    # MTC_ROTARY_MAX_DIM
 CACHED_MAX_TOKENS = 16                   # MTC_CACHED_MAX_TOKENS
 CACHED_MAX_SEQS = 8192                   # MTC_CACHED_MAX_SEQS
 CACHE_MAX_SLOTS = 65536                  # MTC_CACHE_MAX_SLOTS
 CACHE_STATUS = {1: "sequence number out of range or twice in a list", 2: "not enough free pages",
                 4: "a sequence's table row is full", 8: "negative count or present length, or a length above the present one",
                 16: "fork into a sequence that holds tokens or is a source"}
+CACHE_WRITE_STATUS = {32: "append to an 8-bit cache into a page that several sequences hold"}
+CACHE_CODES8 = 16                        # MTC_CACHE_CODES8: flag of MtcCacheDesc.dtype
+CODES8_BLOCK = 16                        # MTC_CODES8_BLOCK
 
 
 class MtcStreamDesc(ctypes.Structure):
@@ -153,6 +157,16 @@ class MtcVerifyArgs(ctypes.Structure):
     ]
 
 
+class MtcRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("rows", ctypes.c_int32), ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("dim", ctypes.c_int32), ("rotated", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("amplitude", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("q", MtcHeads), ("k", MtcHeads), ("oq", MtcHeads), ("ok", MtcHeads),
+        ("positions", ctypes.c_void_p), ("turns", ctypes.c_void_p),
+    ]
+
+
 MAX_GROUP = 4                        # MTC_MAX_GROUP: matrices per mtc_gemv_f32_group launch
 
 
@@ -230,7 +244,10 @@ def declare_serve(lib: ctypes.CDLL) -> None:
             ("mtc_cached_attention_workspace_bytes", sz, [cache, P(MtcCachedArgs)]),
             ("mtc_cached_attention", i32, [cache, P(MtcCachedArgs), vp, sz, vp]),
             ("mtc_verify_workspace_bytes", sz, [P(MtcVerifyArgs)]),
-            ("mtc_verify_drafts", i32, [P(MtcVerifyArgs), vp, sz, vp])):
+            ("mtc_verify_drafts", i32, [P(MtcVerifyArgs), vp, sz, vp]),
+            ("mtc_rotary", i32, [P(MtcRotaryArgs), vp]),
+            ("mtc_cache_read", i32, [cache, i32, P(MtcHeads), P(MtcHeads), i32, i32, vp, vp, i32, vp]),
+            ("mtc_cache_reorder", i32, [cache, vp, vp, i32, vp])):
         getattr(lib, name).restype = res
         getattr(lib, name).argtypes = args
 

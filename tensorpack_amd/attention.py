@@ -30,6 +30,22 @@ def _in_place(x) -> bool:
     return u == 1 and not (h | r) & 7 and x.shape[2] <= r < 1 << 24 and not x.data_ptr() & 15
 
 
+def _aligned_rows(x) -> bool:
+    """x (rows, heads, dim) of any type: unit stride along dim, rows and heads that start at multiples of 16 bytes."""
+    r, h, u = x.stride()
+    return u == 1 and not (h | r) * x.element_size() & 15 and not x.data_ptr() & 15
+
+
+def _apart(x) -> bool:
+    """No two elements of x (rows, heads, dim) share memory."""
+    end = x.shape[2]
+    for stride, size in sorted((s, n) for s, n in zip(x.stride()[:2], x.shape[:2]) if n > 1):
+        if stride < end:
+            return False
+        end += stride * (size - 1)
+    return True
+
+
 def _copy(x):
     """A contiguous copy in memory of its own. (contiguous() returns x itself where only its start or the stride of an
     axis of size 1 is in the way.)"""

@@ -14,7 +14,7 @@ import ctypes
 from typing import Optional
 
 from . import _abi, _native
-from .attention import _copy, _dtype_code, _int32
+from .attention import _aligned_rows, _apart, _copy, _dtype_code, _int32
 from .device import _need, on_device, raw_stream, require_gpu
 
 STATE_WORDS = 4
@@ -24,7 +24,8 @@ class CacheError(RuntimeError):
     """A bookkeeping call could not be done. `bits`: the status word (MTC_CACHE_*)."""
 
     def __init__(self, bits: int):
-        super().__init__("; ".join(t for b, t in _abi.CACHE_STATUS.items() if bits & b) or f"status {bits}")
+        texts = {**_abi.CACHE_STATUS, **_abi.CACHE_WRITE_STATUS}
+        super().__init__("; ".join(t for b, t in texts.items() if bits & b) or f"status {bits}")
         self.bits = bits
 
 
@@ -47,17 +48,17 @@ class PagedCache:
         self.dtype = dtype
         self.n_pages, self.n_layers, self.n_kv_heads, self.head_dim = int(n_pages), int(n_layers), int(n_kv_heads), int(head_dim)
         self.page_size, self.max_seqs, self.max_pages = int(page_size), int(max_seqs), int(max_pages)
-        code = _dtype_code(dtype)
+        code = self._code = _dtype_code(dtype)
         _need(min(self.n_pages, self.n_layers, self.n_kv_heads, self.max_seqs, self.max_pages) > 0, "sizes must be positive")
         _need(8 <= self.head_dim <= _abi.ATTN_MAX_DIM and self.head_dim % 8 == 0,
               f"head_dim must be a multiple of 8 from 8 to {_abi.ATTN_MAX_DIM}, got {head_dim}")
         _need(self.page_size in (16, 32, 64, 128, 256), f"page_size must be a power of two from 16 to 256, got {page_size}")
         _need(self.max_seqs <= _abi.CACHE_MAX_SLOTS, f"at most {_abi.CACHE_MAX_SLOTS} sequences, got {max_seqs}")
-        shape = (self.n_pages, self.n_layers, 2, self.n_kv_heads, self.page_size, self.head_dim)
+        shape, kind = self._pool_form()
         if pool is None:
-            pool = torch.empty(shape, dtype=dtype, device=self.device)
-        _need(tuple(pool.shape) == shape and pool.dtype == dtype and pool.is_contiguous() and pool.data_ptr() % 16 == 0,
-              f"pool must be a contiguous {shape} {dtype} tensor")
+            pool = torch.empty(shape, dtype=kind, device=self.device)
+        _need(tuple(pool.shape) == shape and pool.dtype == kind and pool.is_contiguous() and pool.data_ptr() % 16 == 0,
+              f"pool must be a contiguous {shape} {kind} tensor")
         self.pool = pool
         self.lib = _native.hip_lib()
         # one tensor for the bookkeeping, so that a snapshot is one copy
@@ -68,11 +69,21 @@ class PagedCache:
         self.table.fill_(-1)
         self.scratch = torch.empty(int(self.lib.mtc_cache_scratch_ints(self.n_pages, self.max_seqs)), dtype=torch.int32,
                                    device=self.device)
-        self.desc = _abi.MtcCacheDesc(_abi.ABI_VERSION, code, self.n_pages, self.n_layers, self.n_kv_heads, self.head_dim,
+        self.desc = _abi.MtcCacheDesc(_abi.ABI_VERSION, code | self._flags, self.n_pages, self.n_layers, self.n_kv_heads, self.head_dim,
                                       self.page_size, self.max_seqs, self.max_pages, 0, pool.data_ptr(), self.table.data_ptr(),
                                       self.lens.data_ptr(), self.refs.data_ptr(), self.state.data_ptr(), self.scratch.data_ptr())
         self.desc_ref = ctypes.byref(self.desc)
         _abi.check(self.lib, "mtc_check_cache_desc", self.lib.mtc_check_cache_desc(self.desc_ref))
+
+    _flags = 0                                                   # of the descriptor's dtype
+
+    def _pool_form(self):
+        """(shape, dtype) of the pool."""
+        return (self.n_pages, self.n_layers, 2, self.n_kv_heads, self.page_size, self.head_dim), self.dtype
+
+    def _geometry(self):
+        """What two caches share if pages can be copied between them."""
+        return type(self), self.dtype, self.device, self.n_layers, self.n_kv_heads, self.page_size, self.head_dim
 
     @classmethod
     def from_buffers(cls, pool, table, lens, refs) -> "PagedCache":
@@ -80,10 +91,13 @@ class PagedCache:
         _need(pool.dim() == 6 and table.dim() == 2, "pool has six axes (see PagedCache), table two")
         self = cls(pool.shape[0], pool.shape[1], pool.shape[3], pool.shape[5], max_seqs=table.shape[0], max_pages=table.shape[1],
                    page_size=pool.shape[4], dtype=pool.dtype, pool=pool)
+        self._take_book(table, lens, refs)
+        return self
+
+    def _take_book(self, table, lens, refs):
         for mine, given, name in ((self.table, table, "table"), (self.lens, lens, "lens"), (self.refs, refs, "refs")):
             _need(mine.shape == given.shape, f"{name} must be {tuple(mine.shape)}, got {tuple(given.shape)}")
             mine.copy_(given)
-        return self
 
     # ---- bookkeeping ----------------------------------------------------------------
     def _call(self, name, *args):
@@ -121,13 +135,19 @@ class PagedCache:
         k, v = (x if x.stride(2) == 1 and not (x.stride(0) | x.stride(1)) & mask and not x.data_ptr() & 15 else _copy(x)
                 for x in (k, v))
         hk, hv = (_abi.MtcHeads(x.data_ptr(), x.stride(0), x.stride(1)) for x in (k, v))
-        code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self.desc.dtype
+        code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self._code
         self._call("mtc_cache_append", layer, ctypes.byref(hk), ctypes.byref(hv), code, k.shape[0], p, c, seqs.shape[0])
 
     def fork(self, src, dst) -> None:
         """dst[i] (empty) becomes a second holder of everything src[i] holds. src may name a sequence several times."""
         p = self._list("src", src)
         self._call("mtc_cache_fork", p, self._list("dst", dst, src.shape[0]), src.shape[0])
+
+    def reorder(self, seqs, parents) -> None:
+        """seqs[i] becomes a holder of what seqs[parents[i]] held, all at once, as after a step of beam search (sampling.beam_select gives
+        the parents); pages that nobody holds any more become free. parents are places in the list and may repeat."""
+        p = self._list("seqs", seqs)
+        self._call("mtc_cache_reorder", p, self._list("parents", parents, seqs.shape[0]), seqs.shape[0])
 
     def truncate(self, seqs, new_lens) -> None:
         """seqs[i] keeps its first new_lens[i] tokens; pages that nobody holds any more become free."""
@@ -146,8 +166,7 @@ class PagedCache:
         """Page dst[i] becomes a copy of page src[i] of `source` (a cache of the same geometry; default: this one).
         dst are distinct and none of them is also a src of this cache. Ids out of range copy nothing."""
         source = source or self
-        _need(source.device == self.device and source.dtype == self.dtype and source.pool.shape[1:] == self.pool.shape[1:],
-              "source must have the same page geometry and dtype, on the same device")
+        _need(source._geometry() == self._geometry(), "source must be a cache of the same kind, page geometry and dtype, on the same device")
         p, n = _int32("src", src, None, self.device), src.shape[0]
         self._call("mtc_cache_copy_pages", source.pool.data_ptr(), source.n_pages, p, _int32("dst", dst, n, self.device), n)
 
@@ -172,3 +191,83 @@ class PagedCache:
     def free_pages(self) -> int:
         """Pages that no sequence holds (waits for the GPU)."""
         return int((self.refs == 0).sum().item())
+
+
+class QuantizedCache(PagedCache):
+    """A PagedCache that holds K and V in 8 bits: half the memory, and half the bytes that `cached_attention` reads.
+
+    A value is code * 2 ** e: an int8 code, and an exponent for each block of 16 tokens, K or V and head, the least for which the block's
+    values fit (each is off by half a step at most, 2 ** (e - 1), which is 1 / 127 of the block's largest or less). Powers of two, so that every value is a
+    number of `dtype` and is read back exactly, and so that a block's codes depend on nothing but its values: `append` of a
+    token larger than those that its block holds rounds their codes again, to the larger step.
+    The exponents are bounded: values above 65024 (float16) are cut there, and no step is finer than 2 ** -24 (float16) or
+    2 ** -100 (bfloat16). NaN becomes 0, an infinity the block's largest value.
+
+    pool    (n_pages, page_bytes) int8: the codes of a page, then its scales (see codes and scales)
+    codes   (n_pages, n_layers, 2 (K, V), n_kv_heads, page_size, head_dim) int8, a view of pool
+    scales  (n_pages, n_layers, 2, n_kv_heads, page_size / 16) bfloat16, a view of pool
+
+    All calls are PagedCache's, and the same pages can be shared, copied and moved. `append` quantises (bfloat16, float16 or float32 as
+    they come); it does not write into pages that several sequences hold (`extend` first: it copies them), nor for a sequence that its list
+    names twice: these set the status that `check` raises.
+    """
+
+    _flags = _abi.CACHE_CODES8
+
+    def _pool_form(self):
+        import torch
+        blocks = self.page_size // _abi.CODES8_BLOCK
+        self._codes_bytes = 2 * self.n_layers * self.n_kv_heads * self.page_size * (-(-self.head_dim // 16) * 16)
+        self._scales_bytes = 4 * self.n_layers * self.n_kv_heads * blocks
+        return (self.n_pages, -(-(self._codes_bytes + self._scales_bytes) // 16) * 16), torch.int8
+
+    @classmethod
+    def from_buffers(cls, pool, table, lens, refs, *, n_layers: int, n_kv_heads: int, head_dim: int, page_size: int = 16,
+                     dtype=None) -> "QuantizedCache":
+        """A cache over an existing pool (kept, not copied) with the given bookkeeping (copied)."""
+        _need(pool.dim() == 2 and table.dim() == 2, "pool and table have two axes (see QuantizedCache)")
+        self = cls(pool.shape[0], n_layers, n_kv_heads, head_dim, max_seqs=table.shape[0], max_pages=table.shape[1],
+                   page_size=page_size, dtype=dtype, pool=pool)
+        self._take_book(table, lens, refs)
+        return self
+
+    @property
+    def codes(self):
+        room = -(-self.head_dim // 16) * 16
+        x = self.pool[:, :self._codes_bytes].view(self.n_pages, self.n_layers, 2, self.n_kv_heads, self.page_size, room)
+        return x[..., :self.head_dim]
+
+    @property
+    def scales(self):
+        import torch
+        x = self.pool[:, self._codes_bytes:self._codes_bytes + self._scales_bytes].view(torch.bfloat16)
+        return x.view(self.n_pages, self.n_layers, 2, self.n_kv_heads, self.page_size // _abi.CODES8_BLOCK)
+
+    def read(self, layer: int, seqs, cu, rows: Optional[int] = None, *, dtype=None, out=None):
+        """(K, V) (rows, n_kv_heads, head_dim) of tokens held: rows cu[i]:cu[i+1] are the last tokens of seqs[i] (all of them where cu
+        holds the sums of `lens`), as `prompt_attention` takes them beside the queries of new tokens. dtype: the cache's (exact) or float32. Rows
+        past a sequence's first token or on no page are 0. out: (K, V) to write to instead, whose rows of no sequence stay as they are;
+        those of a new result hold anything."""
+        import torch
+        if not 0 <= layer < self.n_layers:
+            raise ValueError(f"layer {layer} of {self.n_layers}")
+        if (rows is None) == (out is None):
+            raise ValueError("give rows, or out")
+        if out is None:
+            dtype = dtype or self.dtype
+            if rows < 0 or dtype not in (self.dtype, torch.float32):
+                raise ValueError(f"{rows} rows of {dtype}: the cache's {self.dtype} or float32")
+            out = tuple(torch.empty((rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in (0, 1))
+        k, v = out
+        form = (self.n_kv_heads, self.head_dim)
+        for x in (k, v):
+            ok = x.dim() == 3 and tuple(x.shape[1:]) == form and x.shape[0] == k.shape[0] and x.dtype == k.dtype
+            ok = ok and x.dtype in (self.dtype, torch.float32) and x.device == self.device
+            if not (ok and _aligned_rows(x) and _apart(x)):
+                raise ValueError(f"out must be two (rows, {form[0]}, {form[1]}) {self.dtype} or float32 tensors with 16-byte aligned rows")
+        p = self._list("seqs", seqs)
+        c = _int32("cu", cu, seqs.shape[0] + 1, self.device)
+        hk, hv = (_abi.MtcHeads(x.data_ptr(), x.stride(0), x.stride(1)) for x in (k, v))
+        code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self._code
+        self._call("mtc_cache_read", layer, ctypes.byref(hk), ctypes.byref(hv), code, k.shape[0], p, c, seqs.shape[0])
+        return k, v

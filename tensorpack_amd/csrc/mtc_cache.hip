@@ -17,6 +17,7 @@
 #include <algorithm>
 
 #include "mtc_attn.h"
+#include "mtc_codes.h"
 #include "mtc_host.h"
 #include "mtc_serve.h"
 
@@ -26,6 +27,7 @@ using mtc::host::check_launch;
 using mtc::host::fail;
 using mtc::host::ok;
 using namespace mtc::attn;
+namespace codes = mtc::codes;
 
 namespace {
 
@@ -333,6 +335,56 @@ __global__ __launch_bounds__(kThreads) void k_fork(const mtc_cache_desc c, const
   if (threadIdx.x == 0 && bad) c.state[kStatus] |= bad;
 }
 
+// A block takes a few columns of the table, of all the call's rows: what they held is read before anything is written,
+// so that any sequence may take any other's place. Takers are counted before leavers, so that a page that stays held never counts 0.
+// Bound by its chain of loads (list, lengths, table, counts).
+constexpr int kReorderIds = MTC_CACHED_MAX_SEQS;
+__host__ __device__ inline int reorder_columns(int n) { return min(32, max(1, kReorderIds / n)); }
+__global__ __launch_bounds__(kThreads) void k_reorder(const mtc_cache_desc c, const int32_t* seqs, const int32_t* parents, int n) {
+  __shared__ uint32_t marks[kMarkWords];
+  __shared__ int32_t ids[kReorderIds];
+  clear_marks(marks);
+  __syncthreads();
+  int bad = 0, most = 0;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int s = seqs[i];
+    if ((uint32_t)s >= (uint32_t)c.max_seqs || mark(marks, s) || (uint32_t)parents[i] >= (uint32_t)n) bad = MTC_CACHE_BAD_SEQ;
+    else most = max(most, pages_of(c, held(c, s)));
+  }
+  bad = block_or(bad);
+  const int columns = reorder_columns(n), first = blockIdx.x * columns;
+  if (!bad && block_or(most > first)) {
+    for (int x = threadIdx.x; x < n * columns; x += kThreads) {
+      const int s = seqs[x / columns], k = first + x % columns;
+      ids[x] = k < pages_of(c, held(c, s)) ? c.table[(int64_t)s * c.max_pages + k] : -1;
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < n * columns; x += kThreads) {
+      const int i = x / columns, k = x % columns, p = ids[parents[i] * columns + k];
+      if (p == ids[x]) continue;
+      if ((uint32_t)p < (uint32_t)c.n_pages) atomicAdd(&c.refs[p], 1);
+      c.table[(int64_t)seqs[i] * c.max_pages + first + k] = p;         // first + k < max_pages: one of the two rows holds it
+    }
+    __syncthreads();
+    int lowest = c.n_pages;
+    for (int x = threadIdx.x; x < n * columns; x += kThreads) {
+      const int p = ids[x];
+      if (p == ids[parents[x / columns] * columns + x % columns] || (uint32_t)p >= (uint32_t)c.n_pages) continue;
+      if (atomicSub(&c.refs[p], 1) == 1) lowest = min(lowest, p);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) lowest = min(lowest, __shfl_xor(lowest, d));
+    if ((threadIdx.x & 63) == 0 && lowest < c.n_pages) atomicMin(&c.state[kFirstFree], lowest);
+  }
+  if (!last_block(&c.state[kDone])) return;
+  if (!bad) {
+    for (int i = threadIdx.x; i < n; i += kThreads) ids[i] = held(c, seqs[parents[i]]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) c.lens[seqs[i]] = ids[i];
+  }
+  if (threadIdx.x == 0 && bad) c.state[kStatus] |= bad;
+}
+
 // One block; a thread takes four consecutive pages of each round of 4096. A page is held or free (a count below 0 is free),
 // so that there are as many free pages below `live` as held ones from there on.
 __global__ __launch_bounds__(kThreads) void k_compact_plan(const mtc_cache_desc c) {
@@ -435,6 +487,196 @@ __global__ __launch_bounds__(256) void k_append(const mtc_cache_desc c, int laye
   }
   const int64_t to = ((((int64_t)page * c.n_layers + layer) * 2 + is_v) * c.kv_heads + h) * c.page_size + pos % c.page_size;
   *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(c.pool) + to * c.dim + piece * 8) = y;
+}
+
+// ---------------------------------------------------------------------------
+// the 8-bit cache
+// ---------------------------------------------------------------------------
+// Byte offsets, within a page, of the codes of token 0 and of the scales of block 0 of (layer, K or V, head).
+__device__ __forceinline__ int64_t codes_at(const mtc_cache_desc& c, int layer, int is_v, int h) {
+  return (((int64_t)layer * 2 + is_v) * c.kv_heads + h) * c.page_size * codes::row_bytes(c.dim);
+}
+__device__ __forceinline__ int64_t scales_at(const mtc_cache_desc& c, int layer, int is_v, int h) {
+  return codes::code_bytes(c) + (((int64_t)layer * 2 + is_v) * c.kv_heads + h) * (c.page_size / codes::kBlock) * 2;
+}
+
+// 16 elements of a row from `d` on, those past dim 0.
+template <int SRC>
+__device__ __forceinline__ void load16(const mtc_heads& x, int64_t row, int h, int d, int dim, float (&y)[16]) {
+  const int64_t at = row * x.row_stride + (int64_t)h * x.head_stride + d;
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    if (d + i >= dim) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[i + j] = 0.0f;
+    } else if constexpr (SRC == MTC_DTYPE_F32) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(x.data) + at + i);
+      const f32x4 a = p[0], b = p[1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y[i + j] = a[j];
+        y[i + 4 + j] = b[j];
+      }
+    } else {
+      using E = Elem<SRC == MTC_DTYPE_BF16>;
+      const u32x4 a = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(x.data) + at + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = a[j];
+        y[i + 2 * j] = E::widen((uint16_t)u);
+        y[i + 2 * j + 1] = E::widen((uint16_t)(u >> 16));
+      }
+    }
+  }
+}
+__device__ __forceinline__ uint32_t pack_codes(const float* y, float by) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float v = y[j] * by;
+    const int q = v == v ? (int)__builtin_rintf(fminf(fmaxf(v, -127.0f), 127.0f)) : 0;
+    r |= (uint32_t)(q & 0xFF) << (8 * j);
+  }
+  return r;
+}
+
+__device__ __forceinline__ int cut(const int32_t* cu, int i, int rows) { return min(max(cu[i], 0), rows); }
+
+// A wave per block of 16 tokens that gets new ones, K or V, and head: the whole block is in its lanes (16 bytes each, twice at
+// most), so its largest value, and the older codes' rounding to a larger scale, need one exchange and no second pass.
+// Which block: sequence i's blocks have the numbers from cu[i] / 16 + 2 i on. It has at most rows / 16 + 2, so
+// numbers of two never meet, and a bisection of cu finds the sequence.
+template <bool BF, int SRC>
+__global__ __launch_bounds__(256) void k_append8(const mtc_cache_desc c, int layer, const mtc_heads k, const mtc_heads v, int rows,
+                                                 const int32_t* seqs, const int32_t* cu, int n) {
+  using namespace codes;
+  const int u = blockIdx.x, lane = threadIdx.x & 63;
+  auto start = [&](int i) { return cut(cu, i, rows) / kBlock + 2 * i; };
+  int lo = 0, hi = n;                                      // start(lo) <= u < start(hi)
+  if (start(0) > u || start(n) <= u) return;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start(mid) <= u) lo = mid; else hi = mid;
+  }
+  const int r0 = cut(cu, lo, rows), count = cut(cu, lo + 1, rows) - r0, s = seqs[lo];
+  if (count <= 0 || (uint32_t)s >= (uint32_t)c.max_seqs) return;
+  const int len = held(c, s), p0 = max(len - count, 0), skip = max(count - len, 0);     // rows before token 0
+  const int block = p0 / kBlock + (u - start(lo));
+  if (block * kBlock >= len) return;
+  const int at = block * kBlock;
+  int twice = 0;
+  for (int j = threadIdx.x; j < n; j += 256) twice |= j != lo && seqs[j] == s && cut(cu, j + 1, rows) > cut(cu, j, rows);
+  twice = __syncthreads_or(twice);
+  const int page = c.table[(int64_t)s * c.max_pages + at / c.page_size];
+  if ((uint32_t)page >= (uint32_t)c.n_pages) return;
+  const bool shared = c.refs[page] > 1;
+  if (twice || shared) {
+    if (threadIdx.x == 0) atomicOr(&c.state[kStatus], (twice ? MTC_CACHE_BAD_SEQ : 0) | (shared ? MTC_CACHE_SHARED_PAGE : 0));
+    return;
+  }
+  char* const base = (char*)c.pool + (int64_t)page * page_bytes(c);
+  const int room = row_bytes(c.dim), pieces = room / 16, in = at % c.page_size;
+  for (int item = blockIdx.y * 4 + (threadIdx.x >> 6); item < 2 * c.kv_heads; item += gridDim.y * 4) {
+    const int is_v = item & 1, h = item >> 1;
+    u32x4* const to = reinterpret_cast<u32x4*>(base + codes_at(c, layer, is_v, h) + (int64_t)in * room);
+    uint16_t* const scale = reinterpret_cast<uint16_t*>(base + scales_at(c, layer, is_v, h)) + in / kBlock;
+    float y[2][16];
+    int token[2];
+    float top = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int chunk = lane + 64 * x;
+      token[x] = chunk < room ? at + chunk / pieces : len;                 // len: none
+      if (token[x] < p0 || token[x] >= len) continue;
+      load16<SRC>(is_v ? v : k, r0 + skip + token[x] - p0, h, chunk % pieces * 16, c.dim, y[x]);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float a = fabsf(y[x][j]);
+        top = fmaxf(top, a < INFINITY ? a : 0.0f);
+      }
+    }
+    const bool older = at < p0;
+    const int was = older ? exponent_of<BF>(*scale) : Range<BF>::lo;
+    const int e = max(was, exponent_for<BF>(wave_max(top)));
+    if (lane == 0) *scale = (uint16_t)((e + 127) << 7);
+    const float by = power(-e);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int chunk = lane + 64 * x;
+      if (token[x] >= len) continue;
+      u32x4 z;
+      if (token[x] >= p0) {
+        z = u32x4{pack_codes(y[x], by), pack_codes(y[x] + 4, by), pack_codes(y[x] + 8, by), pack_codes(y[x] + 12, by)};
+      } else if (e > was) {
+        const float less = e - was > 40 ? 0.0f : power(was - e);           // codes below 2^7: nothing of them is left
+        z = to[chunk];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = z[i];
+          const float o[4] = {(float)(int8_t)w, (float)(int8_t)(w >> 8), (float)(int8_t)(w >> 16), (float)(int8_t)(w >> 24)};
+          z[i] = pack_codes(o, less);
+        }
+      } else {
+        continue;
+      }
+      to[chunk] = z;
+    }
+  }
+}
+
+// One thread per 16 codes: each finds its row's sequence by bisection.
+template <bool BF, int DST>
+__global__ __launch_bounds__(256) void k_read8(const mtc_cache_desc c, int layer, const mtc_heads k, const mtc_heads v, int rows,
+                                               const int32_t* seqs, const int32_t* cu, int n) {
+  using namespace codes;
+  const int room = row_bytes(c.dim), pieces = room / 16;
+  const int64_t per_row = 2ll * c.kv_heads * pieces;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= per_row * rows) return;
+  const int r = (int)(i / per_row), in = (int)(i % per_row);
+  const int piece = in % pieces, h = in / pieces % c.kv_heads, is_v = in / pieces / c.kv_heads;
+  if (cut(cu, 0, rows) > r || cut(cu, n, rows) <= r) return;
+  int lo = 0, hi = n;                                      // cu[lo] <= r < cu[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cut(cu, mid, rows) <= r) lo = mid; else hi = mid;
+  }
+  const int s = seqs[lo];
+  u32x4 z{};
+  float scale = 0.0f;
+  if ((uint32_t)s < (uint32_t)c.max_seqs) {
+    const int pos = held(c, s) - (cut(cu, lo + 1, rows) - r);
+    if (pos >= 0 && pos < c.max_pages * c.page_size) {
+      const int page = c.table[(int64_t)s * c.max_pages + pos / c.page_size];
+      if ((uint32_t)page < (uint32_t)c.n_pages) {
+        const char* const base = (const char*)c.pool + (int64_t)page * page_bytes(c);
+        const int p = pos % c.page_size;
+        z = *reinterpret_cast<const u32x4*>(base + codes_at(c, layer, is_v, h) + (int64_t)p * room + piece * 16);
+        scale = scale_of<BF>(reinterpret_cast<const uint16_t*>(base + scales_at(c, layer, is_v, h))[p / kBlock]);
+      }
+    }
+  }
+  const mtc_heads& x = is_v ? v : k;
+  const int64_t to = (int64_t)r * x.row_stride + (int64_t)h * x.head_stride + piece * 16;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    if (piece * 16 + half * 8 >= c.dim) break;
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t w = z[2 * half + (j >> 2)];
+      y[j] = (float)(int8_t)(w >> (8 * (j & 3))) * scale;
+    }
+    if constexpr (DST == MTC_DTYPE_F32) {
+      f32x4* p = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(x.data) + to + half * 8);
+      p[0] = f32x4{y[0], y[1], y[2], y[3]};
+      p[1] = f32x4{y[4], y[5], y[6], y[7]};
+    } else {
+      using E = Elem<BF>;
+      *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(x.data) + to + half * 8) =
+          u32x4{E::pack(y[0], y[1]), E::pack(y[2], y[3]), E::pack(y[4], y[5]), E::pack(y[6], y[7])};
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -602,7 +844,9 @@ __global__ __launch_bounds__(64) void k_verify_join(const mtc_verify_args a, con
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-int64_t page_bytes(const mtc_cache_desc* c) { return 2ll * c->n_layers * 2 * c->kv_heads * c->page_size * c->dim; }
+int64_t page_bytes(const mtc_cache_desc* c) {
+  return codes::is_codes(*c) ? codes::page_bytes(*c) : 2ll * c->n_layers * 2 * c->kv_heads * c->page_size * c->dim;
+}
 
 // Blocks that keep every CU's loads in flight, or one per unit of the most pages that may move.
 unsigned copy_grid(const mtc_cache_desc* c, int64_t pages) {
@@ -614,6 +858,22 @@ int check_list(const mtc_cache_desc* c, const int32_t* a, const char* what, int 
   if (int rc = mtc_check_cache_desc(c)) return rc;
   if (n < 0 || n > MTC_CACHED_MAX_SEQS) return fail(MTC_E_SHAPE, "%d sequences: 0 to %d", n, MTC_CACHED_MAX_SEQS);
   if (n && !a) return fail(MTC_E_NULL, "%s is NULL", what);
+  return MTC_OK;
+}
+
+// The checks of append and read.
+int check_rows(const mtc_cache_desc* c, int layer, const mtc_heads* k, const mtc_heads* v, int dtype, int rows, const int32_t* seqs,
+               const int32_t* cu, int n) {
+  if (int rc = check_list(c, seqs, "seqs", n)) return rc;
+  if (layer < 0 || layer >= c->n_layers) return fail(MTC_E_SHAPE, "layer %d of %d", layer, c->n_layers);
+  if (dtype != MTC_DTYPE_F32 && dtype != codes::base_type(*c)) return fail(MTC_E_DTYPE, "k and v of dtype %d, a cache of %d", dtype, c->dtype);
+  if (rows < 0) return fail(MTC_E_SHAPE, "%d rows", rows);
+  if (n == 0 || rows == 0) return MTC_OK;
+  if (!cu || !k || !v || !k->data || !v->data) return fail(MTC_E_NULL, "k, v or cu is NULL");
+  const int align = dtype == MTC_DTYPE_F32 ? 4 : 8;
+  for (const mtc_heads* x : {k, v})
+    if ((uintptr_t)x->data % 16 || x->row_stride % align || x->head_stride % align)
+      return fail(MTC_E_SHAPE, "k and v: 16-byte aligned, strides multiples of 16 bytes");
   return MTC_OK;
 }
 
@@ -656,7 +916,8 @@ int run_verify(const mtc_verify_args& a, Found* found, hipStream_t st) {
 MTC_API int mtc_check_cache_desc(const mtc_cache_desc* c) {
   if (!c) return fail(MTC_E_NULL, "cache descriptor is NULL");
   if (c->abi_version != MTC_ABI_VERSION) return fail(MTC_E_VERSION, "cache descriptor of ABI %u, library %d", c->abi_version, MTC_ABI_VERSION);
-  if (c->dtype != MTC_DTYPE_BF16 && c->dtype != MTC_DTYPE_F16) return fail(MTC_E_DTYPE, "a cache holds bf16 or f16, got dtype %d", c->dtype);
+  const int type = codes::base_type(*c);
+  if (type != MTC_DTYPE_BF16 && type != MTC_DTYPE_F16) return fail(MTC_E_DTYPE, "a cache holds bf16 or f16, or codes of them, got dtype %d", c->dtype);
   if (c->n_pages < 1 || c->n_layers < 1 || c->kv_heads < 1 || c->max_seqs < 1 || c->max_pages < 1 || c->reserved != 0)
     return fail(MTC_E_DESC, "cache of %d pages, %d layers, %d heads, %d sequences of %d pages", c->n_pages, c->n_layers, c->kv_heads,
                 c->max_seqs, c->max_pages);
@@ -699,6 +960,15 @@ MTC_API int mtc_cache_fork(const mtc_cache_desc* c, const int32_t* src, const in
   return check_launch("k_fork");
 }
 
+MTC_API int mtc_cache_reorder(const mtc_cache_desc* c, const int32_t* seqs, const int32_t* parents, int n, void* hip_stream) {
+  if (int rc = check_list(c, seqs, "seqs", n)) return rc;
+  if (n == 0) return ok();
+  if (!parents) return fail(MTC_E_NULL, "parents is NULL");
+  const int columns = reorder_columns(n);
+  k_reorder<<<(c->max_pages + columns - 1) / columns, kThreads, 0, (hipStream_t)hip_stream>>>(*c, seqs, parents, n);
+  return check_launch("k_reorder");
+}
+
 MTC_API int mtc_cache_truncate(const mtc_cache_desc* c, const int32_t* seqs, const int32_t* new_lens, int n, void* hip_stream) {
   if (int rc = check_list(c, seqs, "seqs", n)) return rc;
   if (n == 0) return ok();
@@ -730,26 +1000,47 @@ MTC_API int mtc_cache_copy_pages(const mtc_cache_desc* c, const void* from_pool,
 
 MTC_API int mtc_cache_append(const mtc_cache_desc* c, int layer, const mtc_heads* k, const mtc_heads* v, int src_dtype, int rows,
                              const int32_t* seqs, const int32_t* cu, int n, void* hip_stream) {
-  if (int rc = check_list(c, seqs, "seqs", n)) return rc;
-  if (layer < 0 || layer >= c->n_layers) return fail(MTC_E_SHAPE, "layer %d of %d", layer, c->n_layers);
-  if (src_dtype != MTC_DTYPE_F32 && src_dtype != c->dtype) return fail(MTC_E_DTYPE, "k and v of dtype %d into a cache of %d", src_dtype, c->dtype);
-  if (rows < 0) return fail(MTC_E_SHAPE, "%d rows", rows);
+  if (int rc = check_rows(c, layer, k, v, src_dtype, rows, seqs, cu, n)) return rc;
   if (n == 0 || rows == 0) return ok();
-  if (!cu || !k || !v || !k->data || !v->data) return fail(MTC_E_NULL, "k, v or cu is NULL");
-  const int align = src_dtype == MTC_DTYPE_F32 ? 4 : 8;
-  for (const mtc_heads* x : {k, v})
-    if ((uintptr_t)x->data % 16 || x->row_stride % align || x->head_stride % align)
-      return fail(MTC_E_SHAPE, "k and v: 16-byte aligned, strides multiples of 16 bytes");
+  hipStream_t st = (hipStream_t)hip_stream;
+  const bool bf = codes::base_type(*c) == MTC_DTYPE_BF16, f32 = src_dtype == MTC_DTYPE_F32;
+  if (codes::is_codes(*c)) {
+    const int64_t units = (int64_t)rows / codes::kBlock + 2 * n;
+    // one item a wave, but where the blocks fill the chip already: each reads the list of sequences
+    const int items = (2 * c->kv_heads + 3) / 4;
+    if (units > 0xFFFFFF / items || items > 0xFFFF) return fail(MTC_E_SHAPE, "%d rows of %d heads: too many", rows, c->kv_heads);
+    const dim3 g((unsigned)units, units < 2048 ? items : 1);
+    if (bf && f32) k_append8<true, MTC_DTYPE_F32><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
+    else if (bf) k_append8<true, MTC_DTYPE_BF16><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
+    else if (f32) k_append8<false, MTC_DTYPE_F32><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
+    else k_append8<false, MTC_DTYPE_F16><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
+    return check_launch("k_append8");
+  }
   const int64_t blocks = ((int64_t)rows * 2 * c->kv_heads * (c->dim / 8) + 255) / 256;
   if (blocks > 0xFFFFFF) return fail(MTC_E_SHAPE, "%d rows: too many", rows);
-  hipStream_t st = (hipStream_t)hip_stream;
-  const bool bf = c->dtype == MTC_DTYPE_BF16, f32 = src_dtype == MTC_DTYPE_F32;
   const dim3 g((unsigned)blocks);
   if (bf && f32) k_append<true, true><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
   else if (bf) k_append<true, false><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
   else if (f32) k_append<false, true><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
   else k_append<false, false><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
   return check_launch("k_append");
+}
+
+MTC_API int mtc_cache_read(const mtc_cache_desc* c, int layer, const mtc_heads* k, const mtc_heads* v, int dst_dtype, int rows,
+                           const int32_t* seqs, const int32_t* cu, int n, void* hip_stream) {
+  if (int rc = check_rows(c, layer, k, v, dst_dtype, rows, seqs, cu, n)) return rc;
+  if (!codes::is_codes(*c)) return fail(MTC_E_DTYPE, "a cache of dtype %d holds no codes", c->dtype);
+  if (n == 0 || rows == 0) return ok();
+  hipStream_t st = (hipStream_t)hip_stream;
+  const bool bf = codes::base_type(*c) == MTC_DTYPE_BF16, f32 = dst_dtype == MTC_DTYPE_F32;
+  const int64_t blocks = ((int64_t)rows * 2 * c->kv_heads * (codes::row_bytes(c->dim) / 16) + 255) / 256;
+  if (blocks > 0xFFFFFF) return fail(MTC_E_SHAPE, "%d rows: too many", rows);
+  const dim3 g((unsigned)blocks);
+  if (bf && f32) k_read8<true, MTC_DTYPE_F32><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
+  else if (bf) k_read8<true, MTC_DTYPE_BF16><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
+  else if (f32) k_read8<false, MTC_DTYPE_F32><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
+  else k_read8<false, MTC_DTYPE_F16><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
+  return check_launch("k_read8");
 }
 
 MTC_API size_t mtc_verify_workspace_bytes(const mtc_verify_args* a) {
