@@ -48,7 +48,7 @@ class PagedCache:
         self.dtype = dtype
         self.n_pages, self.n_layers, self.n_kv_heads, self.head_dim = int(n_pages), int(n_layers), int(n_kv_heads), int(head_dim)
         self.page_size, self.max_seqs, self.max_pages = int(page_size), int(max_seqs), int(max_pages)
-        code = self._code = _dtype_code(dtype)
+        code = _dtype_code(dtype)
         _need(min(self.n_pages, self.n_layers, self.n_kv_heads, self.max_seqs, self.max_pages) > 0, "sizes must be positive")
         _need(8 <= self.head_dim <= _abi.ATTN_MAX_DIM and self.head_dim % 8 == 0,
               f"head_dim must be a multiple of 8 from 8 to {_abi.ATTN_MAX_DIM}, got {head_dim}")
@@ -135,7 +135,7 @@ class PagedCache:
         k, v = (x if x.stride(2) == 1 and not (x.stride(0) | x.stride(1)) & mask and not x.data_ptr() & 15 else _copy(x)
                 for x in (k, v))
         hk, hv = (_abi.MtcHeads(x.data_ptr(), x.stride(0), x.stride(1)) for x in (k, v))
-        code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self._code
+        code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self.desc.dtype & ~_abi.CACHE_CODES8
         self._call("mtc_cache_append", layer, ctypes.byref(hk), ctypes.byref(hv), code, k.shape[0], p, c, seqs.shape[0])
 
     def fork(self, src, dst) -> None:
@@ -268,6 +268,6 @@ class QuantizedCache(PagedCache):
         p = self._list("seqs", seqs)
         c = _int32("cu", cu, seqs.shape[0] + 1, self.device)
         hk, hv = (_abi.MtcHeads(x.data_ptr(), x.stride(0), x.stride(1)) for x in (k, v))
-        code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self._code
+        code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self.desc.dtype & ~_abi.CACHE_CODES8
         self._call("mtc_cache_read", layer, ctypes.byref(hk), ctypes.byref(hv), code, k.shape[0], p, c, seqs.shape[0])
         return k, v
