@@ -268,6 +268,40 @@ typedef struct mtc_rotary_args {
 
 int mtc_rotary(const mtc_rotary_args* a, void* hip_stream);
 
+/*
+ * One step of beam search: of every prompt's beams x vocabulary continuations the n with the highest score
+ *   scores[b, w] + logits[b, w, v] - log sum_u exp logits[b, w, u]
+ * in falling order, equal ones in the order of w * vocab + v. A beam with done[b, w] (NULL: none) is not continued: it stands
+ * as one candidate of its present score, with the token `pad` (in the order: v = 0); its logits are not read. Candidates of score -inf or NaN are none
+ * (a logit of -inf is a token that may not come; a NaN or +inf among a beam's logits leaves that beam without candidates). Logarithms and
+ * exponentials are fp32 or better, sums of scores fp64.
+ *   logits (n_prompts, beams, vocab) fp32, bf16 or f16, element strides of the first two axes; scores (n_prompts, beams)
+ *   fp32 and done bytes, contiguous; outputs (n_prompts, n): scores fp32, tokens, parents (b * beams + w). Where there are fewer candidates
+ *   than n: -inf, -1 and the row b * beams + min(place, beams - 1).
+ * Workspace: mtc_beam_workspace_bytes, 256-byte aligned, no initialisation.
+ */
+#define MTC_BEAM_MAX 64                /* beams of a prompt, and n */
+typedef struct mtc_beam_args {
+  uint32_t abi_version;
+  int32_t dtype;
+  int32_t n_prompts;
+  int32_t beams;
+  int32_t vocab;
+  int32_t n;
+  int32_t pad;
+  int32_t reserved;           /* 0 */
+  const void* logits;
+  int64_t stride[2];
+  const float* scores;
+  const uint8_t* done;
+  float* out_scores;
+  int32_t* tokens;
+  int32_t* parents;
+} mtc_beam_args;
+
+size_t mtc_beam_workspace_bytes(const mtc_beam_args* a);
+int mtc_beam_select(const mtc_beam_args* a, void* workspace, size_t workspace_bytes, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

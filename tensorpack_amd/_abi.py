@@ -27,9 +27,11 @@ EXPORTED = ("mtc_abi_version", "mtc_last_error", "mtc_check_desc", "mtc_dequant"
 SERVE_EXPORTED = ("mtc_prompt_attention_workspace_bytes", "mtc_prompt_attention", "mtc_check_cache_desc", "mtc_cache_scratch_ints", "mtc_cache_extend",
                   "mtc_cache_fork", "mtc_cache_truncate", "mtc_cache_compact", "mtc_cache_copy_pages", "mtc_cache_append",
                   "mtc_cached_attention_workspace_bytes", "mtc_cached_attention", "mtc_verify_workspace_bytes",
-                  "mtc_verify_drafts", "mtc_rotary", "mtc_cache_read", "mtc_cache_reorder")
+                  "mtc_verify_drafts", "mtc_rotary", "mtc_cache_read", "mtc_cache_reorder",
+                  "mtc_beam_workspace_bytes", "mtc_beam_select")
 
 ATTN_MAX_DIM = 128                       # MTC_ATTN_MAX_DIM
+BEAM_MAX = 64                            # MTC_BEAM_MAX
 ROTARY_MAX_DIM = 1024                    # MTC_ROTARY_MAX_DIM
 CACHED_MAX_TOKENS = 16                   # MTC_CACHED_MAX_TOKENS
 CACHED_MAX_SEQS = 8192                   # MTC_CACHED_MAX_SEQS
@@ -167,6 +169,15 @@ class MtcRotaryArgs(ctypes.Structure):
     ]
 
 
+class MtcBeamArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("n_prompts", ctypes.c_int32), ("beams", ctypes.c_int32),
+        ("vocab", ctypes.c_int32), ("n", ctypes.c_int32), ("pad", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("logits", ctypes.c_void_p), ("stride", ctypes.c_int64 * 2), ("scores", ctypes.c_void_p), ("done", ctypes.c_void_p),
+        ("out_scores", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("parents", ctypes.c_void_p),
+    ]
+
+
 MAX_GROUP = 4                        # MTC_MAX_GROUP: matrices per mtc_gemv_f32_group launch
 
 
@@ -247,7 +258,9 @@ def declare_serve(lib: ctypes.CDLL) -> None:
             ("mtc_verify_drafts", i32, [P(MtcVerifyArgs), vp, sz, vp]),
             ("mtc_rotary", i32, [P(MtcRotaryArgs), vp]),
             ("mtc_cache_read", i32, [cache, i32, P(MtcHeads), P(MtcHeads), i32, i32, vp, vp, i32, vp]),
-            ("mtc_cache_reorder", i32, [cache, vp, vp, i32, vp])):
+            ("mtc_cache_reorder", i32, [cache, vp, vp, i32, vp]),
+            ("mtc_beam_workspace_bytes", sz, [P(MtcBeamArgs)]),
+            ("mtc_beam_select", i32, [P(MtcBeamArgs), vp, sz, vp])):
         getattr(lib, name).restype = res
         getattr(lib, name).argtypes = args
 

@@ -21,7 +21,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 INCLUDE = os.path.join(ROOT, "include")
 
-HIP_SOURCES = ["mtc_hip.hip", "mtc_gemm.hip", "mtc_attn.hip", "mtc_attn8.hip", "mtc_cache.hip", "mtc_rotary.hip"]
+HIP_SOURCES = ["mtc_hip.hip", "mtc_gemm.hip", "mtc_attn.hip", "mtc_attn8.hip", "mtc_cache.hip", "mtc_rotary.hip", "mtc_beam.hip"]
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # packed fp32 VALU ops stay disabled (known to misbehave on this part)

@@ -11,9 +11,8 @@
 
 #include <cmath>
 
-#include "mtc_attn.h"
 #include "mtc_host.h"
-#include "mtc_serve.h"
+#include "mtc_values.h"
 
 #define MTC_API extern "C" __attribute__((visibility("default")))
 
@@ -25,32 +24,6 @@ using namespace mtc::attn;
 namespace {
 
 constexpr int kRotaryThreads = 256;
-
-template <int DT>
-struct Value;
-template <>
-struct Value<MTC_DTYPE_F32> {
-  typedef float type;
-  static __device__ __forceinline__ float get(float x) { return x; }
-  static __device__ __forceinline__ float put(float x) { return x; }
-};
-template <>
-struct Value<MTC_DTYPE_BF16> {
-  typedef uint16_t type;
-  static __device__ __forceinline__ float get(uint16_t x) { return Elem<true>::widen(x); }
-  static __device__ __forceinline__ uint16_t put(float x) { return Elem<true>::round(x); }
-};
-template <>
-struct Value<MTC_DTYPE_F16> {
-  typedef uint16_t type;
-  static __device__ __forceinline__ float get(uint16_t x) { return Elem<false>::widen(x); }
-  static __device__ __forceinline__ uint16_t put(float x) { return Elem<false>::round(x); }
-};
-
-template <class T, int N>
-struct __attribute__((aligned(sizeof(T) * N < 16 ? sizeof(T) * N : 16))) Run {
-  T x[N];
-};
 
 __device__ __forceinline__ void sin_cos(int32_t position, uint64_t turns, float& s, float& c) {
   const uint64_t turn = (uint64_t)(int64_t)position * turns + 0x80000000u;

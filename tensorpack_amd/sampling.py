@@ -1,4 +1,4 @@
-"""Verification of drafted tokens (include/mtc_serve.h). No counterpart in the reference.
+"""Verification of drafted tokens, and a step of beam search (include/mtc_serve.h). No counterpart in the reference.
 
 A small model drafts a few tokens per sequence; the large one scores them in one pass (at 2 to 16 rows the packed
 matmul reads its weights once, as for one) and keeps a run of them so that the tokens have the large
@@ -6,6 +6,7 @@ model's distribution.
 """
 
 import ctypes
+from typing import Optional
 
 from . import _abi, _native
 from .device import on_device, raw_stream, require_gpu, stream_workspace
@@ -63,3 +64,48 @@ def verify_drafts(drafts, p, q, u, noise, *, n_drafts=None):
         if rc:
             _abi.check(lib, "mtc_verify_drafts", rc)
     return tokens, accepted
+
+
+def beam_select(logits, scores, *, n: Optional[int] = None, done=None, pad: int = 0):
+    """(scores, tokens, parents), each (B, n): the n best continuations of each prompt's W beams (mtc_beam_select).
+
+    logits (B, W, V) fp32, bf16 or f16, unit stride along V; scores (B, W) fp32: the beams' log probabilities so far. n: default W, at
+    most 64, as W. A continuation's score is scores[b, w] + log_softmax(logits[b, w])[v]; the best come first, equal ones
+    in the order of w * V + v. done (B, W) bool: beams that have ended; such a beam stands as one candidate with its score as it is and the token
+    `pad`. Scores of -inf are no candidates (give all beams but one -inf at the first step, or tokens that must not come a logit of -inf).
+    scores fp32, tokens int32, parents int32: the row b * W + w of the beam that goes on, as it stands in `logits.flatten(0, 1)`, and in the
+    list for `PagedCache.reorder` where n = W. Where there are fewer candidates than n: -inf, -1 and some row of the prompt.
+    """
+    import torch
+    dev = logits.device if logits.is_cuda else require_gpu(logits.device)
+    if logits.dim() != 3 or scores.shape != logits.shape[:2]:
+        raise ValueError(f"logits (B, W, V) and scores (B, W), got {tuple(logits.shape)}, {tuple(scores.shape)}")
+    B, W, V = logits.shape
+    n = W if n is None else n
+    code = {torch.float32: _abi.MTC_DTYPE_F32, torch.bfloat16: _abi.MTC_DTYPE_BF16, torch.float16: _abi.MTC_DTYPE_F16}.get(logits.dtype)
+    if code is None or scores.dtype != torch.float32:
+        raise ValueError(f"logits must be fp32, bf16 or f16, scores fp32, got {logits.dtype}, {scores.dtype}")
+    if not 1 <= W <= _abi.BEAM_MAX or not 1 <= n <= _abi.BEAM_MAX or V < 1:
+        raise ValueError(f"1 to {_abi.BEAM_MAX} beams and picks over a vocabulary, got {W}, {n}, {V}")
+    if scores.device != dev or (done is not None and not (done.dtype == torch.bool and done.shape == scores.shape and done.device == dev)):
+        raise ValueError(f"scores must be on {dev}, and done {tuple(scores.shape)} bool there")
+    if not -1 << 31 <= pad < 1 << 31:
+        raise ValueError(f"pad must fit 32 bits, got {pad}")
+    best = torch.empty((B, n), dtype=torch.float32, device=dev)
+    tokens, parents = torch.empty((2, B, n), dtype=torch.int32, device=dev)
+    if B == 0:
+        return best, tokens, parents
+    logits = logits if logits.stride(2) == 1 else logits.contiguous()
+    scores = scores.contiguous()
+    done = None if done is None else done.contiguous()
+    lib = _native.hip_lib()
+    args = _abi.MtcBeamArgs(_abi.ABI_VERSION, code, B, W, V, n, pad, 0, logits.data_ptr(), logits.stride()[:2], scores.data_ptr(),
+                            None if done is None else done.data_ptr(), best.data_ptr(), tokens.data_ptr(), parents.data_ptr())
+    ref, stream = ctypes.byref(args), raw_stream(dev.index)
+    need = lib.mtc_beam_workspace_bytes(ref)
+    with on_device(dev.index):
+        ws = stream_workspace(dev.index, stream, need)
+        rc = lib.mtc_beam_select(ref, ws.data_ptr(), need, stream)
+        if rc:
+            _abi.check(lib, "mtc_beam_select", rc)
+    return best, tokens, parents
