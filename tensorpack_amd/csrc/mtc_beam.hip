@@ -56,8 +56,27 @@ __device__ __forceinline__ float wave_top(float x) {
   x = step(x, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
-// The n-th largest of the lanes' values, -inf if fewer are above that.
-__device__ __forceinline__ float nth_top(float x, int n) {
+// A value that at least n of the lanes' values reach, -inf if fewer than n are above that. Up to 16: lanes that are equal modulo
+// a power of two >= n form a group, and the least of the groups' maxima is reached by one lane of each (n ln n lanes or so in all: six
+// exchanges for that list, where n of them give the n-th largest, 150 cycles each). Lanes without values are the last ones, so that
+// no group is empty while n lanes have some.
+__device__ __forceinline__ float reached(float x, int n) {
+  if (n <= 16) {
+    const int groups = n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1));
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+      const int u = __builtin_bit_cast(int, x);
+      int v;                                                // of the lane at distance d: lanes 2 d apart hold the same already
+      if (d >= 16) v = __shfl_xor(u, d);
+      else if (d == 8) v = __builtin_amdgcn_update_dpp(u, u, 0x128, 0xF, 0xF, false);       // row_ror:8
+      else if (d == 4) v = __builtin_amdgcn_update_dpp(u, u, 0x124, 0xF, 0xF, false);       // row_ror:4
+      else if (d == 2) v = __builtin_amdgcn_update_dpp(u, u, 0x4E, 0xF, 0xF, false);        // quad_perm 2 3 0 1
+      else v = __builtin_amdgcn_update_dpp(u, u, 0xB1, 0xF, 0xF, false);                    // quad_perm 1 0 3 2
+      const float y = __builtin_bit_cast(float, v);
+      x = d >= groups ? fmaxf(x, y) : fminf(x, y);
+    }
+    return x;
+  }
   float t = -INFINITY;
   for (int i = 0; i < n; ++i) {
     t = wave_top(x);
@@ -67,10 +86,11 @@ __device__ __forceinline__ float nth_top(float x, int n) {
   }
   return t;
 }
+constexpr float kLeast = -3.402823466e38f;  // of what is above -inf
 
-// Chunks of 512 ROUNDS logits, 8 ROUNDS a lane. What can be among the n best is not below the n-th largest of the lanes' maxima:
-// mostly n or a few more values, which are ranked in LDS by counting. (Many equal values overflow the list: then the best are
-// taken one after another.)
+// Chunks of 512 ROUNDS logits, 8 ROUNDS a lane. What can be among the n best is not below a value that n of the lanes' maxima reach:
+// a few values, which each lane marks by a bit, reads again (from a cache) and ranks in LDS by counting. (Many equal values overflow the
+// list: then the best are taken one after another.)
 template <int DT, int ROUNDS>
 __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const Parts parts) {
   using V = Value<DT>;
@@ -83,17 +103,18 @@ __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const 
   const T* p = reinterpret_cast<const T*>(a.logits) + (row / a.beams) * a.stride[0] + (row % a.beams) * a.stride[1];
   const int from = chunk * 64 * kEach + lane * 8;          // element e: from + e / 8 * 512 + e % 8
   float x[kEach];
+  if ((chunk + 1) * 64 * kEach <= a.vocab) {               // all loads before the first is looked at
+    Loose<T, 8> y[ROUNDS];
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
-    const int at = from + r * 512;
-    if (at + 8 <= a.vocab) {
-      const Loose<T, 8> y = *reinterpret_cast<const Loose<T, 8>*>(p + at);
+    for (int r = 0; r < ROUNDS; ++r) y[r] = *reinterpret_cast<const Loose<T, 8>*>(p + from + r * 512);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[8 * r + j] = V::get(y.x[j]);
-    } else {
+    for (int e = 0; e < kEach; ++e) x[e] = V::get(y[e / 8].x[e % 8]);
+  } else {
+    T y[kEach];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[8 * r + j] = at + j < a.vocab ? V::get(p[at + j]) : -INFINITY;
-    }
+    for (int e = 0; e < kEach; ++e) y[e] = p[min(from + e / 8 * 512 + e % 8, a.vocab - 1)];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) x[e] = from + e / 8 * 512 + e % 8 < a.vocab ? V::get(y[e]) : -INFINITY;
   }
   float mine = -INFINITY;
 #pragma unroll
@@ -107,16 +128,20 @@ __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const 
   if (lane == 0) parts.stat[part] = Stat{top, sum};
   Candidate* const out = parts.best + part * a.n;
 
-  const float least = nth_top(mine, a.n);
+  const float least = fmaxf(reached(mine, a.n), kLeast);
+  uint32_t low = 0, high = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) (e < 32 ? low : high) |= x[e] >= least ? 1u << (e % 32) : 0u;
+  uint64_t left = (uint64_t)high << 32 | low;
   int count = 0;
   Candidate* const list = lists[wave];
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const bool take = x[e] >= least && x[e] > -INFINITY;
-    const uint64_t all = __ballot(take);
-    if (!all) continue;
+  while (const uint64_t all = __ballot(left != 0)) {
     const int at = count + __popcll(all & ((1ull << lane) - 1));
-    if (take && at < kList) list[at] = Candidate{x[e], from + e / 8 * 512 + e % 8};
+    if (left && at < kList) {
+      const int e = __builtin_ctzll(left), v = from + e / 8 * 512 + e % 8;
+      list[at] = Candidate{V::get(p[v]), v};
+    }
+    left &= left - 1;
     count += __popcll(all);
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
@@ -125,9 +150,10 @@ __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const 
     for (int i = lane; i < count; i += 64) {
       const Candidate me = list[i];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < count; ++j) {
         const Candidate it = list[j];
-        rank += it.x > me.x || (it.x == me.x && it.v < me.v);
+        rank += (int)(it.x > me.x) | ((int)(it.x == me.x) & (int)(it.v < me.v));        // without branches
       }
       if (rank < a.n) out[rank] = me;
     }
@@ -140,8 +166,9 @@ __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const 
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {                      // places ascend in e
       const int v = from + e / 8 * 512 + e % 8;
-      const bool after = x[e] < last.x || (x[e] == last.x && v > last.v);
-      if (after && x[e] > best.x) best = Candidate{x[e], v};
+      const bool take = ((x[e] < last.x) | ((x[e] == last.x) & (v > last.v))) & (x[e] > best.x);
+      best.x = take ? x[e] : best.x;
+      best.v = take ? v : best.v;
     }
     const float t = wave_top(best.x);
     int v = best.x == t ? best.v : 0x7FFFFFFF;
@@ -156,70 +183,100 @@ __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const 
 // logits that decide.
 struct Pick {
   double score;
-  int32_t w, v;
+  uint64_t place;                          // w << 32 | v
 };
-__device__ __forceinline__ bool before(const Pick& a, const Pick& b) {
-  return a.score > b.score || (a.score == b.score && (a.w < b.w || (a.w == b.w && a.v < b.v)));
+__device__ __forceinline__ bool before(const Pick& a, const Pick& b) {      // without branches
+  return (a.score > b.score) | ((a.score == b.score) & (a.place < b.place));
 }
-__global__ __launch_bounds__(kThreads) void k_beam_join(const mtc_beam_args a, const Parts parts) {
+__device__ __forceinline__ uint64_t place_of(int w, int v) { return (uint64_t)w << 32 | (uint32_t)v; }
+// A thread per chunk of a beam (or several), whose candidates fall: the first ones give a bound, and few chunks have more than one
+// above it.
+constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
+constexpr int kAhead = 4;                  // candidates of a chunk that are loaded before the bound is known
+__global__ __launch_bounds__(kJoinThreads) void k_beam_join(const mtc_beam_args a, const Parts parts) {
   __shared__ double offset[MTC_BEAM_MAX];
+  __shared__ int ended[MTC_BEAM_MAX];
   __shared__ Pick list[kJoinList];
-  __shared__ float least[kWaves];
+  __shared__ float least[kJoinWaves];
   __shared__ int count;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int items = a.beams * parts.chunks;
+  const Candidate* const best = parts.best + (int64_t)b * items * a.n;
+  // everything is loaded in one round (of beams that have ended, whatever is there: it is not used)
+  Candidate ahead[kAhead];                                 // of item `tid`
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) ahead[k] = tid < items && k < a.n ? best[(int64_t)tid * a.n + k] : Candidate{-INFINITY, -1};
   if (tid == 0) count = 0;
-  for (int w = wave; w < a.beams; w += kWaves) {
+  for (int w = wave; w < a.beams; w += kJoinWaves) {
     const int row = b * a.beams + w;
-    double o = a.scores[row];
-    if (!(a.done && a.done[row])) {
-      const Stat* s = parts.stat + (int64_t)row * parts.chunks;
-      float top = -INFINITY;
-      for (int c = lane; c < parts.chunks; c += 64) top = fmaxf(top, s[c].top);
-      top = wave_top(top);
-      double sum = 0.0;
-      for (int c = lane; c < parts.chunks; c += 64)
-        if (!(s[c].top == -INFINITY && s[c].sum == 0.0f)) sum += (double)s[c].sum * exp((double)s[c].top - (double)top);
-      sum = wave_sum(sum);
-      o -= (double)top + log(sum);
+    const Stat* s = parts.stat + (int64_t)row * parts.chunks;
+    Stat x = lane < parts.chunks ? s[lane] : Stat{-INFINITY, 0.0f};
+    const double score = a.scores[row];
+    const bool over = a.done && a.done[row];
+    for (int c = lane + 64; c < parts.chunks; c += 64) {
+      const Stat y = s[c];
+      const float t = fmaxf(x.top, y.top), u = t == -INFINITY ? 0.0f : t;
+      x = Stat{t, x.sum * expf(x.top - u) + y.sum * expf(y.top - u)};
     }
-    if (lane == 0) offset[w] = o;
+    const float top = wave_top(x.top), base = top == -INFINITY ? 0.0f : top;
+    const double sum = wave_sum((double)(x.sum * expf(x.top - base)));
+    if (lane == 0) {
+      offset[w] = over ? score : score - ((double)top + log(sum));
+      ended[w] = over;
+    }
   }
   __syncthreads();
-  const int64_t each = (int64_t)parts.chunks * a.n, total = each * a.beams;
-  const Candidate* best = parts.best + (int64_t)b * total;
-  // candidate i: of the chunks, then one per beam that has ended
-  auto pick = [&](int64_t i) {
-    if (i >= total) {
-      const int w = (int)(i - total);
-      return Pick{a.done && a.done[b * a.beams + w] ? offset[w] : -INFINITY, w, 0};
-    }
-    const int w = (int)(i / each);
-    if (a.done && a.done[b * a.beams + w]) return Pick{-INFINITY, w, 0};
-    const Candidate c = best[i];
-    return Pick{offset[w] + (double)c.x, w, c.v};
-  };
-  float mine = -INFINITY;
-  for (int64_t i = tid; i < total + a.beams; i += kThreads) mine = fmaxf(mine, (float)pick(i).score);
-  const float nth = nth_top(mine, a.n);
-  if (lane == 0) least[wave] = nth;
+  const int my_w = min(tid / parts.chunks, a.beams - 1);
+  const bool mine_over = tid < a.beams && ended[tid];      // beam `tid` stands as a candidate
+  auto score = [&](int w, float x) { return offset[w] + (double)x; };
+  const bool go_on = tid < items && !ended[my_w];
+  float mine = mine_over ? (float)offset[tid] : -INFINITY;
+  if (go_on) mine = fmaxf(mine, (float)score(my_w, ahead[0].x));
+  for (int i = tid + kJoinThreads; i < items; i += kJoinThreads) {
+    const int w = i / parts.chunks;
+    if (!ended[w]) mine = fmaxf(mine, (float)score(w, best[(int64_t)i * a.n].x));
+  }
+  const float bound = fmaxf(reached(mine, a.n), kLeast);
+  if (lane == 0) least[wave] = bound;
   __syncthreads();
   float from = least[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) from = fmaxf(from, least[w]);
-  for (int64_t i = tid; i < total + a.beams; i += kThreads) {
-    const Pick p = pick(i);
-    if ((float)p.score >= from && p.score > -INFINITY) {
-      const int at = atomicAdd(&count, 1);
-      if (at < kJoinList) list[at] = p;
+  for (int w = 1; w < kJoinWaves; ++w) from = fmaxf(from, least[w]);
+  auto above = [&](int w, float x) { return (float)score(w, x) >= from; };
+  auto offer = [&](int at, const Pick& p) {
+    if (at < kJoinList) list[at] = p;
+  };
+  auto rest = [&](int i, int w, int k) {                   // of item i, from candidate k on, to the first below the bound
+    for (; k < a.n; ++k) {
+      const Candidate c = best[(int64_t)i * a.n + k];
+      if (!above(w, c.x)) break;
+      offer(atomicAdd(&count, 1), Pick{score(w, c.x), place_of(w, c.v)});
     }
+  };
+  if (mine_over && (float)offset[tid] >= from) offer(atomicAdd(&count, 1), Pick{offset[tid], place_of(tid, 0)});
+  if (go_on) {
+    int some = 0;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) some += above(my_w, ahead[k].x);
+    if (some) {
+      const int at = atomicAdd(&count, some);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (k < some) offer(at + k, Pick{score(my_w, ahead[k].x), place_of(my_w, ahead[k].v)});
+      if (some == kAhead) rest(tid, my_w, kAhead);
+    }
+  }
+  for (int i = tid + kJoinThreads; i < items; i += kJoinThreads) {
+    const int w = i / parts.chunks;
+    if (!ended[w]) rest(i, w, 0);
   }
   __syncthreads();
   const int found = count;
   auto put = [&](int k, const Pick& p) {
-    const int row = b * a.beams + p.w;
+    const int w = (int)(p.place >> 32), row = b * a.beams + w;
     const int64_t at = (int64_t)b * a.n + k;
     a.out_scores[at] = (float)p.score;
-    a.tokens[at] = a.done && a.done[row] ? a.pad : p.v;
+    a.tokens[at] = ended[w] ? a.pad : (int32_t)p.place;
     a.parents[at] = row;
   };
   auto none = [&](int k) {
@@ -229,9 +286,10 @@ __global__ __launch_bounds__(kThreads) void k_beam_join(const mtc_beam_args a, c
     a.parents[at] = b * a.beams + min(k, a.beams - 1);
   };
   if (found <= kJoinList) {
-    for (int i = tid; i < found; i += kThreads) {
+    for (int i = tid; i < found; i += kJoinThreads) {
       const Pick me = list[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < found; ++j) rank += before(list[j], me);
       if (rank < a.n) put(rank, me);
     }
@@ -239,21 +297,31 @@ __global__ __launch_bounds__(kThreads) void k_beam_join(const mtc_beam_args a, c
     return;
   }
   // more equal scores than the list holds: one pick after another
-  Pick last{INFINITY, -1, -1};
+  bool first = true;
+  Pick last{INFINITY, 0};
   for (int k = 0; k < a.n; ++k) {
-    Pick p{-INFINITY, 0x7FFFFFFF, 0};
-    for (int64_t i = tid; i < total + a.beams; i += kThreads) {
-      const Pick q = pick(i);
-      if (q.score > -INFINITY && before(last, q) && before(q, p)) p = q;
+    Pick p{-INFINITY, ~0ull};
+    auto take = [&](const Pick& q) {
+      if ((q.score > -INFINITY) & (first | before(last, q)) & before(q, p)) p = q;
+    };
+    if (mine_over) take(Pick{offset[tid], place_of(tid, 0)});
+    for (int i = tid; i < items; i += kJoinThreads) {
+      const int w = i / parts.chunks;
+      if (ended[w]) continue;
+      for (int j = 0; j < a.n; ++j) {
+        const Candidate c = best[(int64_t)i * a.n + j];
+        take(Pick{score(w, c.x), place_of(w, c.v)});
+      }
     }
     __syncthreads();                                       // the list's last readers
     list[tid] = p;
     __syncthreads();
-    for (int s = kThreads / 2; s; s >>= 1) {
+    for (int s = kJoinThreads / 2; s; s >>= 1) {
       if (tid < s && before(list[tid + s], list[tid])) list[tid] = list[tid + s];
       __syncthreads();
     }
     last = list[0];
+    first = false;
     if (tid == 0) {
       if (last.score > -INFINITY) put(k, last); else none(k);
     }
@@ -295,7 +363,7 @@ int run_beam(const mtc_beam_args& a, const Parts& parts, hipStream_t st) {
   if (beam_rounds(a) == 8) k_beam<DT, 8><<<grid, kThreads, 0, st>>>(a, parts);
   else k_beam<DT, 1><<<grid, kThreads, 0, st>>>(a, parts);
   if (int rc = check_launch("k_beam")) return rc;
-  k_beam_join<<<a.n_prompts, kThreads, 0, st>>>(a, parts);
+  k_beam_join<<<a.n_prompts, kJoinThreads, 0, st>>>(a, parts);
   return check_launch("k_beam_join");
 }
 

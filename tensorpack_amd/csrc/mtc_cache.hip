@@ -339,7 +339,7 @@ __global__ __launch_bounds__(kThreads) void k_fork(const mtc_cache_desc c, const
 // so that any sequence may take any other's place. Takers are counted before leavers, so that a page that stays held never counts 0.
 // Bound by its chain of loads (list, lengths, table, counts).
 constexpr int kReorderIds = MTC_CACHED_MAX_SEQS;
-__host__ __device__ inline int reorder_columns(int n) { return min(32, max(1, kReorderIds / n)); }
+__host__ __device__ inline int reorder_columns(int n) { return min(32, max(1, kThreads / n)); }      // an entry a thread, if they fit
 __global__ __launch_bounds__(kThreads) void k_reorder(const mtc_cache_desc c, const int32_t* seqs, const int32_t* parents, int n) {
   __shared__ uint32_t marks[kMarkWords];
   __shared__ int32_t ids[kReorderIds];
