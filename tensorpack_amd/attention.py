@@ -7,6 +7,7 @@ waits for the GPU, so a serving loop can capture them into a graph.
 """
 
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -21,6 +22,13 @@ def _dtype_code(dtype):
     if dtype == torch.float16:
         return _abi.MTC_DTYPE_F16
     raise ValueError(f"attention takes bfloat16 or float16, got {dtype}")
+
+
+@functools.lru_cache(maxsize=None)
+def _value_code(dtype):
+    """MTC_DTYPE_* of float32, bfloat16 or float16, None for others."""
+    import torch
+    return {torch.float32: _abi.MTC_DTYPE_F32, torch.bfloat16: _abi.MTC_DTYPE_BF16, torch.float16: _abi.MTC_DTYPE_F16}.get(dtype)
 
 
 def _in_place(x) -> bool:

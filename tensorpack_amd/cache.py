@@ -14,7 +14,7 @@ import ctypes
 from typing import Optional
 
 from . import _abi, _native
-from .attention import _aligned_rows, _apart, _copy, _dtype_code, _int32
+from .attention import _aligned_rows, _apart, _copy, _dtype_code, _heads, _int32
 from .device import _need, on_device, raw_stream, require_gpu
 
 STATE_WORDS = 4
@@ -214,6 +214,10 @@ class QuantizedCache(PagedCache):
 
     _flags = _abi.CACHE_CODES8
 
+    @property
+    def _type(self):
+        return self.desc.dtype & ~_abi.CACHE_CODES8
+
     def _pool_form(self):
         import torch
         blocks = self.page_size // _abi.CODES8_BLOCK
@@ -255,19 +259,21 @@ class QuantizedCache(PagedCache):
             raise ValueError("give rows, or out")
         if out is None:
             dtype = dtype or self.dtype
-            if rows < 0 or dtype not in (self.dtype, torch.float32):
+            if rows < 0 or (dtype != self.dtype and dtype != torch.float32):
                 raise ValueError(f"{rows} rows of {dtype}: the cache's {self.dtype} or float32")
-            out = tuple(torch.empty((rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in (0, 1))
-        k, v = out
-        form = (self.n_kv_heads, self.head_dim)
-        for x in (k, v):
-            ok = x.dim() == 3 and tuple(x.shape[1:]) == form and x.shape[0] == k.shape[0] and x.dtype == k.dtype
-            ok = ok and x.dtype in (self.dtype, torch.float32) and x.device == self.device
-            if not (ok and _aligned_rows(x) and _apart(x)):
-                raise ValueError(f"out must be two (rows, {form[0]}, {form[1]}) {self.dtype} or float32 tensors with 16-byte aligned rows")
+            k, v = torch.empty((2, rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+            stride = self.n_kv_heads * self.head_dim, self.head_dim
+            hk, hv = _abi.MtcHeads(k.data_ptr(), *stride), _abi.MtcHeads(v.data_ptr(), *stride)
+        else:
+            k, v = out
+            dtype, rows, form = k.dtype, k.shape[0], (self.n_kv_heads, self.head_dim)
+            for x in (k, v):
+                ok = x.dim() == 3 and tuple(x.shape) == (rows, *form) and x.dtype == dtype and dtype in (self.dtype, torch.float32)
+                if not (ok and x.device == self.device and _aligned_rows(x) and _apart(x)):
+                    raise ValueError(f"out must be two (rows, {form[0]}, {form[1]}) {self.dtype} or float32 tensors with 16-byte aligned rows")
+            hk, hv = _heads(k), _heads(v)
         p = self._list("seqs", seqs)
         c = _int32("cu", cu, seqs.shape[0] + 1, self.device)
-        hk, hv = (_abi.MtcHeads(x.data_ptr(), x.stride(0), x.stride(1)) for x in (k, v))
-        code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self.desc.dtype & ~_abi.CACHE_CODES8
-        self._call("mtc_cache_read", layer, ctypes.byref(hk), ctypes.byref(hv), code, k.shape[0], p, c, seqs.shape[0])
+        code = _abi.MTC_DTYPE_F32 if dtype == torch.float32 else self._type
+        self._call("mtc_cache_read", layer, ctypes.byref(hk), ctypes.byref(hv), code, rows, p, c, seqs.shape[0])
         return k, v

