@@ -379,6 +379,8 @@ __global__ __launch_bounds__(64 * kPromptWaves) void k_prompt_join(const mtc_pro
   }
 }
 
+constexpr int kWaveKeys = 32;                     // split keys: per wave and step
+
 // Buffer over up to 16 rows (of one page) of K or V from token p on, cut at token `to`; no rows if the page id is bad.
 __device__ __forceinline__ u32x4 page_rows(const CachedCall& a, int id, int64_t off, int p, int to) {
   const int rows = min(to - p, 16);
@@ -607,8 +609,12 @@ __device__ void split_rows(const CachedCall& a, const Book& book, char* lds, con
 
 template <bool BF>
 struct Store16 {
+  static constexpr int kKeys = kWaveKeys, kStart = 4, kStartAlone = 4, kShort = 8;
+  static constexpr float kCostRows = 2.2f, kCostKeys = 0.8f;
   typedef CachedCall Call;
   using E = Elem<BF>;
+  template <int DP>
+  static constexpr int kKeysBytes = kCachedWaves * 2 * kWaveKeys * DP * 2;      // one tile of keys, one of values a wave
   template <int DP, int MODE, bool PREFIX>
   static __device__ __forceinline__ void keys(const Call& a, const Book& book, char* lds, const Entry& x, int item, int from, int to, int slot,
                                               bool alone) {

@@ -17,6 +17,313 @@ namespace mtc {
 namespace attn {
 namespace {
 
+// ---------------------------------------------------------------------------
+// few rows: codes in LDS
+// ---------------------------------------------------------------------------
+// Tiles of 32 keys (or their values) as memory has them, a row of DP bytes cut into 16-byte pieces; piece c of row r lies at place
+// c ^ codes_key(r). Both readings take the same piece of rows that differ: keys 16 consecutive rows at a time, values the rows
+// 4 w .. 4 w + 3 and 16 + 4 w .. of two w.
+template <int DP>
+__device__ __forceinline__ uint32_t codes_key(uint32_t row) {
+  return DP == 128 ? (row >> 1 & 7u) ^ (row >> 4 & 1u) << 2 : (row >> 2 & 3u) ^ (row >> 4 & 1u) << 1;
+}
+
+// Codes as f16 numbers of the same value. A byte u under 0x64 is 1024 + u; u = code + 128.
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& a, uint32_t& b) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  w ^= 0x80808080u;
+  const h2 minus = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+  a = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + minus);
+  b = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + minus);
+}
+
+// Transposed read of bytes: of the 16 lanes of a group, lane i fetches 8 bytes (half i & 1 of a 16-byte piece of row i / 2 of 8) and
+// gets column i of these rows.
+__device__ __forceinline__ u32x2 read_transposed8(uint32_t at) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(uintptr_t)at));
+}
+
+// Global -> LDS copy of 4 bytes per lane, to lds + 4 lane. (The wait state after m0 is written stands here, as in copy16.)
+__device__ __forceinline__ void copy4(uint64_t from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dword %0, off" : : "v"(from), "s"(lds) : "memory", "m0");
+}
+// Waits until at most `base` copies and those of `further` whole tiles (EACH copies) are in flight.
+template <int BASE, int EACH, int MOST>
+__device__ __forceinline__ void wait_tiles(int further) {
+  if constexpr (MOST == 0) {
+    wait_copies<BASE>();
+  } else {
+    if (further >= MOST) wait_copies<BASE + MOST * EACH>();
+    else wait_tiles<BASE, EACH, MOST - 1>(further);
+  }
+}
+
+constexpr int kWaveKeys = 64;              // split keys: per wave and step
+constexpr int kSubs = kWaveKeys / 32;      // matrix steps of 32 keys (the depth of a product with the values)
+constexpr int kBlocks = kWaveKeys / codes::kBlock;
+template <int DP>
+struct KeyTiles {
+  static constexpr int kTile = kWaveKeys * DP, kDeep = 128 / DP;                 // bytes of a tile, tiles ahead
+  static constexpr int kScales = 256;                                            // LDS of a tile's scales (2 kBlocks words are used)
+  static constexpr int kBytes = kDeep * (2 * kTile + kScales);                   // of a wave
+};
+
+// One item's keys [from, to) (from a multiple of 16) into a partial result, by the block (the keys split over its waves)
+// or by this wave alone.
+//
+// Codes reach LDS as they are (direct copies, kDeep tiles of 64 keys ahead) and become f16 between LDS and the matrix core, 1.25
+// vector instructions each, for either type of cache: q, scaled by a power of two to f16's range, loses nothing that fp32 sums would
+// keep. Scales are folded in where there is one number per key instead of per element: a key's into its score, a value's into
+// its weight. With s = score (log2), m its running maximum and e = log2 of the value's scale:
+//   l = sum 2^(s - m),   o = sum 2^(s + e - t) code,   t the running maximum of s + e;   result 2^(t - m) o / l
+// so that weights keep f16's precision whatever the scales are. l adds weights in fp32, before they are rounded to f16 (half a step: 2^-12).
+template <bool BF, int DP, int MT, bool PREFIX>
+__device__ void split_keys(const CodesCall& a, const Book& book, char* lds, const Entry& x, int item, int from, int to, int slot, bool alone) {
+  using H = Elem<false>;
+  using Tiles = KeyTiles<DP>;
+  constexpr int kTile = Tiles::kTile, kDeep = Tiles::kDeep, kSub = 32 * DP, kHalf = 16 * DP;      // bytes of 64, 32, 16 keys
+  constexpr int kHalfCopies = kHalf / 1024, kCopyRows = 1024 / DP, kCopies = kBlocks * kHalfCopies;      // of 16 keys, of a tile
+  constexpr int kKeyCopies = kCopies + 1, kBoth = kKeyCopies + kCopies;          // keys with scales; with their values
+  constexpr int kSteps = DP / 32;
+  constexpr float kLag = 8.0f;                           // bits that weights may grow before o is scaled down
+  const int stride = alone ? kWaveKeys : kCachedWaves * kWaveKeys;
+  const Pass& ps = PREFIX ? a.pre : a.own;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, w = lane >> 4;
+  const int D = a.dim;
+  const int kvh = item / x.tiles, row0 = (item % x.tiles) * 16 * MT;
+  const int rows = min(x.rows - row0, 16 * MT);
+
+  PageWindow pages{a.table + (int64_t)x.seq.row * a.max_pages, 0, -1, a.max_pages};
+  const int first = alone ? from : from + kWaveKeys * wave;
+  const int tiles = first < to ? (to - first + stride - 1) / stride : 0;
+  if (tiles) pages.load(first >> a.page_log);
+
+  uint32_t from_lane[2][kHalfCopies];                    // byte offsets within 16 rows
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+    for (int i = 0; i < kHalfCopies; ++i) {
+      const uint32_t r = i * kCopyRows + lane / (DP / 16), c = lane % (DP / 16) ^ codes_key<DP>(16 * hf + r);
+      from_lane[hf][i] = (int)c * 16 < a.room ? r * a.room + c * 16 : kOutOfRange;
+    }
+  char* const mine = lds + wave * Tiles::kBytes;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(mine));
+  const int64_t head = ((int64_t)kvh << a.page_log), head_codes = head * a.room, head_scales = head / codes::kBlock * 2;
+  const int mask = (1 << a.page_log) - 1;
+  auto copy_codes = [&](int p0, int64_t off, uint32_t dst) {
+#pragma unroll
+    for (int hf = 0; hf < kBlocks; ++hf) {
+      const int p = p0 + 16 * hf, id = pages(p >> a.page_log), count = min(to - p, 16);
+      const bool good = count > 0 && (uint32_t)id < (uint32_t)a.n_pages;
+      const char* at = a.codes + (int64_t)(good ? id : 0) * a.page_bytes + off + head_codes + (int64_t)(p & mask) * a.room;
+      const u32x4 r = buffer_rsrc((uint64_t)(uintptr_t)at, good ? (uint32_t)(count * a.room) : 0u);
+#pragma unroll
+      for (int i = 0; i < kHalfCopies; ++i) copy16(r, from_lane[hf & 1][i], __builtin_amdgcn_readfirstlane(dst + hf * kHalf + i * 1024));
+    }
+  };
+  // a word that holds the scale: lanes 0 .. kBlocks - 1 of the keys' blocks, the next ones of the values'
+  auto scale_at = [&](int p, int is_v) { return (is_v ? a.v_scales : a.k_scales) + head_scales + (int64_t)((p & mask) / codes::kBlock * 2); };
+  auto copy_scales = [&](int p0, uint32_t dst) {
+    const int p = p0 + 16 * (lane % kBlocks), id = __shfl(pages.ids, min((p >> a.page_log) - pages.at, 63));
+    const char* page = a.codes + (int64_t)((uint32_t)id < (uint32_t)a.n_pages ? id : 0) * a.page_bytes;
+    copy4((uint64_t)(uintptr_t)(page + (scale_at(p, lane / kBlocks & 1) & ~3ll)), __builtin_amdgcn_readfirstlane(dst));
+  };
+  auto place = [&](int t) { return (uint32_t)(t % kDeep); };
+  auto copy_keys = [&](int t) {
+    const int p = first + t * stride;
+    if (((p + kWaveKeys - 1) >> a.page_log) - pages.at > 63) pages.load(p >> a.page_log);
+    copy_scales(p, lds0 + kDeep * 2 * kTile + place(t) * Tiles::kScales);
+    copy_codes(p, a.k_codes, lds0 + place(t) * 2 * kTile);
+  };
+  auto copy_values = [&](int t) { copy_codes(first + t * stride, a.v_codes, lds0 + place(t) * 2 * kTile + kTile); };
+  // this lane's query rows 16 rt + n: piece 4 j + w of 16 dims is multiplied in steps 2 j and 2 j + 1
+  u32x4 qf[MT][kSteps];
+  int seen[MT], all = 0x7FFFFFFF;                        // keys that a row sees, that all rows see
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt) {
+    const int rr = row0 + rt * 16 + n;
+    const uint16_t* qp = cached_query<PREFIX>(a, book, x, kvh, rr, seen[rt]);
+    if (rr < x.rows) all = min(all, seen[rt]);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int d = 16 * (4 * (s >> 1) + w) + 8 * (s & 1);
+      qf[rt][s] = rr < x.rows && d < D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
+    }
+  }
+  // they are here before the copies start (waits for loads count those too)
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt)
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(qf[rt][s]));
+
+#pragma unroll
+  for (int t = 0; t < kDeep; ++t)
+    if (t < tiles) {
+      copy_keys(t);
+      copy_values(t);
+    }
+
+  float scale[MT];
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt) {
+    scale[rt] = a.c;
+    if constexpr (BF) {
+      uint32_t most = 0;                                 // the row's largest magnitude
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = max(max(most, qf[rt][s][i] << 16 & 0x7FFF0000u), qf[rt][s][i] & 0x7FFF0000u);
+      most = max(most, (uint32_t)__shfl_xor((int)most, 16));
+      most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+      const int exponent = (int)(most >> 23) - 127;
+      const int by = exponent == 128 ? 0 : min(max(exponent, -100), 113) - 14;       // not finite: as it is
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = qf[rt][s][i];
+          qf[rt][s][i] = H::pack(Elem<true>::widen((uint16_t)u) * codes::power(-by), Elem<true>::widen((uint16_t)(u >> 16)) * codes::power(-by));
+        }
+      scale[rt] *= codes::power(by);
+    }
+  }
+#pragma unroll
+  for (int d = 8; d; d >>= 1) all = min(all, __shfl_xor(all, d));
+  all = __builtin_amdgcn_readfirstlane(all);
+
+  const uint32_t v_row = (n < 8 ? 0u : 16u) + 4 * w + (n >> 1 & 3u);      // that this lane fetches for the transposed read
+  const uint32_t v_at = lds0 + kTile + v_row * DP + 8 * (n & 1);
+  const uint32_t v_key = codes_key<DP>(v_row);
+
+  f32x4 o[MT][DP / 16];
+  float top[MT], most[MT], sum[MT];                      // m, t and this lane's share of l
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt) {
+    top[rt] = most[rt] = -INFINITY;
+    sum[rt] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) o[rt][d] = f32x4{};
+  }
+  for (int t = 0; t < tiles; ++t) {
+    const int pos = first + t * stride;
+    const uint32_t buf = place(t) * 2 * kTile;
+    wait_tiles<kCopies, kBoth, kDeep - 1>(tiles - 1 - t);          // keys and scales are there
+    f32x4 s[MT][kBlocks];
+#pragma unroll
+    for (int rt = 0; rt < MT; ++rt)
+#pragma unroll
+      for (int g = 0; g < kBlocks; ++g) s[rt][g] = f32x4{};
+#pragma unroll
+    for (int j = 0; j < kSteps / 2; ++j)
+#pragma unroll
+      for (int g = 0; g < kBlocks; ++g) {
+        const uint32_t r = (g & 1) * 16 + n;             // in its 32 keys
+        const u32x4 k = *reinterpret_cast<const u32x4*>(mine + buf + (g >> 1) * kSub + r * DP + ((4 * j + w) ^ codes_key<DP>(r)) * 16);
+        u32x4 lo, hi;
+        uint32_t u, v;
+        widen4(k[0], u, v);
+        lo[0] = u; lo[1] = v;
+        widen4(k[1], u, v);
+        lo[2] = u; lo[3] = v;
+        widen4(k[2], u, v);
+        hi[0] = u; hi[1] = v;
+        widen4(k[3], u, v);
+        hi[2] = u; hi[3] = v;
+#pragma unroll
+        for (int rt = 0; rt < MT; ++rt) {
+          s[rt][g] = H::mfma16(lo, qf[rt][2 * j], s[rt][g]);
+          s[rt][g] = H::mfma16(hi, qf[rt][2 * j + 1], s[rt][g]);
+        }
+      }
+    float ks[kBlocks], ve[kBlocks];                      // the keys' scale, log2 of the values', of the tile's blocks
+    const char* const sc = mine + kDeep * 2 * kTile + place(t) * Tiles::kScales;
+#pragma unroll
+    for (int g = 0; g < kBlocks; ++g) {
+      const int p = pos + 16 * g;
+      ks[g] = __builtin_bit_cast(float, (uint32_t)(*reinterpret_cast<const uint16_t*>(sc + 4 * g + (scale_at(p, 0) & 2)) & 0x7F80u) << 16);
+      ve[g] = (float)codes::exponent_of<true>(*reinterpret_cast<const uint16_t*>(sc + 4 * (kBlocks + g) + (scale_at(p, 1) & 2)));
+    }
+    wait_lds();
+    if (t + kDeep < tiles) copy_keys(t + kDeep);
+    // element i of s[rt][g]: key pos + 16 g + 4 w + i, query row 16 rt + n
+    u32x4 p[MT][kSubs];
+#pragma unroll
+    for (int rt = 0; rt < MT; ++rt) {
+      const int end = min(seen[rt], to);
+#pragma unroll
+      for (int g = 0; g < kBlocks; ++g) s[rt][g] *= scale[rt] * ks[g];
+      if (pos + kWaveKeys > min(all, to)) {
+#pragma unroll
+        for (int g = 0; g < kBlocks; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (pos + 16 * g + 4 * w + i >= end) s[rt][g][i] = -INFINITY;
+      }
+      float m1 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < kBlocks; ++g) {
+        const float mx = fmaxf(fmaxf(s[rt][g][0], s[rt][g][1]), fmaxf(s[rt][g][2], s[rt][g][3]));
+        m1 = fmaxf(m1, mx);
+        t1 = fmaxf(t1, mx + ve[g]);
+      }
+      m1 = half_max(fmaxf(m1, __shfl_xor(m1, 16)));
+      t1 = half_max(fmaxf(t1, __shfl_xor(t1, 16)));
+      const float was = top[rt];
+      top[rt] = fmaxf(was, m1);
+      const float base = top[rt] == -INFINITY ? 0.0f : top[rt];
+      sum[rt] *= exp2_fast(was - base);
+      if (__ballot(t1 > most[rt] + 15.0f)) {             // weights stay below 2^15 in f16
+        const float before = most[rt];
+        most[rt] = fmaxf(before, t1 - (15.0f - kLag));
+        const float fade = most[rt] == -INFINITY ? 1.0f : exp2_fast(before - most[rt]);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) o[rt][d] *= fade;
+      }
+      const float shift = base - (most[rt] == -INFINITY ? 0.0f : most[rt]);
+      float add[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int g = 0; g < kBlocks; ++g) {
+        const float f = exp2_fast(fminf(ve[g] + shift, 126.0f));
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float y0 = exp2_fast(s[rt][g][i] - base), y1 = exp2_fast(s[rt][g][i + 1] - base);
+          add[i >> 1] += y0 + y1;
+          p[rt][g >> 1][2 * (g & 1) + (i >> 1)] = H::pack(y0 * f, y1 * f);
+        }
+      }
+      sum[rt] += add[0] + add[1];
+    }
+    // values are there
+    if (t + kDeep < tiles) wait_copies<kKeyCopies + (kDeep - 1) * kBoth>();
+    else wait_tiles<0, kBoth, kDeep - 1>(tiles - 1 - t);
+#pragma unroll
+    for (int h = 0; h < kSubs; ++h)
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        const u32x2 c = read_transposed8(v_at + buf + h * kSub + ((d ^ v_key) << 4));
+        uint32_t v0, v1, v2, v3;
+        widen4(c[0], v0, v1);
+        widen4(c[1], v2, v3);
+#pragma unroll
+        for (int rt = 0; rt < MT; ++rt) o[rt][d] = H::mfma16(u32x4{v0, v1, v2, v3}, p[rt][h], o[rt][d]);
+      }
+    wait_lds();
+    if (t + kDeep < tiles) copy_values(t + kDeep);
+  }
+#pragma unroll
+  for (int rt = 0; rt < MT; ++rt) {
+    const float f = most[rt] == -INFINITY ? 1.0f : exp2_fast(most[rt] - top[rt]);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) o[rt][d] *= f;
+  }
+  store_keys<DP, MT>(ps, lds, slot, alone, rows, D, o, top, sum);
+}
+
+// ---------------------------------------------------------------------------
+// many rows: numbers in LDS
+// ---------------------------------------------------------------------------
 // 16 codes as two pieces of 8 numbers: (u - 128) s = u s - 128 s of u = code + 128, exact in fp32.
 template <bool BF>
 __device__ __forceinline__ void expand(u32x4 z, float s, u32x4& lo, u32x4& hi) {
@@ -33,181 +340,45 @@ __device__ __forceinline__ void expand(u32x4 z, float s, u32x4& lo, u32x4& hi) {
   }
 }
 
-// 16 rows (one block of codes: of one page and scale) on their way from memory to a tile: a wave holds them in its lanes.
+// 16 rows (one block: of one page and scale), a wave's share of a tile. The codes are copied into the place of the numbers; each lane
+// then takes back the 16 bytes that it brought, and the wave writes its rows of numbers over them.
 template <bool BF, int DP>
-struct Codes16 {
-  static constexpr int kLanes = DP / 16, kRows = 64 / kLanes, kLoads = 16 / kRows;      // lanes of a row, rows of a load
-  u32x4 z[kLoads];
+struct Rows16 {
+  static constexpr int kLanes = DP / 16, kCopyRows = 64 / kLanes, kCopies = 16 / kCopyRows;      // lanes of a row, rows of a copy
   uint16_t scale;
 
-  // Rows from token p on; none if the page id is bad or p is not below `to`. (Rows past `to` in the block hold something; the weights are 0 there.)
-  __device__ __forceinline__ void load(const CodesCall& a, int id, int64_t codes_off, int64_t scales_off, int p, int to) {
-    const int lane = threadIdx.x & 63, piece = lane % kLanes * 16, in = p & ((1 << a.page_log) - 1);
-    const bool good = p < to && (uint32_t)id < (uint32_t)a.n_pages;
-    scale = 0;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) z[i] = u32x4{0, 0, 0, 0};
-    if (!good) return;
-    const char* const page = a.codes + (int64_t)id * a.page_bytes;
-    if (piece < a.room)
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        z[i] = *reinterpret_cast<const u32x4*>(page + codes_off + (int64_t)(in + i * kRows + lane / kLanes) * a.room + piece);
+  // Rows from token p on into `place`; zeros past token `to`, or if the page id is bad.
+  __device__ __forceinline__ void copy(const CodesCall& a, int id, int64_t codes_off, int64_t scales_off, int p, int to, uint32_t place) {
+    const uint32_t lane = threadIdx.x & 63, piece = lane % kLanes * 16;
+    const int in = p & ((1 << a.page_log) - 1), count = min(to - p, 16);
+    const bool good = count > 0 && (uint32_t)id < (uint32_t)a.n_pages;
+    const char* const page = a.codes + (int64_t)(good ? id : 0) * a.page_bytes;
     scale = *reinterpret_cast<const uint16_t*>(page + scales_off + in / codes::kBlock * 2);
-  }
-  // Into rows 0 .. 15 of a tile whose rows have the key `key`.
-  template <class Key>
-  __device__ __forceinline__ void put(char* tile, Key key) const {
-    const int lane = threadIdx.x & 63, piece = lane % kLanes * 2;
-    const float s = codes::scale_of<BF>(scale);
+    const u32x4 r = buffer_rsrc((uint64_t)(uintptr_t)(page + codes_off + (int64_t)in * a.room), good ? (uint32_t)(count * a.room) : 0u);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const uint32_t row = i * kRows + lane / kLanes;
+    for (int i = 0; i < kCopies; ++i)
+      copy16(r, (int)piece < a.room ? (i * kCopyRows + lane / kLanes) * a.room + piece : kOutOfRange,
+             __builtin_amdgcn_readfirstlane(place + i * 1024));
+  }
+  // When the copies have landed. Rows of a tile whose rows have the key `key`.
+  template <class Key>
+  __device__ __forceinline__ void widen(char* place, Key key) const {
+    const uint32_t lane = threadIdx.x & 63, piece = lane % kLanes * 2;
+    const float s = codes::scale_of<BF>(scale);
+    u32x4 z[kCopies];
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) z[i] = *reinterpret_cast<const u32x4*>(place + i * 1024 + lane * 16);
+    asm volatile("" ::: "memory");                         // (LDS serves a wave in order)
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const uint32_t row = i * kCopyRows + lane / kLanes;
       u32x4 lo, hi;
       expand<BF>(z[i], s, lo, hi);
-      *reinterpret_cast<u32x4*>(tile + row * (DP * 2) + ((piece ^ key(row)) << 4)) = lo;
-      *reinterpret_cast<u32x4*>(tile + row * (DP * 2) + (((piece + 1) ^ key(row)) << 4)) = hi;
+      *reinterpret_cast<u32x4*>(place + row * (DP * 2) + ((piece ^ key(row)) << 4)) = lo;
+      *reinterpret_cast<u32x4*>(place + row * (DP * 2) + (((piece + 1) ^ key(row)) << 4)) = hi;
     }
   }
 };
-
-// Orders this wave's LDS accesses before and after it (LDS serves a wave in order).
-__device__ __forceinline__ void own_lds() { asm volatile("" ::: "memory"); }
-
-// One item's keys [from, to) (from a multiple of 16) into a partial result, by the block (the keys split over its waves)
-// or by this wave alone. Each wave has a tile of 32 keys and one of values of its own; the next ones are in flight in its registers.
-template <bool BF, int DP, int MT, bool PREFIX>
-__device__ void split_keys(const CodesCall& a, const Book& book, char* lds, const Entry& x, int item, int from, int to, int slot, bool alone) {
-  using E = Elem<BF>;
-  constexpr int kHalf = 16 * DP * 2;
-  constexpr int kSteps = DP / 32;
-  const int stride = alone ? kWaveKeys : kCachedWaves * kWaveKeys;
-  const Pass& ps = PREFIX ? a.pre : a.own;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 15, w = lane >> 4;
-  const int D = a.dim;
-  const int kvh = item / x.tiles, row0 = (item % x.tiles) * 16 * MT;
-  const int rows = min(x.rows - row0, 16 * MT);
-
-  PageWindow pages{a.table + (int64_t)x.seq.row * a.max_pages, 0, -1, a.max_pages};
-  int pos = alone ? from : from + kWaveKeys * wave;
-  if (pos < to) pages.load(pos >> a.page_log);
-
-  const int64_t head = ((int64_t)kvh << a.page_log), head_codes = head * a.room, head_scales = head / codes::kBlock * 2;
-  Codes16<BF, DP> kc[2], vc[2];
-  auto load = [&](Codes16<BF, DP>(&to_regs)[2], int at, int64_t codes_off, int64_t scales_off) {
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int p = at + 16 * hf;
-      to_regs[hf].load(a, pages(p >> a.page_log), codes_off + head_codes, scales_off + head_scales, p, to);
-    }
-  };
-  if (pos < to) {
-    load(kc, pos, a.k_codes, a.k_scales);
-    load(vc, pos, a.v_codes, a.v_scales);
-  }
-
-  // this lane's query rows: 16 rt + n
-  u32x4 qf[MT][kSteps];
-  int seen[MT], all = 0x7FFFFFFF;                        // keys that a row sees, that all rows see
-#pragma unroll
-  for (int rt = 0; rt < MT; ++rt) {
-    const int rr = row0 + rt * 16 + n;
-    const uint16_t* qp = cached_query<PREFIX>(a, book, x, kvh, rr, seen[rt]);
-    if (rr < x.rows) all = min(all, seen[rt]);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int d = 32 * s + 8 * w;
-      qf[rt][s] = rr < x.rows && d < D ? *reinterpret_cast<const u32x4*>(qp + d) : u32x4{0, 0, 0, 0};
-    }
-  }
-#pragma unroll
-  for (int d = 8; d; d >>= 1) all = min(all, __shfl_xor(all, d));
-  all = __builtin_amdgcn_readfirstlane(all);
-
-  char* const kt = lds + wave * 4 * kHalf;
-  char* const vt = kt + 2 * kHalf;
-  f32x4 o[MT][DP / 16];
-  float top[MT], sum[MT];
-#pragma unroll
-  for (int rt = 0; rt < MT; ++rt) {
-    top[rt] = -INFINITY;
-    sum[rt] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) o[rt][d] = f32x4{};
-  }
-  while (pos < to) {
-    const int next = pos + stride;
-    const bool more = next < to;
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) kc[hf].put(kt + hf * kHalf, k_key<DP>);
-    own_lds();
-    if (more) {
-      if (((next + kWaveKeys - 1) >> a.page_log) - pages.at > 63) pages.load(next >> a.page_log);
-      load(kc, next, a.k_codes, a.k_scales);
-    }
-    f32x4 s[MT][2];
-#pragma unroll
-    for (int rt = 0; rt < MT; ++rt) s[rt][0] = s[rt][1] = f32x4{};
-#pragma unroll
-    for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const u32x4 kf = read_k<DP>(kt, g * 16 + n, 4 * st + w);
-#pragma unroll
-        for (int rt = 0; rt < MT; ++rt) s[rt][g] = E::mfma16(kf, qf[rt][st], s[rt][g]);
-      }
-    // element i of s[rt][g]: key pos + 16 g + 4 w + i, query row 16 rt + n
-    u32x4 p[MT];
-#pragma unroll
-    for (int rt = 0; rt < MT; ++rt) {
-      const int end = min(seen[rt], to);
-      if (pos + kWaveKeys > min(all, to)) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (pos + 16 * g + 4 * w + i >= end) s[rt][g][i] = -INFINITY;
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][g][i]);
-      mx = half_max(fmaxf(mx, __shfl_xor(mx, 16))) * a.c - E::raise(0.0f);
-      const float was = top[rt];
-      top[rt] = fmaxf(was, mx);
-      const float base = top[rt] == -INFINITY ? 0.0f : top[rt];
-      const float fade = exp2_fast(was - base);
-      sum[rt] *= fade;
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) o[rt][d] *= fade;
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const float y0 = exp2_fast(__builtin_fmaf(s[rt][g][i], a.c, -base));
-          const float y1 = exp2_fast(__builtin_fmaf(s[rt][g][i + 1], a.c, -base));
-          const uint32_t y = E::pack(y0, y1);            // weights of 16 bits: the matrix core's operand
-          sum[rt] = E::add2(y, sum[rt]);                 // and what is summed, so that the quotient's parts agree
-          p[rt][2 * g + (i >> 1)] = y;
-        }
-    }
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) vc[hf].put(vt + hf * kHalf, v_key<DP>);
-    own_lds();
-    if (more) load(vc, next, a.v_codes, a.v_scales);
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) {
-      const u32x2 lo = read_v<DP>(vt, 4 * w, d * 16, n), hi = read_v<DP>(vt, 16 + 4 * w, d * 16, n);
-#pragma unroll
-      for (int rt = 0; rt < MT; ++rt) o[rt][d] = E::mfma16(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[rt], o[rt][d]);
-    }
-    own_lds();
-    pos = next;
-  }
-  store_keys<DP, MT>(ps, lds, slot, alone, rows, D, o, top, sum);
-}
 
 // The same with the rows split over the waves, 32 each, and tiles of 64 keys shared by the block: each wave brings 16 keys.
 template <bool BF, int DP, bool PREFIX>
@@ -235,43 +406,39 @@ __device__ void split_rows(const CodesCall& a, const Book& book, char* lds, cons
   all = max(all, from);
 
   const int64_t head = ((int64_t)kvh << a.page_log), head_codes = head * a.room, head_scales = head / codes::kBlock * 2;
-  Codes16<BF, DP> kc, vc;
+  Rows16<BF, DP> kc, vc;
   char* const mine = lds + wave * 16 * kRow;
-  auto load_keys = [&](int t) {
+  const uint32_t lds0 = lds_addr(mine);
+  auto copy_keys = [&](int t) {
     const int p = from + t * kPromptKeys + wave * 16;
-    kc.load(a, pages(p >> a.page_log), a.k_codes + head_codes, a.k_scales + head_scales, p, to);
+    kc.copy(a, pages(p >> a.page_log), a.k_codes + head_codes, a.k_scales + head_scales, p, to, lds0 + (t & 1) * kTile);
   };
-  auto load_values = [&](int t) {
+  auto copy_values = [&](int t) {
     const int p = from + t * kPromptKeys + wave * 16;
-    vc.load(a, pages(p >> a.page_log), a.v_codes + head_codes, a.v_scales + head_scales, p, to);
+    vc.copy(a, pages(p >> a.page_log), a.v_codes + head_codes, a.v_scales + head_scales, p, to, lds0 + (2 + (t & 1)) * kTile);
   };
-  auto put_keys = [&](int t) { kc.put(mine + (t & 1) * kTile, k_key<DP>); };
-  auto put_values = [&](int t) { vc.put(mine + (2 + (t & 1)) * kTile, v_key<DP>); };
+  auto widen_keys = [&](int t) { kc.widen(mine + (t & 1) * kTile, k_key<DP>); };
+  auto widen_values = [&](int t) { vc.widen(mine + (2 + (t & 1)) * kTile, v_key<DP>); };
   const int steps = (to - from + kPromptKeys - 1) / kPromptKeys;
   rt.run(
       steps, busy ? steps : 0, (all - from) / kPromptKeys, a.c,
       [&]() {
-        load_keys(0);
-        load_values(0);
-        put_keys(0);
-        if (steps > 1) load_keys(1);
-        put_values(0);
-        if (steps > 1) load_values(1);
-        if (steps > 1) put_keys(1);
-        if (steps > 2) load_keys(2);
+        copy_keys(0);
+        wait_copies<0>();
+        widen_keys(0);
+        copy_values(0);
+        if (steps > 1) copy_keys(1);
         lds_barrier();
       },
-      // tile t's values and tile t + 1's keys were put before the barrier; the next ones are put, those after them start
       [&](int t) {
+        wait_copies<0>();
+        widen_values(t);
+        if (t + 1 < steps) widen_keys(t + 1);
         lds_barrier();
-        const int next = from + (t + 2) * kPromptKeys;
-        if (t + 1 < steps) put_values(t + 1);
-        if (t + 2 < steps) put_keys(t + 2);
-        if (t + 2 < steps) {
-          if (((next + 2 * kPromptKeys - 1) >> a.page_log) - pages.at > 63) pages.load(next >> a.page_log);
-          load_values(t + 2);
-        }
-        if (t + 3 < steps) load_keys(t + 3);
+        const int next = from + (t + 1) * kPromptKeys;
+        if (((next + 2 * kPromptKeys - 1) >> a.page_log) - pages.at > 63) pages.load(next >> a.page_log);
+        if (t + 1 < steps) copy_values(t + 1);
+        if (t + 2 < steps) copy_keys(t + 2);
       },
       [&](int t) { return seen - from - t * kPromptKeys; });
   lds_barrier();                                         // the next item may fill the tiles
@@ -282,8 +449,12 @@ __device__ void split_rows(const CodesCall& a, const Book& book, char* lds, cons
 
 template <bool BF>
 struct StoreCodes {
+  static constexpr int kKeys = kWaveKeys, kStart = 5, kStartAlone = 1, kShort = 8;
+  static constexpr float kCostRows = 2.2f, kCostKeys = 0.8f;
   typedef CodesCall Call;
   using E = Elem<BF>;
+  template <int DP>
+  static constexpr int kKeysBytes = kCachedWaves * KeyTiles<DP>::kBytes;
   template <int DP, int MODE, bool PREFIX>
   static __device__ __forceinline__ void keys(const Call& a, const Book& book, char* lds, const Entry& x, int item, int from, int to, int slot,
                                               bool alone) {

@@ -2,6 +2,11 @@
 // templates over a Store, which knows how the cache holds K and V:
 //   Call                         CachedCall, or one that adds to it
 //   E                            the 16-bit type of q, o and the tiles
+//   kKeys                        split keys: keys of a unit, a wave's step (at least kLeastKeys)
+//   kStart, kStartAlone          units that stand for an item's start, in runs of blocks and of single waves (up to kMostStart)
+//   kCostRows, kCostKeys         of a unit of split rows, of split keys, for dealing blocks to prefixes and own parts
+//   kShort                       up to as many units per item on average, runs of single waves
+//   kKeysBytes<DP>               LDS that keys<DP, ...> uses
 //   keys<DP, MODE, PREFIX>(...)  one item's keys [from, to) into a partial result, few rows
 //   rows<DP, PREFIX>(...)        the same, up to 128 rows
 //   join_again(...)              whether the row was computed anew, because of what it does not see
@@ -40,20 +45,21 @@ constexpr int kCachedWaves = 4;
 constexpr int kCachedThreads = 64 * kCachedWaves;
 constexpr int kCachedBlocks = 512;         // two per CU
 constexpr int kXcds = 8;
-constexpr int kWaveKeys = 32;              // split keys: per wave and step
+constexpr int kLeastKeys = 32, kMostStart = 8;   // of any Store
+constexpr int kJoinHead = 8;               // words
 constexpr int kManyRows = 128;             // split rows: rows of a tile
 // Measured on the device with 64 sequences on one prefix of 8192, 16 x 6 drafts on prefixes of 1536, 32 sequences of 0 to
 // 16384 and 64 of 1 to 512 (14/2 heads of 64, 32/8 of 128): starts of 1/2, 2/3, 2/5 and 3/3 units are within 6 %
 // of each other but for 1/2 (32 ragged: 48 us against 43); a prefix's unit at 0.9, 1.5 and 2.8 times a unit of keys
 // gives the first case 47, 37 and 34 us, at 5 times 38.
-constexpr int kStartRows = 2, kStartKeys = 4;    // units that stand for an item's start
-constexpr int kShortItem = 8;                    // split keys: up to as many units per item on average, runs of single waves
+constexpr int kStartRows = 2;              // split rows: units that stand for an item's start
 constexpr int kLeastRows = 2;                    // split rows: units of a run (drafts 14.9 us; 4: 17.4, 8: 21)
-constexpr float kCostRows = 2.2f, kCostKeys = 0.8f;      // of a unit, for dealing blocks to prefixes and own parts
 enum { kNone = 0, kOneTile = 1, kTwoTiles = 2, kRows = 3 };      // 16 rows, 32 rows, split rows
 __host__ __device__ constexpr int mode_rows(int mode) { return mode == kRows ? kManyRows : 16 * mode; }
-__host__ __device__ constexpr int mode_start(int mode) { return mode == kRows ? kStartRows : kStartKeys; }
-__host__ __device__ constexpr int mode_unit(int mode) { return mode == kRows ? kPromptKeys : kWaveKeys; }
+template <class Store>
+__host__ __device__ constexpr int mode_start(int mode, bool alone) { return mode == kRows ? kStartRows : alone ? Store::kStartAlone : Store::kStart; }
+template <class Store>
+__host__ __device__ constexpr int mode_unit(int mode) { return mode == kRows ? kPromptKeys : Store::kKeys; }
 
 struct Pass {                              // the own parts, or the prefixes
   float* part;                             // [slot][stride][dim]
@@ -87,7 +93,7 @@ struct CachedCall {
   int32_t n_seqs, tokens, heads, n_groups;
   float c;
   Pass own, pre;
-  int32_t* join;                           // Deal of the own parts, of the prefixes; then the entries
+  int32_t* join;                           // Deal of the own parts, of the prefixes, their starts (kJoinHead words); then the entries
 };
 
 struct Seq {
@@ -150,12 +156,13 @@ __device__ void fill_book(const CachedCall& a, const Book& k) {
 
 struct Entry {
   int rows, tiles, items;                  // query rows, row tiles, items (tiles of every K/V head)
-  int units;                               // of each item, its start among them; 0: no keys
+  int units;                               // of keys, of each item; 0: none
   int from, to;                            // keys
   int first, group;                        // batch entry that the keys belong to; own part: its group
   Seq seq;                                 // of `first`
+  __device__ __forceinline__ int with(int start) const { return units ? units + start : 0; }
 };
-template <bool PREFIX, int MODE>
+template <class Store, bool PREFIX, int MODE>
 __device__ __forceinline__ Entry cached_entry(const CachedCall& a, const Book& book, int e) {
   Entry r;
   const int per = a.tokens * (a.heads / a.kv_heads);
@@ -176,46 +183,59 @@ __device__ __forceinline__ Entry cached_entry(const CachedCall& a, const Book& b
   }
   r.tiles = (r.rows + mode_rows(MODE) - 1) / mode_rows(MODE);
   r.items = a.kv_heads * r.tiles;
-  r.units = r.to > r.from ? (r.to - r.from + mode_unit(MODE) - 1) / mode_unit(MODE) + mode_start(MODE) : 0;
+  r.units = r.to > r.from ? (r.to - r.from + mode_unit<Store>(MODE) - 1) / mode_unit<Store>(MODE) : 0;
   return r;
 }
 
 // Running sums over the entries: every thread of the block has the sums before its run of entries [e0, e1).
 struct Scan {
-  int e0, e1, units, own, items;
+  int e0, e1, units, own, items;           // own: units of the run
   int total, all_items;
+  int held, own_held, all_held;            // items that have keys
+  // Units of keys become units with `start` more for each item.
+  __device__ __forceinline__ void add_starts(int start) {
+    units += start * held;
+    own += start * own_held;
+    total += start * all_held;
+  }
 };
-template <bool PREFIX, int MODE>
-__device__ Scan cached_scan(const CachedCall& a, const Book& book, int (&shared)[2][kCachedWaves]) {
+template <class Store, bool PREFIX, int MODE>
+__device__ Scan cached_scan(const CachedCall& a, const Book& book, int (&shared)[3][kCachedWaves]) {
   const int n = PREFIX ? a.n_groups : a.n_seqs, per = (n + kCachedThreads - 1) / kCachedThreads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Scan r;
   r.e0 = min((int)threadIdx.x * per, n);
   r.e1 = min(r.e0 + per, n);
-  int u = 0, it = 0;
+  int u = 0, it = 0, held = 0;
   for (int e = r.e0; e < r.e1; ++e) {
-    const Entry x = cached_entry<PREFIX, MODE>(a, book, e);
+    const Entry x = cached_entry<Store, PREFIX, MODE>(a, book, e);
     u += x.items * x.units;
     it += x.items;
+    held += x.units ? x.items : 0;
   }
-  const int su = wave_scan(u), si = wave_scan(it);
+  const int su = wave_scan(u), si = wave_scan(it), sh = wave_scan(held);
   if (lane == 63) {
     shared[0][wave] = su;
     shared[1][wave] = si;
+    shared[2][wave] = sh;
   }
   __syncthreads();
   r.own = u;
+  r.own_held = held;
   r.units = su - u;
   r.items = si - it;
-  r.total = r.all_items = 0;
+  r.held = sh - held;
+  r.total = r.all_items = r.all_held = 0;
 #pragma unroll
   for (int w = 0; w < kCachedWaves; ++w) {
     if (w < wave) {
       r.units += shared[0][w];
       r.items += shared[1][w];
+      r.held += shared[2][w];
     }
     r.total += shared[0][w];
     r.all_items += shared[1][w];
+    r.all_held += shared[2][w];
   }
   return r;
 }
@@ -337,10 +357,20 @@ struct Plan {
   Deal deal;
   int runs;
   bool alone;                              // runs of single waves, not of blocks
+  int start;                               // units of an item's start
 };
-__device__ __forceinline__ Plan deal_out(int units, int items, int blocks, int mode) {
+template <class Store>
+__device__ __forceinline__ bool short_items(const Scan& sc, int mode) {
+  const int start = mode_start<Store>(mode, false);
+  return mode != kRows && sc.total + start * sc.all_held <= (Store::kShort + start) * sc.all_items;
+}
+template <class Store>
+__device__ __forceinline__ Plan deal_out(Scan& sc, int blocks, int mode) {
   Plan p;
-  p.alone = mode != kRows && units <= (kShortItem + mode_start(mode)) * items;
+  p.alone = short_items<Store>(sc, mode);
+  p.start = mode_start<Store>(mode, p.alone);
+  sc.add_starts(p.start);
+  const int units = sc.total;
   const int least = mode == kRows ? kLeastRows : 1;
   p.runs = min(p.alone ? blocks * kCachedWaves : blocks, (units + least - 1) / least);
   p.deal.each = units / max(p.runs, 1);
@@ -362,14 +392,15 @@ __device__ void cached_run(const typename Store::Call& a, const Book& book, char
     if (run >= plan.runs || u < sc.units || u >= sc.units + sc.own) continue;   // one thread: its run of entries holds u
     int before = sc.units, items = sc.items;
     for (int e = sc.e0; e < sc.e1; ++e) {
-      const Entry x = cached_entry<PREFIX, MODE>(a, book, e);
-      if (u < before + x.items * x.units) {
+      const Entry x = cached_entry<Store, PREFIX, MODE>(a, book, e);
+      const int all = x.items * x.with(plan.start);
+      if (u < before + all) {
         found[k][0] = e;
         found[k][1] = u - before;
         found[k][2] = items;
         break;
       }
-      before += x.items * x.units;
+      before += all;
       items += x.items;
     }
   }
@@ -380,13 +411,13 @@ __device__ void cached_run(const typename Store::Call& a, const Book& book, char
   int e = min(max(__builtin_amdgcn_readfirstlane(found[wave][0]), 0), n - 1), items = __builtin_amdgcn_readfirstlane(found[wave][2]);
   const int in = max(__builtin_amdgcn_readfirstlane(found[wave][1]), 0);
   int left = plan.deal.each + (run < plan.deal.rest);
-  Entry x = cached_entry<PREFIX, MODE>(a, book, e);
+  Entry x = cached_entry<Store, PREFIX, MODE>(a, book, e);
   if (x.units == 0 || x.items == 0) return;
-  int item = min(in / x.units, x.items - 1), unit = in % x.units;
+  int item = min(in / x.with(plan.start), x.items - 1), unit = in % x.with(plan.start);
   while (true) {
-    const int units = min(left, x.units - unit);
-    const int from = x.from + max(unit - mode_start(MODE), 0) * mode_unit(MODE);
-    const int to = min(x.from + (unit + units - mode_start(MODE)) * mode_unit(MODE), x.to);
+    const int units = min(left, x.with(plan.start) - unit);
+    const int from = x.from + max(unit - plan.start, 0) * mode_unit<Store>(MODE);
+    const int to = min(x.from + (unit + units - plan.start) * mode_unit<Store>(MODE), x.to);
     if (to > from) {
       if constexpr (MODE == kRows) Store::template rows<DP, PREFIX>(a, book, lds, x, item, from, to, run + items + item);
       else Store::template keys<DP, MODE, PREFIX>(a, book, lds, x, item, from, to, run + items + item, plan.alone);
@@ -399,7 +430,7 @@ __device__ void cached_run(const typename Store::Call& a, const Book& book, char
       do {                                               // left > 0: a further entry has units
         items += x.items;
         if (++e >= n) return;
-        x = cached_entry<PREFIX, MODE>(a, book, e);
+        x = cached_entry<Store, PREFIX, MODE>(a, book, e);
       } while (x.items == 0 || x.units == 0);
     }
   }
@@ -419,47 +450,49 @@ __device__ __forceinline__ int spread(int xcd, int at, int each, int runs) {
 // run) and blocks that share a CU. Smallest calls: 6 us.
 template <class Store, int DP, int OWN, int PRE>
 __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const typename Store::Call a) {
-  constexpr int kStage = kCachedWaves * 2 * kWaveKeys * DP * 2;     // = 2 buffers of K and V tiles of 64 keys for split rows, halved
-  constexpr int kBytes = OWN == kRows || PRE == kRows ? 4 * kPromptKeys * DP * 2 : kStage;
+  constexpr int kStage = Store::template kKeysBytes<DP>, kTiles = 4 * kPromptKeys * DP * 2;
+  constexpr int kBytes = (OWN == kRows || PRE == kRows) && kTiles > kStage ? kTiles : kStage;
   __shared__ __attribute__((aligned(1024))) char lds[kBytes];
-  __shared__ int shared[2][2][kCachedWaves];
+  __shared__ int shared[2][3][kCachedWaves];
   static_assert(kCachedWaves * (16 * (DP + 4) + 32 * 2) * 4 <= kStage, "the join fits the tiles' space");
   __shared__ int2 book_seq[kBook];
   __shared__ int book_group[PRE == kNone ? 1 : kBook + 1], book_prefix[PRE == kNone ? 1 : kBook];
   const Book book{book_seq, book_group, book_prefix, a.n_seqs <= kBook};
   fill_book(a, book);
-  const Scan own = cached_scan<false, OWN>(a, book, shared[0]);
+  Scan own = cached_scan<Store, false, OWN>(a, book, shared[0]);
   Scan pre;
-  pre.total = pre.all_items = 0;
-  if constexpr (PRE != kNone) pre = cached_scan<true, PRE>(a, book, shared[1]);
+  pre.total = pre.all_items = pre.all_held = 0;
+  if constexpr (PRE != kNone) pre = cached_scan<Store, true, PRE>(a, book, shared[1]);
 
   // blocks for the prefixes: their share of the cost
   int n_pre = 0;
   if constexpr (PRE != kNone) {
     auto cost = [](const Scan& sc, int mode) {
-      return sc.total * (mode == kRows ? kCostRows : kCostKeys);
+      return (sc.total + mode_start<Store>(mode, short_items<Store>(sc, mode)) * sc.all_held) * (mode == kRows ? Store::kCostRows : Store::kCostKeys);
     };
     const float wp = cost(pre, PRE), wo = cost(own, OWN);
     if (pre.total) n_pre = own.total ? min(max((int)(kCachedBlocks / kXcds * wp / (wp + wo) + 0.5f), 1), kCachedBlocks / kXcds - 1) * kXcds : kCachedBlocks;
   }
-  const Plan own_plan = deal_out(own.total, own.all_items, kCachedBlocks - n_pre, OWN);
+  const Plan own_plan = deal_out<Store>(own, kCachedBlocks - n_pre, OWN);
   Plan pre_plan = own_plan;
-  if constexpr (PRE != kNone) pre_plan = deal_out(pre.total, pre.all_items, n_pre, PRE);
+  if constexpr (PRE != kNone) pre_plan = deal_out<Store>(pre, n_pre, PRE);
   if (blockIdx.x == kCachedBlocks - 1) {                 // for k_join
     if (threadIdx.x == 0) {
       reinterpret_cast<Deal*>(a.join)[0] = own_plan.deal;
       reinterpret_cast<Deal*>(a.join)[1] = pre_plan.deal;
+      a.join[4] = own_plan.start;
+      a.join[5] = pre_plan.start;
     }
-    JoinEntry* je = reinterpret_cast<JoinEntry*>(a.join + 4);
+    JoinEntry* je = reinterpret_cast<JoinEntry*>(a.join + kJoinHead);
     JoinPart* jg = reinterpret_cast<JoinPart*>(je + a.n_seqs);      // the groups' parts, until the sequences have them
     int u, it;
     if constexpr (PRE != kNone) {
       u = pre.units;
       it = pre.items;
       for (int e = pre.e0; e < pre.e1; ++e) {
-        const Entry x = cached_entry<true, PRE>(a, book, e);
-        jg[e] = JoinPart{u, it, x.units, x.tiles};
-        u += x.items * x.units;
+        const Entry x = cached_entry<Store, true, PRE>(a, book, e);
+        jg[e] = JoinPart{u, it, x.with(pre_plan.start), x.tiles};
+        u += x.items * x.with(pre_plan.start);
         it += x.items;
       }
       __syncthreads();
@@ -467,11 +500,11 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const typename Sto
     u = own.units;
     it = own.items;
     for (int e = own.e0; e < own.e1; ++e) {
-      const Entry x = cached_entry<false, OWN>(a, book, e);
-      je[e].own = JoinPart{u, it, x.units, x.tiles};
+      const Entry x = cached_entry<Store, false, OWN>(a, book, e);
+      je[e].own = JoinPart{u, it, x.with(own_plan.start), x.tiles};
       je[e].pre = PRE != kNone && x.group >= 0 ? jg[x.group] : JoinPart{0, 0, 0, 0};
       je[e].first = PRE != kNone && x.group >= 0 ? book.start(a, x.group) : 0;
-      u += x.items * x.units;
+      u += x.items * x.with(own_plan.start);
       it += x.items;
     }
   }
@@ -490,7 +523,7 @@ __global__ __launch_bounds__(kCachedThreads, 2) void k_cached(const typename Sto
 // four dims: a quarter (DP 64) or half of the wave reads one slot's row, so one load covers several slots, and eight
 // loads are in flight (one dim a lane and four loads: 9 to 15 us for 32 ragged sequences, now 4.8).
 template <class Store, int DP>
-__global__ __launch_bounds__(kCachedThreads) void k_join(const typename Store::Call a, int own_rows, int own_start, int pre_rows, int pre_start) {
+__global__ __launch_bounds__(kCachedThreads) void k_join(const typename Store::Call a, int own_rows, int pre_rows) {
   constexpr int kLanes = DP / 4, kPer = 64 / kLanes, kBatch = 8;      // lanes and slots per load, loads in flight
   const int b = blockIdx.x, lane = threadIdx.x & 63;
   const int G = a.heads / a.kv_heads, D = a.dim;
@@ -498,7 +531,8 @@ __global__ __launch_bounds__(kCachedThreads) void k_join(const typename Store::C
   if (row >= a.tokens * a.heads) return;
   const int t = row / a.heads, h = row % a.heads, kvh = h / G;
   const Deal* deals = reinterpret_cast<const Deal*>(a.join);
-  const JoinEntry je = reinterpret_cast<const JoinEntry*>(a.join + 4)[b];
+  const JoinEntry je = reinterpret_cast<const JoinEntry*>(a.join + kJoinHead)[b];
+  const int own_start = a.join[4], pre_start = a.join[5];
   const int sub = lane / kLanes, dim = lane % kLanes * 4;
   float m = -INFINITY, l = 0.0f;
   f32x4 y = f32x4{};
@@ -597,13 +631,13 @@ inline int plan_cached(const mtc_cache_desc* c, const mtc_cached_args* a, Cached
   p->pre_stride = p->pre_mode ? stride(all, p->pre_mode) : 0;
   p->pre_slots = p->pre_mode ? runs(p->pre_mode) + (int64_t)c->kv_heads * (tiles(all, p->pre_mode) + a->n_groups) : 0;
   // the kernels count units in 32 bits
-  const int64_t units = (int64_t)c->max_pages * c->page_size / kWaveKeys + 1 + std::max(mode_start(kOneTile), mode_start(kRows));
+  const int64_t units = (int64_t)c->max_pages * c->page_size / kLeastKeys + 1 + kMostStart;
   if (units * (p->own_slots + p->pre_slots) > 0x7FFFFFFF)
     return host::fail(MTC_E_SHAPE, "%d sequences of up to %d pages of %d tokens, %d row tiles: too much for one call", a->n_seqs, c->max_pages,
                 c->page_size, (int)tiles(per, p->own_mode));
   p->own_bytes = round_up((size_t)p->own_slots * p->own_stride * (c->dim + 2) * 4, 256);
   p->pre_bytes = round_up((size_t)p->pre_slots * p->pre_stride * (c->dim + 2) * 4, 256);
-  p->join_bytes = round_up(16 + sizeof(JoinEntry) * (size_t)a->n_seqs + sizeof(JoinPart) * (size_t)a->n_groups, 256);
+  p->join_bytes = round_up(4 * kJoinHead + sizeof(JoinEntry) * (size_t)a->n_seqs + sizeof(JoinPart) * (size_t)a->n_groups, 256);
   return MTC_OK;
 }
 
@@ -626,8 +660,8 @@ int run_cached(const typename Store::Call& a, const CachedPlan& p, hipStream_t s
   else launch_cached<Store, 128>(a, p.own_mode, p.pre_mode, st);
   if (int rc = host::check_launch("k_cached")) return rc;
   const dim3 grid(a.n_seqs, (a.tokens * a.heads + kCachedWaves - 1) / kCachedWaves);
-  if (a.dim <= 64) k_join<Store, 64><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_start(p.own_mode), mode_rows(p.pre_mode), mode_start(p.pre_mode));
-  else k_join<Store, 128><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_start(p.own_mode), mode_rows(p.pre_mode), mode_start(p.pre_mode));
+  if (a.dim <= 64) k_join<Store, 64><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_rows(p.pre_mode));
+  else k_join<Store, 128><<<grid, kCachedThreads, 0, st>>>(a, mode_rows(p.own_mode), mode_rows(p.pre_mode));
   return host::check_launch("k_join");
 }
 
