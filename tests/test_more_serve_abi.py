@@ -1,0 +1,152 @@
+"""C-ABI of rotary positions, the 8-bit cache, reordering and the beam step (include/mtc_serve.h) without a GPU: the ctypes structs mirror
+the C ones, and host-side checks turn bad arguments into error codes before any GPU call."""
+
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+from tensorpack_amd import _abi, _native
+
+INCLUDE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _native.hip_lib()
+
+
+def test_constants_and_struct_layouts_match_c(tmp_path):
+    structs = {"mtc_rotary_args": _abi.MtcRotaryArgs, "mtc_beam_args": _abi.MtcBeamArgs}
+    consts = {"MTC_ROTARY_MAX_DIM": _abi.ROTARY_MAX_DIM, "MTC_BEAM_MAX": _abi.BEAM_MAX, "MTC_CACHE_CODES8": _abi.CACHE_CODES8,
+              "MTC_CODES8_BLOCK": _abi.CODES8_BLOCK, "MTC_CACHE_SHARED_PAGE": max(_abi.CACHE_WRITE_STATUS)}
+    src = "#include <stddef.h>\n#include <stdio.h>\n#include \"mtc_serve.h\"\nint main(void){\n"
+    want = []
+    for c, py in structs.items():
+        src += f'printf("%zu\\n", sizeof({c}));\n'
+        want.append(ctypes.sizeof(py))
+        for f, _ in py._fields_:
+            src += f'printf("%zu\\n", offsetof({c}, {f}));\n'
+            want.append(getattr(py, f).offset)
+    for c, v in consts.items():
+        src += f'printf("%zu\\n", (size_t){c});\n'
+        want.append(v)
+    (tmp_path / "t.c").write_text(src + "return 0;}\n")
+    subprocess.run(["gcc", "-I", INCLUDE, str(tmp_path / "t.c"), "-o", str(tmp_path / "t")], check=True)
+    out = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.split()
+    assert [int(x) for x in out] == want
+    assert not set(_abi.CACHE_STATUS) & set(_abi.CACHE_WRITE_STATUS)
+
+
+def _heads(data=0x1000, row=512, head=64):
+    return _abi.MtcHeads(data, row, head)
+
+
+def _rotary(**kw):
+    h = _heads()
+    a = _abi.MtcRotaryArgs(_abi.ABI_VERSION, _abi.MTC_DTYPE_BF16, 4, 8, 2, 64, 64, 0, 1.0, 0, h, h, h, h, 0x2000, 0x3000)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return ctypes.byref(a)
+
+
+def test_rotary_checks(lib):
+    f = lambda a: lib.mtc_rotary(a, None)
+    assert f(None) == -1
+    for kw, code in (({"abi_version": 1}, -7), ({"dtype": 9}, -4), ({"rows": -1}, -3), ({"heads": -1}, -3), ({"kv_heads": 1 << 20}, -3), ({"dim": 60}, -3),
+                     ({"dim": 1032}, -3), ({"dim": 0}, -3), ({"rotated": 0}, -3), ({"rotated": 63}, -3), ({"rotated": 66}, -3),
+                     ({"amplitude": float("nan")}, -3), ({"reserved": 1}, -3), ({"positions": None}, -1), ({"turns": None}, -1), ({"q": _heads(None)}, -1),
+                     ({"k": _heads(0x1008)}, -3), ({"oq": _heads(row=516)}, -3), ({"ok": _heads(head=-64)}, -3),
+                     ({"rows": 0x7FFFFFFF, "heads": 0xFFFF}, -3)):
+        assert f(_rotary(**kw)) == code, kw
+        assert lib.mtc_last_error()
+    assert f(_rotary(rows=0)) == 0 and f(_rotary(heads=0, kv_heads=0)) == 0
+
+
+def _cache(**kw):
+    c = _abi.MtcCacheDesc(_abi.ABI_VERSION, _abi.MTC_DTYPE_BF16 | _abi.CACHE_CODES8, 100, 2, 2, 64, 16, 8, 10, 0, 0x1000, 0x2000, 0x3000, 0x4000, 0x5000, 0x6000)
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return ctypes.byref(c)
+
+
+def test_quantized_cache_checks(lib):
+    bf, f16, f32, flag = _abi.MTC_DTYPE_BF16, _abi.MTC_DTYPE_F16, _abi.MTC_DTYPE_F32, _abi.CACHE_CODES8
+    assert lib.mtc_check_cache_desc(_cache()) == 0 and lib.mtc_check_cache_desc(_cache(dtype=f16 | flag)) == 0
+    for kw, code in (({"dtype": f32 | flag}, -4), ({"dtype": bf | 32}, -4), ({"dtype": 3 | flag}, -4), ({"dim": 12}, -2), ({"page_size": 8}, -2), ({"pool": 0x1008}, -2)):
+        assert lib.mtc_check_cache_desc(_cache(**kw)) == code, kw
+    c, p, h = _cache(), 0x7000, ctypes.byref(_heads())
+    for f in (lib.mtc_cache_append, lib.mtc_cache_read):
+        assert f(c, 2, h, h, bf, 1, p, p, 1, None) == -3 and f(c, -1, h, h, bf, 1, p, p, 1, None) == -3
+        assert f(c, 0, h, h, f16, 1, p, p, 1, None) == -4 and f(c, 0, h, h, bf | flag, 1, p, p, 1, None) == -4
+        assert f(c, 0, h, h, bf, -1, p, p, 1, None) == -3 and f(c, 0, h, h, bf, 1, None, p, 1, None) == -1
+        assert f(c, 0, h, h, bf, 1, p, None, 1, None) == -1 and f(c, 0, None, h, bf, 1, p, p, 1, None) == -1
+        assert f(c, 0, h, ctypes.byref(_heads(None)), bf, 1, p, p, 1, None) == -1
+        assert f(c, 0, ctypes.byref(_heads(0x1004)), h, bf, 1, p, p, 1, None) == -3 and f(c, 0, h, ctypes.byref(_heads(row=260)), bf, 1, p, p, 1, None) == -3
+        assert f(c, 0, h, h, bf, 1, p, p, 8193, None) == -3 and f(_cache(dim=12), 0, h, h, bf, 1, p, p, 1, None) == -2
+        assert f(c, 0, h, h, bf, 0, p, p, 1, None) == 0 and f(c, 0, None, None, bf, 0, None, None, 0, None) == 0
+    assert lib.mtc_cache_read(_cache(dtype=bf), 0, h, h, bf, 1, p, p, 1, None) == -4           # holds no codes
+    a = _abi.MtcCachedArgs(_abi.ABI_VERSION, 1, 4, 2, 8, 0, 0.125, 0, _heads(), _heads(), 0x7000, None, None, None)
+    need = lib.mtc_cached_attention_workspace_bytes(c, ctypes.byref(a))
+    assert need > 0 and lib.mtc_cached_attention(c, ctypes.byref(a), 0x100, need - 1, None) == -5
+
+
+def test_reorder_checks(lib):
+    for c in (_cache(), _cache(dtype=_abi.MTC_DTYPE_F16)):
+        f = lambda *a: lib.mtc_cache_reorder(c, *a, None)
+        assert f(None, 0x7000, 1) == -1 and f(0x7000, None, 1) == -1 and f(0x7000, 0x7000, -1) == -3 and f(0x7000, 0x7000, 8193) == -3
+        assert f(None, None, 0) == 0
+    assert lib.mtc_cache_reorder(_cache(page_size=8), 0x7000, 0x7000, 1, None) == -2
+
+
+def _beam(**kw):
+    two = (ctypes.c_int64 * 2)(400, 100)
+    a = _abi.MtcBeamArgs(_abi.ABI_VERSION, 0, 2, 4, 100, 4, 0, 0, 0x1000, two, 0x2000, None, 0x3000, 0x4000, 0x5000)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return ctypes.byref(a)
+
+
+def test_beam_checks(lib):
+    f, ws = lib.mtc_beam_select, lib.mtc_beam_workspace_bytes
+    need = ws(_beam())
+    assert need > 0 and ws(_beam(n=8)) > need
+    for kw, code in (({"abi_version": 1}, -7), ({"dtype": 3}, -4), ({"beams": 0}, -3), ({"beams": 65}, -3), ({"n": 0}, -3), ({"n": 65}, -3), ({"vocab": 0}, -3),
+                     ({"n_prompts": -1}, -3), ({"n_prompts": 20000}, -3), ({"reserved": 1}, -3), ({"logits": None}, -1), ({"scores": None}, -1),
+                     ({"out_scores": None}, -1), ({"tokens": None}, -1), ({"parents": None}, -1)):
+        assert f(_beam(**kw), 0x100, 1 << 40, None) == code, kw
+    assert f(None, 0x100, need, None) == -1 and f(_beam(), None, need, None) == -5 and f(_beam(), 0x100, need - 1, None) == -5
+    assert f(_beam(), 0x104, need, None) == -5
+    assert f(_beam(n_prompts=0), None, 0, None) == 0
+
+
+def test_frequencies():
+    import math
+    from tensorpack_amd.rotary import rotary_frequencies
+    f = rotary_frequencies(8, base=10000.0)
+    assert f == [1.0, 10000.0 ** -0.25, 10000.0 ** -0.5, 10000.0 ** -0.75]
+    assert rotary_frequencies(8, factor=4.0) == [x / 4 for x in f]
+    g = rotary_frequencies(8, factor=4.0, original=512, ramp=(1.0, 4.0))
+    turns = [512 * x / (2 * math.pi) for x in f]                  # 81, 8.1, 0.81, 0.081
+    assert g[:2] == f[:2] and g[2:] == [x / 4 for x in f[2:]]
+    h = rotary_frequencies(8, factor=4.0, original=1500)          # the third pair turns 2.4 times: between
+    assert f[2] / 4 < h[2] < f[2] and turns[2] < 1
+    for kw in (dict(dim=7), dict(dim=8, factor=0.0), dict(dim=8, base=0.0), dict(dim=8, original=-1), dict(dim=8, original=5, ramp=(3.0, 1.0))):
+        with pytest.raises(ValueError):
+            rotary_frequencies(**kw)
+
+
+def test_without_a_gpu_the_calls_raise():
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is here")
+    from tensorpack_amd.cache import QuantizedCache
+    from tensorpack_amd.rotary import Rotary
+    from tensorpack_amd.sampling import beam_select
+    with pytest.raises(RuntimeError):
+        Rotary(64)
+    with pytest.raises(RuntimeError):
+        QuantizedCache(8, 1, 2, 64, max_seqs=2, max_pages=4)
+    with pytest.raises(RuntimeError):
+        beam_select(torch.zeros(1, 2, 8), torch.zeros(1, 2))
