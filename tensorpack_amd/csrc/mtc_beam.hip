@@ -88,18 +88,25 @@ __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const 
   const T* p = reinterpret_cast<const T*>(a.logits) + (row / a.beams) * a.stride[0] + (row % a.beams) * a.stride[1];
   const int from = chunk * 64 * kEach + lane * 8;          // element e: from + e / 8 * 512 + e % 8
   float x[kEach];
-  if ((chunk + 1) * 64 * kEach <= a.vocab) {               // all loads before the first is looked at
-    Loose<T, 8> y[ROUNDS];
+  const int end = a.vocab - chunk * 64 * kEach;             // of the row, in the chunk
+  Loose<T, 8> y[ROUNDS];                                   // all loads before the first is looked at
+  if (end >= 64 * kEach) {
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) y[r] = *reinterpret_cast<const Loose<T, 8>*>(p + from + r * 512);
 #pragma unroll
     for (int e = 0; e < kEach; ++e) x[e] = V::get(y[e / 8].x[e % 8]);
   } else {
-    T y[kEach];
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) y[e] = p[min(from + e / 8 * 512 + e % 8, a.vocab - 1)];
+    for (int r = 0; r < ROUNDS; ++r) {
+      if ((r + 1) * 512 <= end) {
+        y[r] = *reinterpret_cast<const Loose<T, 8>*>(p + from + r * 512);
+      } else {
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) x[e] = from + e / 8 * 512 + e % 8 < a.vocab ? V::get(y[e]) : -INFINITY;
+        for (int j = 0; j < 8; ++j) y[r].x[j] = r * 512 < end ? p[min(from + r * 512 + j, a.vocab - 1)] : T(0);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) x[e] = from + e / 8 * 512 + e % 8 < a.vocab ? V::get(y[e / 8].x[e % 8]) : -INFINITY;
   }
   float mine = -INFINITY;
 #pragma unroll
@@ -318,10 +325,11 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const mtc_beam_args 
   }
 }
 
-// Chunks of 4096 logits once these fill the chip (two waves a SIMD), else of 512.
-int beam_rounds(const mtc_beam_args& a) { return (int64_t)a.n_prompts * a.beams * a.vocab >= (8 << 20) ? 8 : 1; }
+// Chunks of 512 kManyRounds logits once these fill the chip, else of 512.
+constexpr int kManyRounds = 8;
+int beam_rounds(const mtc_beam_args& a) { return (int64_t)a.n_prompts * a.beams * a.vocab >= (8 << 20) ? kManyRounds : 1; }
 int beam_chunks(const mtc_beam_args& a) {
-  const int size = 512 * (beam_rounds(a) == 8 ? 4 : 1);
+  const int size = 512 * beam_rounds(a);
   return (a.vocab + size - 1) / size;
 }
 size_t stat_bytes(const mtc_beam_args& a) {
@@ -350,7 +358,7 @@ int check_beam(const mtc_beam_args* a) {
 template <int DT>
 int run_beam(const mtc_beam_args& a, const Parts& parts, hipStream_t st) {
   const dim3 grid((parts.chunks + kWaves - 1) / kWaves, a.n_prompts * a.beams);
-  if (beam_rounds(a) == 8) k_beam<DT, 4><<<grid, kThreads, 0, st>>>(a, parts);
+  if (beam_rounds(a) == kManyRounds) k_beam<DT, kManyRounds><<<grid, kThreads, 0, st>>>(a, parts);
   else k_beam<DT, 1><<<grid, kThreads, 0, st>>>(a, parts);
   if (int rc = check_launch("k_beam")) return rc;
   k_beam_join<<<a.n_prompts, kJoinThreads, 0, st>>>(a, parts);

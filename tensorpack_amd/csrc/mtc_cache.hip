@@ -344,33 +344,44 @@ __host__ __device__ inline int reorder_columns(int n) { return min(32, max(1, kT
 __global__ __launch_bounds__(kThreads) void k_reorder(const mtc_cache_desc c, const int32_t* seqs, const int32_t* parents, int n) {
   __shared__ uint32_t marks[kMarkWords];
   __shared__ int32_t ids[kReorderIds];
+  __shared__ int32_t kept_seq[kThreads], kept_from[kThreads], kept_pages[kThreads];      // of the first rows
   clear_marks(marks);
   __syncthreads();
+  const int columns = reorder_columns(n), first = blockIdx.x * columns;
   int bad = 0, most = 0;
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int s = seqs[i];
-    if ((uint32_t)s >= (uint32_t)c.max_seqs || mark(marks, s) || (uint32_t)parents[i] >= (uint32_t)n) bad = MTC_CACHE_BAD_SEQ;
-    else most = max(most, pages_of(c, held(c, s)));
+    const int s = seqs[i], from = parents[i];
+    int pages = 0;
+    if ((uint32_t)s >= (uint32_t)c.max_seqs || mark(marks, s) || (uint32_t)from >= (uint32_t)n) bad = MTC_CACHE_BAD_SEQ;
+    else pages = pages_of(c, held(c, s));
+    most = max(most, pages);
+    if (i < kThreads) {
+      kept_seq[i] = s;
+      kept_from[i] = from;
+      kept_pages[i] = pages;
+    }
   }
-  bad = block_or(bad);
-  const int columns = reorder_columns(n), first = blockIdx.x * columns;
-  if (!bad && block_or(most > first)) {
+  bad = __syncthreads_or(bad) ? MTC_CACHE_BAD_SEQ : 0;
+  const bool any = __syncthreads_or(most > first);
+  auto seq = [&](int i) { return i < kThreads ? kept_seq[i] : seqs[i]; };
+  auto from = [&](int i) { return i < kThreads ? kept_from[i] : parents[i]; };
+  if (!bad && any) {
     for (int x = threadIdx.x; x < n * columns; x += kThreads) {
-      const int s = seqs[x / columns], k = first + x % columns;
-      ids[x] = k < pages_of(c, held(c, s)) ? c.table[(int64_t)s * c.max_pages + k] : -1;
+      const int i = x / columns, s = seq(i), k = first + x % columns;
+      ids[x] = k < (i < kThreads ? kept_pages[i] : pages_of(c, held(c, s))) ? c.table[(int64_t)s * c.max_pages + k] : -1;
     }
     __syncthreads();
     for (int x = threadIdx.x; x < n * columns; x += kThreads) {
-      const int i = x / columns, k = x % columns, p = ids[parents[i] * columns + k];
+      const int i = x / columns, k = x % columns, p = ids[from(i) * columns + k];
       if (p == ids[x]) continue;
       if ((uint32_t)p < (uint32_t)c.n_pages) atomicAdd(&c.refs[p], 1);
-      c.table[(int64_t)seqs[i] * c.max_pages + first + k] = p;         // first + k < max_pages: one of the two rows holds it
+      c.table[(int64_t)seq(i) * c.max_pages + first + k] = p;         // first + k < max_pages: one of the two rows holds it
     }
     __syncthreads();
     int lowest = c.n_pages;
     for (int x = threadIdx.x; x < n * columns; x += kThreads) {
       const int p = ids[x];
-      if (p == ids[parents[x / columns] * columns + x % columns] || (uint32_t)p >= (uint32_t)c.n_pages) continue;
+      if (p == ids[from(x / columns) * columns + x % columns] || (uint32_t)p >= (uint32_t)c.n_pages) continue;
       if (atomicSub(&c.refs[p], 1) == 1) lowest = min(lowest, p);
     }
 #pragma unroll
@@ -379,9 +390,9 @@ __global__ __launch_bounds__(kThreads) void k_reorder(const mtc_cache_desc c, co
   }
   if (!last_block(&c.state[kDone])) return;
   if (!bad) {
-    for (int i = threadIdx.x; i < n; i += kThreads) ids[i] = held(c, seqs[parents[i]]);
+    for (int i = threadIdx.x; i < n; i += kThreads) ids[i] = held(c, seq(from(i)));
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) c.lens[seqs[i]] = ids[i];
+    for (int i = threadIdx.x; i < n; i += kThreads) c.lens[seq(i)] = ids[i];
   }
   if (threadIdx.x == 0 && bad) c.state[kStatus] |= bad;
 }
