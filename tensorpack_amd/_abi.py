@@ -1,6 +1,7 @@
 """ctypes mirror of include/mtc_hip.h and include/mtc_serve.h (struct layout, constants, prototypes)."""
 
 import ctypes
+import struct
 
 ABI_VERSION = 11
 
@@ -167,6 +168,10 @@ class MtcRotaryArgs(ctypes.Structure):
         ("q", MtcHeads), ("k", MtcHeads), ("oq", MtcHeads), ("ok", MtcHeads),
         ("positions", ctypes.c_void_p), ("turns", ctypes.c_void_p),
     ]
+
+
+# MtcRotaryArgs in one go: building its nested structs one by one takes longer than the launch.
+ROTARY_PACK = struct.Struct("<I7ifi12Q2Q").pack
 
 
 class MtcBeamArgs(ctypes.Structure):

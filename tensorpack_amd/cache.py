@@ -66,6 +66,7 @@ class PagedCache:
         self.book = torch.zeros(sum(words) + entries, dtype=torch.int32, device=self.device)
         self.state, self.lens, self.refs, table = self.book.split([*words, entries])
         self.table = table.view(self.max_seqs, self.max_pages)
+        self._but_status = self.book[1:]
         self.table.fill_(-1)
         self.scratch = torch.empty(int(self.lib.mtc_cache_scratch_ints(self.n_pages, self.max_seqs)), dtype=torch.int32,
                                    device=self.device)
@@ -125,18 +126,26 @@ class PagedCache:
         import torch
         if not 0 <= layer < self.n_layers:
             raise ValueError(f"layer {layer} of {self.n_layers}")
-        if k.dim() != 3 or k.shape != v.shape or k.shape[1] != self.n_kv_heads or k.shape[2] != self.head_dim:
+        shape, dtype = k.shape, k.dtype
+        if len(shape) != 3 or shape != v.shape or shape[1] != self.n_kv_heads or shape[2] != self.head_dim:
             raise ValueError(f"k and v must be (rows, {self.n_kv_heads}, {self.head_dim}), got {tuple(k.shape)}, {tuple(v.shape)}")
-        if not (k.dtype == v.dtype and k.dtype in (self.dtype, torch.float32) and k.device == self.device == v.device):
+        if not (dtype == v.dtype and (dtype == self.dtype or dtype == torch.float32) and k.device == self.device == v.device):
             raise ValueError(f"k and v must be {self.dtype} or float32 on {self.device}")
         p = self._list("seqs", seqs)
         c = _int32("cu", cu, seqs.shape[0] + 1, self.device)
-        mask = 16 // k.element_size() - 1                        # rows of 16-byte pieces are read in place, others copied
-        k, v = (x if x.stride(2) == 1 and not (x.stride(0) | x.stride(1)) & mask and not x.data_ptr() & 15 else _copy(x)
-                for x in (k, v))
-        hk, hv = (_abi.MtcHeads(x.data_ptr(), x.stride(0), x.stride(1)) for x in (k, v))
-        code = _abi.MTC_DTYPE_F32 if k.dtype == torch.float32 else self.desc.dtype & ~_abi.CACHE_CODES8
-        self._call("mtc_cache_append", layer, ctypes.byref(hk), ctypes.byref(hv), code, k.shape[0], p, c, seqs.shape[0])
+        mask = 15 // dtype.itemsize                              # rows of 16-byte pieces are read in place, others copied
+        (r, h, u), at = k.stride(), k.data_ptr()
+        if u != 1 or (r | h) & mask or at & 15:
+            k = _copy(k)
+            (r, h, _), at = k.stride(), k.data_ptr()
+        hk = _abi.MtcHeads(at, r, h)
+        (r, h, u), at = v.stride(), v.data_ptr()
+        if u != 1 or (r | h) & mask or at & 15:
+            v = _copy(v)
+            (r, h, _), at = v.stride(), v.data_ptr()
+        hv = _abi.MtcHeads(at, r, h)
+        code = _abi.MTC_DTYPE_F32 if dtype == torch.float32 else self.desc.dtype & ~_abi.CACHE_CODES8
+        self._call("mtc_cache_append", layer, ctypes.byref(hk), ctypes.byref(hv), code, shape[0], p, c, seqs.shape[0])
 
     def fork(self, src, dst) -> None:
         """dst[i] (empty) becomes a second holder of everything src[i] holds. src may name a sequence several times."""
@@ -178,7 +187,7 @@ class PagedCache:
         """Puts the bookkeeping back, but for the status: `check()` still raises, once, for a call since the last check.
         Pages written or moved since hold what was written."""
         _need(snapshot.shape == self.book.shape and snapshot.dtype == self.book.dtype, "not a snapshot of this cache")
-        self.book[1:].copy_(snapshot[1:])
+        self._but_status.copy_(snapshot[1:])
 
     def check(self) -> None:
         """Waits for the GPU; raises CacheError if a call since the last check could not be done."""

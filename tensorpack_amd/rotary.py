@@ -62,9 +62,21 @@ class Rotary:
         self.turns_at = self.turns.data_ptr()
 
 
+_NONE = (0, 0, 0)
+
+
 def _view(x):
     r, h, _ = x.stride()
     return x.data_ptr(), r, h
+
+
+def _readable(x, mask):
+    """x, or a copy that the kernel can read, and its address and strides."""
+    (r, h, u), at = x.stride(), x.data_ptr()
+    if u == 1 and not (r | h) & mask and not at & 15:
+        return x, (at, r, h)
+    x = _copy(x)
+    return x, _view(x)
 
 
 def _like(out, x) -> bool:
@@ -83,33 +95,43 @@ def apply_rotary(rotary: Rotary, q, k, positions, *, out=None):
     if q.dim() != 3 or q.device != dev:
         raise ValueError(f"q must be (rows, heads, dim) on {dev}, got {tuple(q.shape)} on {q.device}")
     rows, heads, dim = q.shape
+    dtype = q.dtype
     kv_heads = 0
     if k is not None:
-        if k.dim() != 3 or k.shape[0] != rows or k.shape[2] != dim or k.dtype != q.dtype or k.device != dev:
-            raise ValueError(f"k must be ({rows}, kv_heads, {dim}) {q.dtype} on {dev}, got {tuple(k.shape)} {k.dtype} on {k.device}")
-        kv_heads = k.shape[1]
-    code = _value_code(q.dtype)
+        if k.dim() != 3 or k.dtype != dtype or k.device != dev:
+            raise ValueError(f"k must be ({rows}, kv_heads, {dim}) {dtype} on {dev}, got {tuple(k.shape)} {k.dtype} on {k.device}")
+        k_rows, kv_heads, k_dim = k.shape
+        if k_rows != rows or k_dim != dim:
+            raise ValueError(f"k must be ({rows}, kv_heads, {dim}), got {tuple(k.shape)}")
+    code = _value_code(dtype)
     if code is None:
-        raise ValueError(f"rotary positions take float32, bfloat16 or float16, got {q.dtype}")
+        raise ValueError(f"rotary positions take float32, bfloat16 or float16, got {dtype}")
     if dim % 8 or not 8 <= dim <= _abi.ROTARY_MAX_DIM or rotary.dim > dim:
         raise ValueError(f"dim must be a multiple of 8 from {max(8, rotary.dim)} to {_abi.ROTARY_MAX_DIM}, got {dim}")
     p = _int32("positions", positions, rows, dev)
-    none = ok = (None, 0, 0)
+    mask = 15 // dtype.itemsize                              # strides of rows of 16-byte pieces have none of these bits
+    q, hq = _readable(q, mask)
+    hk = ok = _NONE
+    if k is not None:
+        k, hk = _readable(k, mask)
     if out is None:
         new = torch.contiguous_format
-        out = torch.empty_like(q, memory_format=new), None if k is None else torch.empty_like(k, memory_format=new)
-        oq = (out[0].data_ptr(), heads * dim, dim)
+        oq = torch.empty_like(q, memory_format=new)
+        ho = oq.data_ptr(), heads * dim, dim
+        out = oq, None
         if k is not None:
-            ok = (out[1].data_ptr(), kv_heads * dim, dim)
+            out = oq, torch.empty_like(k, memory_format=new)
+            ok = out[1].data_ptr(), kv_heads * dim, dim
     else:
         out = tuple(out)
         if len(out) != 2 or not _like(out[0], q) or (k is None) != (out[1] is None) or not (k is None or _like(out[1], k)):
             raise ValueError("out must be a pair of tensors like q and k with 16-byte aligned rows that do not overlap")
-        oq, ok = _view(out[0]), none if k is None else _view(out[1])
-    q = q if _aligned_rows(q) else _copy(q)
-    k = k if k is None or _aligned_rows(k) else _copy(k)
-    args = _abi.MtcRotaryArgs(_abi.ABI_VERSION, code, rows, heads, kv_heads, dim, rotary.dim, rotary.interleaved, rotary.amplitude, 0,
-                              _view(q), none if k is None else _view(k), oq, ok, p, rotary.turns_at)
+        ho = _view(out[0])
+        if k is not None:
+            ok = _view(out[1])
+    args = _abi.MtcRotaryArgs.from_buffer_copy(_abi.ROTARY_PACK(
+        _abi.ABI_VERSION, code, rows, heads, kv_heads, dim, rotary.dim, rotary.interleaved, rotary.amplitude, 0, *hq, *hk, *ho, *ok, p,
+        rotary.turns_at))
     lib = _native.hip_lib()
     with on_device(dev.index):
         rc = lib.mtc_rotary(ctypes.byref(args), raw_stream(dev.index))
