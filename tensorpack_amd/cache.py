@@ -84,7 +84,7 @@ class PagedCache:
 
     def _geometry(self):
         """What two caches share if pages can be copied between them."""
-        return type(self), self.dtype, self.device, self.n_layers, self.n_kv_heads, self.page_size, self.head_dim
+        return self._flags, self.dtype, self.device, self.n_layers, self.n_kv_heads, self.page_size, self.head_dim
 
     @classmethod
     def from_buffers(cls, pool, table, lens, refs) -> "PagedCache":
@@ -206,9 +206,10 @@ class QuantizedCache(PagedCache):
     """A PagedCache that holds K and V in 8 bits: half the memory, and half the bytes that `cached_attention` reads.
 
     A value is code * 2 ** e: an int8 code, and an exponent for each block of 16 tokens, K or V and head, the least for which the block's
-    values fit (each is off by half a step at most, 2 ** (e - 1), which is 1 / 127 of the block's largest or less). Powers of two, so that every value is a
-    number of `dtype` and is read back exactly, and so that a block's codes depend on nothing but its values: `append` of a
-    token larger than those that its block holds rounds their codes again, to the larger step.
+    values fit (each is off by half a step at most, 2 ** (e - 1), which is 1 / 127 of the block's largest or less). Powers of two, so that every
+    value is a number of `dtype` and is read back exactly, and so that rounding is the same in any precision. `append` of a token
+    larger than those that its block holds rounds their codes again, to the larger step; a block keeps its step until its first token is
+    written again, also where `truncate` dropped the token that made it large.
     The exponents are bounded: values above 65024 (float16) are cut there, and no step is finer than 2 ** -24 (float16) or
     2 ** -100 (bfloat16). NaN becomes 0, an infinity the block's largest value.
 

@@ -336,18 +336,21 @@ __global__ __launch_bounds__(kThreads) void k_fork(const mtc_cache_desc c, const
   if (threadIdx.x == 0 && bad) c.state[kStatus] |= bad;
 }
 
-// A block takes a few columns of the table, of all the call's rows: what they held is read before anything is written,
+// A block takes a few columns of the table at a time, of all the call's rows: what they held is read before anything is written,
 // so that any sequence may take any other's place. Takers are counted before leavers, so that a page that stays held never counts 0.
-// Bound by its chain of loads (list, lengths, table, counts).
+// Bound by its chain of loads and atomics (list, lengths, table, counts): 4 beams of 8 pages 4.8 us, 256 of up to 58 7.7 us.
 constexpr int kReorderIds = MTC_CACHED_MAX_SEQS;
+constexpr int kReorderBlocks = 256;
 __host__ __device__ inline int reorder_columns(int n) { return min(32, max(1, kThreads / n)); }      // an entry a thread, if they fit
 __global__ __launch_bounds__(kThreads) void k_reorder(const mtc_cache_desc c, const int32_t* seqs, const int32_t* parents, int n) {
   __shared__ uint32_t marks[kMarkWords];
   __shared__ int32_t ids[kReorderIds];
   __shared__ int32_t kept_seq[kThreads], kept_from[kThreads], kept_pages[kThreads];      // of the first rows
+  __shared__ int longest;
   clear_marks(marks);
+  if (threadIdx.x == 0) longest = 0;
   __syncthreads();
-  const int columns = reorder_columns(n), first = blockIdx.x * columns;
+  const int columns = reorder_columns(n);
   int bad = 0, most = 0;
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int s = seqs[i], from = parents[i];
@@ -361,11 +364,14 @@ __global__ __launch_bounds__(kThreads) void k_reorder(const mtc_cache_desc c, co
       kept_pages[i] = pages;
     }
   }
+  most = (int)wave_umax((uint32_t)most);
+  if ((threadIdx.x & 63) == 0 && most) atomicMax(&longest, most);
   bad = __syncthreads_or(bad) ? MTC_CACHE_BAD_SEQ : 0;
-  const bool any = __syncthreads_or(most > first);
+  most = longest;
   auto seq = [&](int i) { return i < kThreads ? kept_seq[i] : seqs[i]; };
   auto from = [&](int i) { return i < kThreads ? kept_from[i] : parents[i]; };
-  if (!bad && any) {
+  for (int first = blockIdx.x * columns; !bad && first < most; first += gridDim.x * columns) {
+    __syncthreads();                                       // the last readers of ids
     for (int x = threadIdx.x; x < n * columns; x += kThreads) {
       const int i = x / columns, s = seq(i), k = first + x % columns;
       ids[x] = k < (i < kThreads ? kept_pages[i] : pages_of(c, held(c, s))) ? c.table[(int64_t)s * c.max_pages + k] : -1;
@@ -1028,7 +1034,7 @@ MTC_API int mtc_cache_reorder(const mtc_cache_desc* c, const int32_t* seqs, cons
   if (n == 0) return ok();
   if (!parents) return fail(MTC_E_NULL, "parents is NULL");
   const int columns = reorder_columns(n);
-  k_reorder<<<(c->max_pages + columns - 1) / columns, kThreads, 0, (hipStream_t)hip_stream>>>(*c, seqs, parents, n);
+  k_reorder<<<std::min((c->max_pages + columns - 1) / columns, kReorderBlocks), kThreads, 0, (hipStream_t)hip_stream>>>(*c, seqs, parents, n);
   return check_launch("k_reorder");
 }
 

@@ -129,6 +129,8 @@ def apply_rotary(rotary: Rotary, q, k, positions, *, out=None):
         ho = _view(out[0])
         if k is not None:
             ok = _view(out[1])
+            if rows and heads and kv_heads and (ho[0] in (hk[0], ok[0]) or ok[0] == hq[0]):
+                raise ValueError("the results' memory is another's of q, k and the results")
     args = _abi.MtcRotaryArgs.from_buffer_copy(_abi.ROTARY_PACK(
         _abi.ABI_VERSION, code, rows, heads, kv_heads, dim, rotary.dim, rotary.interleaved, rotary.amplitude, 0, *hq, *hk, *ho, *ok, p,
         rotary.turns_at))

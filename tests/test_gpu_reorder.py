@@ -73,6 +73,25 @@ def test_against_lists(gpu, kind, n, width):
     c.check()
 
 
+def test_long_tables(gpu):
+    """More columns than the call's blocks take at a time (1200 sequences: one column a turn), far beyond most sequences."""
+    import torch
+    from tensorpack_amd.cache import PagedCache
+    rng = np.random.RandomState(5)
+    c = PagedCache(6000, 1, 1, 8, max_seqs=1200, max_pages=900, device=gpu)
+    lens = rng.randint(0, 40, 1200)
+    lens[[3, 700]] = 16 * 900, 16 * 600 + 1
+    c.extend(_ints(list(range(1200)), gpu), _ints(lens.tolist(), gpu))
+    c.check()
+    for trial in range(3):
+        seqs, parents = rng.permutation(1200), rng.randint(0, 1200, 1200)
+        parents[:2] = [list(seqs).index(700), list(seqs).index(3)]
+        before = _state(c)
+        c.reorder(_ints(seqs.tolist(), gpu), _ints(parents.tolist(), gpu))
+        c.check()
+        assert all(np.array_equal(a, b) for a, b in zip(_state(c), _expect(before, seqs, parents)))
+
+
 def test_then_extended(gpu):
     """Beams that take the same parent share its pages until they write."""
     import torch

@@ -135,9 +135,11 @@ def test_refusals(gpu):
     from tensorpack_amd.rotary import Rotary, apply_rotary, rotary_frequencies
     r = Rotary(64, device=gpu)
     q, pos = torch.zeros((4, 2, 64), device=gpu), torch.zeros(4, dtype=torch.int32, device=gpu)
+    other = q.clone()
     for bad in (dict(q=q.double()), dict(q=q[0]), dict(q=q[..., :60]), dict(q=q[..., :32]), dict(k=q.half()), dict(k=q[:3]),
                 dict(positions=pos.long()), dict(positions=pos[:3]), dict(positions=pos.cpu()), dict(q=q.cpu()),
                 dict(out=(q, q)), dict(out=(q[..., 1:], None)), dict(out=(q[:1].expand(4, 2, 64), None)),
+                dict(k=q.clone(), out=(other, other)), dict(k=other, out=(other, torch.empty_like(q))), dict(k=other, out=(torch.empty_like(q), q)),
                 dict(out=(torch.zeros((4, 130), device=gpu)[:, :128].unflatten(1, (2, 64)), None))):
         kw = {**dict(q=q, k=None, positions=pos), **bad}
         with pytest.raises(ValueError):
