@@ -170,8 +170,10 @@ class MtcRotaryArgs(ctypes.Structure):
     ]
 
 
-# MtcRotaryArgs in one go: building its nested structs one by one takes longer than the launch.
-ROTARY_PACK = struct.Struct("<I7ifi12Q2Q").pack
+# The structs of calls that a decoder makes per layer or step, packed in one go (building nested structs one by one takes about as
+# long as a launch): bytes for from_buffer_copy.
+ROTARY_PACK = struct.Struct("<I7ifi14Q").pack
+CACHED_PACK = struct.Struct("<I5ifi10Q").pack
 
 
 class MtcBeamArgs(ctypes.Structure):
@@ -181,6 +183,9 @@ class MtcBeamArgs(ctypes.Structure):
         ("logits", ctypes.c_void_p), ("stride", ctypes.c_int64 * 2), ("scores", ctypes.c_void_p), ("done", ctypes.c_void_p),
         ("out_scores", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("parents", ctypes.c_void_p),
     ]
+
+
+BEAM_PACK = struct.Struct("<I7i8Q").pack
 
 
 MAX_GROUP = 4                        # MTC_MAX_GROUP: matrices per mtc_gemv_f32_group launch

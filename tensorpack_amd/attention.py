@@ -195,8 +195,9 @@ def cached_attention(q, cache, layer: int, seqs, *, q_lens=None, groups=None, pr
         q = _copy(q)
         row, head = heads * dim, dim
     lib = cache.lib
-    args = _abi.MtcCachedArgs(_abi.ABI_VERSION, layer, n, tokens, heads, n_groups, scale, 0, _abi.MtcHeads(q.data_ptr(), row, head),
-                              _abi.MtcHeads(out.data_ptr(), heads * dim, dim), sp, qp, gp, pp)
+    args = _abi.MtcCachedArgs.from_buffer_copy(_abi.CACHED_PACK(
+        _abi.ABI_VERSION, layer, n, tokens, heads, n_groups, scale, 0, q.data_ptr(), row, head, out.data_ptr(), heads * dim, dim, sp,
+        qp or 0, gp or 0, pp or 0))
     ref, stream = ctypes.byref(args), raw_stream(dev.index)
     need = lib.mtc_cached_attention_workspace_bytes(cache.desc_ref, ref)
     with on_device(dev.index):

@@ -102,8 +102,9 @@ def beam_select(logits, scores, *, n: Optional[int] = None, done=None, pad: int 
     if done is not None:
         done = done.contiguous()
     lib = _native.hip_lib()
-    args = _abi.MtcBeamArgs(_abi.ABI_VERSION, code, B, W, V, n, pad, 0, logits.data_ptr(), logits.stride()[:2], scores.data_ptr(),
-                            None if done is None else done.data_ptr(), best.data_ptr(), tokens.data_ptr(), parents.data_ptr())
+    args = _abi.MtcBeamArgs.from_buffer_copy(_abi.BEAM_PACK(
+        _abi.ABI_VERSION, code, B, W, V, n, pad, 0, logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(),
+        0 if done is None else done.data_ptr(), best.data_ptr(), tokens.data_ptr(), parents.data_ptr()))
     ref, stream = ctypes.byref(args), raw_stream(dev.index)
     need = lib.mtc_beam_workspace_bytes(ref)
     with on_device(dev.index):

@@ -39,6 +39,18 @@ def test_constants_and_struct_layouts_match_c(tmp_path):
     assert not set(_abi.CACHE_STATUS) & set(_abi.CACHE_WRITE_STATUS)
 
 
+def test_packed_structs():
+    """The bytes that calls pack in one go are those of the structs."""
+    h = lambda i: _abi.MtcHeads(i, i + 1, i + 2)
+    a = _abi.MtcRotaryArgs(1, 2, 3, 4, 5, 6, 7, 1, 0.5, 0, h(10), h(20), h(30), h(40), 50, 60)
+    b = _abi.ROTARY_PACK(1, 2, 3, 4, 5, 6, 7, True, 0.5, 0, 10, 11, 12, 20, 21, 22, 30, 31, 32, 40, 41, 42, 50, 60)
+    assert bytes(a) == b
+    a = _abi.MtcCachedArgs(1, 2, 3, 4, 5, 6, 0.25, 0, h(10), h(20), 30, 40, 50, 60)
+    assert bytes(a) == _abi.CACHED_PACK(1, 2, 3, 4, 5, 6, 0.25, 0, 10, 11, 12, 20, 21, 22, 30, 40, 50, 60)
+    a = _abi.MtcBeamArgs(1, 2, 3, 4, 5, 6, -7, 0, 10, (ctypes.c_int64 * 2)(11, 12), 13, 14, 15, 16, 17)
+    assert bytes(a) == _abi.BEAM_PACK(1, 2, 3, 4, 5, 6, -7, 0, 10, 11, 12, 13, 14, 15, 16, 17)
+
+
 def _heads(data=0x1000, row=512, head=64):
     return _abi.MtcHeads(data, row, head)
 
