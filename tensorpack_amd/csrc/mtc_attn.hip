@@ -1,7 +1,7 @@
 // gfx950 attention kernels and their C-ABI (include/mtc_serve.h).
 //
 //   k_prompt  : whole prompts, packed sequences, causal or not
-//   k_cached  : the newest tokens of each sequence over a paged cache; work split evenly over the blocks
+//   k_cached  : the newest tokens of each sequence over a paged cache (mtc_cached.h), here of 16-bit numbers; work split evenly over the blocks
 //   k_join    : joins k_cached's partial results per row
 //
 // Both multiply keys by queries with the keys as rows: S^T = K Q^T puts one query into each lane's

@@ -1,10 +1,21 @@
 // gfx950 kernels of attention over the 8-bit cache (include/mtc_serve.h): k_cached and k_join of mtc_cached.h over codes.
 //
-// Codes become numbers of the cache's 16-bit type on their way into LDS: code 2^e is one exactly, so nothing is rounded there, and
-// from the tiles on the kernels are those of the 16-bit cache. The bytes that a call reads are half, which is what bounds
-// few rows; the conversion costs 2.75 vector instructions per code (bytes to fp32, one fused multiply-add, pairs packed).
+// The bytes that a call reads are half of a 16-bit cache's, which is what bounds few rows; what the kernels add is the way from
+// codes to the matrix core's 16-bit operands, and it differs:
+//   few rows   codes lie in LDS as they are; each wave makes f16 whole numbers of them, 1.25 vector instructions a code, and scales are
+//              folded into scores and weights
+//   many rows  each code is read by four waves, so a wave makes numbers of the cache's type of its quarter (code 2^e is one exactly,
+//              nothing is rounded; 2.75 instructions a code: bytes to fp32, a fused multiply-add, pairs packed) and puts those into the
+//              tile; from there on the kernel is that of the 16-bit cache
 // Memory cannot hold an infinity or a NaN here (scales are bounded as they are read, codes are integers), so a key that a row does
 // not see has no part in it by its weight of 0 alone, and no row is computed again.
+//
+// 32 sequences of 8192, 32/8 heads of 128, 537 MB: 107 us a pass, 5.0 TB/s (a 1 GiB copy: 5.14; the 16-bit cache: 193). 32 ragged ones up to
+// 16384, 92 MB: 27 us, with the join 31 a pass; its start is much of it (the lists, the table, the first keys: one of 200 keys takes 8 us), and
+// items that change within a block's run. As 16-bit numbers in LDS, 32 keys a step, it took 29.6 us and 32 of 8192 114.
+// 64 sequences on a prefix of 8192: 35 us, of which some 21 are start, fill and the partial results of 64 KB a run; a step of 64 keys
+// takes 3.1 us with two blocks a CU, half of it conversions. Runs of 4 or 8 units at least (fewer partial results): 43.4 and 48.5 us a
+// pass against 43.8; the first two tiles' copies issued together: 43.5 and 43.5.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -449,6 +460,9 @@ __device__ void split_rows(const CodesCall& a, const Book& book, char* lds, cons
 
 template <bool BF>
 struct StoreCodes {
+  // Starts measured on 32 and 96 ragged sequences up to 16384 and 4000 (blocks: 2, 3, 4, 5, 6, 8 units give 36, 32.6, 30.3, 30.7, 30.6, 30.6
+  // and 92, 82, 72.7, 68.9, 69.2, 71.2 us), on 64 up to 512 (waves: 1, 2, 4 units give 16.8, 17.2, 19.9) and on 8 up to 2048 (items of up to 4,
+  // 6, 8 units taken by waves: 16.5, 15.0, 14.3).
   static constexpr int kKeys = kWaveKeys, kStart = 5, kStartAlone = 1, kShort = 8;
   static constexpr float kCostRows = 2.2f, kCostKeys = 0.8f;
   typedef CodesCall Call;

@@ -25,7 +25,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kList = 256;                 // candidates that a wave's list holds
-constexpr int kJoinList = 1024;            // and the join's
+constexpr int kJoinList = 2048;            // and the join's
 
 struct Candidate {
   float x;
@@ -41,41 +41,38 @@ struct Parts {
   int32_t chunks;
 };
 
-// A value that at least n of the lanes' values reach, -inf if fewer than n are above that. Up to 16: lanes that are equal modulo
-// a power of two >= n form a group, and the least of the groups' maxima is reached by one lane of each (n ln n lanes or so in all: six
-// exchanges for that list, where n of them give the n-th largest, 150 cycles each). Lanes without values are the last ones, so that
-// no group is empty while n lanes have some.
+// A value that n or a few more of the lanes' values reach, -inf if fewer than n are above that: the n-th largest, but for its distance to
+// the largest, of which 5 bits behind the leading one are found, bit by bit by counting lanes. (Taking the largest away n times costs 150
+// cycles each; the least maximum of n groups of lanes is as quick as this, but n ln n values reach it, twice as many in the worst of a hundred
+// chunks, which the others wait for: a row of 32000 and 16 picks takes 19 us by that, 10 by this.)
 __device__ __forceinline__ float reached(float x, int n) {
-  if (n <= 16) {
-    const int groups = n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1));
+  const float top = wave_top(x);
+  if (top == -INFINITY) return top;
+  const uint32_t far = __builtin_bit_cast(uint32_t, top - x);                // not negative
+  uint32_t t = 0;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) {
-      const int u = __builtin_bit_cast(int, x);
-      int v;                                                // of the lane at distance d: lanes 2 d apart hold the same already
-      if (d >= 16) v = __shfl_xor(u, d);
-      else if (d == 8) v = __builtin_amdgcn_update_dpp(u, u, 0x128, 0xF, 0xF, false);       // row_ror:8
-      else if (d == 4) v = __builtin_amdgcn_update_dpp(u, u, 0x124, 0xF, 0xF, false);       // row_ror:4
-      else if (d == 2) v = __builtin_amdgcn_update_dpp(u, u, 0x4E, 0xF, 0xF, false);        // quad_perm 2 3 0 1
-      else v = __builtin_amdgcn_update_dpp(u, u, 0xB1, 0xF, 0xF, false);                    // quad_perm 1 0 3 2
-      const float y = __builtin_bit_cast(float, v);
-      x = d >= groups ? fmaxf(x, y) : fminf(x, y);
-    }
-    return x;
+  for (int bit = 30; bit >= 18; --bit) {
+    const uint32_t to = t | ((1u << bit) - 1);
+    t |= __popcll(__ballot(far <= to)) < n ? 1u << bit : 0u;
   }
-  float t = -INFINITY;
-  for (int i = 0; i < n; ++i) {
-    t = wave_top(x);
-    if (t == -INFINITY) break;
-    const uint64_t at = __ballot(x == t);
-    if ((int)(threadIdx.x & 63) == __ffsll((unsigned long long)at) - 1) x = -INFINITY;
-  }
-  return t;
+  if (t >= 0x7F800000u) return -INFINITY;
+  return -wave_top(far <= (t | ((1u << 18) - 1)) ? -x : -INFINITY);
 }
 constexpr float kLeast = -3.402823466e38f;  // of what is above -inf
+constexpr int kTwo = 24;                   // picks beyond which a bound is made of lanes' second values
+// As above, from each lane's largest value and another: more than kTwo picks are bounded by the others of half as many lanes, where the lanes'
+// maxima alone give little (64 picks: the least of all; 64 beams of 32000 and 64 picks 1170 us without, 43 with; 32 of 8 beams 19.4 and 16.9; 17
+// of 8 beams 11.2 and 15.6).
+__device__ __forceinline__ float reached(float x, float second, int n) {
+  return n > kTwo ? reached(second, (n + 1) / 2) : reached(x, n);
+}
 
 // Chunks of 512 ROUNDS logits, 8 ROUNDS a lane. What can be among the n best is not below a value that n of the lanes' maxima reach:
 // a few values, which each lane marks by a bit, reads again (from a cache) and ranks in LDS by counting. (Many equal values overflow the
 // list: then the best are taken one after another.)
+// 256 rows of 128003 bf16, a fifth of them ended, 52 MB: 22.4 us, of which the loads and the maxima take 13 (memory alone 10): all waves'
+// loads arrive at much the same time, so little of the selection lies under them. Blocks that load their next chunk ahead were slower (34 to
+// 42 us), sums kept round by round no faster (24). Four rows of 32000 fp32: 4.4 us.
 template <int DT, int ROUNDS>
 __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const Parts parts) {
   using V = Value<DT>;
@@ -108,9 +105,10 @@ __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const 
 #pragma unroll
     for (int e = 0; e < kEach; ++e) x[e] = from + e / 8 * 512 + e % 8 < a.vocab ? V::get(y[e / 8].x[e % 8]) : -INFINITY;
   }
-  float mine = -INFINITY;
+  float half[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) mine = fmaxf(mine, x[e]);
+  for (int e = 0; e < kEach; ++e) half[e / 4 % 2] = fmaxf(half[e / 4 % 2], x[e]);
+  const float mine = fmaxf(half[0], half[1]);
   const float top = wave_top(mine), base = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f;
 #pragma unroll
@@ -120,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const 
   if (lane == 0) parts.stat[part] = Stat{top, sum};
   Candidate* const out = parts.best + part * a.n;
 
-  const float least = fmaxf(reached(mine, a.n), kLeast);
+  const float least = fmaxf(reached(mine, fminf(half[0], half[1]), a.n), kLeast);
   uint32_t low = 0, high = 0;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) (e < 32 ? low : high) |= x[e] >= least ? 1u << (e % 32) : 0u;
@@ -187,14 +185,14 @@ __device__ __forceinline__ bool before(const Pick& a, const Pick& b) {      // w
 }
 __device__ __forceinline__ uint64_t place_of(int w, int v) { return (uint64_t)w << 32 | (uint32_t)v; }
 // A thread per chunk of a beam (or several), whose candidates fall: the first ones give a bound, and few chunks have more than one
-// above it.
+// above it. Bound by its chain (loads, log sums, bound, ranks): 4 beams of 63 chunks 4.6 us, 32 prompts of 8 beams of 32 chunks 5.9 us.
 constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
 constexpr int kAhead = 4;                  // candidates of a chunk that are loaded before the bound is known
 __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const mtc_beam_args a, const Parts parts) {
   __shared__ double offset[MTC_BEAM_MAX];
   __shared__ int ended[MTC_BEAM_MAX];
   __shared__ Pick list[kJoinList];
-  __shared__ float least[kJoinWaves];
+  __shared__ float firsts[kJoinThreads], seconds[kJoinThreads];
   __shared__ int count;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int items = a.beams * parts.chunks;
@@ -227,18 +225,32 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const mtc_beam_args 
   const bool mine_over = tid < a.beams && ended[tid];      // beam `tid` stands as a candidate
   auto score = [&](int w, float x) { return offset[w] + (double)x; };
   const bool go_on = tid < items && !ended[my_w];
-  float mine = mine_over ? (float)offset[tid] : -INFINITY;
-  if (go_on) mine = fmaxf(mine, (float)score(my_w, ahead[0].x));
+  // The block's bound: a lane of each wave makes one of 64 groups, of which every wave finds the same bound.
+  float mine = -INFINITY, second = -INFINITY;
+  auto hold = [&](float x) {
+    x = fmaxf(x, -INFINITY);                               // NaN, of a row that has no candidates
+    second = fmaxf(second, fminf(mine, x));
+    mine = fmaxf(mine, x);
+  };
+  if (mine_over) hold((float)offset[tid]);
+  if (go_on) {
+    hold((float)score(my_w, ahead[0].x));
+    hold((float)score(my_w, ahead[1].x));
+  }
   for (int i = tid + kJoinThreads; i < items; i += kJoinThreads) {
     const int w = i / parts.chunks;
-    if (!ended[w]) mine = fmaxf(mine, (float)score(w, best[(int64_t)i * a.n].x));
+    if (!ended[w]) hold((float)score(w, best[(int64_t)i * a.n].x));
   }
-  const float bound = fmaxf(reached(mine, a.n), kLeast);
-  if (lane == 0) least[wave] = bound;
+  firsts[tid] = mine;
+  seconds[tid] = second;
   __syncthreads();
-  float from = least[0];
 #pragma unroll
-  for (int w = 1; w < kJoinWaves; ++w) from = fmaxf(from, least[w]);
+  for (int w = 1; w < kJoinWaves; ++w) {
+    const int at = (tid + 64 * w) % kJoinThreads;
+    hold(firsts[at]);
+    hold(seconds[at]);
+  }
+  const float from = fmaxf(reached(mine, second, a.n), kLeast);
   auto above = [&](int w, float x) { return (float)score(w, x) >= from; };
   auto offer = [&](int at, const Pick& p) {
     if (at < kJoinList) list[at] = p;
@@ -307,7 +319,9 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const mtc_beam_args 
       if (ended[w]) continue;
       for (int j = 0; j < a.n; ++j) {
         const Candidate c = best[(int64_t)i * a.n + j];
-        take(Pick{score(w, c.x), place_of(w, c.v)});
+        const Pick q{score(w, c.x), place_of(w, c.v)};
+        if (q.score < p.score) break;                      // nor is any after it better
+        take(q);
       }
     }
     __syncthreads();                                       // the list's last readers
@@ -325,9 +339,15 @@ __global__ __launch_bounds__(kJoinThreads) void k_beam_join(const mtc_beam_args 
   }
 }
 
-// Chunks of 512 kManyRounds logits once these fill the chip, else of 512.
+// Chunks of 512 logits, which spread few rows over the chip, or of 4096, which leave the join fewer candidates and fill the chip with many rows.
+// Measured, us a call, chunks of 4096 and of 512: 1 x 4 beams of 32000 10.3, 8.9; 16 x 4 10.8, 10.0; 32 x 4 11.0, 11.9; 64 x 4 13.3, 15.9; 1 x 4 of 128003
+// 10.5, 10.5; 1 x 8 11.4, 13.1; 1 x 16 14.4, 21.4; 32 x 8 27.6, 43.1; short rows: 256 x 8 of 8192 18.8, 25.0; 256 x 4 of 5003 13.9, 13.9; 1024 x 4 of
+// 1500 24.9, 19.0.
 constexpr int kManyRounds = 8;
-int beam_rounds(const mtc_beam_args& a) { return (int64_t)a.n_prompts * a.beams * a.vocab >= (8 << 20) ? kManyRounds : 1; }
+int beam_rounds(const mtc_beam_args& a) {
+  const int64_t prompt = (int64_t)a.beams * a.vocab;
+  return a.vocab >= 8192 && (prompt >= (512 << 10) || a.n_prompts * prompt >= (3 << 20)) ? kManyRounds : 1;
+}
 int beam_chunks(const mtc_beam_args& a) {
   const int size = 512 * beam_rounds(a);
   return (a.vocab + size - 1) / size;

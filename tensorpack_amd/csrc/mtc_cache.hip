@@ -588,6 +588,7 @@ __device__ __forceinline__ int cut(const int32_t* cu, int i, int rows) { return 
 // Which block: sequence i's blocks have the numbers from cu[i] / 16 + 2 i on. It has at most rows / 16 + 2, so that
 // numbers of two never meet, and a bisection of cu finds the sequence. The new rows, and the block's old codes and scale, are on
 // their way while the list and the page's holders are checked.
+// 16384 tokens of 8 heads of 128 (67 MB bf16 in, 34 MB out) 20.8 us, 4.8 TB/s; one token of 64 sequences 6.6 us, the chain of loads.
 template <bool BF, int SRC>
 __global__ __launch_bounds__(256) void k_append8(const mtc_cache_desc c, int layer, const mtc_heads k, const mtc_heads v, int rows,
                                                  const int32_t* seqs, const int32_t* cu, int n) {
@@ -693,7 +694,8 @@ __global__ __launch_bounds__(256) void k_append8(const mtc_cache_desc c, int lay
   }
 }
 
-// One thread per 16 codes: each finds its row's sequence by bisection.
+// One thread per 16 codes: each finds its row's sequence by bisection (counted by the block in one round of loads instead: 25 us for
+// the first of these). 16384 tokens of 8 heads of 128 (34 MB in, 67 MB bf16 out) 22 us, 4.6 TB/s; 32 tokens of 64 sequences 5.9 us.
 template <bool BF, int DST>
 __global__ __launch_bounds__(256) void k_read8(const mtc_cache_desc c, int layer, const mtc_heads k, const mtc_heads v, int rows,
                                                const int32_t* seqs, const int32_t* cu, int n) {
@@ -1075,10 +1077,12 @@ MTC_API int mtc_cache_append(const mtc_cache_desc* c, int layer, const mtc_heads
   const bool bf = codes::base_type(*c) == MTC_DTYPE_BF16, f32 = src_dtype == MTC_DTYPE_F32;
   if (codes::is_codes(*c)) {
     const int64_t units = (int64_t)rows / codes::kBlock + 2 * n;
-    // one item a wave, but where the blocks fill the chip already: each reads the list of sequences
+    // one item a wave, but where the blocks fill the chip already: each reads the list of sequences. Measured with a read of the newest
+    // tokens, one and several items a wave: 8 heads of 128, 64 sequences of 1 token 9.5, 12.1 us; 64 of 100 17.8, 18.2; 512 of 1 23.4, 20.8; 1
+    // of 16384 24.5, 22.9; 64 of 512 55.4, 51.3
     const int items = (2 * c->kv_heads + 3) / 4;
     if (units > 0xFFFFFF / items || items > 0xFFFF) return fail(MTC_E_SHAPE, "%d rows of %d heads: too many", rows, c->kv_heads);
-    const dim3 g((unsigned)units, units < 2048 ? items : 1);
+    const dim3 g((unsigned)units, units < 1024 ? items : 1);
     if (bf && f32) k_append8<true, MTC_DTYPE_F32><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
     else if (bf) k_append8<true, MTC_DTYPE_BF16><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);
     else if (f32) k_append8<false, MTC_DTYPE_F32><<<g, 256, 0, st>>>(*c, layer, *k, *v, rows, seqs, cu, n);

@@ -47,7 +47,8 @@ __device__ __forceinline__ void sin_cos(int32_t position, uint64_t turns, float&
 
 // One thread per VEC pairs of a token, for HEADS heads: their sines and cosines serve all of them. Slots past the
 // turned dims copy 2 VEC elements each.
-// Bound by memory where there are many tokens, by the launch where there are few.
+// Bound by memory where there are many tokens (16384 of 32 + 8 heads of 128 bf16: 336 MB in 69 us, 4.9 TB/s; a 1 GiB copy: 5.14), by the
+// launch where there are few (one token 2.6 to 3.1 us).
 template <int DT, int VEC, int HEADS>
 __global__ __launch_bounds__(kRotaryThreads) void k_rotary(const mtc_rotary_args a) {
   using V = Value<DT>;
@@ -141,9 +142,10 @@ int check_rotary_heads(const char* what, const mtc_heads& x, int align) {
 template <int DT, int VEC>
 int launch_rotary(const mtc_rotary_args& a, hipStream_t st) {
   const int64_t units = (int64_t)a.rows * (a.dim / (2 * VEC)), all = a.heads + a.kv_heads;
-  // sines for four heads at once where that still fills the chip
+  // sines for four heads at once where that still fills the chip, 512 threads a CU. Measured, one head and four a thread: 32 + 8 heads of 128, 64
+  // tokens 3.4, 4.9 us; 1024 6.8, 7.6; 1500 9.7, 8.7; 4096 18.3, 15.4; 16384 70.5, 68.3; 14 + 2 of 64, 4096 5.7, 6.5; 8192 9.7, 9.2; 16384 15.2, 13.7
   constexpr int kHeads = 4;
-  const bool few = units * ((all + kHeads - 1) / kHeads) < 256 * 1024;
+  const bool few = units * ((all + kHeads - 1) / kHeads) < 128 * 1024;
   const int64_t threads = units * (few ? all : (all + kHeads - 1) / kHeads);
   const int64_t blocks = (threads + kRotaryThreads - 1) / kRotaryThreads;
   if (blocks > 0xFFFFFF) return fail(MTC_E_SHAPE, "%d rows of %d heads: too many", a.rows, (int)all);

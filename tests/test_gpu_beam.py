@@ -13,6 +13,8 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 LOG_ERROR = 80 * 2.0 ** -24
+MANY = [(500, 1, 0), (500, 16, 0), (500, 31, 0), (500, 33, 0), (500, 64, 0), (9000, 1, 0), (9000, 16, 0), (9000, 31, 0),
+        (9000, 33, 0), (9000, 64, 0), (32000, 1, 0), (32000, 16, 0), (32000, 31, 0), (32000, 33, 0), (32000, 64, 0)]                  # vocabulary, beams that go on, seed
 
 
 def _ints(x, dev):
@@ -86,6 +88,30 @@ def test_ended_beams_and_first_steps(gpu, V):
     many = beam_select(logits, scores, n=9, done=torch.tensor(done, device=gpu), pad=-5)
     _check(many, _want(logits, scores, 9, done, -5))
     assert many[1][3].tolist() == [-1] * 9 and many[0][2][4:].tolist() == [-math.inf] * 5
+
+
+def _many(V, live, seed):
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    logits = torch.randn((2, 64, V), generator=g) * 3 + 100
+    scores = torch.full((2, 64), -math.inf)
+    scores[0, :live] = torch.randn(live, generator=g)
+    scores[1, 64 - live:] = torch.randn(live, generator=g) * 100
+    logits[1, 63, 5:] = -math.inf
+    logits[0, 0, 70:] = -math.inf
+    if live > 16:
+        logits[0, 7] = math.nan
+    return logits, scores
+
+
+@pytest.mark.parametrize("V,live,seed", MANY)
+def test_many_picks(gpu, V, live, seed):
+    """64 picks of 64 beams: few beams that go on (the rest wait at -inf), rows with few tokens allowed, a row that has none."""
+    from tensorpack_amd.sampling import beam_select
+    logits, scores = _many(V, live, seed)
+    for n in (17, 25, 64):
+        want = _want(logits, scores, n)
+        _check(beam_select(logits.to(gpu), scores.to(gpu), n=n), want)
 
 
 @pytest.mark.parametrize("V,W", [(40, 2), (3000, 3), (600000, 16)])
