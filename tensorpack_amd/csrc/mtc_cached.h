@@ -35,7 +35,7 @@ namespace attn {
 // raises one of them, so no two share a slot.
 //
 // Three ways through an item's keys:
-//   split keys   16 or 32 rows, units of 32 keys: for few rows the keys' bytes are all that counts, and every wave keeps
+//   split keys   16 or 32 rows, units of kKeys keys (32 of 16-bit numbers, 64 of codes): for few rows the keys' bytes are all that counts, and every wave keeps
 //                loads of its own in flight. A run belongs to a block, whose waves take every fourth unit and are joined
 //                at the end, or, where items are short, to a single wave (64 sequences of 100 keys, 8 K/V heads: an item
 //                takes a block or a wave about 5 us of waiting whatever its length)
@@ -48,7 +48,7 @@ constexpr int kXcds = 8;
 constexpr int kLeastKeys = 32, kMostStart = 8;   // of any Store
 constexpr int kJoinHead = 8;               // words
 constexpr int kManyRows = 128;             // split rows: rows of a tile
-// Measured on the device with 64 sequences on one prefix of 8192, 16 x 6 drafts on prefixes of 1536, 32 sequences of 0 to
+// Measured over the 16-bit cache with 64 sequences on one prefix of 8192, 16 x 6 drafts on prefixes of 1536, 32 sequences of 0 to
 // 16384 and 64 of 1 to 512 (14/2 heads of 64, 32/8 of 128): starts of 1/2, 2/3, 2/5 and 3/3 units are within 6 %
 // of each other but for 1/2 (32 ragged: 48 us against 43); a prefix's unit at 0.9, 1.5 and 2.8 times a unit of keys
 // gives the first case 47, 37 and 34 us, at 5 times 38.

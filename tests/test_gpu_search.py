@@ -66,3 +66,78 @@ def test_ended_beams_stay(example, decoder, gpu):
     ended = [t for best in out for _, t in best if end in t]
     assert ended and all(t.index(end) == len(t) - 1 for t in ended)
     assert all(np.isfinite(s) for best in out for s, _ in best)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_a_captured_step(gpu, dtype):
+    """A step of all calls (a token more of each beam, positions, append, attention with the prompts shared, selection, reordering)
+    captured once and replayed, against eager steps on a cache of its own, bit by bit; the eager ones run between the replays."""
+    import torch
+    from tensorpack_amd.attention import cached_attention
+    from tensorpack_amd.cache import QuantizedCache
+    from tensorpack_amd.rotary import Rotary, apply_rotary
+    from tensorpack_amd.sampling import beam_select
+    dtype = getattr(torch, dtype)
+    n, beams, heads, kv, dim, vocab = 3, 4, 6, 2, 40, 1500
+    rows = n * beams
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu)
+    g = torch.Generator().manual_seed(5)
+    rand = lambda *shape: torch.randn(shape, generator=g).to(gpu).to(dtype)
+    lens = [37, 1, 64]
+    rotary = Rotary(32, interleaved=True, device=gpu)
+    roots, seqs, cu, ones = ints(range(n)), ints(range(n, n + rows)), ints(range(rows + 1)), ints([1] * rows)
+    groups, prefix, starts = ints(range(0, rows + 1, beams)), ints(lens), ints(np.concatenate([[0], np.cumsum(lens)]).tolist())
+    first = rand(2, sum(lens), kv, dim)
+
+    class Side:
+        def __init__(self):
+            self.cache = QuantizedCache(200, 1, kv, dim, max_seqs=n + rows, max_pages=8, dtype=dtype, device=gpu)
+            self.cache.extend(roots, prefix)
+            self.cache.append(0, first[0], first[1], roots, starts)
+            self.cache.fork(roots.repeat_interleave(beams), seqs)
+            self.q, self.k, self.v = (torch.empty((rows, h, dim), dtype=dtype, device=gpu) for h in (heads, kv, kv))
+            self.logits = torch.empty((n, beams, vocab), device=gpu)
+            self.scores, self.done = torch.zeros((n, beams), device=gpu), torch.zeros((n, beams), dtype=torch.bool, device=gpu)
+
+        def take(self, inputs):
+            for a, b in zip((self.q, self.k, self.v, self.logits), inputs):
+                a.copy_(b)
+
+        def step(self):
+            c = self.cache
+            c.extend(seqs, ones)
+            q, k = apply_rotary(rotary, self.q, self.k, c.lens[seqs.long()] - 1)
+            c.append(0, k, self.v, seqs, cu)
+            self.o = cached_attention(q[:, None], c, 0, seqs, groups=groups, prefix_lens=prefix)
+            scores, self.tokens, self.parents = beam_select(self.logits, self.scores, done=self.done, pad=9)
+            self.scores.copy_(scores)
+            self.done.copy_(self.done.gather(1, self.parents.long() % beams) | (self.tokens % 50 == 3))
+            c.reorder(seqs, self.parents.view(-1))
+
+    eager, captured = Side(), Side()
+    inputs = lambda: (rand(rows, heads, dim), rand(rows, kv, dim), rand(rows, kv, dim) * 3, rand(n, beams, vocab).float() * 4)
+    x = inputs()
+    for side in (eager, captured):
+        side.take(x)
+        side.step()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        captured.step()
+    for i in range(30):
+        x = inputs()
+        captured.take(x)
+        graph.replay()
+        if i % 3 == 0:
+            torch.cuda.synchronize()
+        eager.take(x)
+        eager.step()
+        assert torch.isfinite(eager.o).all() and bool(eager.o.abs().sum(-1).min() > 0)
+        for name in ("o", "tokens", "parents", "scores", "done"):
+            assert torch.equal(getattr(eager, name), getattr(captured, name)), (i, name)
+        assert torch.equal(eager.cache.lens, captured.cache.lens) and torch.equal(eager.cache.table, captured.cache.table)
+    assert int(eager.cache.lens[int(seqs[0])]) == lens[0] + 31
+    for side in (eager, captured):
+        side.cache.check()
+        side.cache.free(torch.cat([roots, seqs]))
+        assert side.cache.free_pages == 200
