@@ -72,7 +72,7 @@ __device__ __forceinline__ float reached(float x, float second, int n) {
 // list: then the best are taken one after another.)
 // 256 rows of 128003 bf16, a fifth of them ended, 52 MB: 22.4 us, of which the loads and the maxima take 13 (memory alone 10): all waves'
 // loads arrive at much the same time, so little of the selection lies under them. Blocks that load their next chunk ahead were slower (34 to
-// 42 us), sums kept round by round no faster (24). Four rows of 32000 fp32: 4.4 us.
+// 42 us), as were waves that load two chunks and then select from each (of 2048 23.4, of 4096 27.4); sums kept round by round no faster (24). Four rows of 32000 fp32: 4.4 us.
 template <int DT, int ROUNDS>
 __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const Parts parts) {
   using V = Value<DT>;
