@@ -179,6 +179,18 @@ def test_views(gpu):
     assert all(torch.equal(a, b) for a, b in zip(got, beam_select(base[:, 1], scores)))
 
 
+def test_rows_far_apart(gpu):
+    """Rows 2 GiB apart: offsets pass 32 bits."""
+    import torch
+    from tensorpack_amd.sampling import beam_select
+    buf = torch.empty((3 << 30) + 4096, dtype=torch.bfloat16, device=gpu)
+    far = buf.as_strided((2, 2, 2003), (2 << 30, 1 << 30, 1), 5)
+    near = torch.randn((2, 2, 2003), generator=torch.Generator().manual_seed(6)).bfloat16().to(gpu)
+    far.copy_(near)
+    scores = torch.tensor([[-1.0, -1.5], [-3.0, -2.0]], device=gpu)
+    assert all(torch.equal(a, b) for a, b in zip(beam_select(far, scores), beam_select(near, scores)))
+
+
 def test_capture_and_stream(gpu):
     import torch
     from tensorpack_amd.sampling import beam_select

@@ -259,6 +259,26 @@ def test_read_windows(gpu):
     assert np.array_equal(far[0].double().cpu().numpy(), np.concatenate([m.values(1, 0, 0)[-4:], m.values(1, 3, 0)[-4:]]))
 
 
+def test_rows_far_apart(gpu):
+    """K and V, and results, of rows 2 GiB apart: offsets pass 32 bits."""
+    import torch
+    c, _ = _cache(gpu, kv=2, dim=40)
+    buf = torch.empty((3 << 30) + 4096, dtype=torch.bfloat16, device=gpu)
+    far = lambda at: buf.as_strided((4, 2, 40), (1 << 30, 40, 1), at)
+    near = torch.randn((2, 4, 2, 40), generator=torch.Generator().manual_seed(1)).bfloat16().to(gpu)
+    k, v, to = far(0), far(256), (far(512), far(768))
+    k.copy_(near[0])
+    v.copy_(near[1])
+    seqs, cu = _ints([0, 1], gpu), _ints([0, 3, 4], gpu)
+    c.extend(seqs, _ints([3, 1], gpu))
+    c.append(0, k, v, seqs, cu)
+    c.append(1, near[0], near[1], seqs, cu)
+    c.check()
+    want = c.read(1, seqs, cu, 4)
+    c.read(0, seqs, cu, out=to)
+    assert all(torch.equal(a, b) for a, b in zip(to, want)) and all(bool(x.any(-1).all()) for x in want)
+
+
 def test_more_rows_than_tokens(gpu):
     """Rows that would fall before token 0 are left out, and have no part in the scales."""
     rng = np.random.RandomState(8)

@@ -92,6 +92,23 @@ def test_views_in_place_and_copies(gpu):
     assert torch.equal(apply_rotary(r, q, None, pos, out=(by_heads, None))[0], want[0])
 
 
+def test_rows_far_apart(gpu):
+    """Rows 2 GiB apart, in and out: offsets pass 32 bits."""
+    import torch
+    from tensorpack_amd.rotary import Rotary, apply_rotary
+    r = Rotary(64, device=gpu)
+    pos = torch.tensor([3, 70, 1000, 5], dtype=torch.int32, device=gpu)
+    buf = torch.empty((3 << 30) + 4096, dtype=torch.bfloat16, device=gpu)
+    far = lambda at, h: buf.as_strided((4, h, 64), (1 << 30, 64, 1), at)
+    near = [torch.randn((4, h, 64), generator=torch.Generator().manual_seed(h)).bfloat16().to(gpu) for h in (4, 2)]
+    q, k, to = far(0, 4), far(512, 2), (far(1024, 4), far(2048, 2))
+    q.copy_(near[0])
+    k.copy_(near[1])
+    apply_rotary(r, q, k, pos, out=to)
+    assert all(torch.equal(a, b) for a, b in zip(to, apply_rotary(r, *near, pos)))
+    assert torch.equal(q, near[0]) and torch.equal(k, near[1])
+
+
 def test_nothing_to_do_and_infinities(gpu):
     import torch
     from tensorpack_amd.rotary import Rotary, apply_rotary
