@@ -7,8 +7,8 @@
 //   many rows  each code is read by four waves, so a wave makes numbers of the cache's type of its quarter (code 2^e is one exactly,
 //              nothing is rounded; 2.75 instructions a code: bytes to fp32, a fused multiply-add, pairs packed) and puts those into the
 //              tile; from there on the kernel is that of the 16-bit cache
-// Memory cannot hold an infinity or a NaN here (scales are bounded as they are read, codes are integers), so a key that a row does
-// not see has no part in it by its weight of 0 alone, and no row is computed again.
+// Memory cannot hold an infinity or a NaN here (scales are bounded as they are read, K's and V's alike, codes are integers), so a key that a
+// row does not see has no part in it by its weight of 0 alone, and no row is computed again.
 //
 // 32 sequences of 8192, 32/8 heads of 128, 537 MB: 107 us a pass, 5.0 TB/s (a 1 GiB copy: 5.14; the 16-bit cache: 193). 32 ragged ones up to
 // 16384, 92 MB: 27 us, with the join 31 a pass; its start is much of it (the lists, the table, the first keys: one of 200 keys takes 8 us), and
@@ -69,6 +69,8 @@ __device__ __forceinline__ void wait_tiles(int further) {
     else wait_tiles<BASE, EACH, MOST - 1>(further);
   }
 }
+
+__device__ const uint32_t no_scale = 0;    // of keys on no page: the least there is, so that their zeros never are the largest values
 
 constexpr int kWaveKeys = 64;              // split keys: per wave and step
 constexpr int kSubs = kWaveKeys / 32;      // matrix steps of 32 keys (the depth of a product with the values)
@@ -134,12 +136,12 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
       for (int i = 0; i < kHalfCopies; ++i) copy16(r, from_lane[hf & 1][i], __builtin_amdgcn_readfirstlane(dst + hf * kHalf + i * 1024));
     }
   };
-  // a word that holds the scale: lanes 0 .. kBlocks - 1 of the keys' blocks, the next ones of the values'
+  // a word that holds the scale (every lane copies one, so that copies can be counted): lanes 0 .. kBlocks - 1 of the keys' blocks, the next ones of the values'
   auto scale_at = [&](int p, int is_v) { return (is_v ? a.v_scales : a.k_scales) + head_scales + (int64_t)((p & mask) / codes::kBlock * 2); };
   auto copy_scales = [&](int p0, uint32_t dst) {
     const int p = p0 + 16 * (lane % kBlocks), id = __shfl(pages.ids, min((p >> a.page_log) - pages.at, 63));
-    const char* page = a.codes + (int64_t)((uint32_t)id < (uint32_t)a.n_pages ? id : 0) * a.page_bytes;
-    copy4((uint64_t)(uintptr_t)(page + (scale_at(p, lane / kBlocks & 1) & ~3ll)), __builtin_amdgcn_readfirstlane(dst));
+    const char* at = a.codes + (int64_t)id * a.page_bytes + (scale_at(p, lane / kBlocks & 1) & ~3ll);
+    copy4((uint64_t)(uintptr_t)((uint32_t)id < (uint32_t)a.n_pages ? at : (const char*)&no_scale), __builtin_amdgcn_readfirstlane(dst));
   };
   auto place = [&](int t) { return (uint32_t)(t % kDeep); };
   auto copy_keys = [&](int t) {
@@ -253,8 +255,8 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
 #pragma unroll
     for (int g = 0; g < kBlocks; ++g) {
       const int p = pos + 16 * g;
-      ks[g] = __builtin_bit_cast(float, (uint32_t)(*reinterpret_cast<const uint16_t*>(sc + 4 * g + (scale_at(p, 0) & 2)) & 0x7F80u) << 16);
-      ve[g] = (float)codes::exponent_of<true>(*reinterpret_cast<const uint16_t*>(sc + 4 * (kBlocks + g) + (scale_at(p, 1) & 2)));
+      ks[g] = codes::power(codes::exponent_of<BF>(*reinterpret_cast<const uint16_t*>(sc + 4 * g + (scale_at(p, 0) & 2))));
+      ve[g] = (float)codes::exponent_of<BF>(*reinterpret_cast<const uint16_t*>(sc + 4 * (kBlocks + g) + (scale_at(p, 1) & 2)));
     }
     wait_lds();
     if (t + kDeep < tiles) copy_keys(t + kDeep);
