@@ -86,8 +86,8 @@ struct KeyTiles {
 // or by this wave alone.
 //
 // Codes reach LDS as they are (direct copies, kDeep tiles of 64 keys ahead) and become f16 between LDS and the matrix core, 1.25
-// vector instructions each, for either type of cache: q, scaled by a power of two to f16's range, loses nothing that fp32 sums would
-// keep. Scales are folded in where there is one number per key instead of per element: a key's into its score, a value's into
+// vector instructions each, for either type of cache: bf16 q are scaled by a power of two, the row's largest to 2^15 or more, so that an
+// element loses at most 2^-40 of the largest (a score 2^-40 max |q| sum |k|, less than its fp32 sum does unless K is 0 where q is large). Scales are folded in where there is one number per key instead of per element: a key's into its score, a value's into
 // its weight. With s = score (log2), m its running maximum and e = log2 of the value's scale:
 //   l = sum 2^(s - m),   o = sum 2^(s + e - t) code,   t the running maximum of s + e;   result 2^(t - m) o / l
 // so that weights keep f16's precision whatever the scales are. l adds weights in fp32, before they are rounded to f16 (half a step: 2^-12).
@@ -178,10 +178,10 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
       copy_values(t);
     }
 
-  float scale[MT];
+  int raised[MT];                                        // q is scaled by 2^-raised
 #pragma unroll
   for (int rt = 0; rt < MT; ++rt) {
-    scale[rt] = a.c;
+    raised[rt] = 0;
     if constexpr (BF) {
       uint32_t most = 0;                                 // the row's largest magnitude
 #pragma unroll
@@ -190,16 +190,15 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
         for (int i = 0; i < 4; ++i) most = max(max(most, qf[rt][s][i] << 16 & 0x7FFF0000u), qf[rt][s][i] & 0x7FFF0000u);
       most = max(most, (uint32_t)__shfl_xor((int)most, 16));
       most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-      const int exponent = (int)(most >> 23) - 127;
-      const int by = exponent == 128 ? 0 : min(max(exponent, -100), 113) - 14;       // not finite: as it is
+      raised[rt] = min(max((int)(most >> 23) - 127, -100), 127) - 15;      // -115 to 112: a normal number, its inverse too
+      const float by = codes::power(-raised[rt]);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t u = qf[rt][s][i];
-          qf[rt][s][i] = H::pack(Elem<true>::widen((uint16_t)u) * codes::power(-by), Elem<true>::widen((uint16_t)(u >> 16)) * codes::power(-by));
+          qf[rt][s][i] = H::pack(Elem<true>::widen((uint16_t)u) * by, Elem<true>::widen((uint16_t)(u >> 16)) * by);
         }
-      scale[rt] *= codes::power(by);
     }
   }
 #pragma unroll
@@ -250,12 +249,13 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
           s[rt][g] = H::mfma16(hi, qf[rt][2 * j + 1], s[rt][g]);
         }
       }
-    float ks[kBlocks], ve[kBlocks];                      // the keys' scale, log2 of the values', of the tile's blocks
+    int ks[kBlocks];                                     // log2 of the keys' scales, of the values', of the tile's blocks
+    float ve[kBlocks];
     const char* const sc = mine + kDeep * 2 * kTile + place(t) * Tiles::kScales;
 #pragma unroll
     for (int g = 0; g < kBlocks; ++g) {
       const int p = pos + 16 * g;
-      ks[g] = codes::power(codes::exponent_of<BF>(*reinterpret_cast<const uint16_t*>(sc + 4 * g + (scale_at(p, 0) & 2))));
+      ks[g] = codes::exponent_of<BF>(*reinterpret_cast<const uint16_t*>(sc + 4 * g + (scale_at(p, 0) & 2)));
       ve[g] = (float)codes::exponent_of<BF>(*reinterpret_cast<const uint16_t*>(sc + 4 * (kBlocks + g) + (scale_at(p, 1) & 2)));
     }
     wait_lds();
@@ -266,7 +266,15 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
     for (int rt = 0; rt < MT; ++rt) {
       const int end = min(seen[rt], to);
 #pragma unroll
-      for (int g = 0; g < kBlocks; ++g) s[rt][g] *= scale[rt] * ks[g];
+      for (int g = 0; g < kBlocks; ++g) {
+        if constexpr (BF) {                              // 2^-215 to 2^212, by halves: neither leaves the range of its own accord
+          const int e = raised[rt] + ks[g];
+          s[rt][g] *= codes::power(e >> 1);
+          s[rt][g] *= a.c * codes::power(e - (e >> 1));
+        } else {
+          s[rt][g] *= a.c * codes::power(ks[g]);
+        }
+      }
       if (pos + kWaveKeys > min(all, to)) {
 #pragma unroll
         for (int g = 0; g < kBlocks; ++g)
