@@ -72,6 +72,11 @@ __device__ __forceinline__ void wait_tiles(int further) {
 
 __device__ const uint32_t no_scale = 0;    // of keys on no page: the least there is, so that their zeros never are the largest values
 
+// The nearest number of 11 bits. (NaN stays NaN: matrix instructions and exponentials give no payload that could carry over.)
+__device__ __forceinline__ float round11(float x) {
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) + 0x1000u) & ~0x1FFFu);
+}
+
 constexpr int kWaveKeys = 64;              // split keys: per wave and step
 constexpr int kSubs = kWaveKeys / 32;      // matrix steps of 32 keys (the depth of a product with the values)
 constexpr int kBlocks = kWaveKeys / codes::kBlock;
@@ -90,7 +95,9 @@ struct KeyTiles {
 // element loses at most 2^-40 of the largest (a score 2^-40 max |q| sum |k|, less than its fp32 sum does unless K is 0 where q is large). Scales are folded in where there is one number per key instead of per element: a key's into its score, a value's into
 // its weight. With s = score (log2), m its running maximum and e = log2 of the value's scale:
 //   l = sum 2^(s - m),   o = sum 2^(s + e - t) code,   t the running maximum of s + e;   result 2^(t - m) o / l
-// so that weights keep f16's precision whatever the scales are. l adds weights in fp32, before they are rounded to f16 (half a step: 2^-12).
+// so that weights keep f16's precision whatever the scales are. m and t are rounded up to whole numbers: a key's weights in l and o then differ
+// by a power of two, and one rounding, to f16's 11 bits (half a step: 2^-11), serves both, so that a constant V comes out as itself. (f16 has a
+// weight's rounded bits from 2^-14 on; below that it loses less than 2^-24 of one, where the row's largest is 2^6 or more.)
 template <bool BF, int DP, int MT, bool PREFIX>
 __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, const Entry& x, int item, int from, int to, int slot, bool alone) {
   using H = Elem<false>;
@@ -292,12 +299,12 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
       m1 = half_max(fmaxf(m1, __shfl_xor(m1, 16)));
       t1 = half_max(fmaxf(t1, __shfl_xor(t1, 16)));
       const float was = top[rt];
-      top[rt] = fmaxf(was, m1);
+      top[rt] = fmaxf(was, __builtin_ceilf(m1));
       const float base = top[rt] == -INFINITY ? 0.0f : top[rt];
       sum[rt] *= exp2_fast(was - base);
       if (__ballot(t1 > most[rt] + 15.0f)) {             // weights stay below 2^15 in f16
         const float before = most[rt];
-        most[rt] = fmaxf(before, t1 - (15.0f - kLag));
+        most[rt] = fmaxf(before, __builtin_ceilf(t1) - (15.0f - kLag));
         const float fade = most[rt] == -INFINITY ? 1.0f : exp2_fast(before - most[rt]);
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d) o[rt][d] *= fade;
@@ -306,10 +313,10 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
       float add[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int g = 0; g < kBlocks; ++g) {
-        const float f = exp2_fast(fminf(ve[g] + shift, 126.0f));
+        const float f = codes::power((int)fminf(fmaxf(ve[g] + shift, -126.0f), 126.0f));
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          const float y0 = exp2_fast(s[rt][g][i] - base), y1 = exp2_fast(s[rt][g][i + 1] - base);
+          const float y0 = round11(exp2_fast(s[rt][g][i] - base)), y1 = round11(exp2_fast(s[rt][g][i + 1] - base));
           add[i >> 1] += y0 + y1;
           p[rt][g >> 1][2 * (g & 1) + (i >> 1)] = H::pack(y0 * f, y1 * f);
         }
