@@ -609,6 +609,7 @@ __device__ void split_rows(const CachedCall& a, const Book& book, char* lds, con
 
 template <bool BF>
 struct Store16 {
+  static constexpr bool kCodes = false;
   static constexpr int kKeys = kWaveKeys, kStart = 4, kStartAlone = 4, kShort = 8;
   static constexpr float kCostRows = 2.2f, kCostKeys = 0.8f;
   typedef CachedCall Call;

@@ -480,6 +480,7 @@ struct StoreCodes {
   // Starts measured on 32 and 96 ragged sequences up to 16384 and 4000 (blocks: 2, 3, 4, 5, 6, 8 units give 36, 32.6, 30.3, 30.7, 30.6, 30.6
   // and 92, 82, 72.7, 68.9, 69.2, 71.2 us), on 64 up to 512 (waves: 1, 2, 4 units give 16.8, 17.2, 19.9) and on 8 up to 2048 (items of up to 4,
   // 6, 8 units taken by waves: 16.5, 15.0, 14.3). A unit of keys at 0.8, 1.6, 2.5 beside one of rows at 2.2: 64 on a prefix of 8192 43.2, 47.8, 45.5.
+  static constexpr bool kCodes = true;
   static constexpr int kKeys = kWaveKeys, kStart = 5, kStartAlone = 1, kShort = 8;
   static constexpr float kCostRows = 2.2f, kCostKeys = 0.8f;
   typedef CodesCall Call;

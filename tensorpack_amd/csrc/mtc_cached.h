@@ -3,7 +3,8 @@
 //   Call                         CachedCall, or one that adds to it
 //   E                            the 16-bit type of q, o and the tiles
 //   kKeys                        split keys: keys of a unit, a wave's step (at least kLeastKeys)
-//   kStart, kStartAlone          units that stand for an item's start, in runs of blocks and of single waves (up to kMostStart)
+//   kCodes                       whether the cache is MTC_CACHE_CODES8
+//   kStart, kStartAlone          units that stand for an item's start, in runs of blocks and of single waves (up to most_start(kCodes))
 //   kCostRows, kCostKeys         of a unit of split rows, of split keys, for dealing blocks to prefixes and own parts
 //   kShort                       up to as many units per item on average, runs of single waves
 //   kKeysBytes<DP>               LDS that keys<DP, ...> uses
@@ -34,9 +35,9 @@ namespace attn {
 // result (maximum, sum, weighted values). Its slot is run + item: both only grow along the runs and every crossing
 // raises one of them, so no two share a slot.
 //
-// Three ways through an item's keys:
-//   split keys   16 or 32 rows, units of kKeys keys (32 of 16-bit numbers, 64 of codes): for few rows the keys' bytes are all that counts, and every wave keeps
-//                loads of its own in flight. A run belongs to a block, whose waves take every fourth unit and are joined
+// Three ways through an item's keys, for 16, 32 and 128 rows:
+//   split keys   16 or 32 rows (the first two), units of kKeys keys (32 of 16-bit numbers, 64 of codes): for few rows the
+//                keys' bytes are all that counts, and every wave keeps loads of its own in flight. A run belongs to a block, whose waves take every fourth unit and are joined
 //                at the end, or, where items are short, to a single wave (64 sequences of 100 keys, 8 K/V heads: an item
 //                takes a block or a wave about 5 us of waiting whatever its length)
 //   split rows   up to 128 rows, units of 64 keys, a run per block: as in k_prompt, 32 rows per wave, and the waves share
@@ -45,7 +46,8 @@ constexpr int kCachedWaves = 4;
 constexpr int kCachedThreads = 64 * kCachedWaves;
 constexpr int kCachedBlocks = 512;         // two per CU
 constexpr int kXcds = 8;
-constexpr int kLeastKeys = 32, kMostStart = 8;   // of any Store
+constexpr int kLeastKeys = 32;             // of any Store
+constexpr int most_start(bool codes) { return codes ? 5 : 4; }
 constexpr int kJoinHead = 8;               // words
 constexpr int kManyRows = 128;             // split rows: rows of a tile
 // Measured over the 16-bit cache with 64 sequences on one prefix of 8192, 16 x 6 drafts on prefixes of 1536, 32 sequences of 0 to
@@ -57,7 +59,10 @@ constexpr int kLeastRows = 2;                    // split rows: units of a run (
 enum { kNone = 0, kOneTile = 1, kTwoTiles = 2, kRows = 3 };      // 16 rows, 32 rows, split rows
 __host__ __device__ constexpr int mode_rows(int mode) { return mode == kRows ? kManyRows : 16 * mode; }
 template <class Store>
-__host__ __device__ constexpr int mode_start(int mode, bool alone) { return mode == kRows ? kStartRows : alone ? Store::kStartAlone : Store::kStart; }
+__host__ __device__ constexpr int mode_start(int mode, bool alone) {
+  static_assert(std::max({Store::kStart, Store::kStartAlone, kStartRows}) <= most_start(Store::kCodes), "plan_cached counts with it");
+  return mode == kRows ? kStartRows : alone ? Store::kStartAlone : Store::kStart;
+}
 template <class Store>
 __host__ __device__ constexpr int mode_unit(int mode) { return mode == kRows ? kPromptKeys : Store::kKeys; }
 
@@ -631,7 +636,7 @@ inline int plan_cached(const mtc_cache_desc* c, const mtc_cached_args* a, Cached
   p->pre_stride = p->pre_mode ? stride(all, p->pre_mode) : 0;
   p->pre_slots = p->pre_mode ? runs(p->pre_mode) + (int64_t)c->kv_heads * (tiles(all, p->pre_mode) + a->n_groups) : 0;
   // the kernels count units in 32 bits
-  const int64_t units = (int64_t)c->max_pages * c->page_size / kLeastKeys + 1 + kMostStart;
+  const int64_t units = (int64_t)c->max_pages * c->page_size / kLeastKeys + 1 + most_start(codes::is_codes(*c));
   if (units * (p->own_slots + p->pre_slots) > 0x7FFFFFFF)
     return host::fail(MTC_E_SHAPE, "%d sequences of up to %d pages of %d tokens, %d row tiles: too much for one call", a->n_seqs, c->max_pages,
                 c->page_size, (int)tiles(per, p->own_mode));
