@@ -54,6 +54,27 @@ def _apart(x) -> bool:
     return True
 
 
+def _meet(a, a_shape, b, b_shape, size: int) -> bool:
+    """Two views of (rows, heads, dim) elements of `size` bytes, each given as (address, row stride, head stride) with unit stride along
+    the same dim, share memory. Addresses are multiples of `size`."""
+    (at, r, h), (rows, heads, dim) = a, a_shape
+    (at2, r2, h2), (rows2, heads2, _) = b, b_shape
+    if not (rows and heads and rows2 and heads2):
+        return False
+    apart, block, block2 = (at2 - at) // size, (heads - 1) * h + dim, (heads2 - 1) * h2 + dim
+    if apart >= (rows - 1) * r + block or -apart >= (rows2 - 1) * r2 + block2:
+        return False
+    if r == r2 and r and block <= apart % r <= r - block2:         # parts of the rows of one buffer
+        return False
+    import torch
+    first = (torch.arange(rows)[:, None] * r + torch.arange(heads) * h).flatten().sort().values
+    second = (torch.arange(rows2)[:, None] * r2 + torch.arange(heads2) * h2).flatten() + apart
+    after = torch.searchsorted(first, second, right=True)
+    low = second - first[(after - 1).clamp(min=0)] < dim
+    high = first[after.clamp(max=first.numel() - 1)] - second < dim
+    return bool(((after > 0) & low | (after < first.numel()) & high).any())
+
+
 def _copy(x):
     """A contiguous copy in memory of its own. (contiguous() returns x itself where only its start or the stride of an
     axis of size 1 is in the way.)"""

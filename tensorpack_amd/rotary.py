@@ -11,7 +11,7 @@ from fractions import Fraction
 from typing import Optional, Sequence
 
 from . import _abi, _native
-from .attention import _aligned_rows, _apart, _copy, _int32, _value_code
+from .attention import _aligned_rows, _apart, _copy, _int32, _meet, _value_code
 from .device import on_device, raw_stream, require_gpu
 
 _PI = Fraction(3141592653589793238462643383279502884197169399375105820974944592307816406286, 10 ** 75)
@@ -83,13 +83,22 @@ def _like(out, x) -> bool:
     return out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and _aligned_rows(out) and _apart(out)
 
 
+def _clash(hq, ho, heads, hk, ok, kv_heads, rows, dim, size) -> bool:
+    """A result (ho, ok: address, strides) shares memory with anything but its own input, element by element."""
+    q, k = (rows, heads, dim), (rows, kv_heads, dim)
+    own = lambda a, b, n: a[0] == b[0] and (rows < 2 or a[1] == b[1]) and (n < 2 or a[2] == b[2])
+    q_own, k_own = own(hq, ho, heads), own(hk, ok, kv_heads)         # an input in the place of its result: one pair less
+    return (not q_own and _meet(ho, q, hq, q, size)) or (not k_own and _meet(ok, k, hk, k, size)) or _meet(ho, q, ok, k, size) or \
+        (not k_own and _meet(ho, q, hk, k, size)) or (not q_own and _meet(ok, k, hq, q, size))
+
+
 def apply_rotary(rotary: Rotary, q, k, positions, *, out=None):
     """(q', k'): q (rows, heads, dim) and k (rows, kv_heads, dim; or None) turned by their tokens' positions (mtc_rotary), in one launch.
 
     bf16, f16 or fp32; dim a multiple of 8 up to 1024; dims past rotary.dim are copied. positions (rows) int32 on the
     device, negative ones too. Strided views whose rows and heads are 16-byte aligned are read in place, others are copied.
-    Angles, products and sums are fp32 or better, results rounded once. out: (q', k') to write to, which may be q and k themselves but
-    share no other memory with them; default: new contiguous tensors."""
+    Angles, products and sums are fp32 or better, results rounded once. out: (q', k') to write to, which may be q and k themselves (the
+    same elements in the same places) but share no other memory with them or with each other; default: new contiguous tensors."""
     import torch
     dev = rotary.device
     if q.dim() != 3 or q.device != dev:
@@ -129,8 +138,8 @@ def apply_rotary(rotary: Rotary, q, k, positions, *, out=None):
         ho = _view(out[0])
         if k is not None:
             ok = _view(out[1])
-            if rows and heads and kv_heads and (ho[0] in (hk[0], ok[0]) or ok[0] == hq[0]):
-                raise ValueError("the results' memory is another's of q, k and the results")
+        if _clash(hq, ho, heads, hk, ok, kv_heads, rows, dim, dtype.itemsize):
+            raise ValueError("the results share memory with each other, with the other one's input, or with their own at other places")
     args = _abi.MtcRotaryArgs.from_buffer_copy(_abi.ROTARY_PACK(
         _abi.ABI_VERSION, code, rows, heads, kv_heads, dim, rotary.dim, rotary.interleaved, rotary.amplitude, 0, *hq, *hk, *ho, *ok, p,
         rotary.turns_at))
