@@ -14,7 +14,7 @@ import ctypes
 from typing import Optional
 
 from . import _abi, _native
-from .attention import _aligned_rows, _apart, _copy, _dtype_code, _heads, _int32
+from .attention import _aligned_rows, _apart, _copy, _dtype_code, _heads, _int32, _meet
 from .device import _need, on_device, raw_stream, require_gpu
 
 STATE_WORDS = 4
@@ -260,8 +260,8 @@ class QuantizedCache(PagedCache):
     def read(self, layer: int, seqs, cu, rows: Optional[int] = None, *, dtype=None, out=None):
         """(K, V) (rows, n_kv_heads, head_dim) of tokens held: rows cu[i]:cu[i+1] are the last tokens of seqs[i] (all of them where cu
         holds the sums of `lens`), as `prompt_attention` takes them beside the queries of new tokens. dtype: the cache's (exact) or float32. Rows
-        past a sequence's first token or on no page are 0. out: (K, V) to write to instead, whose rows of no sequence stay as they are;
-        those of a new result hold anything."""
+        past a sequence's first token or on no page are 0. out: (K, V) to write to instead (apart from each other), whose rows of no
+        sequence stay as they are; those of a new result hold anything."""
         import torch
         if not 0 <= layer < self.n_layers:
             raise ValueError(f"layer {layer} of {self.n_layers}")
@@ -282,6 +282,8 @@ class QuantizedCache(PagedCache):
                 if not (ok and x.device == self.device and _aligned_rows(x) and _apart(x)):
                     raise ValueError(f"out must be two (rows, {form[0]}, {form[1]}) {self.dtype} or float32 tensors with 16-byte aligned rows")
             hk, hv = _heads(k), _heads(v)
+            if _meet((hk.data, hk.row_stride, hk.head_stride), k.shape, (hv.data, hv.row_stride, hv.head_stride), v.shape, dtype.itemsize):
+                raise ValueError("out: K and V share memory")
         p = self._list("seqs", seqs)
         c = _int32("cu", cu, seqs.shape[0] + 1, self.device)
         code = _abi.MTC_DTYPE_F32 if dtype == torch.float32 else self._type

@@ -1,5 +1,5 @@
-"""Results that share memory with what a call still reads are refused, without a GPU: apply_rotary's own check, and the question
-that it and QuantizedCache.read ask, against a count of every element's address."""
+"""Results that share memory with each other, or with what a call still reads, are refused, without a GPU: apply_rotary's and
+QuantizedCache.read's checks, and the question that both ask, against a count of every element's address."""
 
 import itertools
 
@@ -65,3 +65,25 @@ def test_rotary_results():
     assert not clash(one, one.as_strided((1, 4, 64), (64, 64, 1)), torch.zeros((1, 2, 64)), torch.zeros((1, 2, 64)))
     heads_first = torch.zeros((6, 5, 64)).transpose(0, 1)
     assert not clash(heads_first[:, :4], heads_first[:, :4], heads_first[:, 4:], heads_first[:, 4:])
+
+
+def test_read_results():
+    from tensorpack_amd.cache import QuantizedCache
+    cache = object.__new__(QuantizedCache)
+    cache.n_layers, cache.n_kv_heads, cache.head_dim, cache.dtype, cache.device = 1, 2, 64, torch.bfloat16, torch.device("cpu")
+    seqs, cu = torch.zeros(1, dtype=torch.int32), torch.tensor([0, 5], dtype=torch.int32)
+    x = torch.zeros((8, 2, 64), dtype=torch.bfloat16)
+    for k, v in ((x[:5], x[:5]), (x[:5], x[3:]), (x[3:], x[:5]), (x[:5].float(), x[:5].float()[:4])):
+        with pytest.raises(ValueError):
+            cache.read(0, seqs, cu, out=(k, v))
+    both = torch.zeros((5, 2, 2, 64), dtype=torch.bfloat16)
+
+    class Passed(Exception):
+        pass
+
+    def passed(*_):
+        raise Passed
+    cache._list = passed                                            # the next step: the arguments were taken
+    for k, v in ((both[:, 0], both[:, 1]), (both[:, :, 0], both[:, :, 1]), (x[:4], x[4:])):
+        with pytest.raises(Passed):
+            cache.read(0, seqs, cu, out=(k, v))
