@@ -142,8 +142,10 @@ int check_rotary_heads(const char* what, const mtc_heads& x, int align) {
 template <int DT, int VEC>
 int launch_rotary(const mtc_rotary_args& a, hipStream_t st) {
   const int64_t units = (int64_t)a.rows * (a.dim / (2 * VEC)), all = a.heads + a.kv_heads;
-  // sines for four heads at once where that still fills the chip, 512 threads a CU. Measured, one head and four a thread: 32 + 8 heads of 128, 64
-  // tokens 3.4, 4.9 us; 1024 6.8, 7.6; 1500 9.7, 8.7; 4096 18.3, 15.4; 16384 70.5, 68.3; 14 + 2 of 64, 4096 5.7, 6.5; 8192 9.7, 9.2; 16384 15.2, 13.7
+  // sines for four heads at once where that still fills the chip, 512 threads a CU. Measured in a graph, one head and four a thread, by the
+  // count of threads of four (K): 32 + 8 heads of 128, 512 tokens (40) 4.5, 5.3 us; 1228 (96) 6.8, 7.1; 1400 (109) 7.4, 7.6; 1500 (117) 8.2, 7.8; 1638
+  // (128) 8.3, 8.2; 2048 (160) 10.8, 9.5; 4096 17.0, 15.1; 14 + 2 of 64, 6000 (94) 6.7, 7.3; 8192 (128) 8.4, 8.1; 8 + 1 of 128, 6144 (144) 7.7, 8.6;
+  // 8192 (192) 9.9, 9.1; 16 + 16 of 80, 32 turned, 3200 (125) 8.3, 9.1. fp32 would cross later: 32 + 8 of 128, 2048 (160) 16.0, 17.5.
   constexpr int kHeads = 4;
   const bool few = units * ((all + kHeads - 1) / kHeads) < 128 * 1024;
   const int64_t threads = units * (few ? all : (all + kHeads - 1) / kHeads);
