@@ -110,10 +110,14 @@ __global__ __launch_bounds__(kThreads) void k_beam(const mtc_beam_args a, const 
   for (int e = 0; e < kEach; ++e) half[e / 4 % 2] = fmaxf(half[e / 4 % 2], x[e]);
   const float mine = fmaxf(half[0], half[1]);
   const float top = wave_top(mine), base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
+  float sums[8] = {};                                      // a term is rounded with ROUNDS sums, then 3 and 6, not with 64: the log is off by 20 * 2^-24 at most
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) sum += exp2_fast((x[e] - base) * kLog2e);
-  sum = wave_sum(sum);
+  for (int e = 0; e < kEach; ++e) sums[e % 8] += exp2_fast((x[e] - base) * kLog2e);
+#pragma unroll
+  for (int d = 4; d; d >>= 1)
+#pragma unroll
+    for (int e = 0; e < d; ++e) sums[e] += sums[e + d];
+  const float sum = wave_sum(sums[0]);
   const int64_t part = (int64_t)row * parts.chunks + chunk;
   if (lane == 0) parts.stat[part] = Stat{top, sum};
   Candidate* const out = parts.best + part * a.n;
