@@ -8,7 +8,6 @@ waits for the GPU, so a serving loop can capture them into a graph.
 
 import ctypes
 import functools
-import math
 from typing import Optional
 
 from . import _abi, _native
@@ -100,10 +99,13 @@ def _int32(name, x, n, device):
     return x.data_ptr()
 
 
+_F32_MAX = (2 - 2 ** -23) * 2.0 ** 127
+
+
 def _scale(scale: Optional[float], dim: int) -> float:
     if scale is None:
         return dim ** -0.5
-    if not (math.isfinite(scale) and scale > 0):
+    if not 0 < scale <= _F32_MAX:
         raise ValueError(f"scale must be positive and finite, got {scale}")
     return float(scale)
 

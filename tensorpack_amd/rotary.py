@@ -11,7 +11,7 @@ from fractions import Fraction
 from typing import Optional, Sequence
 
 from . import _abi, _native
-from .attention import _aligned_rows, _apart, _copy, _int32, _meet, _value_code
+from .attention import _F32_MAX, _aligned_rows, _apart, _copy, _int32, _meet, _value_code
 from .device import on_device, raw_stream, require_gpu
 
 _PI = Fraction(3141592653589793238462643383279502884197169399375105820974944592307816406286, 10 ** 75)
@@ -48,8 +48,8 @@ class Rotary:
         import torch
         self.device = require_gpu(device)
         self.dim, self.interleaved, self.amplitude = int(dim), bool(interleaved), float(amplitude)
-        if not math.isfinite(self.amplitude):
-            raise ValueError(f"amplitude must be finite, got {amplitude}")
+        if not abs(self.amplitude) <= _F32_MAX:
+            raise ValueError(f"amplitude must be a finite fp32 number, got {amplitude}")
         f = rotary_frequencies(dim, base=base, factor=factor, original=original, ramp=ramp)
         if frequencies is not None:
             given = [float(x) for x in frequencies]
