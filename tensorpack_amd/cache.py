@@ -205,11 +205,14 @@ class PagedCache:
 class QuantizedCache(PagedCache):
     """A PagedCache that holds K and V in 8 bits: half the memory, and half the bytes that `cached_attention` reads.
 
-    A value is code * 2 ** e: an int8 code, and an exponent for each block of 16 tokens, K or V and head, the least for which the block's
-    values fit (each is off by half a step at most, 2 ** (e - 1), which is 1 / 127 of the block's largest or less). Powers of two, so that every
-    value is a number of `dtype` and is read back exactly, and so that rounding is the same in any precision. `append` of a token
-    larger than those that its block holds rounds their codes again, to the larger step; a block keeps its step until its first token is
-    written again, also where `truncate` dropped the token that made it large.
+    A value is code * 2 ** e: an int8 code, and an exponent for each block of 16 tokens, K or V and head: at each `append` the least for which the
+    new values fit, or the block's own if that is larger. Powers of two, so that every value is a number of `dtype` and is read back exactly, and
+    so that rounding is the same in any precision. A value is off by half a step at most, 2 ** (e - 1), which is 1 / 127 of the block's largest or less,
+    while its block keeps the step that it was written with. `append` of a token larger than those that its block holds rounds their codes
+    again, to the larger step: they are then off by less than one step of the present e (half a step of each that the block has had).
+    A block keeps its step until its first token is written again, also where `truncate` or `restore` dropped the token that made it large: the tokens
+    before it in its block of 16 stay as coarse as it made them, and the next ones are rounded to that step too. Where drafts are
+    taken back, their K and V should be of the size of the others.
     The exponents are bounded: values above 65024 (float16) are cut there, and no step is finer than 2 ** -24 (float16) or
     2 ** -100 (bfloat16). NaN becomes 0, an infinity the block's largest value.
 
