@@ -185,10 +185,14 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
       copy_values(t);
     }
 
-  int raised[MT];                                        // q is scaled by 2^-raised
+  // A score in log2 is a product of q and codes, times scale, times 2^(rest + the exponent of K's scale): of the powers of two, -115 to 112 of q's
+  // scaling and -100 to 100, neither factor leaves fp32's range, nor becomes 0.
+  float scale[MT];
+  int rest[MT];
 #pragma unroll
   for (int rt = 0; rt < MT; ++rt) {
-    raised[rt] = 0;
+    scale[rt] = a.c;
+    rest[rt] = 0;
     if constexpr (BF) {
       uint32_t most = 0;                                 // the row's largest magnitude
 #pragma unroll
@@ -197,8 +201,8 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
         for (int i = 0; i < 4; ++i) most = max(max(most, qf[rt][s][i] << 16 & 0x7FFF0000u), qf[rt][s][i] & 0x7FFF0000u);
       most = max(most, (uint32_t)__shfl_xor((int)most, 16));
       most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-      raised[rt] = min(max((int)(most >> 23) - 127, -100), 127) - 15;      // -115 to 112: a normal number, its inverse too
-      const float by = codes::power(-raised[rt]);
+      const int raised = min(max((int)(most >> 23) - 127, -100), 127) - 15;      // q is scaled by 2^-raised: a normal number, its inverse too
+      const float by = codes::power(-raised);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
 #pragma unroll
@@ -206,6 +210,9 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
           const uint32_t u = qf[rt][s][i];
           qf[rt][s][i] = H::pack(Elem<true>::widen((uint16_t)u) * by, Elem<true>::widen((uint16_t)(u >> 16)) * by);
         }
+      const int now = min(max(raised, -90), 90);
+      scale[rt] = fminf(scale[rt] * codes::power(now), 3.40282347e+38f);
+      rest[rt] = raised - now;
     }
   }
 #pragma unroll
@@ -273,15 +280,7 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
     for (int rt = 0; rt < MT; ++rt) {
       const int end = min(seen[rt], to);
 #pragma unroll
-      for (int g = 0; g < kBlocks; ++g) {
-        if constexpr (BF) {                              // 2^-215 to 2^212, by halves: neither leaves the range of its own accord
-          const int e = raised[rt] + ks[g];
-          s[rt][g] *= codes::power(e >> 1);
-          s[rt][g] *= a.c * codes::power(e - (e >> 1));
-        } else {
-          s[rt][g] *= a.c * codes::power(ks[g]);
-        }
-      }
+      for (int g = 0; g < kBlocks; ++g) s[rt][g] *= scale[rt];
       if (pos + kWaveKeys > min(all, to)) {
 #pragma unroll
         for (int g = 0; g < kBlocks; ++g)
@@ -289,12 +288,13 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
           for (int i = 0; i < 4; ++i)
             if (pos + 16 * g + 4 * w + i >= end) s[rt][g][i] = -INFINITY;
       }
-      float m1 = -INFINITY, t1 = -INFINITY;
+      float m1 = -INFINITY, t1 = -INFINITY, by[kBlocks];
 #pragma unroll
       for (int g = 0; g < kBlocks; ++g) {
         const float mx = fmaxf(fmaxf(s[rt][g][0], s[rt][g][1]), fmaxf(s[rt][g][2], s[rt][g][3]));
-        m1 = fmaxf(m1, mx);
-        t1 = fmaxf(t1, mx + ve[g]);
+        by[g] = codes::power(rest[rt] + ks[g]);
+        m1 = fmaxf(m1, mx * by[g]);
+        t1 = fmaxf(t1, __builtin_fmaf(mx, by[g], ve[g]));
       }
       m1 = half_max(fmaxf(m1, __shfl_xor(m1, 16)));
       t1 = half_max(fmaxf(t1, __shfl_xor(t1, 16)));
@@ -316,7 +316,8 @@ __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, cons
         const float f = codes::power((int)fminf(fmaxf(ve[g] + shift, -126.0f), 126.0f));
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          const float y0 = round11(exp2_fast(s[rt][g][i] - base)), y1 = round11(exp2_fast(s[rt][g][i + 1] - base));
+          const float y0 = round11(exp2_fast(__builtin_fmaf(s[rt][g][i], by[g], -base)));
+          const float y1 = round11(exp2_fast(__builtin_fmaf(s[rt][g][i + 1], by[g], -base)));
           add[i >> 1] += y0 + y1;
           p[rt][g >> 1][2 * (g & 1) + (i >> 1)] = H::pack(y0 * f, y1 * f);
         }
