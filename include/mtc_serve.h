@@ -87,7 +87,7 @@ int mtc_prompt_attention(const mtc_prompt_args* a, void* workspace, size_t works
  * 8-bit caches: dtype MTC_DTYPE_BF16 or MTC_DTYPE_F16 with MTC_CACHE_CODES8. A page is
  *   [n_layers][2 (K, V)][kv_heads][page_size][dim rounded up to a multiple of 16] int8 codes, then
  *   [n_layers][2][kv_heads][page_size / MTC_CODES8_BLOCK] bf16 scales, rounded up to a multiple of 16 bytes;
- * a value is code * scale, of a scale for each MTC_CODES8_BLOCK tokens of one head, a power of two from 2^-100 to 2^100 (bf16)
+ * a value is code * scale, of a code from -127 to 127 and a scale for each MTC_CODES8_BLOCK tokens of one head, a power of two from 2^-100 to 2^100 (bf16)
  * or 2^-24 to 2^9 (f16): every value is a number of the dtype. Bookkeeping calls and mtc_cached_attention take both kinds.
  */
 enum {

@@ -7,13 +7,17 @@
 //   many rows  each code is read by four waves, so a wave makes numbers of the cache's type of its quarter (code 2^e is one exactly,
 //              nothing is rounded; 2.75 instructions a code: bytes to fp32, a fused multiply-add, pairs packed) and puts those into the
 //              tile; from there on the kernel is that of the 16-bit cache
+// Weights are rounded to 16 bits once, as the matrix core's operands have to be, and summed as rounded: to f16's 11 bits by few rows over
+// either cache, to the cache's type by many, bf16's 8 bits among them (as over the 16-bit cache). Relative error against 64 bits, rounding
+// of the result included: 64 sequences on one prefix (bf16, many rows) 2.1e-3, fp32 weights 1.7e-3; 16 x 6 drafts (f16) 2.4e-4 and 2.1e-4; bf16, few
+// rows 1.5e-3 both.
 // Memory cannot hold an infinity or a NaN here (scales are bounded as they are read, K's and V's alike, codes are integers), so a key that a
 // row does not see has no part in it by its weight of 0 alone, and no row is computed again.
 //
-// 32 sequences of 8192, 32/8 heads of 128, 537 MB: 107 us a pass, 5.0 TB/s (a 1 GiB copy: 5.14; the 16-bit cache: 193). 32 ragged ones up to
-// 16384, 92 MB: 27 us, with the join 31 a pass; its start is much of it (the lists, the table, the first keys: one of 200 keys takes 8 us), and
+// 32 sequences of 8192, 32/8 heads of 128, 537 MB: 109 us a pass, 4.9 TB/s (a 1 GiB copy: 5.14; the 16-bit cache: 193). 32 ragged ones up to
+// 16384, 92 MB: 27.6 us, with the join 31 a pass; its start is much of it (the lists, the table, the first keys: one of 200 keys takes 8 us), and
 // items that change within a block's run. As 16-bit numbers in LDS, 32 keys a step, it took 29.6 us and 32 of 8192 114.
-// 64 sequences on a prefix of 8192: 35 us, of which some 21 are start, fill and the partial results of 64 KB a run; a step of 64 keys
+// 64 sequences on a prefix of 8192: 36 us, of which some 21 are start, fill and the partial results of 64 KB a run; a step of 64 keys
 // takes 3.1 us with two blocks a CU, half of it conversions. Runs of 4 or 8 units at least (fewer partial results): 43.4 and 48.5 us a
 // pass against 43.8; the first two tiles' copies issued together: 43.5 and 43.5.
 
@@ -91,13 +95,15 @@ struct KeyTiles {
 // or by this wave alone.
 //
 // Codes reach LDS as they are (direct copies, kDeep tiles of 64 keys ahead) and become f16 between LDS and the matrix core, 1.25
-// vector instructions each, for either type of cache: bf16 q are scaled by a power of two, the row's largest to 2^15 or more, so that an
-// element loses at most 2^-40 of the largest (a score 2^-40 max |q| sum |k|, less than its fp32 sum does unless K is 0 where q is large). Scales are folded in where there is one number per key instead of per element: a key's into its score, a value's into
+// vector instructions each, for either type of cache. bf16 q are scaled by a power of two, the row's largest to 2^15 or more, so that an
+// element loses at most 2^-40 of the largest (a score 2^-40 max |q| sum |k|: less than its fp32 sum does, unless K is 0 where q is
+// large). Scales are folded in where there is one number per key instead of per element: a key's into its score, a value's into
 // its weight. With s = score (log2), m its running maximum and e = log2 of the value's scale:
 //   l = sum 2^(s - m),   o = sum 2^(s + e - t) code,   t the running maximum of s + e;   result 2^(t - m) o / l
-// so that weights keep f16's precision whatever the scales are. m and t are rounded up to whole numbers: a key's weights in l and o then differ
-// by a power of two, and one rounding, to f16's 11 bits (half a step: 2^-11), serves both, so that a constant V comes out as itself. (f16 has a
-// weight's rounded bits from 2^-14 on; below that it loses less than 2^-24 of one, where the row's largest is 2^6 or more.)
+// so that weights keep f16's precision whatever the scales are. m and t are rounded up to whole numbers: a key's weights in l and o
+// then differ by a power of two, and one rounding, to f16's 11 bits (half a step: 2^-11), serves both, so that a constant V comes out as
+// itself. (f16 has a weight's rounded bits from 2^-14 on; below that it loses less than 2^-24 of one, where the row's largest is 2^6 or
+// more.) Bounds, any q, and one rounding cost 2 % (32 ragged sequences: 30.3 -> 30.9 us a pass; heads of 64: 26.7 -> 27.7).
 template <bool BF, int DP, int MT, bool PREFIX>
 __device__ void split_keys(const CodesCall& a, const Book& book, char* lds, const Entry& x, int item, int from, int to, int slot, bool alone) {
   using H = Elem<false>;

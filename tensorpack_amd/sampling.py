@@ -70,10 +70,12 @@ def verify_drafts(drafts, p, q, u, noise, *, n_drafts=None):
 def beam_select(logits, scores, *, n: Optional[int] = None, done=None, pad: int = 0):
     """(scores, tokens, parents), each (B, n): the n best continuations of each prompt's W beams (mtc_beam_select).
 
-    logits (B, W, V) fp32, bf16 or f16, unit stride along V; scores (B, W) fp32: the beams' log probabilities so far. n: default W, at
-    most 64, as W. A continuation's score is scores[b, w] + log_softmax(logits[b, w])[v]; the best come first, equal ones
-    in the order of w * V + v. done (B, W) bool: beams that have ended; such a beam stands as one candidate with its score as it is and the token
-    `pad`. Scores of -inf are no candidates (give all beams but one -inf at the first step, or tokens that must not come a logit of -inf).
+    logits (B, W, V) fp32, bf16 or f16, unit stride along V (else copied), up to 65535 rows; scores (B, W) fp32: the beams' log
+    probabilities so far. n: default W, at most 64, as W. A continuation's score is scores[b, w] + log_softmax(logits[b, w])[v]; the best
+    come first, equal ones in the order of w * V + v. A log sum is off by less than 2.7e-6 (V up to 2 ** 20; usually a tenth of that): of two beams'
+    continuations that lie closer, either may come first. done (B, W) bool: beams that have ended; such a beam stands as one candidate
+    with its score as it is and the token `pad`. Scores of -inf are no candidates (give all beams but one -inf at the first step, or tokens
+    that must not come a logit of -inf).
     scores fp32, tokens int32, parents int32: the row b * W + w of the beam that goes on, as it stands in `logits.flatten(0, 1)`, and in the
     list for `PagedCache.reorder` where n = W. Where there are fewer candidates than n: -inf, -1 and some row of the prompt.
     """

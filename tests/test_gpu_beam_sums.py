@@ -1,7 +1,7 @@
 """beam_select: beams whose scores differ by little, where terms of the sum of exponentials are small against it.
 
-A term goes through 8 sums in a lane, 3 that put a lane's together and 6 over the lanes, is off by 3 * 2^-24 itself, and the chunks are put together by fp32
-factors of two roundings each and fp64 sums: a log sum is off by less than 20 * 2^-24 = 1.2e-6."""
+A term goes through 8 sums in a lane, 3 that put a lane's together and 6 over the lanes, and is off by 3 * 2^-24 itself: a log sum is off by less than 20 * 2^-24
+= 1.2e-6 where, as here, nearly all of it comes from terms at the maximum (others are off by 2.3 * 2^-24 times their distance from it besides)."""
 
 import math
 
